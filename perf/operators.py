@@ -347,7 +347,7 @@ def _quantise(x):
     b = x.reshape(*x.shape[:-1], -1, 32)
     at = b.abs().argmax(-1, keepdim=True)  # the first of the largest
     m = torch.gather(b, -1, at)[..., 0]
-    d = (m / -8).float().bfloat16().float().clamp(-8160, 8160).half()
+    d = (m / -8).float().bfloat16().float().clamp(-2720, 2720).half()
     dd = d.double()[..., None]
     n = torch.where(dd != 0, torch.floor(b / torch.where(dd != 0, dd, 1.0) + 8.5), 8.0).clamp(0, 15)
     return n.to(torch.int32).reshape(x.shape), d
