@@ -417,6 +417,81 @@ bool zlm_gpu_attention_decode_enqueue_noalloc(zlm_device *dev, const float *qkv,
                                               uint16_t *k_cache, uint16_t *v_cache, uint32_t max_seq, float scale,
                                               float *out);
 
+/* ---- a paged KV cache: several sequences' keys and values in pages of one pool ----
+ * No reference counterpart (its caches are one sequence's, contiguous).  A page
+ * holds `page_size` positions of every kv head; K and V have a pool of `n_pages`
+ * pages each, zlm_gpu_paged_page_bytes a page (so n_pages times that a pool),
+ * 16-byte aligned.  Per head, at head * (page bytes / n_kv_heads) of its page:
+ *   K  f16   [page_size][head_dim]
+ *      q4_0  [page_size][head_dim/32][16], the nibble bytes of GGUF q4_0 blocks,
+ *            then their f16 scales [page_size][head_dim/32]
+ *   V, by groups of 8 positions
+ *      f16   [page_size/8][head_dim][8]
+ *      q4_0  one 32-bit word of 8 nibbles per group and dim, position j's at bits
+ *            4*(j/2) + 16*(j%2), [page_size/8][head_dim], then the f16 scales
+ *            [page_size/8][head_dim/32][8]
+ * A q4_0 value is d * (nibble - 8).  d holds at most 8 significant bits and at
+ * most 2720 in size, so a value is exact in f16; the append writes such scales,
+ * and a cache filled elsewhere has to.  Pages need no clearing: what lies past a
+ * sequence's length is never used, whatever bits it holds. */
+typedef struct {
+    void *k, *v;           /* device pools */
+    uint32_t type;         /* ZLM_GGML_F16 or ZLM_GGML_Q4_0 */
+    uint32_t n_kv_heads;
+    uint32_t head_dim;     /* 64, 128 or 256 */
+    uint32_t page_size;    /* 16, 32, 64, 128 or 256 positions */
+    uint32_t n_pages;
+} zlm_paged_cache;
+/* A batch of tokens, any number a sequence.  The arrays are device memory, read
+ * when the work runs: a captured graph replays with what they hold then.  Rows
+ * q_start[s] .. q_start[s+1]-1 of the token buffers are sequence s's newest
+ * tokens, the last at position kv_len[s] - 1; position p of s lies in page
+ * table[s * table_stride + p / page_size].  q_start never decreases.  A sequence
+ * may have no rows.  Rows at negative positions (kv_len below the row count)
+ * are padding, rows from q_start[n_seqs] on are not touched.  A page number
+ * outside [0, n_pages) is no page: nothing is appended there, and what reads a
+ * position there becomes NaN.  Sequences may share pages that none of them
+ * appends to; two rows of one call never write one position. */
+typedef struct {
+    uint32_t n_seqs;         /* at most 1024 */
+    uint32_t n_tokens;       /* rows of the token buffers, at most 2^24 */
+    const int32_t *q_start;  /* n_seqs + 1 */
+    const int32_t *kv_len;   /* n_seqs: positions of each sequence, these rows included */
+    const int32_t *table;    /* n_seqs x table_stride page numbers */
+    uint32_t table_stride;
+} zlm_paged_batch;
+/* Bytes of one page of one pool; 0 for a type or size that is not supported. */
+uint64_t zlm_gpu_paged_page_bytes(uint32_t type, uint32_t n_kv_heads, uint32_t head_dim, uint32_t page_size);
+/* The batch form of zlm_gpu_qk_norm_rope_kv_enqueue: per row q/k head RMSNorm
+ * (weights of head_dim floats; both null: none), rotate-half RoPE at the row's
+ * position and the append of K and V to its page.  qkv rows are [q: n_heads*hd |
+ * k: n_kv_heads*hd | v: n_kv_heads*hd] floats, qkv_stride floats apart (0:
+ * packed); q_out: n_tokens x n_heads*hd floats, 0 in padding rows.  The angle
+ * (position * freq_base^(-2i/hd)), the norm and the choice of 4-bit values are
+ * formed in 64 bits.  q4_0: d = -m/8 of the block's value m of the largest size
+ * (the first of several), rounded to 8 significant bits, n = floor(x/d + 8.5)
+ * within 0..15; a block with a NaN reads back as NaN, values past 21760 saturate.
+ * f16: rounded to nearest, infinite past its range. */
+bool zlm_gpu_paged_append_enqueue(zlm_device *dev, const zlm_paged_cache *cache, const zlm_paged_batch *batch,
+                                  const float *qkv, uint64_t qkv_stride, const float *q_norm_w,
+                                  const float *k_norm_w, uint32_t n_heads, float eps, float freq_base, float *q_out);
+/* The batch's own rows as the cache holds them: k_out and v_out, n_tokens x
+ * n_kv_heads*hd floats; 0 in padding rows. */
+bool zlm_gpu_paged_read_enqueue(zlm_device *dev, const zlm_paged_cache *cache, const zlm_paged_batch *batch,
+                                float *k_out, float *v_out);
+/* Attention of every row over the positions [max(0, p - window + 1), p] of its
+ * sequence (p: the row's position; window 0: all from 0), scores scaled by
+ * `scale`, q heads dealt to kv heads in order (n_heads / n_kv_heads each); q and
+ * out: n_tokens x n_heads*hd floats, 16-byte aligned.  One token a sequence, a
+ * prompt's chunk, or both in one batch.  The results have the accuracy of 32-bit
+ * products and sums over the cached values.  A padding row's output is 0.  NaN or
+ * infinite K reaches the rows that see its position only; such a V may make NaN
+ * of other rows of its sequence in the same call, never of another sequence's.
+ * Partial results live in the library scratch of zlm_gpu_attention_enqueue (call
+ * once before capture). */
+bool zlm_gpu_paged_attention_enqueue(zlm_device *dev, const zlm_paged_cache *cache, const zlm_paged_batch *batch,
+                                     const float *q, uint32_t n_heads, uint32_t window, float scale, float *out);
+
 /* ---- HIP graphs over the device stream ----
  * Everything enqueued between capture_begin and capture_end is recorded, not
  * run.  Only the *_enqueue entry points can be captured: the host-buffer

@@ -1,0 +1,122 @@
+"""What the serving operators' entry points refuse, launch and allocate, without a
+GPU: the host library over the stand-in runtime (tests/fake_hip.cpp), whose
+kernels do nothing.  Addresses are not read here."""
+import ctypes
+
+import pytest
+
+from zlm_amd import device as zd
+from tests.test_host_routes import MALLOCS, _Box, fake  # noqa: F401
+
+
+@pytest.fixture
+def box(fake):  # noqa: F811
+    b = _Box(fake, 1 << 16, 1 << 16)
+    b.mod = fake
+    yield b
+    b.dev.deinit()
+
+
+def _cache(mod, k=1 << 20, v=1 << 21, type=zd.Q4_0, kv=2, hd=128, page=64, pages=4):
+    return mod.PagedCache(k, v, type, kv, hd, page, pages)
+
+
+def _batch(mod, seqs=2, tokens=3, q_start=1 << 12, kv_len=1 << 13, table=1 << 14, stride=2):
+    return mod.PagedBatch(seqs, tokens, q_start, kv_len, table, stride)
+
+
+BAD_CACHES = [dict(type=zd.Q8_0), dict(type=zd.F32), dict(hd=96), dict(hd=0), dict(kv=0), dict(kv=2000), dict(page=8),
+              dict(page=48), dict(page=512), dict(page=0), dict(k=0), dict(v=0), dict(k=(1 << 20) + 8), dict(pages=0),
+              dict(pages=0x80000000)]
+BAD_BATCHES = [dict(seqs=1025), dict(tokens=(1 << 24) + 1), dict(q_start=0), dict(kv_len=0), dict(table=0),
+               dict(stride=0)]
+
+
+def _calls(box, cache, batch):
+    d, p = box.dev, 1 << 16
+    return {"append": lambda: d.paged_append_enqueue(cache, batch, p, p, 8, 1e-6, 1e6),
+            "read": lambda: d.paged_read_enqueue(cache, batch, p, p),
+            "attention": lambda: d.paged_attention_enqueue(cache, batch, p, p, 8, 0.1)}
+
+
+@pytest.mark.parametrize("op", ["append", "read", "attention"])
+def test_bad_caches_and_batches_are_refused(box, op):
+    for bad in BAD_CACHES:
+        assert not _calls(box, _cache(box.mod, **bad), _batch(box.mod))[op](), bad
+        assert box.dev.last_error()
+    for bad in BAD_BATCHES:
+        assert not _calls(box, _cache(box.mod), _batch(box.mod, **bad))[op](), bad
+        assert box.dev.last_error()
+    assert _calls(box, _cache(box.mod), _batch(box.mod))[op](), box.dev.last_error()
+
+
+def test_other_arguments_are_refused(box):
+    d, p, c, b = box.dev, 1 << 16, _cache(box.mod), _batch(box.mod)
+    for heads in (0, 3, 16386):
+        assert not d.paged_attention_enqueue(c, b, p, p, heads, 0.1), heads
+    for q, out in ((0, p), (p, 0), (p + 4, p), (p, p + 8)):
+        assert not d.paged_attention_enqueue(c, b, q, out, 8, 0.1), (q, out)
+    assert not d.paged_attention_enqueue(c, b, p, p, 8, 0.1, window=1 << 31)
+    # 2^24 tokens of 128 q heads over sequences of 2^24 positions: more work than a call counts
+    big = _batch(box.mod, seqs=1000, tokens=1 << 24, stride=1 << 18)
+    assert not d.paged_attention_enqueue(_cache(box.mod, kv=8), big, p, p, 128, 0.1)
+    assert "too large" in d.last_error()
+    assert not d.paged_append_enqueue(c, b, 0, p, 8, 1e-6, 1e6)
+    assert not d.paged_append_enqueue(c, b, p, 0, 8, 1e-6, 1e6)
+    assert not d.paged_append_enqueue(c, b, p, p, 0, 1e-6, 1e6)
+    assert not d.paged_append_enqueue(c, b, p, p, 8, 1e-6, 0.0)
+    assert not d.paged_append_enqueue(c, b, p, p, 8, 1e-6, float("nan"))
+    assert not d.paged_append_enqueue(c, b, p, p, 8, 1e-6, 1e6, q_norm_w=p)  # weights of q alone
+    assert not d.paged_append_enqueue(c, b, p, p, 8, 1e-6, 1e6, qkv_stride=12 * 128 - 1)
+    assert d.paged_append_enqueue(c, b, p, p, 8, 1e-6, 1e6, qkv_stride=12 * 128)
+    assert not d.paged_read_enqueue(c, b, 0, p) and not d.paged_read_enqueue(c, b, p, 0)
+    raw = box.raw
+    assert not raw.zlm_gpu_paged_read_enqueue(d._h, None, ctypes.byref(b.c), p, p)
+    assert not raw.zlm_gpu_paged_read_enqueue(d._h, ctypes.byref(c.c), None, p, p)
+
+
+def test_an_empty_batch_launches_nothing(box):
+    box.dev.launch_log(True)
+    for empty in (dict(seqs=0), dict(tokens=0)):
+        b = _batch(box.mod, q_start=0, kv_len=0, table=0, **empty)
+        for op, call in _calls(box, _cache(box.mod, k=0, v=0), b).items():
+            assert call(), (op, box.dev.last_error())
+    assert box.dev.launch_log_read() == []
+
+
+def test_attention_scratch_is_sized_eagerly(box):
+    """Under capture the attention runs in the scratch that an eager call made, and fails without one."""
+    d, call = box.dev, _calls(box, _cache(box.mod), _batch(box.mod))["attention"]
+    assert d.capture_begin()
+    assert not call() and "before capture" in d.last_error()
+    d.graph_destroy(d.capture_end())
+    assert call(), d.last_error()
+    mallocs = box.stat(MALLOCS)
+    assert d.capture_begin()
+    assert call(), d.last_error()
+    g = d.capture_end()
+    assert call() and box.stat(MALLOCS) == mallocs
+    # a call that needs more scratch than the graph's leaves it alone
+    wide = _calls(box, _cache(box.mod, hd=256), _batch(box.mod))["attention"]
+    assert not wide() and "captured graph" in d.last_error()
+    d.graph_destroy(g)
+    assert wide(), d.last_error()
+
+
+def test_page_bytes():
+    assert zd.paged_page_bytes(zd.F16, 8, 128, 64) == 8 * 64 * 256
+    assert zd.paged_page_bytes(zd.Q4_0, 8, 128, 64) == 8 * 64 * 72
+    assert zd.paged_page_bytes(zd.Q4_0, 1, 64, 16) == 16 * 36
+    for bad in ((zd.Q8_0, 8, 128, 64), (zd.F16, 8, 96, 64), (zd.F16, 8, 128, 24)):
+        assert zd.paged_page_bytes(*bad) == 0
+
+
+def test_an_inert_device_refuses():
+    dev = zd.Device()
+    if dev.available():
+        pytest.skip("a GPU is present")
+    c, b = zd.PagedCache(16, 16, zd.F16, 1, 64, 16, 1), zd.PagedBatch(1, 1, 16, 16, 16, 1)
+    assert not dev.paged_append_enqueue(c, b, 16, 16, 1, 1e-6, 1e6)
+    assert not dev.paged_read_enqueue(c, b, 16, 16)
+    assert not dev.paged_attention_enqueue(c, b, 16, 16, 1, 1.0)
+    dev.deinit()

@@ -3,8 +3,9 @@
 //
 // The kernels live in gfx950 code objects next to this library, loaded with
 // hipModuleLoad: zlm_kernels_gfx950.hsaco (layout, dequant, quantizer, GEMM,
-// decode glue; $ZLM_HIP_CODE_OBJECT overrides its path) and one
-// zlm_gemv_<quant>_gfx950.hsaco per quant with that quant's GEMV forms.  One HIP
+// decode glue; $ZLM_HIP_CODE_OBJECT overrides its path), one
+// zlm_gemv_<quant>_gfx950.hsaco per quant with that quant's GEMV forms and
+// zlm_paged_gfx950.hsaco (the paged KV cache's append and attention).  One HIP
 // stream per device carries every copy and launch in order, so a burst's
 // shared activation and a resident's layout conversion are ordered before the
 // kernels that read them without extra synchronisation.
@@ -19,6 +20,7 @@
 //     first submit (reference pipeline.zig:264-276 only documents it).
 #include "zlm_gpu_hip.h"
 
+#include "paged_args.h"
 #include "zlm_static_scratch.h"
 
 #include <dlfcn.h>
@@ -46,6 +48,7 @@ constexpr uint32_t kNoLayout = 0xffffffffu;
 // Library scratch kinds a captured graph can reference.
 constexpr uint32_t kUsesAttn = 1u;  // the attention partials
 constexpr uint32_t kUsesGemm = 2u;  // the GEMM's quantized activations and the residents' GEMM tiles
+constexpr int kPagedDims[] = {64, 128, 256};  // head sizes of the paged kernels
 constexpr uint32_t kQ4kRecords = 0xfffffffeu;
 constexpr uint32_t kQ6kRecords = 0xfffffffdu;
 
@@ -215,6 +218,11 @@ struct zlm_device {
     hipFunction_t attn_combine = nullptr;
     hipFunction_t attn_combine_wide = nullptr;
     hipFunction_t attn_decode = nullptr;
+    // the paged cache's kernels, by cache type (f16, q4_0) and head size (kPagedDims)
+    hipModule_t paged_mod = nullptr;
+    struct PagedKernels {
+        hipFunction_t append = nullptr, read = nullptr, few = nullptr, merge_few = nullptr;
+    } paged[2][3];
     hipFunction_t synth_blocks = nullptr;
     hipFunction_t synth_f16 = nullptr;
 
@@ -306,6 +314,8 @@ std::string library_dir() {
 void unload_modules(zlm_device* d) {
     if (d->mod) hipModuleUnload(d->mod);
     d->mod = nullptr;
+    if (d->paged_mod) hipModuleUnload(d->paged_mod);
+    d->paged_mod = nullptr;
     for (hipModule_t& m : d->gemv_mod) {
         if (m) hipModuleUnload(m);
         m = nullptr;
@@ -378,6 +388,20 @@ bool load_kernels(zlm_device* d) {
             if (!ok(d, hipModuleGetFunction(&d->gemm_tall[qi.slot][tier], d->mod, nm), nm)) return false;
         }
     }
+    const std::string pp = dir + "/zlm_paged_gfx950.hsaco";
+    if (!ok(d, hipModuleLoad(&d->paged_mod, pp.c_str()), pp.c_str())) return false;
+    for (int t = 0; t < 2; t++)
+        for (int i = 0; i < 3; i++) {
+            zlm_device::PagedKernels& k = d->paged[t][i];
+            const struct {
+                hipFunction_t* f;
+                const char* name;
+            } fns[] = {{&k.append, "append"}, {&k.read, "read"}, {&k.few, "attend_few"}, {&k.merge_few, "merge_few"}};
+            for (const auto& fn : fns) {
+                snprintf(nm, sizeof nm, "zlm_paged_%s_%s_%d", fn.name, t ? "q4_0" : "f16", kPagedDims[i]);
+                if (!ok(d, hipModuleGetFunction(fn.f, d->paged_mod, nm), nm)) return false;
+            }
+        }
     return true;
 }
 
@@ -2934,6 +2958,125 @@ extern "C" bool zlm_gpu_attention_enqueue(zlm_device* d, const float* q, const u
         if (!launch3(d, d->attn_partial, n_kv_heads, nsplit, 1, 256, args, "attention")) return false;
     }
     return enqueue_attn_merge(d, part, nsplit, n_heads, out);
+}
+
+// ---- the paged KV cache: append, read back, attention ----
+
+namespace {
+
+// Checks what can be checked on the host and fills the kernels' block.  *k =
+// the cache's kernels; null when the batch is empty (nothing to launch).
+bool paged_block(zlm_device* d, const zlm_paged_cache* c, const zlm_paged_batch* b, zlm::Paged* p,
+                 const zlm_device::PagedKernels** k) {
+    *k = nullptr;
+    if (!c || !b) return fail(d, "null cache or batch");
+    if (c->type != ZLM_GGML_F16 && c->type != ZLM_GGML_Q4_0) return fail(d, "a paged cache is f16 or q4_0 (got type %u)", c->type);
+    int dim = 0;
+    while (dim < 3 && kPagedDims[dim] != static_cast<int>(c->head_dim)) dim++;
+    if (dim == 3) return fail(d, "a paged cache has heads of 64, 128 or 256 (got %u)", c->head_dim);
+    if (c->n_kv_heads == 0 || c->n_kv_heads > 1024) return fail(d, "bad kv head count %u", c->n_kv_heads);
+    uint32_t shift = 4;
+    while (shift < 9 && (1u << shift) != c->page_size) shift++;
+    if (shift == 9) return fail(d, "pages hold 16, 32, 64, 128 or 256 positions (got %u)", c->page_size);
+    if (b->n_seqs > zlm::kPagedMaxSeqs) return fail(d, "a batch holds at most %u sequences (got %u)", zlm::kPagedMaxSeqs, b->n_seqs);
+    if (b->n_tokens > (1u << 24)) return fail(d, "a batch holds at most %u tokens (got %u)", 1u << 24, b->n_tokens);
+    if (b->n_seqs == 0 || b->n_tokens == 0) return true;
+    if (!c->k || !c->v || !b->q_start || !b->kv_len || !b->table) return fail(d, "null buffer");
+    if (reinterpret_cast<uintptr_t>(c->k) % 16 || reinterpret_cast<uintptr_t>(c->v) % 16)
+        return fail(d, "cache pools need 16-byte alignment");
+    if (c->n_pages == 0 || c->n_pages > 0x7fffffffu || b->table_stride == 0) return fail(d, "no pages");
+    *p = {static_cast<uint8_t*>(c->k), static_cast<uint8_t*>(c->v), b->q_start, b->kv_len, b->table, b->n_seqs,
+          b->n_tokens, b->table_stride, c->n_pages, c->n_kv_heads, shift};
+    *k = &d->paged[c->type == ZLM_GGML_Q4_0][dim];
+    return true;
+}
+
+}  // namespace
+
+extern "C" uint64_t zlm_gpu_paged_page_bytes(uint32_t type, uint32_t n_kv_heads, uint32_t head_dim, uint32_t page_size) {
+    const bool dim_ok = head_dim == 64 || head_dim == 128 || head_dim == 256;
+    const bool page_ok = page_size >= 16 && page_size <= 256 && (page_size & (page_size - 1)) == 0;
+    if (!dim_ok || !page_ok || (type != ZLM_GGML_F16 && type != ZLM_GGML_Q4_0)) return 0;
+    const uint64_t row = type == ZLM_GGML_F16 ? 2 * head_dim : head_dim / 2 + head_dim / 16;
+    return row * page_size * n_kv_heads;
+}
+
+extern "C" bool zlm_gpu_paged_append_enqueue(zlm_device* d, const zlm_paged_cache* cache, const zlm_paged_batch* batch,
+                                             const float* qkv, uint64_t qkv_stride, const float* q_norm_w,
+                                             const float* k_norm_w, uint32_t n_heads, float eps, float freq_base,
+                                             float* q_out) {
+    if (!d || !d->avail) return false;
+    zlm::PagedAppend a = {};
+    const zlm_device::PagedKernels* k = nullptr;
+    if (!paged_block(d, cache, batch, &a.p, &k)) return false;
+    if (n_heads == 0 || n_heads > 16384) return fail(d, "bad head count %u", n_heads);
+    const uint64_t packed = (static_cast<uint64_t>(n_heads) + 2 * cache->n_kv_heads) * cache->head_dim;
+    if (qkv_stride == 0) qkv_stride = packed;
+    if (qkv_stride < packed) return fail(d, "qkv rows of %llu floats overlap", static_cast<unsigned long long>(qkv_stride));
+    if (!(freq_base > 0.0f)) return fail(d, "the rotation's base must be positive");
+    if (!k) return true;
+    if (!qkv || !q_out) return fail(d, "null buffer");
+    if (!q_norm_w != !k_norm_w) return fail(d, "head norm weights come for q and k or for neither");
+    a.qkv = qkv;
+    a.q_norm = q_norm_w;
+    a.k_norm = k_norm_w;
+    a.q_out = q_out;
+    a.stride = qkv_stride;
+    a.n_heads = n_heads;
+    a.eps = eps;
+    a.base = freq_base;
+    void* args[] = {&a};
+    const unsigned waves = (n_heads + 2 * cache->n_kv_heads + 3) / 4;
+    return launch3(d, k->append, batch->n_tokens, waves, 1, 256, args, "paged append");
+}
+
+extern "C" bool zlm_gpu_paged_read_enqueue(zlm_device* d, const zlm_paged_cache* cache, const zlm_paged_batch* batch,
+                                           float* k_out, float* v_out) {
+    if (!d || !d->avail) return false;
+    zlm::PagedRead a = {};
+    const zlm_device::PagedKernels* k = nullptr;
+    if (!paged_block(d, cache, batch, &a.p, &k)) return false;
+    if (!k) return true;
+    if (!k_out || !v_out) return fail(d, "null buffer");
+    a.k_out = k_out;
+    a.v_out = v_out;
+    void* args[] = {&a};
+    return launch3(d, k->read, batch->n_tokens, (cache->n_kv_heads + 3) / 4, 1, 256, args, "paged read");
+}
+
+extern "C" bool zlm_gpu_paged_attention_enqueue(zlm_device* d, const zlm_paged_cache* cache,
+                                                const zlm_paged_batch* batch, const float* q, uint32_t n_heads,
+                                                uint32_t window, float scale, float* out) {
+    if (!d || !d->avail) return false;
+    zlm::PagedAttend a = {};
+    const zlm_device::PagedKernels* k = nullptr;
+    if (!paged_block(d, cache, batch, &a.p, &k)) return false;
+    if (n_heads == 0 || n_heads > 16384 || n_heads % cache->n_kv_heads)
+        return fail(d, "%u q heads over %u kv heads", n_heads, cache->n_kv_heads);
+    if (window > 0x7fffffffu) return fail(d, "bad attention window");
+    if (!k) return true;
+    if (!q || !out) return fail(d, "null buffer");
+    if (reinterpret_cast<uintptr_t>(q) % 16 || reinterpret_cast<uintptr_t>(out) % 16)
+        return fail(d, "q and out need 16-byte alignment");
+    const uint32_t hd = cache->head_dim, group = n_heads / cache->n_kv_heads;
+    const uint64_t tiles = static_cast<uint64_t>(batch->n_tokens) * group / 16 + batch->n_seqs;
+    const uint64_t depth = (static_cast<uint64_t>(batch->table_stride) * cache->page_size) / 128 + 2;
+    if (tiles * cache->n_kv_heads * std::min<uint64_t>(depth, (1u << 24) + 2) >= (1ull << 31))
+        return fail(d, "attention of %u tokens over up to %u pages a sequence is too large for one call",
+                    batch->n_tokens, batch->table_stride);
+    const uint32_t grid = static_cast<uint32_t>(d->cus) * 2;
+    if (!ensure_attn_scratch(d, static_cast<size_t>(grid) * 2 * 16 * (hd + 2))) return false;
+    a.q = q;
+    a.out = out;
+    a.part = d->attn_part;
+    a.n_heads = n_heads;
+    a.group = group;
+    a.window = window;
+    a.scale = scale * 1.44269504088896340736f;
+    uint32_t g = grid;
+    void* args[] = {&a, &g};
+    return launch3(d, k->few, grid, 1, 1, 256, args, "paged attention") &&
+           launch3(d, k->merge_few, grid - 1, 1, 1, 256, args, "paged attention merge");
 }
 
 struct zlm_graph {

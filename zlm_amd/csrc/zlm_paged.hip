@@ -1,0 +1,849 @@
+// zlm_paged.hip -- CDNA4 (gfx950) kernels over a paged KV cache: q/k head norm,
+// RoPE and the append of a batch's K and V (f16 or 4-bit q4_0 blocks), the rows
+// read back, and the attention of the batch over its sequences' pages.  Built as a
+// device-only code object (hipcc --genco) and loaded by the host library.
+//
+// A page holds `page` positions of every kv head, K and V in a pool each.  The
+// two layouts are the MFMA operand orders of the attention below, so that its
+// lanes load whole operands from memory without a transpose.  Per head of a page:
+//   K  f16  [page][hd]
+//      q4_0 [page][hd/32][16 nibble bytes in GGUF order], then f16 [page][hd/32]
+//   V, by groups of 8 positions
+//      f16  [page/8][hd][8]
+//      q4_0 one word of 8 nibbles per (group, dim), position j's at bits
+//           4*(j/2) + 16*(j%2): [page/8][hd], then f16 scales [page/8][hd/32][8]
+// A q4_0 value is d * (nibble - 8).  d has at most 8 significant bits, so that
+// d * (nibble - 8) is exact in f16, and is at most 2720 in size, so that 24 d is
+// finite in f16: the decode below is one exact fma.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "paged_args.h"
+
+namespace {
+
+using zlm::Paged;
+using AppendArgs = zlm::PagedAppend;
+using ReadArgs = zlm::PagedRead;
+using AttnArgs = zlm::PagedAttend;
+
+constexpr uint32_t kWave = 64;
+constexpr uint32_t kMaxSeqs = zlm::kPagedMaxSeqs;
+
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+
+template <int HD, bool Q4>
+struct Row {
+    static constexpr uint32_t kBytes = Q4 ? HD / 2 + HD / 16 : HD * 2;
+};
+
+// The sequence of row t (n_seqs when it lies behind the last one): the number of
+// sequences that end at or before t, counted by the whole wave (all of q_start is
+// loaded at once, one memory latency).
+__device__ __forceinline__ uint32_t seq_of(const Paged& p, int32_t t, uint32_t lane) {
+    uint32_t s = 0;
+    for (uint32_t b = 0; b < p.n_seqs; b += kWave) {
+        const bool done = b + lane < p.n_seqs && p.q_start[b + lane + 1] <= t;
+        s += __builtin_popcountll(__ballot(done));
+    }
+    return __builtin_amdgcn_readfirstlane(s);
+}
+
+// Row t's sequence and position; false for a row that belongs to none.  What the
+// batch's arrays hold never leads outside the buffers: rows end at n_tokens.
+struct RowAt {
+    uint32_t s;
+    int32_t row0, row1;  // the sequence's rows
+    int32_t pos, first;  // t's position, that of row0
+};
+
+__device__ __forceinline__ bool row_at(const Paged& p, uint32_t t, uint32_t lane, RowAt& r) {
+    r.s = seq_of(p, static_cast<int32_t>(t), lane);
+    if (r.s >= p.n_seqs) return false;
+    r.row0 = p.q_start[r.s];
+    const int32_t row1 = p.q_start[r.s + 1];
+    r.row1 = min(row1, static_cast<int32_t>(p.n_tokens));
+    if (static_cast<int32_t>(t) < r.row0 || static_cast<int32_t>(t) >= r.row1 || r.row0 < 0) return false;
+    const uint32_t past = static_cast<uint32_t>(p.kv_len[r.s]) - static_cast<uint32_t>(row1);
+    r.pos = static_cast<int32_t>(past + t);
+    r.first = static_cast<int32_t>(past + static_cast<uint32_t>(r.row0));
+    return true;
+}
+
+// The page of position `pos` of sequence s, or -1.
+__device__ __forceinline__ int32_t page_of(const Paged& p, uint32_t s, int32_t pos) {
+    if (pos < 0 || (static_cast<uint32_t>(pos) >> p.page_shift) >= p.table_stride) return -1;
+    const int32_t id = p.table[static_cast<size_t>(s) * p.table_stride + (static_cast<uint32_t>(pos) >> p.page_shift)];
+    return static_cast<uint32_t>(id) < p.n_pages ? id : -1;
+}
+
+template <int HD, bool Q4>
+__device__ __forceinline__ size_t head_base(const Paged& p, uint32_t page, uint32_t h) {
+    const uint32_t head_bytes = Row<HD, Q4>::kBytes << p.page_shift;
+    return (static_cast<size_t>(page) * p.n_kv + h) * head_bytes;
+}
+
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+
+// The q4_0 block of 32 values, one a lane of each half wave: d from the first of
+// the largest, and this lane's nibble.
+__device__ __forceinline__ uint32_t quantise(double x, uint32_t lane, _Float16* d_out) {
+    const double a = __builtin_fabs(x);
+    double mx = a;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = __builtin_fmax(mx, __shfl_xor(mx, o));
+    const uint64_t at = __ballot(a == mx) >> (lane & 32);
+    const int first = at & 0xffffffffu ? __builtin_ctz(static_cast<uint32_t>(at)) : 0;
+    const double m = __shfl(x, static_cast<int>(lane & 32) + first);
+    const bool nan = ((__ballot(x != x) >> (lane & 32)) & 0xffffffffu) != 0;
+    // -m/8 to 8 significant bits (bf16), then to f16 (further only below its normal range)
+    const float f = static_cast<float>(m * -0.125);
+    const uint32_t u = __builtin_bit_cast(uint32_t, f);
+    const float r = __builtin_bit_cast(float, (u + 0x7fffu + ((u >> 16) & 1u)) & 0xffff0000u);
+    _Float16 d = static_cast<_Float16>(__builtin_fminf(__builtin_fmaxf(r, -2720.0f), 2720.0f));
+    const double dd = static_cast<double>(d);
+    const double n = dd != 0.0 ? __builtin_floor(x / dd + 8.5) : 8.0;
+    if (nan) d = __builtin_bit_cast(_Float16, static_cast<uint16_t>(0x7e00));  // a block with a NaN reads back as NaN
+    *d_out = d;
+    return static_cast<uint32_t>(__builtin_fmin(__builtin_fmax(n, 0.0), 15.0));
+}
+
+// One wave: one row's head (or several, `waves` apart).  A lane holds dims lane +
+// 64 j; the rotation's pair (i, i + hd/2) is in one lane for hd 128 and 256 and in
+// lanes i and i + 32 for hd 64.  Angles, norm, rotation and the 4-bit decisions are
+// formed in 64 bits: a rounding of the angle at position 1e5 in 32 bits is 4e-3.
+// V's 8-position groups are written by the wave of the group's first row in this
+// call, which takes the group's other rows along: no two waves write one word.
+template <int HD, bool Q4>
+__device__ __forceinline__ void append(const AppendArgs& a) {
+    const Paged& p = a.p;
+    constexpr int N = HD / 64;  // dims a lane
+    const uint32_t lane = threadIdx.x & (kWave - 1);
+    const uint32_t t = blockIdx.x;
+    RowAt at;
+    if (!row_at(p, t, lane, at)) return;  // a row behind the last sequence: left as it was
+    const uint32_t s = at.s;
+    const int32_t pos = at.pos;
+    const uint32_t page = 1u << p.page_shift;
+    const uint32_t waves = gridDim.y * (blockDim.x / kWave);
+    uint32_t h = blockIdx.y * (blockDim.x / kWave) + threadIdx.x / kWave;
+    const uint32_t heads = a.n_heads + p.n_kv;
+    if (h < heads) {
+        const int32_t id = page_of(p, s, pos);
+        // the rotation of this lane's pairs
+        double cs[N], sn[N];
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            const uint32_t i = (lane + 64 * j) % (HD / 2);
+            const double turn = static_cast<double>(pos) * pow(a.base, static_cast<double>(i) * (-2.0 / HD));
+            sincos(turn, &sn[j], &cs[j]);
+        }
+        for (; h < heads; h += waves) {
+            const bool is_q = h < a.n_heads;
+            const float* src = a.qkv + t * a.stride + static_cast<size_t>(h) * HD;
+            const float* w = is_q ? a.q_norm : a.k_norm;
+            double x[N], y[N];
+            double ss = 0.0;
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                x[j] = src[lane + 64 * j];
+                ss += x[j] * x[j];
+            }
+            if (w) {
+                const double inv = 1.0 / sqrt(wave_sum(ss) * (1.0 / HD) + static_cast<double>(a.eps));
+#pragma unroll
+                for (int j = 0; j < N; j++) x[j] = x[j] * inv * static_cast<double>(w[lane + 64 * j]);
+            }
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                double other;
+                bool upper;
+                if constexpr (HD == 64) {
+                    other = __shfl_xor(x[0], 32);
+                    upper = lane >= 32;
+                } else {
+                    other = x[(j + N / 2) % N];
+                    upper = j >= N / 2;
+                }
+                y[j] = x[j] * cs[j] + (upper ? other : -other) * sn[j];
+            }
+            if (is_q) {
+                float* dst = a.q_out + (static_cast<size_t>(t) * a.n_heads + h) * HD;
+#pragma unroll
+                for (int j = 0; j < N; j++) dst[lane + 64 * j] = pos < 0 ? 0.0f : static_cast<float>(y[j]);
+                continue;
+            }
+            if (id < 0) continue;
+            uint8_t* base = p.k + head_base<HD, Q4>(p, id, h - a.n_heads);
+            const uint32_t off = static_cast<uint32_t>(pos) & (page - 1);
+            if constexpr (!Q4) {
+                _Float16* dst = reinterpret_cast<_Float16*>(base) + off * HD;
+#pragma unroll
+                for (int j = 0; j < N; j++) dst[lane + 64 * j] = static_cast<_Float16>(static_cast<float>(y[j]));
+            } else {
+#pragma unroll
+                for (int j = 0; j < N; j++) {
+                    _Float16 d;
+                    const uint32_t n = quantise(y[j], lane, &d);
+                    const uint32_t hi = __shfl(n, (lane & 32) + ((lane + 16) & 31));
+                    const uint32_t blk = 2 * j + lane / 32, e = lane & 31;
+                    if (e < 16) base[off * (HD / 2) + blk * 16 + e] = static_cast<uint8_t>(n | (hi << 4));
+                    if (e == 0) reinterpret_cast<_Float16*>(base + page * (HD / 2))[off * (HD / 32) + blk] = d;
+                }
+            }
+        }
+    }
+    if (h >= heads + p.n_kv) return;
+    // V: the first row of each 8-position group in this call
+    if (pos < 0 || ((pos & 7) != 0 && pos != at.first)) return;  // position 0 starts a group too
+    const int32_t id = page_of(p, s, pos);
+    if (id < 0) return;
+    const uint32_t j0 = static_cast<uint32_t>(pos) & 7;
+    const uint32_t n_rows = min(8u - j0, static_cast<uint32_t>(at.row1) - t);
+    const uint32_t grp = (static_cast<uint32_t>(pos) & (page - 1)) >> 3;
+    for (; h < heads + p.n_kv; h += waves) {
+        uint8_t* base = p.v + head_base<HD, Q4>(p, id, h - heads);
+        const float* src = a.qkv + t * a.stride + static_cast<size_t>(h) * HD;
+        float x[8][N];
+#pragma unroll
+        for (uint32_t r = 0; r < 8; r++)
+#pragma unroll
+            for (int j = 0; j < N; j++) x[r][j] = r < n_rows ? src[r * a.stride + lane + 64 * j] : 0.0f;
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            const uint32_t dim = lane + 64 * j;
+            if constexpr (!Q4) {
+                _Float16* dst = reinterpret_cast<_Float16*>(base) + (grp * HD + dim) * 8;
+                if (n_rows == 8) {
+                    v8h o;
+#pragma unroll
+                    for (int r = 0; r < 8; r++) o[r] = static_cast<_Float16>(x[r][j]);
+                    *reinterpret_cast<v8h*>(dst) = o;
+                } else {
+#pragma unroll
+                    for (uint32_t r = 0; r < 8; r++)
+                        if (r < n_rows) dst[j0 + r] = static_cast<_Float16>(x[r][j]);
+                }
+            } else {
+                uint32_t* word = reinterpret_cast<uint32_t*>(base) + grp * HD + dim;
+                _Float16* sc = reinterpret_cast<_Float16*>(base + page * (HD / 2)) + (grp * (HD / 32) + dim / 32) * 8;
+                uint32_t bits = 0, mask = 0;
+#pragma unroll
+                for (uint32_t r = 0; r < 8; r++) {
+                    if (r < n_rows) {  // wave-uniform
+                        _Float16 d;
+                        const uint32_t n = quantise(x[r][j], lane, &d);
+                        const uint32_t at = j0 + r, sh = 4 * (at >> 1) + 16 * (at & 1);
+                        bits |= n << sh;
+                        mask |= 15u << sh;
+                        if ((lane & 31) == 0) sc[at] = d;
+                    }
+                }
+                *word = n_rows == 8 ? bits : ((*word & ~mask) | bits);
+            }
+        }
+    }
+}
+
+// The batch's rows of the cache as f32, [n_tokens][n_kv][hd]; NaN where a
+// position has no page, rows of negative positions 0.
+template <int HD, bool Q4>
+__device__ __forceinline__ void read_rows(const ReadArgs& a) {
+    const Paged& p = a.p;
+    const uint32_t lane = threadIdx.x & (kWave - 1), t = blockIdx.x;
+    RowAt at;
+    if (!row_at(p, t, lane, at)) return;
+    const int32_t pos = at.pos, id = page_of(p, at.s, pos);
+    const uint32_t page = 1u << p.page_shift, off = static_cast<uint32_t>(pos) & (page - 1);
+    const uint32_t grp = off >> 3, j = off & 7;
+    for (uint32_t h = blockIdx.y * 4 + threadIdx.x / kWave; h < p.n_kv; h += gridDim.y * 4) {
+        const size_t o = (static_cast<size_t>(t) * p.n_kv + h) * HD;
+#pragma unroll
+        for (int i = 0; i < HD / 64; i++) {
+            const uint32_t dim = lane + 64 * i;
+            float k = pos < 0 ? 0.0f : __builtin_nanf(""), v = k;
+            if (id >= 0) {
+                const uint8_t* kb = p.k + head_base<HD, Q4>(p, id, h);
+                const uint8_t* vb = p.v + head_base<HD, Q4>(p, id, h);
+                if constexpr (!Q4) {
+                    k = static_cast<float>(reinterpret_cast<const _Float16*>(kb)[off * HD + dim]);
+                    v = static_cast<float>(reinterpret_cast<const _Float16*>(vb)[(grp * HD + dim) * 8 + j]);
+                } else {
+                    const uint32_t b = kb[off * (HD / 2) + dim / 32 * 16 + (dim & 15)];
+                    const float dk = reinterpret_cast<const _Float16*>(kb + page * (HD / 2))[off * (HD / 32) + dim / 32];
+                    k = (static_cast<float>((b >> (dim & 16 ? 4 : 0)) & 15) - 8.0f) * dk;
+                    const uint32_t w = reinterpret_cast<const uint32_t*>(vb)[grp * HD + dim];
+                    const float dv =
+                        reinterpret_cast<const _Float16*>(vb + page * (HD / 2))[(grp * (HD / 32) + dim / 32) * 8 + j];
+                    v = (static_cast<float>((w >> (4 * (j >> 1) + 16 * (j & 1))) & 15) - 8.0f) * dv;
+                }
+            }
+            a.k_out[o + dim] = k;
+            a.v_out[o + dim] = v;
+        }
+    }
+}
+
+// ---- attention ---------------------------------------------------------------
+//
+// out[t, head] = sum_j softmax_j(scale q . k_j) v_j over the positions
+// [max(0, pos - window + 1), pos] of the row's sequence.
+//
+// Both products run on v_mfma_f32_16x16x32_f16 with the queries in the N
+// dimension: S^T = K Q^T, O^T = V^T P^T.  A lane then holds, of query row n =
+// lane % 16, the scores of 8 consecutive positions 8q .. 8q+7 (q = lane / 16) --
+// the K rows of the two 16-row tiles of a 32-position block are dealt so -- which
+// is just the B operand of the second product: the probabilities go from the first
+// product to the second without leaving the lane, and a row's maximum, sum and
+// rescale are one register for all of the lane's output.
+//
+// K and V are exact in f16 (4-bit values by the choice of their scales).  q and
+// the probabilities enter as a sum of two f16 each, about 22 bits, so the result
+// has the accuracy of f32 products at half of f16's matrix rate.  q is scaled by a
+// power of two of its row's own, so neither part leaves f16's range.
+constexpr uint32_t kUnit = 128;  // positions of a unit of work: 32 for each of a workgroup's 4 waves
+
+__device__ __forceinline__ float max_over_q(float x) {  // over the four lanes of a query row
+    x = __builtin_fmaxf(x, __shfl_xor(x, 16));
+    return __builtin_fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ float sum_over_q(float x) {
+    x += __shfl_xor(x, 16);
+    return x + __shfl_xor(x, 32);
+}
+
+// Eight 4-bit values of a word as f16, in the order nibble 0, 4, 1, 5, 2, 6, 3, 7.
+// A nibble in mantissa bits 9..6 of 16.0 is 16 + n; (16 + n) d - 24 d is exact.
+__device__ __forceinline__ v8h decode8(uint32_t w, v2h d0, v2h d1, v2h d2, v2h d3) {
+    constexpr uint32_t kMask = 0x03c003c0u, kOr = 0x4c004c00u;
+    const v2h x0 = __builtin_bit_cast(v2h, ((w << 6) & kMask) | kOr), x1 = __builtin_bit_cast(v2h, ((w << 2) & kMask) | kOr);
+    const v2h x2 = __builtin_bit_cast(v2h, ((w >> 2) & kMask) | kOr), x3 = __builtin_bit_cast(v2h, ((w >> 6) & kMask) | kOr);
+    const v2h c = {static_cast<_Float16>(-24.0f), static_cast<_Float16>(-24.0f)};
+    const v2h y0 = __builtin_elementwise_fma(x0, d0, c * d0), y1 = __builtin_elementwise_fma(x1, d1, c * d1);
+    const v2h y2 = __builtin_elementwise_fma(x2, d2, c * d2), y3 = __builtin_elementwise_fma(x3, d3, c * d3);
+    return v8h{y0.x, y0.y, y1.x, y1.y, y2.x, y2.y, y3.x, y3.y};
+}
+
+// The operands of 32 positions as loaded.
+template <int HD, bool Q4>
+struct KRaw {
+    uint32_t w[2][HD / 32][Q4 ? 1 : 4];
+    uint16_t d[2][HD / 128 ? HD / 128 : 1];
+};
+template <int HD, bool Q4>
+struct VRaw {
+    uint32_t w[HD / 16][Q4 ? 1 : 4];
+    v4u d[Q4 ? HD / 64 : 1];
+};
+
+// The pages of a 32-position block: one, or two of 16 positions.  -1: none.
+struct Pages {
+    int32_t id[2];
+};
+
+__device__ __forceinline__ Pages pages_at(const Paged& p, uint32_t s, uint32_t kb) {
+    Pages g;
+    g.id[0] = __builtin_amdgcn_readfirstlane(page_of(p, s, static_cast<int32_t>(kb)));
+    g.id[1] = p.page_shift > 4 ? g.id[0] : __builtin_amdgcn_readfirstlane(page_of(p, s, static_cast<int32_t>(kb) + 16));
+    return g;
+}
+
+// K position of matrix row m (0..15) of tile t in a 32-position block.
+__device__ __forceinline__ uint32_t k_row(uint32_t m, int t) { return 8 * (m >> 2) + (m & 3) + 4 * t; }
+
+template <int HD, bool Q4>
+__device__ __forceinline__ void load_k(const Paged& p, const Pages& g, uint32_t h, uint32_t kb, uint32_t lane,
+                                       KRaw<HD, Q4>& r) {
+    const uint32_t m = lane & 15, q = lane >> 4, page = 1u << p.page_shift;
+    const size_t b0 = head_base<HD, Q4>(p, max(g.id[0], 0), h), b1 = head_base<HD, Q4>(p, max(g.id[1], 0), h);
+    const uint8_t* base = p.k + (m >= 8 ? b1 : b0);
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+        const uint32_t off = (kb + k_row(m, t)) & (page - 1);
+        if constexpr (!Q4) {
+#pragma unroll
+            for (int i = 0; i < HD / 32; i++)
+                *reinterpret_cast<v4u*>(r.w[t][i]) = *reinterpret_cast<const v4u*>(base + off * (HD * 2) + 64 * i + 16 * q);
+        } else {
+            const uint8_t* row = base + off * (HD / 2);
+            const uint16_t* sc = reinterpret_cast<const uint16_t*>(base + page * (HD / 2)) + off * (HD / 32);
+            if constexpr (HD == 64) {  // half of block q / 2
+                const v2u x = *reinterpret_cast<const v2u*>(row + 8 * q);
+                r.w[t][0][0] = x.x;
+                r.w[t][1][0] = x.y;
+                r.d[t][0] = sc[q >> 1];
+            } else {
+#pragma unroll
+                for (int b = 0; b < HD / 128; b++) {  // block q + 4 b
+                    const v4u x = *reinterpret_cast<const v4u*>(row + 16 * q + 64 * b);
+                    r.w[t][4 * b][0] = x.x;
+                    r.w[t][4 * b + 1][0] = x.y;
+                    r.w[t][4 * b + 2][0] = x.z;
+                    r.w[t][4 * b + 3][0] = x.w;
+                    r.d[t][b] = sc[q + 4 * b];
+                }
+            }
+        }
+    }
+}
+
+template <int HD, bool Q4>
+__device__ __forceinline__ v8h k_operand(const KRaw<HD, Q4>& r, int t, int i) {
+    if constexpr (!Q4) {
+        return __builtin_bit_cast(v8h, *reinterpret_cast<const v4u*>(r.w[t][i]));
+    } else {
+        const _Float16 d = __builtin_bit_cast(_Float16, r.d[t][HD == 64 ? 0 : i / 4]);
+        const v2h dd = {d, d};
+        return decode8(r.w[t][i][0], dd, dd, dd, dd);
+    }
+}
+
+// The dim of slot j (0..7) of k-step i for lane quarter q: the order in which
+// load_k's operands hold the head's dims.
+template <int HD, bool Q4>
+__device__ __forceinline__ constexpr uint32_t k_dim(uint32_t q, int i, int j) {
+    if (!Q4) return 32 * i + 8 * q + j;
+    // word w of block b: nibbles 0, 4, 1, 5, 2, 6, 3, 7; nibble n of a GGUF block word is
+    // element 4 w + n / 2 + 16 (n % 2)
+    const uint32_t b = HD == 64 ? q >> 1 : q + 4 * (i / 4), w = HD == 64 ? 2 * (q & 1) + i : i % 4;
+    const uint32_t n = (j >> 1) + 4 * (j & 1);
+    return 32 * b + 4 * w + n / 2 + 16 * (n & 1);
+}
+
+template <int HD, bool Q4>
+__device__ __forceinline__ void load_v(const Paged& p, const Pages& g, uint32_t h, uint32_t kb, uint32_t lane,
+                                       VRaw<HD, Q4>& r) {
+    const uint32_t m = lane & 15, q = lane >> 4, page = 1u << p.page_shift;
+    const size_t b0 = head_base<HD, Q4>(p, max(g.id[0], 0), h), b1 = head_base<HD, Q4>(p, max(g.id[1], 0), h);
+    const uint8_t* base = p.v + (q >= 2 ? b1 : b0);
+    const uint32_t grp = ((kb + 8 * q) & (page - 1)) >> 3;
+    if constexpr (!Q4) {
+#pragma unroll
+        for (int c = 0; c < HD / 16; c++)
+            *reinterpret_cast<v4u*>(r.w[c]) = *reinterpret_cast<const v4u*>(base + (grp * HD + 16 * c + m) * 16);
+    } else {
+        const v4u* sc = reinterpret_cast<const v4u*>(base + page * (HD / 2)) + grp * (HD / 32) + (m >> 3);
+#pragma unroll
+        for (int b = 0; b < HD / 64; b++) {  // dims 64 b + 4 m + {0, 1, 2, 3}
+            const v4u x = *reinterpret_cast<const v4u*>(base + (grp * HD + 64 * b + 4 * m) * 4);
+            r.w[4 * b][0] = x.x;
+            r.w[4 * b + 1][0] = x.y;
+            r.w[4 * b + 2][0] = x.z;
+            r.w[4 * b + 3][0] = x.w;
+            r.d[b] = sc[2 * b];
+        }
+    }
+}
+
+// The dim of matrix row m of V's tile c.
+template <int HD, bool Q4>
+__device__ __forceinline__ constexpr uint32_t v_dim(int c, uint32_t m) {
+    return Q4 ? 64 * (c / 4) + 4 * m + c % 4 : 16 * c + m;
+}
+
+template <int HD, bool Q4>
+__device__ __forceinline__ v8h v_operand(const VRaw<HD, Q4>& r, int c) {
+    if constexpr (!Q4) {
+        return __builtin_bit_cast(v8h, *reinterpret_cast<const v4u*>(r.w[c]));
+    } else {
+        // (a bit cast of a vector's element takes the first one's bits: each goes through a scalar)
+        const uint32_t d0 = r.d[c / 4].x, d1 = r.d[c / 4].y, d2 = r.d[c / 4].z, d3 = r.d[c / 4].w;
+        return decode8(r.w[c][0], __builtin_bit_cast(v2h, d0), __builtin_bit_cast(v2h, d1),
+                       __builtin_bit_cast(v2h, d2), __builtin_bit_cast(v2h, d3));
+    }
+}
+
+// V's operands with the positions outside [lo, hi) zero: what lies there may be
+// anything, and 0 times a NaN is a NaN.
+template <int HD, bool Q4>
+__device__ __forceinline__ void clear_v(VRaw<HD, Q4>& r, int32_t at, int32_t lo, int32_t hi) {
+    uint32_t keep[4];  // by pair of positions
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int32_t a = at + 2 * i;
+        keep[i] = (a >= lo && a < hi ? 0xffffu : 0u) | (a + 1 >= lo && a + 1 < hi ? 0xffff0000u : 0u);
+    }
+    const v4u k = {keep[0], keep[1], keep[2], keep[3]};
+    if constexpr (Q4) {  // a scale of 0 makes the value 0
+#pragma unroll
+        for (int b = 0; b < HD / 64; b++) r.d[b] &= k;
+    } else {
+#pragma unroll
+        for (int c = 0; c < HD / 16; c++) *reinterpret_cast<v4u*>(r.w[c]) &= k;
+    }
+}
+
+// A wave's 16 query rows: the operand parts of q and the factor that takes a
+// product of theirs to the softmax's exponent of two.
+template <int HD>
+struct QTile {
+    v8h hi[HD / 32], lo[HD / 32];
+    float factor;
+};
+
+template <int HD, bool Q4>
+__device__ __forceinline__ void load_q(QTile<HD>& qt, const float* row, uint32_t q, float scale) {
+    float x[HD / 32][8];
+    float mx = 0.0f;
+#pragma unroll
+    for (int i = 0; i < HD / 32; i++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            x[i][j] = row ? row[k_dim<HD, Q4>(q, i, j)] : 0.0f;
+            mx = __builtin_fmaxf(mx, __builtin_fabsf(x[i][j]));
+        }
+    mx = max_over_q(mx);
+    // the row's largest to [2^13, 2^14); a row of zeros, infinities or NaN stays as it is
+    int e = 0;
+    if (mx > 0.0f && mx < INFINITY) e = 14 - __builtin_amdgcn_frexp_expf(mx);
+    qt.factor = ldexpf(scale, -e);
+#pragma unroll
+    for (int i = 0; i < HD / 32; i++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float y = ldexpf(x[i][j], e);
+            const _Float16 a = static_cast<_Float16>(y);
+            qt.hi[i][j] = a;
+            qt.lo[i][j] = static_cast<_Float16>(y - static_cast<float>(a));
+        }
+}
+
+// The running softmax of a wave's 16 rows over blocks of 32 positions.
+// Probabilities are 2^(s - m + kLift) with m the maximum when it last moved: it
+// moves only when a score exceeds it by kSlack, so that the output is rescaled
+// rarely; kLift + kSlack keep the largest below f16's 65504 and put the smallest
+// that the pair of f16 resolves 2^-30 below a weight of 1.
+constexpr float kLift = 6.0f, kSlack = 8.0f;
+
+template <int HD>
+struct Soft {
+    float m, l;  // l: this lane's share of the row's sum
+    v4f o[HD / 16];
+};
+
+template <int HD>
+__device__ __forceinline__ void soft_clear(Soft<HD>& st) {
+    st.m = -INFINITY;
+    st.l = 0.0f;
+#pragma unroll
+    for (int c = 0; c < HD / 16; c++) st.o[c] = v4f{0, 0, 0, 0};
+}
+
+template <int HD, bool Q4>
+__device__ __forceinline__ void scores(const KRaw<HD, Q4>& k, const QTile<HD>& qt, v4f s[2]) {
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+        s[t] = v4f{0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < HD / 32; i++) {
+            const v8h a = k_operand<HD, Q4>(k, t, i);
+            s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qt.hi[i], s[t], 0, 0, 0);
+            s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qt.lo[i], s[t], 0, 0, 0);
+        }
+        s[t] *= qt.factor;
+    }
+}
+
+// s: scores in units of log2; -inf where masked.  Makes the two parts of P.
+template <int HD>
+__device__ __forceinline__ void soft_step(Soft<HD>& st, const v4f s[2], v8h& hi, v8h& lo) {
+    float mx = s[0][0];
+#pragma unroll
+    for (int i = 1; i < 8; i++) mx = __builtin_fmaxf(mx, s[i / 4][i % 4]);
+    if (__any(mx > st.m + kSlack)) {
+        mx = __builtin_fmaxf(max_over_q(mx), st.m);
+        const float f = st.m == mx ? 1.0f : __builtin_amdgcn_exp2f(st.m - mx);  // -inf stays with -inf
+        st.m = mx;
+        st.l *= f;
+#pragma unroll
+        for (int c = 0; c < HD / 16; c++) st.o[c] *= f;
+    }
+    const float base = (st.m == -INFINITY ? 0.0f : st.m) - kLift;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float e = __builtin_amdgcn_exp2f(s[i / 4][i % 4] - base);
+        sum += e;
+        const _Float16 a = static_cast<_Float16>(e);
+        hi[i] = a;
+        lo[i] = static_cast<_Float16>(e - static_cast<float>(a));
+    }
+    st.l += sum;
+}
+
+template <int HD, bool Q4>
+__device__ __forceinline__ void values(Soft<HD>& st, const VRaw<HD, Q4>& v, const v8h& hi, const v8h& lo) {
+#pragma unroll
+    for (int c = 0; c < HD / 16; c++) {
+        const v8h a = v_operand<HD, Q4>(v, c);
+        st.o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, hi, st.o[c], 0, 0, 0);
+        st.o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, lo, st.o[c], 0, 0, 0);
+    }
+}
+
+// Sequence s in units of work: its rows in tiles of 16 (rows x heads of a kv
+// head's group), per tile and kv head the positions [lo, end) in units.
+struct SeqWork {
+    int32_t row0, len, end, first;  // rows, positions with them, position of the first row
+    int32_t lo;                     // first position any row sees, down to a multiple of 32
+    uint32_t tiles, units;          // per tile and head
+};
+
+// Positions that a sequence's pages can hold.  A row past them sees positions
+// that are nowhere: it becomes NaN.
+__device__ __forceinline__ uint64_t capacity(const Paged& p) {
+    return static_cast<uint64_t>(p.table_stride) << p.page_shift;
+}
+
+__device__ __forceinline__ SeqWork seq_work(const AttnArgs& a, uint32_t s) {
+    SeqWork w;
+    const int32_t n = static_cast<int32_t>(a.p.n_tokens);
+    w.row0 = min(max(a.p.q_start[s], 0), n);
+    w.len = max(min(a.p.q_start[s + 1], n) - w.row0, 0);
+    const int32_t kv = a.p.kv_len[s];
+    w.first = static_cast<int32_t>(static_cast<uint32_t>(kv) - static_cast<uint32_t>(w.len));
+    w.end = static_cast<int32_t>(min(static_cast<uint64_t>(max(kv, 0)), capacity(a.p)));
+    const int32_t lo = a.window && w.first >= static_cast<int32_t>(a.window) ? w.first - static_cast<int32_t>(a.window) + 1 : 0;
+    w.lo = min(lo, w.end) & ~31;
+    w.tiles = (static_cast<uint32_t>(w.len) * a.group + 15) / 16;
+    w.units = max((static_cast<uint32_t>(w.end - w.lo) + kUnit - 1) / kUnit, 1u);
+    return w;
+}
+
+// Prefix sums of the sequences' units (all tiles and heads) into LDS; returns the total.
+__device__ __forceinline__ uint32_t scan_units(const AttnArgs& a, uint32_t* prefix, uint32_t* sums) {
+    const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1), wid = tid / kWave;
+    uint32_t base = 0;
+    for (uint32_t b = 0; b < a.p.n_seqs; b += 256) {
+        uint32_t x = 0;
+        if (b + tid < a.p.n_seqs) {
+            const SeqWork w = seq_work(a, b + tid);
+            x = w.tiles * a.p.n_kv * w.units;
+        }
+        uint32_t run = x;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t y = __shfl_up(run, o);
+            if (static_cast<int>(lane) >= o) run += y;
+        }
+        if (lane == 63) sums[wid] = run;
+        __syncthreads();
+        uint32_t before = base, all = 0;
+        for (uint32_t i = 0; i < 4; i++) {
+            if (i < wid) before += sums[i];
+            all += sums[i];
+        }
+        if (b + tid < a.p.n_seqs) prefix[b + tid] = before + run - x;
+        base += all;
+        __syncthreads();
+    }
+    if (tid == 0) prefix[a.p.n_seqs] = base;
+    __syncthreads();
+    return base;
+}
+
+// Where unit u lies.
+struct Place {
+    uint32_t s, tile, h, unit;  // unit within the item (s, tile, h)
+};
+
+__device__ __forceinline__ Place place_of(const AttnArgs& a, const uint32_t* prefix, uint32_t u, SeqWork& w) {
+    uint32_t lo = 0, hi = a.p.n_seqs;  // prefix[lo] <= u < prefix[hi]
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (prefix[mid] <= u) lo = mid;
+        else hi = mid;
+    }
+    Place at;
+    at.s = __builtin_amdgcn_readfirstlane(lo);
+    w = seq_work(a, at.s);
+    const uint32_t r = u - prefix[at.s], item = r / w.units;
+    at.unit = __builtin_amdgcn_readfirstlane(r % w.units);
+    at.tile = __builtin_amdgcn_readfirstlane(item / a.p.n_kv);
+    at.h = __builtin_amdgcn_readfirstlane(item % a.p.n_kv);
+    return at;
+}
+
+// Units of each workgroup: all alike.  Every kernel of a call computes the same.
+__device__ __forceinline__ uint32_t share_of(uint32_t total, uint32_t grid) { return (total + grid - 1) / grid; }
+
+// A partial result: 16 rows of hd sums, then the rows' maxima and sums.
+template <int HD>
+__device__ __forceinline__ float* part_slot(const AttnArgs& a, uint32_t slot) {
+    return a.part + static_cast<size_t>(slot) * (16 * (HD + 2));
+}
+
+// Attention by few rows: the units of all sequences are laid end to end and cut
+// into equal shares, one a workgroup, whatever the lengths are; a workgroup's
+// shares of an item it does not finish alone go to memory and are joined by the
+// merge.  Within an item the four waves take every fourth 32 positions, and their
+// sums are joined through LDS.
+template <int HD, bool Q4>
+__device__ __forceinline__ void attend_few(const AttnArgs& a) {
+    __shared__ uint32_t prefix[kMaxSeqs + 1];
+    __shared__ uint32_t sums[4];
+    __shared__ float sm_m[4][16], sm_l[4][16];
+    __shared__ __attribute__((aligned(16))) float sm_o[4][16][HD + 4];
+    const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const uint32_t n = lane & 15, q = lane >> 4;
+    const uint32_t total = scan_units(a, prefix, sums);
+    const uint32_t share = share_of(total, gridDim.x);
+    uint32_t u = blockIdx.x * share;
+    const uint32_t u_end = min(u + share, total);
+    while (u < u_end) {
+        SeqWork w;
+        const Place at = place_of(a, prefix, u, w);
+        const uint32_t units = min(w.units - at.unit, u_end - u);
+        const uint32_t rows = static_cast<uint32_t>(w.len) * a.group;
+        const uint32_t r = 16 * at.tile + n;
+        const bool live = r < rows;
+        const uint32_t tok = live ? r / a.group : 0, head = at.h * a.group + (live ? r % a.group : 0);
+        const int32_t pos = w.first + static_cast<int32_t>(tok);
+        const int32_t hi = live ? pos + 1 : 0;
+        const int32_t lo = a.window && hi > static_cast<int32_t>(a.window) ? hi - static_cast<int32_t>(a.window) : 0;
+        // what any row of the tile sees, for V; rows are in order of position
+        const uint32_t last_tok = (min(16 * at.tile + 16, rows) - 1) / a.group;
+        const int32_t tile_hi = min(w.first + static_cast<int32_t>(last_tok) + 1, w.end);
+        const int32_t first_hi = w.first + static_cast<int32_t>(16 * at.tile / a.group) + 1;
+        const int32_t tile_lo =
+            a.window && first_hi > static_cast<int32_t>(a.window) ? first_hi - static_cast<int32_t>(a.window) : 0;
+        QTile<HD> qt;
+        load_q<HD, Q4>(qt, live ? a.q + (static_cast<size_t>(w.row0 + tok) * a.n_heads + head) * HD : nullptr, q, a.scale);
+        Soft<HD> st;
+        soft_clear<HD>(st);
+        if (!live) st.m = 0.0f;  // no row: its maximum never moves
+        if (live && pos >= 0 && static_cast<uint64_t>(pos) >= capacity(a.p)) st.l = __builtin_nanf("");
+        for (uint32_t i = 0; i < units; i++) {
+            const uint32_t kb = static_cast<uint32_t>(w.lo) + (at.unit + i) * kUnit + 32 * wid;
+            if (static_cast<int32_t>(kb) >= tile_hi || static_cast<int32_t>(kb) + 32 <= tile_lo) continue;
+            const Pages g = pages_at(a.p, at.s, kb);
+            KRaw<HD, Q4> kr;
+            load_k<HD, Q4>(a.p, g, at.h, kb, lane, kr);
+            VRaw<HD, Q4> vr;
+            load_v<HD, Q4>(a.p, g, at.h, kb, lane, vr);
+            v4f s[2];
+            scores<HD, Q4>(kr, qt, s);
+            const int32_t p0 = static_cast<int32_t>(kb + 8 * q);
+            const bool no_page = g.id[q >> 1] < 0;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int32_t x = p0 + j;
+                float v = s[j / 4][j % 4];
+                if (no_page) v = __builtin_nanf("");
+                s[j / 4][j % 4] = x < lo || x >= hi ? -INFINITY : v;
+            }
+            clear_v<HD, Q4>(vr, p0, tile_lo, no_page ? tile_lo : tile_hi);
+            v8h ph, pl;
+            soft_step<HD>(st, s, ph, pl);
+            values<HD, Q4>(st, vr, ph, pl);
+        }
+        // join the waves
+        const float l = sum_over_q(st.l);
+        if (q == 0) {
+            sm_m[wid][n] = st.m;
+            sm_l[wid][n] = l;
+        }
+#pragma unroll
+        for (int c = 0; c < HD / 16; c++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) sm_o[wid][n][v_dim<HD, Q4>(c, 4 * q + i)] = st.o[c][i];
+        __syncthreads();
+        const bool whole = units == w.units;
+        float* slot = part_slot<HD>(a, 2 * blockIdx.x + (at.unit == 0 ? 1 : 0));
+        for (uint32_t e = tid; e < 16 * HD / 4; e += 256) {
+            const uint32_t row = e / (HD / 4), d = 4 * (e % (HD / 4));
+            const uint32_t rr = 16 * at.tile + row;
+            if (rr >= rows) continue;
+            float m = sm_m[0][row];
+            for (int i = 1; i < 4; i++) m = __builtin_fmaxf(m, sm_m[i][row]);
+            float sum = 0.0f;
+            v4f o = {0, 0, 0, 0};
+            for (int i = 0; i < 4; i++) {
+                const float f = sm_m[i][row] == -INFINITY ? (sm_l[i][row] == 0.0f ? 0.0f : 1.0f)
+                                                          : __builtin_amdgcn_exp2f(sm_m[i][row] - m);
+                sum += sm_l[i][row] * f;
+                o += *reinterpret_cast<const v4f*>(&sm_o[i][row][d]) * f;
+            }
+            if (whole) {
+                if (sum != 0.0f) o /= sum;  // a row that sees nothing: 0
+                const uint32_t tk = rr / a.group, hd = at.h * a.group + rr % a.group;
+                *reinterpret_cast<v4f*>(a.out + (static_cast<size_t>(w.row0 + tk) * a.n_heads + hd) * HD + d) = o;
+            } else {
+                *reinterpret_cast<v4f*>(slot + row * HD + d) = o;
+                if (d == 0) {
+                    slot[16 * HD + row] = m;
+                    slot[16 * HD + 16 + row] = sum;
+                }
+            }
+        }
+        __syncthreads();
+        u += units;
+    }
+}
+
+// The join of an item's shares: the workgroup of the first cut through the item
+// (blockIdx.x + 1 shares lie before it) adds them in the order of the shares.
+template <int HD, bool Q4>
+__device__ __forceinline__ void merge_few(const AttnArgs& a, uint32_t grid) {
+    __shared__ uint32_t prefix[kMaxSeqs + 1];
+    __shared__ uint32_t sums[4];
+    const uint32_t total = scan_units(a, prefix, sums);
+    const uint32_t share = share_of(total, grid);
+    const uint32_t u = (blockIdx.x + 1) * share;
+    if (u >= total) return;
+    SeqWork w;
+    const Place at = place_of(a, prefix, u, w);
+    if (at.unit == 0 || u - at.unit < blockIdx.x * share) return;  // no item cut here, or cut before
+    const uint32_t last = (u - at.unit + w.units - 1) / share;      // the item's last share
+    const uint32_t all = static_cast<uint32_t>(w.len) * a.group;
+    const uint32_t rows = all > 16 * at.tile ? min(all - 16 * at.tile, 16u) : 0u;
+    for (uint32_t e = threadIdx.x; e < rows * HD / 4; e += 256) {
+        const uint32_t row = e / (HD / 4), d = 4 * (e % (HD / 4));
+        float m = -INFINITY;
+        for (uint32_t b = blockIdx.x; b <= last; b++)
+            m = __builtin_fmaxf(m, part_slot<HD>(a, 2 * b + (b == blockIdx.x ? 1 : 0))[16 * HD + row]);
+        float sum = 0.0f;
+        v4f o = {0, 0, 0, 0};
+        for (uint32_t b = blockIdx.x; b <= last; b++) {
+            const float* slot = part_slot<HD>(a, 2 * b + (b == blockIdx.x ? 1 : 0));
+            const float pm = slot[16 * HD + row], pl = slot[16 * HD + 16 + row];
+            const float f = pm == -INFINITY ? (pl == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(pm - m);
+            sum += pl * f;
+            o += *reinterpret_cast<const v4f*>(slot + row * HD + d) * f;
+        }
+        if (sum != 0.0f) o /= sum;
+        const uint32_t rr = 16 * at.tile + row, tk = rr / a.group, hd = at.h * a.group + rr % a.group;
+        *reinterpret_cast<v4f*>(a.out + (static_cast<size_t>(w.row0 + tk) * a.n_heads + hd) * HD + d) = o;
+    }
+}
+
+}  // namespace
+
+#define ZLM_PAGED(HD, NAME, Q4)                                                                               \
+    extern "C" __global__ void __launch_bounds__(256) zlm_paged_append_##NAME##_##HD(AppendArgs a) {          \
+        append<HD, Q4>(a);                                                                                    \
+    }                                                                                                         \
+    extern "C" __global__ void __launch_bounds__(256) zlm_paged_read_##NAME##_##HD(ReadArgs a) {              \
+        read_rows<HD, Q4>(a);                                                                                 \
+    }                                                                                                         \
+    extern "C" __global__ void __launch_bounds__(256) zlm_paged_attend_few_##NAME##_##HD(AttnArgs a) {        \
+        attend_few<HD, Q4>(a);                                                                                \
+    }                                                                                                         \
+    extern "C" __global__ void __launch_bounds__(256) zlm_paged_merge_few_##NAME##_##HD(AttnArgs a, uint32_t grid) { \
+        merge_few<HD, Q4>(a, grid);                                                                           \
+    }
+
+ZLM_PAGED(64, f16, false)
+ZLM_PAGED(64, q4_0, true)
+ZLM_PAGED(128, f16, false)
+ZLM_PAGED(128, q4_0, true)
+ZLM_PAGED(256, f16, false)
+ZLM_PAGED(256, q4_0, true)

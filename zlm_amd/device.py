@@ -24,8 +24,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_DIR = os.path.join(_HERE, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libzlm_gpu_hip.so")
 CODE_OBJECT_PATH = os.path.join(LIB_DIR, "zlm_kernels_gfx950.hsaco")
-# Every code object the library loads: the common kernels and one GEMV object per quant.
-CODE_OBJECT_PATHS = [CODE_OBJECT_PATH] + [os.path.join(LIB_DIR, f"zlm_gemv_{q}_gfx950.hsaco")
+# Every code object the library loads: the common kernels, the paged cache's and one GEMV object per quant.
+CODE_OBJECT_PATHS = [CODE_OBJECT_PATH, os.path.join(LIB_DIR, "zlm_paged_gfx950.hsaco")] + [os.path.join(LIB_DIR, f"zlm_gemv_{q}_gfx950.hsaco")
                                           for q in ("q4_0", "q8_0", "q4_k", "q6_k", "q4_1", "f32", "f16", "bf16")]
 
 RING_SIZE = 8
@@ -89,6 +89,17 @@ class _GemvOp(ctypes.Structure):
         ("res", ctypes.c_void_p),
         ("y", ctypes.c_void_p),
     ]
+
+
+class _PagedCache(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("type", ctypes.c_uint32),
+                ("n_kv_heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32), ("page_size", ctypes.c_uint32),
+                ("n_pages", ctypes.c_uint32)]
+
+
+class _PagedBatch(ctypes.Structure):
+    _fields_ = [("n_seqs", ctypes.c_uint32), ("n_tokens", ctypes.c_uint32), ("q_start", ctypes.c_void_p),
+                ("kv_len", ctypes.c_void_p), ("table", ctypes.c_void_p), ("table_stride", ctypes.c_uint32)]
 
 
 class LaunchRecord(ctypes.Structure):
@@ -188,6 +199,10 @@ def lib() -> ctypes.CDLL:
                                                          P, U, ctypes.c_float, P]),
         "zlm_gpu_attention_decode_window_enqueue": (B, [P, P, P, P, U, U, U, ctypes.c_float, ctypes.c_float, P, P,
                                                         P, U, U, ctypes.c_float, P]),
+        "zlm_gpu_paged_page_bytes": (ctypes.c_uint64, [U, U, U, U]),
+        "zlm_gpu_paged_append_enqueue": (B, [P, P, P, P, ctypes.c_uint64, P, P, U, ctypes.c_float, ctypes.c_float, P]),
+        "zlm_gpu_paged_read_enqueue": (B, [P, P, P, P, P]),
+        "zlm_gpu_paged_attention_enqueue": (B, [P, P, P, P, U, U, ctypes.c_float, P]),
         "zlm_gpu_resident_device_bytes": (ctypes.c_uint64, [P]),
         "zlm_gpu_layout_bytes": (ctypes.c_uint64, [U, S, S, ctypes.c_bool]),
         "zlm_gpu_release_gemm_tiles": (B, [P, P]),
@@ -267,6 +282,25 @@ class Probe:
             return self.fields[name]
         except KeyError as e:
             raise AttributeError(name) from e
+
+
+class PagedCache:
+    """A paged KV cache's pools and sizes (zlm_paged_cache; see the C header for the pages' layout)."""
+
+    def __init__(self, k: int, v: int, type: int, n_kv_heads: int, head_dim: int, page_size: int, n_pages: int):
+        self.c = _PagedCache(k, v, type, n_kv_heads, head_dim, page_size, n_pages)
+
+
+class PagedBatch:
+    """A batch of tokens over a paged cache (zlm_paged_batch); q_start, kv_len and table are device addresses."""
+
+    def __init__(self, n_seqs: int, n_tokens: int, q_start: int, kv_len: int, table: int, table_stride: int):
+        self.c = _PagedBatch(n_seqs, n_tokens, q_start, kv_len, table, table_stride)
+
+
+def paged_page_bytes(type: int, n_kv_heads: int, head_dim: int, page_size: int) -> int:
+    """Bytes of one page of one pool; 0 for a type or size that is not supported.  No GPU needed."""
+    return int(lib().zlm_gpu_paged_page_bytes(type, n_kv_heads, head_dim, page_size))
 
 
 class Device:
@@ -531,6 +565,25 @@ class Device:
         return bool(self._L.zlm_gpu_attention_decode_enqueue_noalloc(self._h, qkv, q_norm_w, k_norm_w, n_heads,
                                                                      n_kv_heads, head_dim, eps, freq_base, pos,
                                                                      k_cache, v_cache, max_seq, scale, out))
+
+    def paged_append_enqueue(self, cache: PagedCache, batch: PagedBatch, qkv: int, q_out: int, n_heads: int,
+                             eps: float, freq_base: float, q_norm_w: int = 0, k_norm_w: int = 0,
+                             qkv_stride: int = 0) -> bool:
+        """Head norm (without weights: none), RoPE and the append of a batch's K and V (no wait)."""
+        return bool(self._L.zlm_gpu_paged_append_enqueue(self._h, ctypes.byref(cache.c), ctypes.byref(batch.c), qkv,
+                                                         qkv_stride, q_norm_w or None, k_norm_w or None, n_heads, eps,
+                                                         freq_base, q_out))
+
+    def paged_read_enqueue(self, cache: PagedCache, batch: PagedBatch, k_out: int, v_out: int) -> bool:
+        """The batch's rows as the cache holds them, f32 (no wait)."""
+        return bool(self._L.zlm_gpu_paged_read_enqueue(self._h, ctypes.byref(cache.c), ctypes.byref(batch.c), k_out,
+                                                       v_out))
+
+    def paged_attention_enqueue(self, cache: PagedCache, batch: PagedBatch, q: int, out: int, n_heads: int,
+                                scale: float, window: int = 0) -> bool:
+        """Attention of a batch's rows over their sequences' pages (no wait)."""
+        return bool(self._L.zlm_gpu_paged_attention_enqueue(self._h, ctypes.byref(cache.c), ctypes.byref(batch.c), q,
+                                                            n_heads, window, scale, out))
 
     def probe_rates(self, ggml_type: int, gate_up: bool, rows: int, k: int) -> Optional[np.ndarray]:
         """GB/s of each GpuVariant for one quant (resident GEMV or fused gate_up); None if one did not run."""
