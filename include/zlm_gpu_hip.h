@@ -492,6 +492,36 @@ bool zlm_gpu_paged_read_enqueue(zlm_device *dev, const zlm_paged_cache *cache, c
 bool zlm_gpu_paged_attention_enqueue(zlm_device *dev, const zlm_paged_cache *cache, const zlm_paged_batch *batch,
                                      const float *q, uint32_t n_heads, uint32_t window, float scale, float *out);
 
+/* ---- sampling (device buffers): a token from each row of logits ----
+ * No reference counterpart on the device (its sampler runs on the CPU over the
+ * downloaded row).  Arrays of one value a row, in device memory; a null array
+ * leaves its filter off (temperature: 1).  The tokens of a row in order of
+ * logit, the lower index first among equals; the filters in this order:
+ *   temperature  weights e^((x - max) / T); T of 0, below or NaN: the largest
+ *                logit's token, whatever the filters say
+ *   top_k        the first k (0 and below: all)
+ *   top_p        the first whose weight reaches top_p of those (1 and above, NaN:
+ *                all; always one)
+ *   min_p        those of at least min_p of the largest weight (0, NaN: all)
+ * and the token is the first whose cumulative weight exceeds u times the weight
+ * of those that are left.  Weights are formed and summed in 64 bits; a token
+ * e^-32 below the largest has none.  -inf and NaN logits are never drawn, +inf
+ * counts as the largest finite number. */
+typedef struct {
+    const float *temperature;
+    const int32_t *top_k;
+    const float *top_p;
+    const float *min_p;
+} zlm_sampling;
+/* logits: `rows` rows of `vocab` floats (1 to 2^20), `stride` floats apart (0:
+ * packed).  u: a number in [0, 1) per row.  token[r]: the token, -1 in a row
+ * whose logits are all -inf or NaN.  prob (or null): its share of the weight of
+ * the tokens left (1 for the largest logit's, 0 for -1).  how null: all filters
+ * off.  Histograms live in the library scratch of zlm_gpu_attention_enqueue (call
+ * once before capture). */
+bool zlm_gpu_sample_enqueue(zlm_device *dev, const float *logits, uint64_t stride, uint32_t rows, uint32_t vocab,
+                            const zlm_sampling *how, const float *u, int32_t *token, float *prob);
+
 /* ---- HIP graphs over the device stream ----
  * Everything enqueued between capture_begin and capture_end is recorded, not
  * run.  Only the *_enqueue entry points can be captured: the host-buffer

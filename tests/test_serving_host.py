@@ -103,6 +103,40 @@ def test_attention_scratch_is_sized_eagerly(box):
     assert wide(), d.last_error()
 
 
+def test_sampling_refusals(box):
+    d, p = box.dev, 1 << 16
+    assert d.sample_enqueue(p, 3, 1000, p, p, temperature=p, top_k=p, top_p=p, min_p=p, prob=p), d.last_error()
+    assert d.sample_enqueue(p, 3, 1000, p, p, stride=1001), d.last_error()
+    assert d.sample_enqueue(p, 3, 1 << 20, p, p), d.last_error()
+    for vocab, more in ((0, {}), ((1 << 20) + 1, {}), (1000, dict(stride=999))):
+        assert not d.sample_enqueue(p, 3, vocab, p, p, **more) and d.last_error()
+    for bad in ((0, 3, 10, p, p), (p, 3, 10, 0, p), (p, 3, 10, p, 0)):
+        assert not d.sample_enqueue(*bad) and "null" in d.last_error()
+    d.launch_log(True)
+    assert d.sample_enqueue(0, 0, 10, 0, 0) and d.launch_log_read() == []
+    # rows in as many launches as the scratch takes
+    assert d.sample_enqueue(p, 40000, 262144, p, p), d.last_error()
+    launches = [r for r in d.launch_log_read() if r["what"] == "sample"]
+    assert sum(r["grid_x"] for r in launches) == 40000 and len(launches) > 1
+    assert d.scratch_device_bytes() <= 65 << 20
+    raw = box.raw
+    assert raw.zlm_gpu_sample_enqueue(d._h, p, 0, 1, 10, None, p, p, None)  # all filters off
+
+
+def test_sampling_scratch_is_sized_eagerly(box):
+    d, p = box.dev, 1 << 16
+    assert d.capture_begin()
+    assert not d.sample_enqueue(p, 4, 150000, p, p) and "sampling scratch" in d.last_error()
+    d.graph_destroy(d.capture_end())
+    assert d.sample_enqueue(p, 4, 150000, p, p)
+    assert d.capture_begin()
+    assert d.sample_enqueue(p, 4, 150000, p, p), d.last_error()
+    g = d.capture_end()
+    assert not d.sample_enqueue(p, 800, 150000, p, p) and "captured graph" in d.last_error()
+    d.graph_destroy(g)
+    assert d.sample_enqueue(p, 800, 150000, p, p), d.last_error()
+
+
 def test_page_bytes():
     assert zd.paged_page_bytes(zd.F16, 8, 128, 64) == 8 * 64 * 256
     assert zd.paged_page_bytes(zd.Q4_0, 8, 128, 64) == 8 * 64 * 72

@@ -4,8 +4,9 @@
 // The kernels live in gfx950 code objects next to this library, loaded with
 // hipModuleLoad: zlm_kernels_gfx950.hsaco (layout, dequant, quantizer, GEMM,
 // decode glue; $ZLM_HIP_CODE_OBJECT overrides its path), one
-// zlm_gemv_<quant>_gfx950.hsaco per quant with that quant's GEMV forms and
-// zlm_paged_gfx950.hsaco (the paged KV cache's append and attention).  One HIP
+// zlm_gemv_<quant>_gfx950.hsaco per quant with that quant's GEMV forms,
+// zlm_paged_gfx950.hsaco (the paged KV cache's append and attention) and
+// zlm_sample_gfx950.hsaco (the sampler).  One HIP
 // stream per device carries every copy and launch in order, so a burst's
 // shared activation and a resident's layout conversion are ordered before the
 // kernels that read them without extra synchronisation.
@@ -21,6 +22,7 @@
 #include "zlm_gpu_hip.h"
 
 #include "paged_args.h"
+#include "sample_args.h"
 #include "zlm_static_scratch.h"
 
 #include <dlfcn.h>
@@ -223,6 +225,9 @@ struct zlm_device {
     struct PagedKernels {
         hipFunction_t append = nullptr, read = nullptr, few = nullptr, merge_few = nullptr;
     } paged[2][3];
+    hipModule_t sample_mod = nullptr;
+    hipFunction_t sample_hist = nullptr;
+    hipFunction_t sample_pick = nullptr;
     hipFunction_t synth_blocks = nullptr;
     hipFunction_t synth_f16 = nullptr;
 
@@ -314,8 +319,10 @@ std::string library_dir() {
 void unload_modules(zlm_device* d) {
     if (d->mod) hipModuleUnload(d->mod);
     d->mod = nullptr;
-    if (d->paged_mod) hipModuleUnload(d->paged_mod);
-    d->paged_mod = nullptr;
+    for (hipModule_t* m : {&d->paged_mod, &d->sample_mod}) {
+        if (*m) hipModuleUnload(*m);
+        *m = nullptr;
+    }
     for (hipModule_t& m : d->gemv_mod) {
         if (m) hipModuleUnload(m);
         m = nullptr;
@@ -402,6 +409,10 @@ bool load_kernels(zlm_device* d) {
                 if (!ok(d, hipModuleGetFunction(fn.f, d->paged_mod, nm), nm)) return false;
             }
         }
+    const std::string sp = dir + "/zlm_sample_gfx950.hsaco";
+    if (!ok(d, hipModuleLoad(&d->sample_mod, sp.c_str()), sp.c_str())) return false;
+    if (!ok(d, hipModuleGetFunction(&d->sample_hist, d->sample_mod, "zlm_sample_hist"), "zlm_sample_hist")) return false;
+    if (!ok(d, hipModuleGetFunction(&d->sample_pick, d->sample_mod, "zlm_sample_pick"), "zlm_sample_pick")) return false;
     return true;
 }
 
@@ -2835,11 +2846,12 @@ extern "C" bool zlm_gpu_qk_norm_rope_kv_enqueue(zlm_device* d, const float* qkv,
 
 namespace {
 
-// Size the attention partials (floats).  Allocation happens on an eager call;
-// a call under capture that would need it fails.
-bool ensure_attn_scratch(zlm_device* d, size_t need) {
+// Size the attention partials (floats); the sampler's histograms live there
+// too.  Allocation happens on an eager call; a call under capture that would
+// need it fails.
+bool ensure_attn_scratch(zlm_device* d, size_t need, const char* what = "the attention scratch") {
     if (need > d->attn_part_cap) {
-        if (!may_replace_scratch(d, kUsesAttn, "the attention scratch")) return false;
+        if (!may_replace_scratch(d, kUsesAttn, what)) return false;
         if (d->attn_part) {
             hipStreamSynchronize(d->stream);
             hipFree(d->attn_part);
@@ -3077,6 +3089,48 @@ extern "C" bool zlm_gpu_paged_attention_enqueue(zlm_device* d, const zlm_paged_c
     void* args[] = {&a, &g};
     return launch3(d, k->few, grid, 1, 1, 256, args, "paged attention") &&
            launch3(d, k->merge_few, grid - 1, 1, 1, 256, args, "paged attention merge");
+}
+
+// ---- sampling ----
+
+// Rows of one launch: their histograms take at most this much scratch.
+constexpr uint64_t kSampleScratch = 64ull << 20;
+
+extern "C" bool zlm_gpu_sample_enqueue(zlm_device* d, const float* logits, uint64_t stride, uint32_t rows,
+                                       uint32_t vocab, const zlm_sampling* how, const float* u, int32_t* token,
+                                       float* prob) {
+    if (!d || !d->avail) return false;
+    if (vocab == 0 || vocab > zlm::kSampleSlice * zlm::kSampleSlices)
+        return fail(d, "sampling takes 1 to %u logits a row (got %u)", zlm::kSampleSlice * zlm::kSampleSlices, vocab);
+    if (stride == 0) stride = vocab;
+    if (stride < vocab) return fail(d, "logits rows of %llu floats overlap", static_cast<unsigned long long>(stride));
+    if (rows == 0) return true;
+    if (!logits || !u || !token) return fail(d, "null buffer");
+    zlm::SampleArgs a = {};
+    a.stride = stride;
+    a.vocab = vocab;
+    a.slices = (vocab + zlm::kSampleSlice - 1) / zlm::kSampleSlice;
+    const uint64_t slice_bytes = zlm::kSampleBins * sizeof(uint64_t) + sizeof(zlm::SampleSlice);
+    const uint32_t most = static_cast<uint32_t>(std::min<uint64_t>(kSampleScratch / (slice_bytes * a.slices), rows));
+    if (!ensure_attn_scratch(d, slice_bytes * a.slices * most / sizeof(float), "the sampling scratch")) return false;
+    a.hist = reinterpret_cast<uint64_t*>(d->attn_part);
+    a.info = reinterpret_cast<zlm::SampleSlice*>(a.hist + static_cast<size_t>(most) * a.slices * zlm::kSampleBins);
+    for (uint32_t r = 0; r < rows; r += most) {
+        a.rows = std::min(most, rows - r);
+        a.logits = logits + r * stride;
+        a.temperature = how && how->temperature ? how->temperature + r : nullptr;
+        a.top_k = how && how->top_k ? how->top_k + r : nullptr;
+        a.top_p = how && how->top_p ? how->top_p + r : nullptr;
+        a.min_p = how && how->min_p ? how->min_p + r : nullptr;
+        a.u = u + r;
+        a.token = token + r;
+        a.prob = prob ? prob + r : nullptr;
+        void* args[] = {&a};
+        if (!launch3(d, d->sample_hist, a.slices, a.rows, 1, 1024, args, "sample histogram") ||
+            !launch(d, d->sample_pick, a.rows, 1024, args, "sample"))
+            return false;
+    }
+    return true;
 }
 
 struct zlm_graph {

@@ -24,8 +24,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_DIR = os.path.join(_HERE, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libzlm_gpu_hip.so")
 CODE_OBJECT_PATH = os.path.join(LIB_DIR, "zlm_kernels_gfx950.hsaco")
-# Every code object the library loads: the common kernels, the paged cache's and one GEMV object per quant.
-CODE_OBJECT_PATHS = [CODE_OBJECT_PATH, os.path.join(LIB_DIR, "zlm_paged_gfx950.hsaco")] + [os.path.join(LIB_DIR, f"zlm_gemv_{q}_gfx950.hsaco")
+# Every code object the library loads: the common kernels, the paged cache's, the sampler's and one GEMV object per quant.
+CODE_OBJECT_PATHS = [CODE_OBJECT_PATH] + [os.path.join(LIB_DIR, f"zlm_{n}_gfx950.hsaco") for n in ("paged", "sample")] + [os.path.join(LIB_DIR, f"zlm_gemv_{q}_gfx950.hsaco")
                                           for q in ("q4_0", "q8_0", "q4_k", "q6_k", "q4_1", "f32", "f16", "bf16")]
 
 RING_SIZE = 8
@@ -100,6 +100,11 @@ class _PagedCache(ctypes.Structure):
 class _PagedBatch(ctypes.Structure):
     _fields_ = [("n_seqs", ctypes.c_uint32), ("n_tokens", ctypes.c_uint32), ("q_start", ctypes.c_void_p),
                 ("kv_len", ctypes.c_void_p), ("table", ctypes.c_void_p), ("table_stride", ctypes.c_uint32)]
+
+
+class _Sampling(ctypes.Structure):
+    _fields_ = [("temperature", ctypes.c_void_p), ("top_k", ctypes.c_void_p), ("top_p", ctypes.c_void_p),
+                ("min_p", ctypes.c_void_p)]
 
 
 class LaunchRecord(ctypes.Structure):
@@ -203,6 +208,7 @@ def lib() -> ctypes.CDLL:
         "zlm_gpu_paged_append_enqueue": (B, [P, P, P, P, ctypes.c_uint64, P, P, U, ctypes.c_float, ctypes.c_float, P]),
         "zlm_gpu_paged_read_enqueue": (B, [P, P, P, P, P]),
         "zlm_gpu_paged_attention_enqueue": (B, [P, P, P, P, U, U, ctypes.c_float, P]),
+        "zlm_gpu_sample_enqueue": (B, [P, P, ctypes.c_uint64, U, U, P, P, P, P]),
         "zlm_gpu_resident_device_bytes": (ctypes.c_uint64, [P]),
         "zlm_gpu_layout_bytes": (ctypes.c_uint64, [U, S, S, ctypes.c_bool]),
         "zlm_gpu_release_gemm_tiles": (B, [P, P]),
@@ -584,6 +590,14 @@ class Device:
         """Attention of a batch's rows over their sequences' pages (no wait)."""
         return bool(self._L.zlm_gpu_paged_attention_enqueue(self._h, ctypes.byref(cache.c), ctypes.byref(batch.c), q,
                                                             n_heads, window, scale, out))
+
+    def sample_enqueue(self, logits: int, rows: int, vocab: int, u: int, token: int, temperature: int = 0,
+                       top_k: int = 0, top_p: int = 0, min_p: int = 0, prob: int = 0, stride: int = 0) -> bool:
+        """Draw a token from each row of device logits (no wait); the parameters are device arrays of one value a
+        row, 0 leaves a filter off."""
+        how = _Sampling(temperature or None, top_k or None, top_p or None, min_p or None)
+        return bool(self._L.zlm_gpu_sample_enqueue(self._h, logits, stride, rows, vocab, ctypes.byref(how), u, token,
+                                                   prob or None))
 
     def probe_rates(self, ggml_type: int, gate_up: bool, rows: int, k: int) -> Optional[np.ndarray]:
         """GB/s of each GpuVariant for one quant (resident GEMV or fused gate_up); None if one did not run."""
