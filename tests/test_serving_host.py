@@ -96,11 +96,10 @@ def test_attention_scratch_is_sized_eagerly(box):
     assert call(), d.last_error()
     g = d.capture_end()
     assert call() and box.stat(MALLOCS) == mallocs
-    # a call that needs more scratch than the graph's leaves it alone
-    wide = _calls(box, _cache(box.mod, hd=256), _batch(box.mod))["attention"]
-    assert not wide() and "captured graph" in d.last_error()
+    # the scratch has room for every shape: calls of another beside the graph need no other
+    wide = _calls(box, _cache(box.mod, hd=256), _batch(box.mod, seqs=1, tokens=300))["attention"]
+    assert wide() and d.sample_enqueue(1 << 16, 800, 150000, 1 << 16, 1 << 16) and box.stat(MALLOCS) == mallocs
     d.graph_destroy(g)
-    assert wide(), d.last_error()
 
 
 def test_sampling_refusals(box):
@@ -131,10 +130,30 @@ def test_sampling_scratch_is_sized_eagerly(box):
     assert d.sample_enqueue(p, 4, 150000, p, p)
     assert d.capture_begin()
     assert d.sample_enqueue(p, 4, 150000, p, p), d.last_error()
-    g = d.capture_end()
-    assert not d.sample_enqueue(p, 800, 150000, p, p) and "captured graph" in d.last_error()
-    d.graph_destroy(g)
-    assert d.sample_enqueue(p, 800, 150000, p, p), d.last_error()
+    d.graph_destroy(d.capture_end())
+
+
+@pytest.mark.parametrize("seqs,tokens,group,want", [
+    # one token a sequence, and few tokens each: the few-row kernel alone
+    (1, 1, 4, ["few"]), (64, 64, 8, ["few"]), (8, 40, 4, ["few"]), (2, 2, 33, ["few"]),
+    # one sequence of more rows than it takes: the many-row kernel alone, its positions split while it has few items
+    (1, 9, 4, ["many", "merge"]), (1, 2048, 4, ["many"]), (1, 300, 4, ["many", "merge"]),
+    # prompts beside other sequences: both
+    (16, 1015, 2, ["many", "merge", "few"]), (200, 500, 4, ["many", "few"]), (2, 4000, 4, ["many", "few"])])
+def test_attention_routes(box, seqs, tokens, group, want):
+    d, p = box.dev, 1 << 16
+    d.launch_log(True)
+    assert d.paged_attention_enqueue(_cache(box.mod, kv=8), _batch(box.mod, seqs=seqs, tokens=tokens), p, p, 8 * group,
+                                     0.1), d.last_error()
+    names = {"paged attention of many rows": "many", "paged attention of many rows, merge": "merge",
+             "paged attention": "few"}
+    log = d.launch_log_read()
+    assert [names[r["what"]] for r in log if r["what"] in names] == want
+    # a workgroup for every tile that the rows may make, kv head and split
+    for r in log:
+        if r["what"] == "paged attention of many rows":
+            rows = tokens * group
+            assert r["grid_x"] % 8 == 0 and r["grid_x"] // 8 >= -(-rows // 128)
 
 
 def test_page_bytes():

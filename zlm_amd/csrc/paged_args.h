@@ -45,6 +45,8 @@ struct PagedAttend {
     uint32_t n_heads, group;
     uint32_t window;  // 0: all
     float scale;      // times log2(e)
+    uint32_t few_rows;  // sequences with more rows (tokens x group) are the many-row kernel's
+    uint32_t splits;    // its splits of the positions
 };
 
 }  // namespace zlm

@@ -223,7 +223,7 @@ struct zlm_device {
     // the paged cache's kernels, by cache type (f16, q4_0) and head size (kPagedDims)
     hipModule_t paged_mod = nullptr;
     struct PagedKernels {
-        hipFunction_t append = nullptr, read = nullptr, few = nullptr, merge_few = nullptr;
+        hipFunction_t append = nullptr, read = nullptr, few = nullptr, merge_few = nullptr, many = nullptr, merge_many = nullptr;
     } paged[2][3];
     hipModule_t sample_mod = nullptr;
     hipFunction_t sample_hist = nullptr;
@@ -403,7 +403,8 @@ bool load_kernels(zlm_device* d) {
             const struct {
                 hipFunction_t* f;
                 const char* name;
-            } fns[] = {{&k.append, "append"}, {&k.read, "read"}, {&k.few, "attend_few"}, {&k.merge_few, "merge_few"}};
+            } fns[] = {{&k.append, "append"}, {&k.read, "read"}, {&k.few, "attend_few"}, {&k.merge_few, "merge_few"},
+                       {&k.many, "attend_many"}, {&k.merge_many, "merge_many"}};
             for (const auto& fn : fns) {
                 snprintf(nm, sizeof nm, "zlm_paged_%s_%s_%d", fn.name, t ? "q4_0" : "f16", kPagedDims[i]);
                 if (!ok(d, hipModuleGetFunction(fn.f, d->paged_mod, nm), nm)) return false;
@@ -2972,6 +2973,11 @@ extern "C" bool zlm_gpu_attention_enqueue(zlm_device* d, const float* q, const u
     return enqueue_attn_merge(d, part, nsplit, n_heads, out);
 }
 
+// The scratch that any paged attention or draw sizes at least: what the largest of
+// their launches need (34 MB the attention's partials with two workgroups a CU of
+// 256 CUs), so that a captured graph of one call never stands in another's way.
+constexpr uint64_t kServingScratch = 64ull << 20;
+
 // ---- the paged KV cache: append, read back, attention ----
 
 namespace {
@@ -3076,8 +3082,25 @@ extern "C" bool zlm_gpu_paged_attention_enqueue(zlm_device* d, const zlm_paged_c
     if (tiles * cache->n_kv_heads * std::min<uint64_t>(depth, (1u << 24) + 2) >= (1ull << 31))
         return fail(d, "attention of %u tokens over up to %u pages a sequence is too large for one call",
                     batch->n_tokens, batch->table_stride);
+    // Sequences of more than kFewRows rows go to the many-row kernel.  Which there
+    // are is known on the device only: both kernels run where the batch may hold such
+    // a sequence beside others, or is made of them.
+    constexpr uint32_t kFewRows = 32;
+    const uint64_t rows = static_cast<uint64_t>(batch->n_tokens) * group;
+    const bool many = batch->n_tokens > batch->n_seqs && (rows > 512 || rows > static_cast<uint64_t>(batch->n_seqs) * kFewRows);
+    const bool few = !many || batch->n_seqs > 1;
     const uint32_t grid = static_cast<uint32_t>(d->cus) * 2;
-    if (!ensure_attn_scratch(d, static_cast<size_t>(grid) * 2 * 16 * (hd + 2))) return false;
+    const uint32_t tile_rows = hd == 256 ? 64 : 128;
+    // a tile for each tile_rows rows and one a sequence begun, as far as there are rows for it
+    const uint64_t many_tiles = rows / tile_rows + std::min<uint64_t>(batch->n_seqs, rows / kFewRows);
+    const uint64_t items = many_tiles * cache->n_kv_heads;
+    if (many && items >= (1ull << 23)) return fail(d, "attention of %u tokens is too large for one call", batch->n_tokens);
+    // positions are split until two workgroups a CU have work
+    const uint64_t want = static_cast<uint64_t>(d->cus) * 2;
+    const uint32_t splits = many ? static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(16, want / items))) : 1;
+    const size_t few_part = few ? static_cast<size_t>(grid) * 2 * 16 * (hd + 2) : 0;
+    const size_t many_part = splits > 1 ? items * splits * tile_rows * (hd + 2) : 0;
+    if (!ensure_attn_scratch(d, std::max({few_part, many_part, kServingScratch / sizeof(float)}))) return false;
     a.q = q;
     a.out = out;
     a.part = d->attn_part;
@@ -3085,16 +3108,20 @@ extern "C" bool zlm_gpu_paged_attention_enqueue(zlm_device* d, const zlm_paged_c
     a.group = group;
     a.window = window;
     a.scale = scale * 1.44269504088896340736f;
+    a.few_rows = many ? kFewRows : 0xffffffffu;
+    a.splits = splits;
     uint32_t g = grid;
     void* args[] = {&a, &g};
-    return launch3(d, k->few, grid, 1, 1, 256, args, "paged attention") &&
-           launch3(d, k->merge_few, grid - 1, 1, 1, 256, args, "paged attention merge");
+    if (many && !(launch(d, k->many, static_cast<uint32_t>(items * splits), 256, args, "paged attention of many rows") &&
+                  (splits == 1 || launch3(d, k->merge_many, static_cast<uint32_t>(items), tile_rows / 16, 1, 256, args,
+                                          "paged attention of many rows, merge"))))
+        return false;
+    if (!few) return true;
+    return launch(d, k->few, grid, 256, args, "paged attention") &&
+           launch(d, k->merge_few, grid - 1, 256, args, "paged attention merge");
 }
 
 // ---- sampling ----
-
-// Rows of one launch: their histograms take at most this much scratch.
-constexpr uint64_t kSampleScratch = 64ull << 20;
 
 extern "C" bool zlm_gpu_sample_enqueue(zlm_device* d, const float* logits, uint64_t stride, uint32_t rows,
                                        uint32_t vocab, const zlm_sampling* how, const float* u, int32_t* token,
@@ -3111,8 +3138,9 @@ extern "C" bool zlm_gpu_sample_enqueue(zlm_device* d, const float* logits, uint6
     a.vocab = vocab;
     a.slices = (vocab + zlm::kSampleSlice - 1) / zlm::kSampleSlice;
     const uint64_t slice_bytes = zlm::kSampleBins * sizeof(uint64_t) + sizeof(zlm::SampleSlice);
-    const uint32_t most = static_cast<uint32_t>(std::min<uint64_t>(kSampleScratch / (slice_bytes * a.slices), rows));
-    if (!ensure_attn_scratch(d, slice_bytes * a.slices * most / sizeof(float), "the sampling scratch")) return false;
+    // rows of one launch: as many as the scratch has room for
+    const uint32_t most = static_cast<uint32_t>(std::min<uint64_t>(kServingScratch / (slice_bytes * a.slices), rows));
+    if (!ensure_attn_scratch(d, kServingScratch / sizeof(float), "the sampling scratch")) return false;
     a.hist = reinterpret_cast<uint64_t*>(d->attn_part);
     a.info = reinterpret_cast<zlm::SampleSlice*>(a.hist + static_cast<size_t>(most) * a.slices * zlm::kSampleBins);
     for (uint32_t r = 0; r < rows; r += most) {

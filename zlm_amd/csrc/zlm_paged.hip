@@ -626,7 +626,7 @@ __device__ __forceinline__ uint32_t scan_units(const AttnArgs& a, uint32_t* pref
         uint32_t x = 0;
         if (b + tid < a.p.n_seqs) {
             const SeqWork w = seq_work(a, b + tid);
-            x = w.tiles * a.p.n_kv * w.units;
+            if (static_cast<uint32_t>(w.len) * a.group <= a.few_rows) x = w.tiles * a.p.n_kv * w.units;
         }
         uint32_t run = x;
 #pragma unroll
@@ -732,7 +732,7 @@ __device__ __forceinline__ void attend_few(const AttnArgs& a) {
             v4f s[2];
             scores<HD, Q4>(kr, qt, s);
             const int32_t p0 = static_cast<int32_t>(kb + 8 * q);
-            const bool no_page = g.id[q >> 1] < 0;
+            const bool no_page = (q >= 2 ? g.id[1] : g.id[0]) < 0;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const int32_t x = p0 + j;
@@ -825,6 +825,414 @@ __device__ __forceinline__ void merge_few(const AttnArgs& a, uint32_t grid) {
     }
 }
 
+// ---- many rows ----
+//
+// A workgroup owns 16 kRt rows a wave of one kv head (the rows of consecutive
+// tokens, each with its group of q heads) and walks the positions they see, 32 kBlocks
+// at a time: the four waves load and decode a quarter each of the K and V operands
+// into LDS, in the lanes' order, while all four multiply from the other buffer.
+template <int HD>
+struct Many {
+    static constexpr int kRt = HD == 256 ? 1 : 2;      // tiles of 16 rows a wave
+    static constexpr int kBlocks = HD == 256 ? 1 : 2;  // 32-position blocks a stage
+    static constexpr uint32_t kRows = 64 * kRt;
+    static constexpr uint32_t kStage = 32 * kBlocks;
+};
+
+template <int HD>
+struct Operands {  // one stage
+    v8h k[Many<HD>::kBlocks][2][HD / 32][kWave];
+    v8h v[Many<HD>::kBlocks][HD / 16][kWave];
+};
+
+// A wave's share of a stage as loaded: K's and V's four operands of a block (hd 64:
+// the even waves load K's, the odd ones V's).
+template <int HD, bool Q4>
+struct Share {
+    static constexpr int kN = HD == 64 ? 4 : 8;
+    v4u w[Q4 ? 2 : kN];
+    v4u vd;
+    uint32_t kd;
+    Pages g;
+    uint32_t kb;
+};
+
+template <int HD>
+struct Job {  // which: block, K tile, 4-operand run of K and of V
+    uint32_t blk, t, kb, vb;
+    bool k, v;
+};
+
+template <int HD>
+__device__ __forceinline__ Job<HD> job_of(uint32_t w) {
+    if constexpr (HD == 256) return {0, w & 1, w >> 1, w, true, true};
+    if constexpr (HD == 128) return {w >> 1, w & 1, 0, w & 1, true, true};
+    return {w >> 1, 0, 0, 0, (w & 1) == 0, (w & 1) != 0};
+}
+
+template <int HD, bool Q4>
+__device__ __forceinline__ void share_load(const Paged& p, const Job<HD>& job, uint32_t h, uint32_t lane,
+                                           Share<HD, Q4>& r) {
+    const uint32_t m = lane & 15, q = lane >> 4, page = 1u << p.page_shift;
+    const size_t b0 = head_base<HD, Q4>(p, max(r.g.id[0], 0), h), b1 = head_base<HD, Q4>(p, max(r.g.id[1], 0), h);
+    const uint8_t* kbase = p.k + (m >= 8 ? b1 : b0);
+    const uint8_t* vbase = p.v + (q >= 2 ? b1 : b0);
+    const uint32_t grp = ((r.kb + 8 * q) & (page - 1)) >> 3;
+    if (job.k) {
+        const uint32_t off = (r.kb + k_row(m, job.t)) & (page - 1);
+        if constexpr (HD == 64) {
+            const uint32_t off1 = (r.kb + k_row(m, 1)) & (page - 1);
+            if constexpr (Q4) {
+                const v2u x = *reinterpret_cast<const v2u*>(kbase + off * 32 + 8 * q);
+                const v2u y = *reinterpret_cast<const v2u*>(kbase + off1 * 32 + 8 * q);
+                r.w[0] = v4u{x.x, x.y, y.x, y.y};
+                const uint16_t* sc = reinterpret_cast<const uint16_t*>(kbase + page * 32) + (q >> 1);
+                r.kd = sc[off * 2] | static_cast<uint32_t>(sc[off1 * 2]) << 16;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    r.w[i] = *reinterpret_cast<const v4u*>(kbase + off * 128 + 64 * i + 16 * q);
+                    r.w[2 + i] = *reinterpret_cast<const v4u*>(kbase + off1 * 128 + 64 * i + 16 * q);
+                }
+            }
+        } else if constexpr (Q4) {
+            r.w[0] = *reinterpret_cast<const v4u*>(kbase + off * (HD / 2) + 16 * q + 64 * job.kb);
+            r.kd = reinterpret_cast<const uint16_t*>(kbase + page * (HD / 2))[off * (HD / 32) + q + 4 * job.kb];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                r.w[i] = *reinterpret_cast<const v4u*>(kbase + off * (HD * 2) + 64 * (4 * job.kb + i) + 16 * q);
+        }
+    }
+    if (job.v) {
+        if constexpr (Q4) {
+            r.w[1] = *reinterpret_cast<const v4u*>(vbase + (grp * HD + 64 * job.vb + 4 * m) * 4);
+            r.vd = reinterpret_cast<const v4u*>(vbase + page * (HD / 2))[grp * (HD / 32) + 2 * job.vb + (m >> 3)];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                r.w[(HD == 64 ? 0 : 4) + i] =
+                    *reinterpret_cast<const v4u*>(vbase + (grp * HD + 16 * (4 * job.vb + i) + m) * 16);
+        }
+    }
+}
+
+// The share decoded into the stage's operands.  `edge`: positions outside [lo, hi)
+// or without a page may be among them: their V becomes 0, a K without a page NaN.
+template <int HD, bool Q4>
+__device__ __forceinline__ void share_store(const Job<HD>& job, Share<HD, Q4>& r, Operands<HD>& to, uint32_t lane,
+                                            int32_t lo, int32_t hi) {
+    const uint32_t m = lane & 15, q = lane >> 4;
+    const bool edge = static_cast<int32_t>(r.kb) < lo || static_cast<int32_t>(r.kb) + 32 > hi || r.g.id[0] < 0 || r.g.id[1] < 0;
+    v4u keep = {~0u, ~0u, ~0u, ~0u};
+    bool no_k = false;
+    if (edge) {
+        no_k = (m >= 8 ? r.g.id[1] : r.g.id[0]) < 0;
+        const int32_t at = static_cast<int32_t>(r.kb + 8 * q), end = (q >= 2 ? r.g.id[1] : r.g.id[0]) < 0 ? lo : hi;
+        uint32_t x[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int32_t a = at + 2 * i;
+            x[i] = (a >= lo && a < end ? 0xffffu : 0u) | (a + 1 >= lo && a + 1 < end ? 0xffff0000u : 0u);
+        }
+        keep = v4u{x[0], x[1], x[2], x[3]};
+    }
+    if (job.k) {
+        v8h o[4];
+        if constexpr (Q4) {
+            const uint32_t x[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
+            const uint32_t d0 = (r.kd & 0xffffu) * 0x10001u, d1 = HD == 64 ? (r.kd >> 16) * 0x10001u : d0;
+            const v2h s0 = __builtin_bit_cast(v2h, d0), s1 = __builtin_bit_cast(v2h, d1);
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[i] = i < 2 ? decode8(x[i], s0, s0, s0, s0) : decode8(x[i], s1, s1, s1, s1);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[i] = __builtin_bit_cast(v8h, r.w[i]);
+        }
+        const _Float16 nan = __builtin_bit_cast(_Float16, static_cast<uint16_t>(0x7e00));
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (edge && no_k) o[i] = v8h{nan, nan, nan, nan, nan, nan, nan, nan};
+            if constexpr (HD == 64) to.k[job.blk][i / 2][i % 2][lane] = o[i];
+            else to.k[job.blk][job.t][4 * job.kb + i][lane] = o[i];
+        }
+    }
+    if (job.v) {
+        if constexpr (Q4) {
+            const v4u d = r.vd & keep;
+            const uint32_t d0 = d.x, d1 = d.y, d2 = d.z, d3 = d.w;
+            const uint32_t x[4] = {r.w[1].x, r.w[1].y, r.w[1].z, r.w[1].w};
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                to.v[job.blk][4 * job.vb + i][lane] =
+                    decode8(x[i], __builtin_bit_cast(v2h, d0), __builtin_bit_cast(v2h, d1), __builtin_bit_cast(v2h, d2),
+                            __builtin_bit_cast(v2h, d3));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const v4u x = r.w[(HD == 64 ? 0 : 4) + i] & keep;
+                to.v[job.blk][4 * job.vb + i][lane] = __builtin_bit_cast(v8h, x);
+            }
+        }
+    }
+}
+
+// A workgroup's item: tile `tile` of the rows of sequence s.
+struct Item {
+    uint32_t s, tile, h, split;
+    bool any;
+};
+
+// Tiles of the sequences with more than few_rows rows, in order; the grid has one
+// workgroup for each (a bound of their number), kv head and split.
+template <int HD>
+__device__ __forceinline__ Item item_of(const AttnArgs& a, uint32_t block, uint32_t* prefix, uint32_t* sums, SeqWork& w) {
+    constexpr uint32_t kRows = Many<HD>::kRows;
+    Item it;
+    it.h = block % a.p.n_kv;
+    it.split = block / a.p.n_kv % a.splits;
+    const uint32_t tile = block / a.p.n_kv / a.splits;
+    const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1), wid = tid / kWave;
+    uint32_t base = 0;
+    it.any = false;
+    for (uint32_t b = 0; b < a.p.n_seqs; b += 256) {
+        uint32_t x = 0;
+        if (b + tid < a.p.n_seqs) {
+            const uint32_t rows = static_cast<uint32_t>(seq_work(a, b + tid).len) * a.group;
+            x = rows > a.few_rows ? (rows + kRows - 1) / kRows : 0;
+        }
+        uint32_t run = x;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t y = __shfl_up(run, o);
+            if (static_cast<int>(lane) >= o) run += y;
+        }
+        if (lane == 63) sums[wid] = run;
+        __syncthreads();
+        uint32_t before = base;
+        for (uint32_t i = 0; i < 4; i++) {
+            if (i < wid) before += sums[i];
+            base += sums[i];
+        }
+        const uint32_t end = before + run;
+        if (tile >= end - x && tile < end) {  // one thread at most
+            prefix[0] = b + tid;
+            prefix[1] = end - 1 - tile;  // the last tile first: it sees the most
+        }
+        if (tile < base) {
+            it.any = true;
+            break;
+        }
+        __syncthreads();
+    }
+    __syncthreads();
+    if (!it.any) return it;
+    it.s = __builtin_amdgcn_readfirstlane(prefix[0]);
+    it.tile = __builtin_amdgcn_readfirstlane(prefix[1]);
+    w = seq_work(a, it.s);
+    return it;
+}
+
+// The positions that an item's rows see, and its split's part of them.
+struct Span {
+    int32_t lo, hi;      // of the item
+    int32_t from, to;    // of the split
+    uint32_t parts;      // splits that have any
+};
+
+template <int HD>
+__device__ __forceinline__ Span span_of(const AttnArgs& a, const Item& it, const SeqWork& w) {
+    constexpr uint32_t kRows = Many<HD>::kRows;
+    const uint32_t rows = static_cast<uint32_t>(w.len) * a.group;
+    const uint32_t first_tok = kRows * it.tile / a.group, last_tok = (min(kRows * (it.tile + 1), rows) - 1) / a.group;
+    Span s;
+    s.hi = max(min(w.first + static_cast<int32_t>(last_tok) + 1, w.end), 0);
+    const int32_t first_hi = w.first + static_cast<int32_t>(first_tok) + 1;
+    s.lo = a.window && first_hi > static_cast<int32_t>(a.window) ? first_hi - static_cast<int32_t>(a.window) : 0;
+    const int32_t start = min(s.lo, s.hi) & ~31;
+    // splits of at least 256 positions, in whole stages
+    const uint32_t n = static_cast<uint32_t>(s.hi - start), step = Many<HD>::kStage;
+    const uint32_t each = max((n + a.splits - 1) / a.splits, 256u);
+    const uint32_t part = (each + step - 1) / step * step;
+    s.parts = max((n + part - 1) / part, 1u);
+    s.from = static_cast<int32_t>(min(static_cast<uint64_t>(start) + static_cast<uint64_t>(part) * it.split, static_cast<uint64_t>(s.hi)));
+    s.to = static_cast<int32_t>(min(static_cast<uint64_t>(s.from) + part, static_cast<uint64_t>(s.hi)));
+    return s;
+}
+
+template <int HD>
+__device__ __forceinline__ float* many_slot(const AttnArgs& a, uint32_t block) {
+    return a.part + static_cast<size_t>(block) * (Many<HD>::kRows * (HD + 2));
+}
+
+template <int HD, bool Q4>
+__device__ __forceinline__ void attend_many(const AttnArgs& a) {
+    using M = Many<HD>;
+    __shared__ __attribute__((aligned(16))) Operands<HD> ops[2];
+    __shared__ uint32_t prefix[2], sums[4];
+    const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const uint32_t n = lane & 15, q = lane >> 4;
+    SeqWork w;
+    const Item it = item_of<HD>(a, blockIdx.x, prefix, sums, w);
+    if (!it.any) return;
+    const Span sp = span_of<HD>(a, it, w);
+    if (it.split >= sp.parts) return;
+    const uint32_t rows = static_cast<uint32_t>(w.len) * a.group;
+    const uint32_t row0 = M::kRows * it.tile + 16 * M::kRt * wid;
+    QTile<HD> qt[M::kRt];
+    Soft<HD> st[M::kRt];
+    int32_t hi[M::kRt], lo[M::kRt];
+#pragma unroll
+    for (int i = 0; i < M::kRt; i++) {
+        const uint32_t r = row0 + 16 * i + n;
+        const bool live = r < rows;
+        const uint32_t tok = live ? r / a.group : 0, head = it.h * a.group + (live ? r % a.group : 0);
+        const int32_t pos = w.first + static_cast<int32_t>(tok);
+        hi[i] = live ? pos + 1 : 0;
+        lo[i] = a.window && hi[i] > static_cast<int32_t>(a.window) ? hi[i] - static_cast<int32_t>(a.window) : 0;
+        load_q<HD, Q4>(qt[i], live ? a.q + (static_cast<size_t>(w.row0 + tok) * a.n_heads + head) * HD : nullptr, q, a.scale);
+        soft_clear<HD>(st[i]);
+        if (!live) st[i].m = 0.0f;
+        if (live && pos >= 0 && static_cast<uint64_t>(pos) >= capacity(a.p)) st[i].l = __builtin_nanf("");
+    }
+    // the wave's rows are in order of position: what any of them and what all of them see
+    const bool wave_live = row0 < rows;
+    const uint32_t tok_a = min(row0, rows - 1) / a.group, tok_b = (min(row0 + 16 * M::kRt, rows) - 1) / a.group;
+    const int32_t win = static_cast<int32_t>(a.window);
+    const int32_t hi_a = w.first + static_cast<int32_t>(tok_a) + 1, hi_b = w.first + static_cast<int32_t>(tok_b) + 1;
+    const int32_t any_lo = win && hi_a > win ? hi_a - win : 0, all_lo = win && hi_b > win ? hi_b - win : 0;
+    const bool full_tile = row0 + 16 * M::kRt <= rows;
+
+    const Job<HD> job = job_of<HD>(wid);
+    Share<HD, Q4> sh;
+    const auto start_load = [&](uint32_t at) {
+        sh.kb = at + 32 * job.blk;
+        sh.g = pages_at(a.p, it.s, sh.kb);
+        share_load<HD, Q4>(a.p, job, it.h, lane, sh);
+    };
+    uint32_t at = static_cast<uint32_t>(sp.from), buf = 0;
+    const uint32_t to = static_cast<uint32_t>(sp.to);
+    if (at < to) {
+        start_load(at);
+        share_store<HD, Q4>(job, sh, ops[0], lane, sp.lo, sp.hi);
+    }
+    __syncthreads();
+    for (; at < to; at += M::kStage) {
+        const bool more = at + M::kStage < to;
+        if (more) start_load(at + M::kStage);
+        const Operands<HD>& op = ops[buf];
+#pragma unroll
+        for (int b = 0; b < M::kBlocks; b++) {
+            const int32_t kb = static_cast<int32_t>(at) + 32 * b;
+            if (!wave_live || kb >= hi_b || kb + 32 <= any_lo) continue;
+            v4f s[M::kRt][2];
+#pragma unroll
+            for (int r = 0; r < M::kRt; r++) s[r][0] = s[r][1] = v4f{0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < HD / 32; i++)
+#pragma unroll
+                for (int t = 0; t < 2; t++) {
+                    const v8h x = op.k[b][t][i][lane];
+#pragma unroll
+                    for (int r = 0; r < M::kRt; r++) {
+                        s[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qt[r].hi[i], s[r][t], 0, 0, 0);
+                        s[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qt[r].lo[i], s[r][t], 0, 0, 0);
+                    }
+                }
+            v8h ph[M::kRt], pl[M::kRt];
+            const bool masked = kb < all_lo || kb + 32 > hi_a || !full_tile;
+#pragma unroll
+            for (int r = 0; r < M::kRt; r++) {
+                s[r][0] *= qt[r].factor;
+                s[r][1] *= qt[r].factor;
+                if (masked) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const int32_t x = kb + static_cast<int32_t>(8 * q) + j;
+                        s[r][j / 4][j % 4] = x < lo[r] || x >= hi[r] ? -INFINITY : s[r][j / 4][j % 4];
+                    }
+                }
+                soft_step<HD>(st[r], s[r], ph[r], pl[r]);
+            }
+#pragma unroll
+            for (int c = 0; c < HD / 16; c++) {
+                const v8h x = op.v[b][c][lane];
+#pragma unroll
+                for (int r = 0; r < M::kRt; r++) {
+                    st[r].o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, ph[r], st[r].o[c], 0, 0, 0);
+                    st[r].o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, pl[r], st[r].o[c], 0, 0, 0);
+                }
+            }
+        }
+        if (more) share_store<HD, Q4>(job, sh, ops[buf ^ 1], lane, sp.lo, sp.hi);
+        __syncthreads();
+        buf ^= 1;
+    }
+    float* slot = many_slot<HD>(a, blockIdx.x);
+#pragma unroll
+    for (int i = 0; i < M::kRt; i++) {
+        const uint32_t r = row0 + 16 * i + n;
+        const float l = sum_over_q(st[i].l);
+        if (r >= rows) continue;
+        const uint32_t tok = r / a.group, head = it.h * a.group + r % a.group, in_tile = r - M::kRows * it.tile;
+        const bool whole = sp.parts == 1;
+        float* dst = whole ? a.out + (static_cast<size_t>(w.row0 + tok) * a.n_heads + head) * HD : slot + in_tile * HD;
+        const float f = whole && l != 0.0f ? 1.0f / l : 1.0f;
+#pragma unroll
+        for (int c = 0; c < HD / 16; c++) {
+            if constexpr (Q4) {
+                // tiles 4 k .. 4 k + 3 hold runs of dims: 64 k + 16 q + 4 i + {0 .. 3}
+                if (c % 4 == 0) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const v4f o = {st[i].o[c][e], st[i].o[c + 1][e], st[i].o[c + 2][e], st[i].o[c + 3][e]};
+                        *reinterpret_cast<v4f*>(dst + 16 * c + 16 * q + 4 * e) = o * f;
+                    }
+                }
+            } else {
+                *reinterpret_cast<v4f*>(dst + 16 * c + 4 * q) = st[i].o[c] * f;
+            }
+        }
+        if (!whole && q == 0) {
+            slot[M::kRows * HD + in_tile] = st[i].m;
+            slot[M::kRows * HD + M::kRows + in_tile] = l;
+        }
+    }
+}
+
+// The join of an item's splits: a workgroup an item and 16 of its rows.
+template <int HD, bool Q4>
+__device__ __forceinline__ void merge_many(const AttnArgs& a) {
+    using M = Many<HD>;
+    __shared__ uint32_t prefix[2], sums[4];
+    const uint32_t block = blockIdx.x / a.p.n_kv * a.p.n_kv * a.splits + blockIdx.x % a.p.n_kv;  // its first split's
+    SeqWork w;
+    const Item it = item_of<HD>(a, block, prefix, sums, w);
+    if (!it.any) return;
+    const Span sp = span_of<HD>(a, it, w);
+    if (sp.parts == 1) return;
+    const uint32_t rows = static_cast<uint32_t>(w.len) * a.group;
+    for (uint32_t e = threadIdx.x; e < 16 * HD / 4; e += 256) {
+        const uint32_t row = 16 * blockIdx.y + e / (HD / 4), d = 4 * (e % (HD / 4)), rr = M::kRows * it.tile + row;
+        if (rr >= rows) continue;
+        float m = -INFINITY;
+        for (uint32_t i = 0; i < sp.parts; i++)
+            m = __builtin_fmaxf(m, many_slot<HD>(a, block + i * a.p.n_kv)[M::kRows * HD + row]);
+        float sum = 0.0f;
+        v4f o = {0, 0, 0, 0};
+        for (uint32_t i = 0; i < sp.parts; i++) {
+            const float* slot = many_slot<HD>(a, block + i * a.p.n_kv);
+            const float pm = slot[M::kRows * HD + row], pl = slot[M::kRows * HD + M::kRows + row];
+            const float f = pm == -INFINITY ? (pl == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(pm - m);
+            sum += pl * f;
+            o += *reinterpret_cast<const v4f*>(slot + row * HD + d) * f;
+        }
+        if (sum != 0.0f) o /= sum;
+        const uint32_t tk = rr / a.group, hd = it.h * a.group + rr % a.group;
+        *reinterpret_cast<v4f*>(a.out + (static_cast<size_t>(w.row0 + tk) * a.n_heads + hd) * HD + d) = o;
+    }
+}
+
 }  // namespace
 
 #define ZLM_PAGED(HD, NAME, Q4)                                                                               \
@@ -839,6 +1247,12 @@ __device__ __forceinline__ void merge_few(const AttnArgs& a, uint32_t grid) {
     }                                                                                                         \
     extern "C" __global__ void __launch_bounds__(256) zlm_paged_merge_few_##NAME##_##HD(AttnArgs a, uint32_t grid) { \
         merge_few<HD, Q4>(a, grid);                                                                           \
+    }                                                                                                         \
+    extern "C" __global__ void __launch_bounds__(256, 2) zlm_paged_attend_many_##NAME##_##HD(AttnArgs a) {    \
+        attend_many<HD, Q4>(a);                                                                               \
+    }                                                                                                         \
+    extern "C" __global__ void __launch_bounds__(256) zlm_paged_merge_many_##NAME##_##HD(AttnArgs a) {        \
+        merge_many<HD, Q4>(a);                                                                                \
     }
 
 ZLM_PAGED(64, f16, false)
