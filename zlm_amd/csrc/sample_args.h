@@ -8,12 +8,13 @@ namespace zlm {
 constexpr uint32_t kSampleSlice = 8192;  // logits of one histogram
 constexpr uint32_t kSampleBins = 512;
 constexpr uint32_t kSampleSlices = 128;  // slices of a row: vocabularies up to 2^20
+constexpr uint32_t kSampleShort = 256;   // tokens of a slice's short list
 
-// A slice of a row: the bin (on the row's absolute grid) of its largest logit and
-// that logit as (key, ~index); best 0: no logit that may be drawn.
+// A slice of a row: its largest logit as (key, ~index) (0: no logit that may be
+// drawn) and its short list, all tokens of its first `bins` bins.
 struct SampleSlice {
-    double top;
     uint64_t best;
+    uint32_t bins, n;
 };
 
 struct SampleArgs {
@@ -27,8 +28,9 @@ struct SampleArgs {
     const float* u;
     int32_t* token;
     float* prob;     // or null
-    uint64_t* hist;  // rows x slices x kSampleBins
-    SampleSlice* info;  // rows x slices
+    uint64_t* hist;      // rows x slices x kSampleBins
+    uint64_t* shorts;    // rows x slices x kSampleShort
+    SampleSlice* info;   // rows x slices
 };
 
 }  // namespace zlm

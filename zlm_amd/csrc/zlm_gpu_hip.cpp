@@ -3044,8 +3044,13 @@ extern "C" bool zlm_gpu_paged_append_enqueue(zlm_device* d, const zlm_paged_cach
     a.eps = eps;
     a.base = freq_base;
     void* args[] = {&a};
-    const unsigned waves = (n_heads + 2 * cache->n_kv_heads + 3) / 4;
-    return launch3(d, k->append, batch->n_tokens, waves, 1, 256, args, "paged append");
+    // A head a wave while rows are few (the call is one memory latency then); a row's
+    // heads in one workgroup where rows alone fill the CUs, so that it forms the
+    // rotation once.
+    const uint64_t most = (n_heads + 2 * static_cast<uint64_t>(cache->n_kv_heads) + 3) / 4;
+    const uint64_t fill = (8ull * d->cus + batch->n_tokens - 1) / batch->n_tokens;
+    const unsigned groups = static_cast<unsigned>(std::min(most, std::max<uint64_t>(fill, 1)));
+    return launch3(d, k->append, batch->n_tokens, groups, 1, 256, args, "paged append");
 }
 
 extern "C" bool zlm_gpu_paged_read_enqueue(zlm_device* d, const zlm_paged_cache* cache, const zlm_paged_batch* batch,
@@ -3137,12 +3142,13 @@ extern "C" bool zlm_gpu_sample_enqueue(zlm_device* d, const float* logits, uint6
     a.stride = stride;
     a.vocab = vocab;
     a.slices = (vocab + zlm::kSampleSlice - 1) / zlm::kSampleSlice;
-    const uint64_t slice_bytes = zlm::kSampleBins * sizeof(uint64_t) + sizeof(zlm::SampleSlice);
+    const uint64_t slice_bytes = (zlm::kSampleBins + zlm::kSampleShort) * sizeof(uint64_t) + sizeof(zlm::SampleSlice);
     // rows of one launch: as many as the scratch has room for
     const uint32_t most = static_cast<uint32_t>(std::min<uint64_t>(kServingScratch / (slice_bytes * a.slices), rows));
     if (!ensure_attn_scratch(d, kServingScratch / sizeof(float), "the sampling scratch")) return false;
     a.hist = reinterpret_cast<uint64_t*>(d->attn_part);
-    a.info = reinterpret_cast<zlm::SampleSlice*>(a.hist + static_cast<size_t>(most) * a.slices * zlm::kSampleBins);
+    a.shorts = a.hist + static_cast<size_t>(most) * a.slices * zlm::kSampleBins;
+    a.info = reinterpret_cast<zlm::SampleSlice*>(a.shorts + static_cast<size_t>(most) * a.slices * zlm::kSampleShort);
     for (uint32_t r = 0; r < rows; r += most) {
         a.rows = std::min(most, rows - r);
         a.logits = logits + r * stride;

@@ -87,10 +87,44 @@ __device__ __forceinline__ size_t head_base(const Paged& p, uint32_t page, uint3
     return (static_cast<size_t>(page) * p.n_kv + h) * head_bytes;
 }
 
+// The value of another lane: its place within the row of 16 by a DPP control, then
+// the neighbouring row and the other half by swaps.
+template <int kCtrl>
+__device__ __forceinline__ double dpp(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(u), kCtrl, 0xf, 0xf, true);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(u >> 32), kCtrl, 0xf, 0xf, true);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+constexpr int kXor1 = 0xb1, kXor2 = 0x4e, kHalfMirror = 0x141, kMirror = 0x140;
+
+template <bool kHalves>  // rows 0 and 1 (2 and 3) exchanged, or the wave's halves
+__device__ __forceinline__ double swapped(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = static_cast<uint32_t>(u), hi = static_cast<uint32_t>(u >> 32);
+    const bool upper = (threadIdx.x & (kHalves ? 32 : 16)) != 0;
+    uint32_t x, y;
+    if constexpr (kHalves) {
+        const auto a = __builtin_amdgcn_permlane32_swap(lo, lo, false, false);
+        const auto b = __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
+        x = upper ? a[0] : a[1];
+        y = upper ? b[0] : b[1];
+    } else {
+        const auto a = __builtin_amdgcn_permlane16_swap(lo, lo, false, false);
+        const auto b = __builtin_amdgcn_permlane16_swap(hi, hi, false, false);
+        x = upper ? a[0] : a[1];
+        y = upper ? b[0] : b[1];
+    }
+    return __builtin_bit_cast(double, static_cast<uint64_t>(y) << 32 | x);
+}
+
 __device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
+    v += dpp<kXor1>(v);
+    v += dpp<kXor2>(v);
+    v += dpp<kHalfMirror>(v);
+    v += dpp<kMirror>(v);
+    v += swapped<false>(v);
+    return v + swapped<true>(v);
 }
 
 // The q4_0 block of 32 values, one a lane of each half wave: d from the first of
@@ -98,8 +132,11 @@ __device__ __forceinline__ double wave_sum(double v) {
 __device__ __forceinline__ uint32_t quantise(double x, uint32_t lane, _Float16* d_out) {
     const double a = __builtin_fabs(x);
     double mx = a;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = __builtin_fmax(mx, __shfl_xor(mx, o));
+    mx = __builtin_fmax(mx, dpp<kXor1>(mx));
+    mx = __builtin_fmax(mx, dpp<kXor2>(mx));
+    mx = __builtin_fmax(mx, dpp<kHalfMirror>(mx));
+    mx = __builtin_fmax(mx, dpp<kMirror>(mx));
+    mx = __builtin_fmax(mx, swapped<false>(mx));
     const uint64_t at = __ballot(a == mx) >> (lane & 32);
     const int first = at & 0xffffffffu ? __builtin_ctz(static_cast<uint32_t>(at)) : 0;
     const double m = __shfl(x, static_cast<int>(lane & 32) + first);
@@ -116,95 +153,104 @@ __device__ __forceinline__ uint32_t quantise(double x, uint32_t lane, _Float16* 
     return static_cast<uint32_t>(__builtin_fmin(__builtin_fmax(n, 0.0), 15.0));
 }
 
-// One wave: one row's head (or several, `waves` apart).  A lane holds dims lane +
-// 64 j; the rotation's pair (i, i + hd/2) is in one lane for hd 128 and 256 and in
-// lanes i and i + 32 for hd 64.  Angles, norm, rotation and the 4-bit decisions are
-// formed in 64 bits: a rounding of the angle at position 1e5 in 32 bits is 4e-3.
+// A workgroup: one row; its waves (and those of the row's other workgroups) deal the
+// heads.  A lane holds dims lane + 64 j; the rotation's pair (i, i + hd/2) is in one
+// lane for hd 128 and 256 and in lanes i and i + 32 for hd 64.  Angles, norm,
+// rotation and the 4-bit decisions are formed in 64 bits: a rounding of the angle at
+// position 1e5 in 32 bits is 4e-3.  The angles' functions are most of the
+// arithmetic; the workgroup forms them once for all of its heads.
 // V's 8-position groups are written by the wave of the group's first row in this
 // call, which takes the group's other rows along: no two waves write one word.
 template <int HD, bool Q4>
 __device__ __forceinline__ void append(const AppendArgs& a) {
     const Paged& p = a.p;
     constexpr int N = HD / 64;  // dims a lane
-    const uint32_t lane = threadIdx.x & (kWave - 1);
+    __shared__ double turns[2][HD / 2];
+    const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1);
     const uint32_t t = blockIdx.x;
+    const uint32_t waves = gridDim.y * 4;
+    uint32_t h = __builtin_amdgcn_readfirstlane(blockIdx.y * 4 + tid / kWave);
+    const uint32_t heads = a.n_heads + p.n_kv;
+    const float* row = a.qkv + t * a.stride + lane;
+    float next[N];  // the next head's values, on their way while this one's are worked on
+#pragma unroll
+    for (int j = 0; j < N; j++) next[j] = h < heads ? row[static_cast<size_t>(h) * HD + 64 * j] : 0.0f;
     RowAt at;
     if (!row_at(p, t, lane, at)) return;  // a row behind the last sequence: left as it was
     const uint32_t s = at.s;
     const int32_t pos = at.pos;
     const uint32_t page = 1u << p.page_shift;
-    const uint32_t waves = gridDim.y * (blockDim.x / kWave);
-    uint32_t h = blockIdx.y * (blockDim.x / kWave) + threadIdx.x / kWave;
-    const uint32_t heads = a.n_heads + p.n_kv;
-    if (h < heads) {
-        const int32_t id = page_of(p, s, pos);
-        // the rotation of this lane's pairs
-        double cs[N], sn[N];
+    const int32_t id = __builtin_amdgcn_readfirstlane(page_of(p, s, pos));
+    if (tid < HD / 2) {
+        const double turn = static_cast<double>(pos) * pow(a.base, static_cast<double>(tid) * (-2.0 / HD));
+        sincos(turn, &turns[1][tid], &turns[0][tid]);
+    }
+    __syncthreads();
+    double cs[N], sn[N];
 #pragma unroll
-        for (int j = 0; j < N; j++) {
-            const uint32_t i = (lane + 64 * j) % (HD / 2);
-            const double turn = static_cast<double>(pos) * pow(a.base, static_cast<double>(i) * (-2.0 / HD));
-            sincos(turn, &sn[j], &cs[j]);
+    for (int j = 0; j < N; j++) {
+        cs[j] = turns[0][(lane + 64 * j) % (HD / 2)];
+        sn[j] = turns[1][(lane + 64 * j) % (HD / 2)];
+    }
+    for (; h < heads; h += waves) {
+        const bool is_q = h < a.n_heads;
+        const float* w = is_q ? a.q_norm : a.k_norm;
+        double x[N], y[N];
+#pragma unroll
+        for (int j = 0; j < N; j++) x[j] = next[j];
+        if (h + waves < heads) {
+#pragma unroll
+            for (int j = 0; j < N; j++) next[j] = row[static_cast<size_t>(h + waves) * HD + 64 * j];
         }
-        for (; h < heads; h += waves) {
-            const bool is_q = h < a.n_heads;
-            const float* src = a.qkv + t * a.stride + static_cast<size_t>(h) * HD;
-            const float* w = is_q ? a.q_norm : a.k_norm;
-            double x[N], y[N];
+        if (w) {
             double ss = 0.0;
 #pragma unroll
-            for (int j = 0; j < N; j++) {
-                x[j] = src[lane + 64 * j];
-                ss += x[j] * x[j];
-            }
-            if (w) {
-                const double inv = 1.0 / sqrt(wave_sum(ss) * (1.0 / HD) + static_cast<double>(a.eps));
+            for (int j = 0; j < N; j++) ss = __builtin_fma(x[j], x[j], ss);
+            const double inv = 1.0 / sqrt(wave_sum(ss) * (1.0 / HD) + static_cast<double>(a.eps));
 #pragma unroll
-                for (int j = 0; j < N; j++) x[j] = x[j] * inv * static_cast<double>(w[lane + 64 * j]);
-            }
+            for (int j = 0; j < N; j++) x[j] = x[j] * inv * static_cast<double>(w[lane + 64 * j]);
+        }
 #pragma unroll
-            for (int j = 0; j < N; j++) {
-                double other;
-                bool upper;
-                if constexpr (HD == 64) {
-                    other = __shfl_xor(x[0], 32);
-                    upper = lane >= 32;
-                } else {
-                    other = x[(j + N / 2) % N];
-                    upper = j >= N / 2;
-                }
-                y[j] = x[j] * cs[j] + (upper ? other : -other) * sn[j];
-            }
-            if (is_q) {
-                float* dst = a.q_out + (static_cast<size_t>(t) * a.n_heads + h) * HD;
-#pragma unroll
-                for (int j = 0; j < N; j++) dst[lane + 64 * j] = pos < 0 ? 0.0f : static_cast<float>(y[j]);
-                continue;
-            }
-            if (id < 0) continue;
-            uint8_t* base = p.k + head_base<HD, Q4>(p, id, h - a.n_heads);
-            const uint32_t off = static_cast<uint32_t>(pos) & (page - 1);
-            if constexpr (!Q4) {
-                _Float16* dst = reinterpret_cast<_Float16*>(base) + off * HD;
-#pragma unroll
-                for (int j = 0; j < N; j++) dst[lane + 64 * j] = static_cast<_Float16>(static_cast<float>(y[j]));
+        for (int j = 0; j < N; j++) {
+            double other;
+            bool upper;
+            if constexpr (HD == 64) {
+                other = swapped<true>(x[0]);
+                upper = lane >= 32;
             } else {
+                other = x[(j + N / 2) % N];
+                upper = j >= N / 2;
+            }
+            y[j] = x[j] * cs[j] + (upper ? other : -other) * sn[j];
+        }
+        if (is_q) {
+            float* dst = a.q_out + (static_cast<size_t>(t) * a.n_heads + h) * HD;
 #pragma unroll
-                for (int j = 0; j < N; j++) {
-                    _Float16 d;
-                    const uint32_t n = quantise(y[j], lane, &d);
-                    const uint32_t hi = __shfl(n, (lane & 32) + ((lane + 16) & 31));
-                    const uint32_t blk = 2 * j + lane / 32, e = lane & 31;
-                    if (e < 16) base[off * (HD / 2) + blk * 16 + e] = static_cast<uint8_t>(n | (hi << 4));
-                    if (e == 0) reinterpret_cast<_Float16*>(base + page * (HD / 2))[off * (HD / 32) + blk] = d;
-                }
+            for (int j = 0; j < N; j++) dst[lane + 64 * j] = pos < 0 ? 0.0f : static_cast<float>(y[j]);
+            continue;
+        }
+        if (id < 0) continue;
+        uint8_t* base = p.k + head_base<HD, Q4>(p, id, h - a.n_heads);
+        const uint32_t off = static_cast<uint32_t>(pos) & (page - 1);
+        if constexpr (!Q4) {
+            _Float16* dst = reinterpret_cast<_Float16*>(base) + off * HD;
+#pragma unroll
+            for (int j = 0; j < N; j++) dst[lane + 64 * j] = static_cast<_Float16>(static_cast<float>(y[j]));
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                _Float16 d;
+                const uint32_t n = quantise(y[j], lane, &d);
+                const uint32_t hi = __shfl(n, (lane & 32) + ((lane + 16) & 31));
+                const uint32_t blk = 2 * j + lane / 32, e = lane & 31;
+                if (e < 16) base[off * (HD / 2) + blk * 16 + e] = static_cast<uint8_t>(n | (hi << 4));
+                if (e == 0) reinterpret_cast<_Float16*>(base + page * (HD / 2))[off * (HD / 32) + blk] = d;
             }
         }
     }
     if (h >= heads + p.n_kv) return;
     // V: the first row of each 8-position group in this call
     if (pos < 0 || ((pos & 7) != 0 && pos != at.first)) return;  // position 0 starts a group too
-    const int32_t id = page_of(p, s, pos);
     if (id < 0) return;
     const uint32_t j0 = static_cast<uint32_t>(pos) & 7;
     const uint32_t n_rows = min(8u - j0, static_cast<uint32_t>(at.row1) - t);
@@ -311,13 +357,23 @@ __device__ __forceinline__ void read_rows(const ReadArgs& a) {
 // power of two of its row's own, so neither part leaves f16's range.
 constexpr uint32_t kUnit = 128;  // positions of a unit of work: 32 for each of a workgroup's 4 waves
 
-__device__ __forceinline__ float max_over_q(float x) {  // over the four lanes of a query row
-    x = __builtin_fmaxf(x, __shfl_xor(x, 16));
-    return __builtin_fmaxf(x, __shfl_xor(x, 32));
+// Over the four lanes of a query row (lane % 16): a swap gives a lane both its own
+// and the other's value, in some order.
+template <class F>
+__device__ __forceinline__ float over_q(float x, const F& f) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const uint32_t a0 = a[0], a1 = a[1];
+    const uint32_t v = __builtin_bit_cast(uint32_t, f(__builtin_bit_cast(float, a0), __builtin_bit_cast(float, a1)));
+    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    const uint32_t b0 = b[0], b1 = b[1];
+    return f(__builtin_bit_cast(float, b0), __builtin_bit_cast(float, b1));
+}
+__device__ __forceinline__ float max_over_q(float x) {
+    return over_q(x, [](float y, float z) { return __builtin_fmaxf(y, z); });
 }
 __device__ __forceinline__ float sum_over_q(float x) {
-    x += __shfl_xor(x, 16);
-    return x + __shfl_xor(x, 32);
+    return over_q(x, [](float y, float z) { return y + z; });
 }
 
 // Eight 4-bit values of a word as f16, in the order nibble 0, 4, 1, 5, 2, 6, 3, 7.

@@ -32,6 +32,7 @@ using Args = zlm::SampleArgs;
 using zlm::SampleSlice;
 constexpr uint32_t kWave = 64, kThreads = 1024;
 constexpr uint32_t kSlice = zlm::kSampleSlice, kBins = zlm::kSampleBins, kSlices = zlm::kSampleSlices;
+constexpr uint32_t kShort = zlm::kSampleShort;
 constexpr uint32_t kPer = kSlice / kThreads;
 constexpr uint32_t kList = 4096;  // tokens that are looked at one by one
 constexpr double kUnit = 17179869184.0;  // 2^34: the weight at a bin's edge
@@ -48,12 +49,10 @@ __device__ __forceinline__ float value_of(uint32_t key) {
     return __builtin_bit_cast(float, key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-// e^z, z in [-1/16, 0]: the series to z^9 (the rest is under 3e-19).
+// e^z, z in [-1/16, 0]: the series to z^6 (the rest is under 8e-13, a fiftieth of
+// the unit that weights are held in).
 __device__ __forceinline__ double exp_small(double z) {
-    double r = 1.0 / 362880;
-    r = __builtin_fma(r, z, 1.0 / 40320);
-    r = __builtin_fma(r, z, 1.0 / 5040);
-    r = __builtin_fma(r, z, 1.0 / 720);
+    double r = 1.0 / 720;
     r = __builtin_fma(r, z, 1.0 / 120);
     r = __builtin_fma(r, z, 1.0 / 24);
     r = __builtin_fma(r, z, 1.0 / 6);
@@ -83,11 +82,13 @@ __device__ __forceinline__ uint64_t wave_max(uint64_t v) {
     return v;
 }
 
-// One slice of a row: its largest logit, and the histogram below it.
+// One slice of a row: its largest logit, the histogram below it, and the short list
+// of the tokens that most draws are decided among.
 __device__ __forceinline__ void slice_hist(const Args& a) {
     __shared__ unsigned long long hist[kBins];
     __shared__ uint64_t best_of[kThreads / kWave];
-    const uint32_t tid = threadIdx.x, s = blockIdx.x, row = blockIdx.y;
+    __shared__ uint32_t ends[kBins / kWave], n_short, n_bins;
+    const uint32_t tid = threadIdx.x, s = blockIdx.x, row = blockIdx.y, lane = tid & (kWave - 1), wid = tid / kWave;
     const float* x = a.logits + row * a.stride;
     const double rate = rate_of(a, row);
     uint32_t key[kPer];
@@ -104,24 +105,58 @@ __device__ __forceinline__ void slice_hist(const Args& a) {
         best = c > best ? c : best;
     }
     best = wave_max(best);
-    if ((tid & (kWave - 1)) == 0) best_of[tid / kWave] = best;
+    if (lane == 0) best_of[wid] = best;
     if (tid < kBins) hist[tid] = 0;
+    if (tid == 0) n_short = n_bins = 0;
     __syncthreads();
 #pragma unroll
     for (uint32_t w = 0; w < kThreads / kWave; w++) best = best_of[w] > best ? best_of[w] : best;
     const size_t at = static_cast<size_t>(row) * a.slices + s;
+    if (best == 0 || rate == 0.0) {
+        if (tid == 0) a.info[at] = {best, 0, 0};
+        return;
+    }
     const double top = __builtin_floor(static_cast<double>(value_of(static_cast<uint32_t>(best >> 32))) * rate);
-    if (tid == 0) a.info[at] = {top, best};
-    if (best == 0 || rate == 0.0) return;
+    uint32_t bin[kPer];
 #pragma unroll
     for (uint32_t j = 0; j < kPer; j++) {
         const double y = static_cast<double>(value_of(key[j])) * rate, b = __builtin_floor(y);
         const double d = top - b;
-        if (key[j] && d < static_cast<double>(kBins))
-            atomicAdd(&hist[static_cast<uint32_t>(d)], (1ull << kCountShift) + weight_of(y, b));
+        bin[j] = kBins;
+        if (key[j] && d < static_cast<double>(kBins)) {
+            bin[j] = static_cast<uint32_t>(d);
+            atomicAdd(&hist[bin[j]], (1ull << kCountShift) + weight_of(y, b));
+        }
     }
     __syncthreads();
-    if (tid < kBins) a.hist[at * kBins + tid] = hist[tid];
+    // the bins that the short list has room for
+    uint32_t c = 0;
+    if (tid < kBins) {
+        const uint64_t h = hist[tid];
+        a.hist[at * kBins + tid] = h;
+        c = static_cast<uint32_t>(h >> kCountShift);
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t y = __shfl_up(c, o);
+            if (static_cast<int>(lane) >= o) c += y;
+        }
+        if (lane == kWave - 1) ends[wid] = c;
+    }
+    __syncthreads();
+    if (tid < kBins) {
+        for (uint32_t w = 0; w < wid; w++) c += ends[w];
+        const uint64_t fits = __ballot(c <= kShort);
+        if (lane == 0 && fits) atomicAdd(&n_bins, static_cast<uint32_t>(__builtin_popcountll(fits)));
+    }
+    __syncthreads();
+    const uint32_t bins = n_bins;
+#pragma unroll
+    for (uint32_t j = 0; j < kPer; j++)
+        if (bin[j] < bins)
+            a.shorts[at * kShort + atomicAdd(&n_short, 1u)] =
+                static_cast<uint64_t>(key[j]) << 32 | ~(s * kSlice + j * kThreads + tid);
+    __syncthreads();
+    if (tid == 0) a.info[at] = {best, bins, n_short};
 }
 
 struct Shared {
@@ -129,13 +164,15 @@ struct Shared {
     double cum[kList];     // their cumulative weights
     double weight[kBins];  // cumulative, all bins up to and with this one
     uint32_t count[kBins];
-    double top[kSlices];  // the slices' shifts below the row's top bin
-    uint32_t need[kSlices];
+    uint64_t best[kSlices];
+    uint32_t shift[kSlices];  // a slice's top bin below the row's (kBins: no tokens with weight)
+    uint32_t bins[kSlices], n_short[kSlices];
+    uint32_t need[kSlices];  // the slices to look through
+    uint32_t n_need;
     uint32_t sub_count[kThreads];
     unsigned long long sub_weight[kThreads];
     double part_w[kThreads / kWave];
     uint32_t part_c[kThreads / kWave];
-    uint64_t best[kThreads / kWave];
     uint32_t n, at, lo, hi;
     double base;
 };
@@ -201,26 +238,38 @@ public:
         : a_(a), sm_(sm), row_(row), rate_(rate), x_(a.logits + row * a.stride), tid_(threadIdx.x) {}
 
     // The slices' histograms as the row's: cumulative counts and weights by bin.
-    __device__ void join() {
-        const SampleSlice* info = a_.info + static_cast<size_t>(row_) * a_.slices;
-        top_ = -INFINITY;
-        for (uint32_t s = 0; s < a_.slices; s++)
-            if (info[s].best) top_ = __builtin_fmax(top_, info[s].top);
-        if (tid_ < a_.slices) sm_.top[tid_] = info[tid_].best ? __builtin_fmin(top_ - info[tid_].top, 1.0 * kBins) : 1.0 * kBins;
+    __device__ __forceinline__ void join(uint64_t best) {
+        best_ = best;
+        top_ = edge_of(static_cast<uint32_t>(best >> 32));
+        if (tid_ < a_.slices) {
+            const uint64_t b = sm_.best[tid_];
+            sm_.shift[tid_] = b ? static_cast<uint32_t>(__builtin_fmin(top_ - edge_of(static_cast<uint32_t>(b >> 32)), 1.0 * kBins)) : kBins;
+        }
         __syncthreads();
+        // the lower half of the threads takes the even slices, the upper the odd ones
+        const uint32_t bin = tid_ % kBins;
         uint32_t c = 0;
         uint64_t w = 0;
-        if (tid_ < kBins) {
-            const uint64_t* hist = a_.hist + static_cast<size_t>(row_) * a_.slices * kBins;
-            for (uint32_t s = 0; s < a_.slices; s++) {
-                const uint32_t shift = static_cast<uint32_t>(sm_.top[s]);
-                if (tid_ < shift) continue;
-                const uint64_t h = hist[static_cast<size_t>(s) * kBins + tid_ - shift];
-                c += static_cast<uint32_t>(h >> kCountShift);
-                w += h & ((1ull << kCountShift) - 1);
-            }
+        const uint64_t* hist = a_.hist + static_cast<size_t>(row_) * a_.slices * kBins;
+#pragma unroll 4
+        for (uint32_t s = tid_ / kBins; s < a_.slices; s += kThreads / kBins) {
+            const uint32_t shift = sm_.shift[s];
+            const uint64_t h = bin >= shift ? hist[static_cast<size_t>(s) * kBins + bin - shift] : 0;
+            c += static_cast<uint32_t>(h >> kCountShift);
+            w += h & ((1ull << kCountShift) - 1);
         }
-        double ww = static_cast<double>(w) * scale_of(tid_);
+        if (tid_ >= kBins) {
+            sm_.sub_count[bin] = c;
+            sm_.sub_weight[bin] = w;
+        }
+        __syncthreads();
+        double ww = 0.0;
+        if (tid_ < kBins) {
+            c += sm_.sub_count[bin];
+            ww = static_cast<double>(w + sm_.sub_weight[bin]) * scale_of(bin);
+        } else {
+            c = 0;
+        }
         block_scan(sm_, c, ww);
         if (tid_ < kBins) {
             sm_.count[tid_] = c;
@@ -229,17 +278,30 @@ public:
         __syncthreads();
     }
 
-    __device__ double total() const { return sm_.weight[kBins - 1]; }
-    __device__ uint32_t tokens() const { return sm_.count[kBins - 1]; }
-    __device__ uint32_t count_to(uint32_t bin) const { return sm_.count[bin]; }
+    __device__ __forceinline__ double total() const { return sm_.weight[kBins - 1]; }
+    __device__ __forceinline__ uint32_t tokens() const { return sm_.count[kBins - 1]; }
+    __device__ __forceinline__ uint32_t count_to(uint32_t bin) const { return sm_.count[bin]; }
 
-    __device__ uint32_t bin_of(uint32_t key) const {  // kBins: below them
-        const double d = top_ - __builtin_floor(static_cast<double>(value_of(key)) * rate_);
+    // The smallest and the largest key of a bin: the border is known to a rounding,
+    // the wave's lanes try the 64 keys around it.
+    __device__ __forceinline__ uint32_t first_key(uint32_t bin) const {
+        const double edge = top_ - static_cast<double>(bin);
+        const double e = __builtin_fmax(__builtin_fmin(edge / rate_, 3.402823466e38), -3.402823466e38);
+        const uint32_t k = key_of(static_cast<float>(e)) - 31 + (tid_ & (kWave - 1));
+        const uint64_t in = __ballot(static_cast<double>(value_of(k)) * rate_ >= edge);
+        return key_of(static_cast<float>(e)) - 31 + (in ? __builtin_ctzll(in) : kWave);
+    }
+    __device__ __forceinline__ uint32_t last_key(uint32_t bin) const {
+        return bin ? first_key(bin - 1) - 1 : static_cast<uint32_t>(best_ >> 32);
+    }
+
+    __device__ __forceinline__ uint32_t bin_of(uint32_t key) const {  // kBins: below them
+        const double d = top_ - edge_of(key);
         return d < 1.0 * kBins ? static_cast<uint32_t>(__builtin_fmax(d, 0.0)) : kBins;
     }
 
     // The first bin by whose end the goal is reached (kBins: none).
-    __device__ uint32_t bin_for(const Goal& g) {
+    __device__ __forceinline__ uint32_t bin_for(const Goal& g) {
         if (g.mode == kKey) return bin_of(g.n);
         const uint32_t b = first_of(sm_, tid_ < kBins && g.reached(sm_.count[tid_ % kBins], sm_.weight[tid_ % kBins]));
         return b < kBins ? b : kBins;
@@ -247,24 +309,25 @@ public:
 
     // The list: tokens of bins g0 .. g1 with keys lo .. hi, sorted, with cumulative
     // weights from `base`.  The caller knows that there are at most kList.
-    __device__ void gather(uint32_t g0, uint32_t g1, uint32_t lo, uint32_t hi, double base) {
+    __device__ __forceinline__ void gather(uint32_t g0, uint32_t g1, uint32_t lo, uint32_t hi, double base) {
         __syncthreads();
         if (tid_ == 0) sm_.n = 0;
-        mark(g0, g1);
-        for (uint32_t s = 0; s < a_.slices; s++) {
-            if (!sm_.need[s]) continue;
-            float x[kPer];
-            load(s, x);
-#pragma unroll
-            for (uint32_t j = 0; j < kPer; j++) {
-                const uint32_t key = key_of(x[j]);
-                if (key < lo || key > hi || !key) continue;
-                const uint32_t b = bin_of(key);
-                if (b < g0 || b > g1) continue;
-                const uint32_t at = atomicAdd(&sm_.n, 1u);
-                if (at < kList) sm_.list[at] = static_cast<uint64_t>(key) << 32 | ~(s * kSlice + j * kThreads + tid_);
-            }
+        mark(g0, g1, true);
+        const auto take = [&](uint32_t key, uint32_t i) {
+            if (key < lo || key > hi) return;
+            const uint32_t at = atomicAdd(&sm_.n, 1u);
+            if (at < kList) sm_.list[at] = static_cast<uint64_t>(key) << 32 | ~i;
+        };
+        // short lists, four slices at a time
+        const uint64_t* shorts = a_.shorts + static_cast<size_t>(row_) * a_.slices * kShort;
+#pragma unroll 4
+        for (uint32_t s = tid_ / kShort; s < a_.slices; s += kThreads / kShort) {
+            const uint32_t shift = sm_.shift[s];
+            if (shift > g1 || g1 - shift >= sm_.bins[s] || tid_ % kShort >= sm_.n_short[s]) continue;
+            const uint64_t t = shorts[static_cast<size_t>(s) * kShort + tid_ % kShort];
+            take(static_cast<uint32_t>(t >> 32), ~static_cast<uint32_t>(t));
         }
+        each_needed([&](uint32_t key, uint32_t i) { take(key, i); });
         __syncthreads();
         n_ = min(sm_.n, kList);
         uint32_t len = 64;
@@ -295,7 +358,7 @@ public:
         __syncthreads();
     }
 
-    __device__ Found find(const Goal& g) {
+    __device__ __forceinline__ Found find(const Goal& g) {
         uint32_t b = bin_for(g);
         if (b >= kBins) {  // all that has weight (a goal missed by a rounding, or a key under all)
             return {0, total()};
@@ -304,40 +367,62 @@ public:
         const double base = b ? sm_.weight[b - 1] : 0.0;
         if (b < g0_ || b > g1_) {
             if (sm_.count[b] - before > kList) return refine(g, b, before, base);
-            gather(b, b, 1, 0xffffffffu, base);
+            gather(b, b, first_key(b), last_key(b), base);
         }
         return in_list(g, g0_ ? sm_.count[g0_ - 1] : 0, g0_ ? sm_.weight[g0_ - 1] : 0.0);
     }
 
-    __device__ double weight_at(uint32_t key) const {
+    __device__ __forceinline__ double weight_at(uint32_t key) const {
         const double y = static_cast<double>(value_of(key)) * rate_, b = __builtin_floor(y);
         return static_cast<double>(weight_of(y, b)) * scale_of(static_cast<uint32_t>(top_ - b));
     }
 
 private:
-    __device__ static double scale_of(uint32_t bin) { return exp(static_cast<double>(bin) * -0.0625) / kUnit; }
+    __device__ __forceinline__ static double scale_of(uint32_t bin) { return exp(static_cast<double>(bin) * -0.0625) / kUnit; }
 
-    __device__ void load(uint32_t s, float x[kPer]) const {
-#pragma unroll
-        for (uint32_t j = 0; j < kPer; j++) {
-            const uint32_t i = s * kSlice + j * kThreads + tid_;
-            x[j] = i < a_.vocab ? x_[i] : -INFINITY;
-        }
+    __device__ __forceinline__ double edge_of(uint32_t key) const {
+        return __builtin_floor(static_cast<double>(value_of(key)) * rate_);
     }
 
-    // Which slices have tokens in bins g0 .. g1 (more than one bin: may have).
-    __device__ void mark(uint32_t g0, uint32_t g1) {
+    // Which slices have tokens in bins g0 .. g1 (more than one bin: may have), but not
+    // (with `beyond`) all of them in their short lists.
+    __device__ __forceinline__ void mark(uint32_t g0, uint32_t g1, bool beyond) {
+        if (tid_ == 0) sm_.n_need = 0;
+        __syncthreads();
         if (tid_ < a_.slices) {
-            const uint32_t shift = static_cast<uint32_t>(sm_.top[tid_]);
-            bool need = shift <= g1;
+            const uint32_t shift = sm_.shift[tid_];
+            bool need = shift <= g1 && !(beyond && g1 - shift < sm_.bins[tid_]);
             if (need && g0 == g1)
                 need = (a_.hist[(static_cast<size_t>(row_) * a_.slices + tid_) * kBins + g0 - shift] >> kCountShift) != 0;
-            sm_.need[tid_] = need;
+            if (need) sm_.need[atomicAdd(&sm_.n_need, 1u)] = tid_;
         }
         __syncthreads();
     }
 
-    __device__ void sort(uint32_t len) {  // largest first; len a power of two
+    // f(key, index) for every logit of the needed slices (key 0: not to be drawn), four
+    // slices' loads in flight at once.
+    template <class F>
+    __device__ __forceinline__ void each_needed(const F& f) const {
+        constexpr uint32_t kAtOnce = 4;
+        const uint32_t n = sm_.n_need;
+        for (uint32_t b = 0; b < n; b += kAtOnce) {
+            float x[kAtOnce][kPer];
+            uint32_t i0[kAtOnce];
+#pragma unroll
+            for (uint32_t g = 0; g < kAtOnce; g++) {
+                i0[g] = b + g < n ? sm_.need[b + g] * kSlice + tid_ : a_.vocab;
+#pragma unroll
+                for (uint32_t j = 0; j < kPer; j++)
+                    x[g][j] = i0[g] + j * kThreads < a_.vocab ? x_[i0[g] + j * kThreads] : -INFINITY;
+            }
+#pragma unroll
+            for (uint32_t g = 0; g < kAtOnce; g++)
+#pragma unroll
+                for (uint32_t j = 0; j < kPer; j++) f(key_of(x[g][j]), i0[g] + j * kThreads);
+        }
+    }
+
+    __device__ __forceinline__ void sort(uint32_t len) {  // largest first; len a power of two
         for (uint32_t size = 2; size <= len; size *= 2)
             for (uint32_t step = size / 2; step > 0; step /= 2) {
                 __syncthreads();
@@ -354,7 +439,7 @@ private:
     }
 
     // The goal in the list, whose tokens come after `before` others with weight `base`.
-    __device__ Found in_list(const Goal& g, uint32_t before, double base) {
+    __device__ __forceinline__ Found in_list(const Goal& g, uint32_t before, double base) {
         __syncthreads();
         if (tid_ == 0) sm_.lo = n_;
         __syncthreads();
@@ -376,33 +461,10 @@ private:
     // A goal in a bin of more than kList tokens: histograms of ever narrower ranges
     // of keys, until the list holds one, or one key is left: then its tokens count
     // in order of their index.
-    __device__ Found refine(const Goal& g, uint32_t b, uint32_t before, double base) {
+    __device__ __forceinline__ Found refine(const Goal& g, uint32_t b, uint32_t before, double base) {
         const double scale = scale_of(b);
-        __syncthreads();
-        if (tid_ == 0) {
-            sm_.lo = 0xffffffffu;
-            sm_.hi = 0;
-        }
-        mark(b, b);
-        uint32_t lo = 0xffffffffu, hi = 0;
-        for (uint32_t s = 0; s < a_.slices; s++) {
-            if (!sm_.need[s]) continue;
-            float x[kPer];
-            load(s, x);
-#pragma unroll
-            for (uint32_t j = 0; j < kPer; j++) {
-                const uint32_t key = key_of(x[j]);
-                if (key && bin_of(key) == b) {
-                    lo = min(lo, key);
-                    hi = max(hi, key);
-                }
-            }
-        }
-        atomicMin(&sm_.lo, lo);
-        atomicMax(&sm_.hi, hi);
-        __syncthreads();
-        lo = sm_.lo;
-        hi = sm_.hi;
+        mark(b, b, false);
+        uint32_t lo = first_key(b), hi = last_key(b);
         if (g.mode == kKey && g.n > hi) return {static_cast<uint64_t>(g.n) << 32, base};
         for (;;) {
             uint32_t sh = 0;
@@ -411,19 +473,12 @@ private:
             sm_.sub_count[tid_] = 0;
             sm_.sub_weight[tid_] = 0;
             __syncthreads();
-            for (uint32_t s = 0; s < a_.slices; s++) {
-                if (!sm_.need[s]) continue;
-                float x[kPer];
-                load(s, x);
-#pragma unroll
-                for (uint32_t j = 0; j < kPer; j++) {
-                    const uint32_t key = key_of(x[j]);
-                    if (key < lo || key > hi) continue;
-                    const double y = static_cast<double>(value_of(key)) * rate_;
-                    atomicAdd(&sm_.sub_count[(hi - key) >> sh], 1u);
-                    atomicAdd(&sm_.sub_weight[(hi - key) >> sh], static_cast<unsigned long long>(weight_of(y, __builtin_floor(y))));
-                }
-            }
+            each_needed([&](uint32_t key, uint32_t) {
+                if (key < lo || key > hi) return;
+                const double y = static_cast<double>(value_of(key)) * rate_;
+                atomicAdd(&sm_.sub_count[(hi - key) >> sh], 1u);
+                atomicAdd(&sm_.sub_weight[(hi - key) >> sh], static_cast<unsigned long long>(weight_of(y, __builtin_floor(y))));
+            });
             __syncthreads();
             const uint32_t own = sm_.sub_count[tid_];
             const double own_w = static_cast<double>(sm_.sub_weight[tid_]);
@@ -457,7 +512,7 @@ private:
     }
 
     // A goal among n tokens of one key.
-    __device__ Found in_ties(const Goal& g, uint32_t b, uint32_t key, uint32_t n, uint32_t before, double base) {
+    __device__ __forceinline__ Found in_ties(const Goal& g, uint32_t b, uint32_t key, uint32_t n, uint32_t before, double base) {
         const double w = weight_at(key);
         uint32_t t = n;  // how many of them the goal takes
         if (g.mode == kKey) return {static_cast<uint64_t>(g.n) << 32, base + (key >= g.n ? n * w : 0.0)};
@@ -471,7 +526,7 @@ private:
         // the t-th in order of index
         uint32_t left = t, at = 0;
         for (uint32_t s = 0; s < a_.slices; s++) {
-            if (!sm_.need[s]) continue;
+            if (sm_.shift[s] > b) continue;
             for (uint32_t j = 0; j < kPer; j++) {
                 const uint32_t i = s * kSlice + j * kThreads + tid_;
                 const bool yes = i < a_.vocab && key_of(x_[i]) == key;
@@ -499,6 +554,7 @@ private:
     const float* x_;
     uint32_t tid_;
     double top_ = 0.0;
+    uint64_t best_ = 0;
     uint32_t n_ = 0, g0_ = 1, g1_ = 0;  // the list's tokens and bins
 };
 
@@ -530,9 +586,17 @@ __device__ __forceinline__ void pick(const Args& a) {
     __shared__ Shared sm;
     const uint32_t tid = threadIdx.x, row = blockIdx.x;
     const double rate = rate_of(a, row);
-    uint64_t best = 0;
-    const SampleSlice* info = a.info + static_cast<size_t>(row) * a.slices;
-    for (uint32_t s = 0; s < a.slices; s++) best = info[s].best > best ? info[s].best : best;
+    if (tid < a.slices) {
+        const SampleSlice s = a.info[static_cast<size_t>(row) * a.slices + tid];
+        sm.best[tid] = s.best;
+        sm.bins[tid] = s.bins;
+        sm.n_short[tid] = s.n;
+    }
+    __syncthreads();
+    const uint32_t lane = tid & (kWave - 1);
+    uint64_t best = lane < a.slices ? sm.best[lane] : 0;
+    if (lane + kWave < a.slices && sm.best[lane + kWave] > best) best = sm.best[lane + kWave];
+    best = wave_max(best);
     if (best == 0 || rate == 0.0) {  // nothing to draw; temperature 0: the largest
         if (tid == 0) {
             a.token[row] = best ? static_cast<int32_t>(~static_cast<uint32_t>(best)) : -1;
@@ -541,7 +605,7 @@ __device__ __forceinline__ void pick(const Args& a) {
         return;
     }
     Row r(a, sm, row, rate);
-    r.join();
+    r.join(best);
     const int32_t k = a.top_k ? a.top_k[row] : 0;
     const float p = a.top_p ? a.top_p[row] : 1.0f, mp = a.min_p ? a.min_p[row] : 0.0f;
     const bool by_k = k > 0 && static_cast<uint32_t>(k) < r.tokens(), by_p = p < 1.0f, by_min = mp > 0.0f;
@@ -553,7 +617,7 @@ __device__ __forceinline__ void pick(const Args& a) {
     if (by_p) last = min(last, r.bin_for({kAtLeast, r.total() * p, 0}));
     if (by_min) last = min(last, r.bin_of(min_key));
     last = min(last, kBins - 1);
-    if (r.count_to(last) <= kList) r.gather(0, last, 1, 0xffffffffu, 0.0);
+    if (r.count_to(last) <= kList) r.gather(0, last, r.first_key(last), r.last_key(0), 0.0);
     // u in [0, 1): what lies outside counts as the nearest that does not
     const double u = __builtin_fminf(__builtin_fmaxf(a.u[row], 0.0f), 0x1.fffffep-1f);
     Found cut = {0, r.total()};  // the last token kept, and the weight of all that are
