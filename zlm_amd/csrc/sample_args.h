@@ -27,10 +27,10 @@ struct SampleArgs {
     const float* min_p;
     const float* u;
     int32_t* token;
-    float* prob;     // or null
-    uint64_t* hist;      // rows x slices x kSampleBins
-    uint64_t* shorts;    // rows x slices x kSampleShort
-    SampleSlice* info;   // rows x slices
+    float* prob;        // or null
+    uint64_t* hist;     // rows x slices x kSampleBins
+    uint64_t* shorts;   // rows x slices x kSampleShort
+    SampleSlice* info;  // rows x slices
 };
 
 }  // namespace zlm

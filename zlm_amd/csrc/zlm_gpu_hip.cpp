@@ -227,6 +227,7 @@ struct zlm_device {
     } paged[2][3];
     hipModule_t sample_mod = nullptr;
     hipFunction_t sample_hist = nullptr;
+    hipFunction_t sample_hist_wide = nullptr;
     hipFunction_t sample_pick = nullptr;
     hipFunction_t synth_blocks = nullptr;
     hipFunction_t synth_f16 = nullptr;
@@ -412,8 +413,13 @@ bool load_kernels(zlm_device* d) {
         }
     const std::string sp = dir + "/zlm_sample_gfx950.hsaco";
     if (!ok(d, hipModuleLoad(&d->sample_mod, sp.c_str()), sp.c_str())) return false;
-    if (!ok(d, hipModuleGetFunction(&d->sample_hist, d->sample_mod, "zlm_sample_hist"), "zlm_sample_hist")) return false;
-    if (!ok(d, hipModuleGetFunction(&d->sample_pick, d->sample_mod, "zlm_sample_pick"), "zlm_sample_pick")) return false;
+    const struct {
+        hipFunction_t* f;
+        const char* name;
+    } sampling[] = {{&d->sample_hist, "zlm_sample_hist"}, {&d->sample_hist_wide, "zlm_sample_hist_wide"},
+                    {&d->sample_pick, "zlm_sample_pick"}};
+    for (const auto& m : sampling)
+        if (!ok(d, hipModuleGetFunction(m.f, d->sample_mod, m.name), m.name)) return false;
     return true;
 }
 
@@ -3142,13 +3148,15 @@ extern "C" bool zlm_gpu_sample_enqueue(zlm_device* d, const float* logits, uint6
     a.stride = stride;
     a.vocab = vocab;
     a.slices = (vocab + zlm::kSampleSlice - 1) / zlm::kSampleSlice;
-    const uint64_t slice_bytes = (zlm::kSampleBins + zlm::kSampleShort) * sizeof(uint64_t) + sizeof(zlm::SampleSlice);
+    const uint64_t row_bytes =
+        a.slices * ((zlm::kSampleBins + zlm::kSampleShort) * sizeof(uint64_t) + sizeof(zlm::SampleSlice));
     // rows of one launch: as many as the scratch has room for
-    const uint32_t most = static_cast<uint32_t>(std::min<uint64_t>(kServingScratch / (slice_bytes * a.slices), rows));
+    const uint32_t most = static_cast<uint32_t>(std::min<uint64_t>(kServingScratch / row_bytes, rows));
     if (!ensure_attn_scratch(d, kServingScratch / sizeof(float), "the sampling scratch")) return false;
+    const size_t all = static_cast<size_t>(most) * a.slices;
     a.hist = reinterpret_cast<uint64_t*>(d->attn_part);
-    a.shorts = a.hist + static_cast<size_t>(most) * a.slices * zlm::kSampleBins;
-    a.info = reinterpret_cast<zlm::SampleSlice*>(a.shorts + static_cast<size_t>(most) * a.slices * zlm::kSampleShort);
+    a.shorts = a.hist + all * zlm::kSampleBins;
+    a.info = reinterpret_cast<zlm::SampleSlice*>(a.shorts + all * zlm::kSampleShort);
     for (uint32_t r = 0; r < rows; r += most) {
         a.rows = std::min(most, rows - r);
         a.logits = logits + r * stride;
@@ -3160,8 +3168,11 @@ extern "C" bool zlm_gpu_sample_enqueue(zlm_device* d, const float* logits, uint6
         a.token = token + r;
         a.prob = prob ? prob + r : nullptr;
         void* args[] = {&a};
-        if (!launch3(d, d->sample_hist, a.slices, a.rows, 1, 1024, args, "sample histogram") ||
-            !launch(d, d->sample_pick, a.rows, 1024, args, "sample"))
+        // up to two slices a CU: 1024 threads each
+        const bool wide = static_cast<uint64_t>(a.slices) * a.rows <= 2ull * d->cus;
+        if (!launch3(d, wide ? d->sample_hist_wide : d->sample_hist, a.slices, a.rows, 1, wide ? 1024 : 256, args,
+                     "sample histogram") ||
+            !launch(d, d->sample_pick, a.rows, 512, args, "sample"))
             return false;
     }
     return true;

@@ -7,8 +7,11 @@
 // x_1 >= x_2 >= ..; every filter keeps a prefix of that order, and the draw takes
 // the first token whose cumulative weight exceeds u times that of the prefix.  So
 // each step asks where a cumulative count or weight is reached, and no sort of the
-// row is needed: a histogram by value answers to within a bin, and only the bin in
-// question is looked at token by token.
+// row is needed.  Two launches:
+//   hist  a histogram by value of each 8192 logits, and the slice's largest tokens
+//   pick  a workgroup a row joins the histograms: they answer to within a bin.  The
+//         tokens of the bins in question are mostly among the slices' largest; else the
+//         workgroup looks the row through for them, once
 //
 // Weights.  y = 16 x / T in 64 bits; bin floor(y), 1/16 of a temperature wide, on a
 // grid that does not depend on the row's maximum, so the slices of a row need no
@@ -30,7 +33,7 @@ namespace {
 
 using Args = zlm::SampleArgs;
 using zlm::SampleSlice;
-constexpr uint32_t kWave = 64, kThreads = 1024;
+constexpr uint32_t kWave = 64, kThreads = 512;  // of a row's workgroup
 constexpr uint32_t kSlice = zlm::kSampleSlice, kBins = zlm::kSampleBins, kSlices = zlm::kSampleSlices;
 constexpr uint32_t kShort = zlm::kSampleShort;
 constexpr uint32_t kPer = kSlice / kThreads;
@@ -49,175 +52,265 @@ __device__ __forceinline__ float value_of(uint32_t key) {
     return __builtin_bit_cast(float, key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-// e^z, z in [-1/16, 0]: the series to z^6 (the rest is under 8e-13, a fiftieth of
-// the unit that weights are held in).
-__device__ __forceinline__ double exp_small(double z) {
-    double r = 1.0 / 720;
-    r = __builtin_fma(r, z, 1.0 / 120);
-    r = __builtin_fma(r, z, 1.0 / 24);
-    r = __builtin_fma(r, z, 1.0 / 6);
-    r = __builtin_fma(r, z, 0.5);
-    r = __builtin_fma(r, z, 1.0);
-    return __builtin_fma(r, z, 1.0);
-}
-
-// The weight of y in its bin, in units of 2^-34.
-__device__ __forceinline__ uint64_t weight_of(double y, double bin) {
-    const double e = exp_small((y - (bin + 1.0)) * 0.0625);
-    const double d = __builtin_fma(e, kUnit, 4503599627370496.0);  // + 2^52: the integer in the low bits
-    return __builtin_bit_cast(uint64_t, d) & 0xfffffffffffffull;
-}
+// The weight of a token that lies f = y - floor(y) above its bin's lower edge,
+// e^((f - 1) / 16) in units of 2^-34: a polynomial of degree 5 through the
+// Chebyshev nodes of [0, 1], good to 5e-14, a six hundredth of the unit.  Its
+// coefficients stay in scalar registers.
+struct Weight {
+    double c[6];
+    __device__ Weight() {
+        const double k[6] = {0.939413062813436,     0.05871331642866946,   0.0018347911054814223,
+                             3.822495502710707e-05, 5.969942951840798e-07, 7.703050641794107e-09};
+#pragma unroll
+        for (int i = 0; i < 6; i++) {
+            c[i] = k[i] * kUnit;
+            asm("" : "+s"(c[i]));
+        }
+    }
+    __device__ __forceinline__ uint64_t operator()(double f) const {
+        double r = __builtin_fma(c[5], f, c[4]);
+        r = __builtin_fma(r, f, c[3]);
+        r = __builtin_fma(r, f, c[2]);
+        r = __builtin_fma(r, f, c[1]);
+        r = __builtin_fma(r, f, c[0]) + 4503599627370496.0;  // + 2^52: the integer in the low bits
+        return __builtin_bit_cast(uint64_t, r) & 0xfffffffffffffull;
+    }
+};
 
 __device__ __forceinline__ double rate_of(const Args& a, uint32_t row) {  // 16 / T; 0: greedy
     const float t = a.temperature ? a.temperature[row] : 1.0f;
     return t > 0.0f ? 16.0 / static_cast<double>(__builtin_fminf(t, 3.402823466e38f)) : 0.0;
 }
 
-__device__ __forceinline__ uint64_t wave_max(uint64_t v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const uint64_t w = __shfl_xor(v, o);
-        v = w > v ? w : v;
-    }
+// Another lane's value by a DPP control; 0 where the control has no source or the
+// row is not in kRows.
+template <int kCtrl, int kRows = 0xf>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), kCtrl, kRows, 0xf, false));
+}
+template <int kCtrl, int kRows = 0xf>
+__device__ __forceinline__ uint64_t dpp(uint64_t v) {
+    return static_cast<uint64_t>(dpp<kCtrl, kRows>(static_cast<uint32_t>(v >> 32))) << 32 | dpp<kCtrl, kRows>(static_cast<uint32_t>(v));
+}
+template <int kCtrl, int kRows = 0xf>
+__device__ __forceinline__ double dpp(double v) {
+    return __builtin_bit_cast(double, dpp<kCtrl, kRows>(__builtin_bit_cast(uint64_t, v)));
+}
+
+// Inclusive sums over the wave: within rows of 16, then row 0's and 2's last to
+// rows 1 and 3, then the lower half's last to the upper.
+template <class T>
+__device__ __forceinline__ T wave_scan(T v) {
+    v += dpp<0x111>(v);
+    v += dpp<0x112>(v);
+    v += dpp<0x114>(v);
+    v += dpp<0x118>(v);
+    v += dpp<0x142, 0xa>(v);
+    return v + dpp<0x143, 0xc>(v);
+}
+
+// The largest of the wave (0 if none is larger), in every lane.
+template <class T>
+__device__ __forceinline__ T wave_max(T v) {
+    const auto more = [&](T w) { v = w > v ? w : v; };
+    more(dpp<0x111>(v));
+    more(dpp<0x112>(v));
+    more(dpp<0x114>(v));
+    more(dpp<0x118>(v));
+    more(dpp<0x142, 0xa>(v));
+    more(dpp<0x143, 0xc>(v));
     return v;
+}
+template <class T>
+__device__ __forceinline__ T last_lane(T v);
+template <>
+__device__ __forceinline__ uint32_t last_lane(uint32_t v) {
+    return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 63));
+}
+template <>
+__device__ __forceinline__ uint64_t last_lane(uint64_t v) {
+    return static_cast<uint64_t>(last_lane(static_cast<uint32_t>(v >> 32))) << 32 | last_lane(static_cast<uint32_t>(v));
+}
+
+// The smallest key of a bin whose lower edge is at y = edge: the border is known to
+// a rounding, the wave's lanes try the 64 keys around it.
+__device__ __forceinline__ uint32_t key_at(double edge, double rate) {
+    const double e = __builtin_fmax(__builtin_fmin(edge / rate, 3.402823466e38), -3.402823466e38);
+    const uint32_t k = key_of(static_cast<float>(e)) - 31;
+    const uint64_t in = __ballot(static_cast<double>(value_of(k + (threadIdx.x & (kWave - 1)))) * rate >= edge);
+    return k + (in ? __builtin_ctzll(in) : kWave);
 }
 
 // One slice of a row: its largest logit, the histogram below it, and the short list
-// of the tokens that most draws are decided among.
+// of the tokens that most draws are decided among.  256 threads hold the slice in
+// registers: eight workgroups a CU are at different steps of it, and all of a
+// slice's loads are in flight at once.  Where there are too few slices for that,
+// 1024 threads a slice finish it sooner.
+template <uint32_t kHistThreads>
 __device__ __forceinline__ void slice_hist(const Args& a) {
-    __shared__ unsigned long long hist[kBins];
-    __shared__ uint64_t best_of[kThreads / kWave];
-    __shared__ uint32_t ends[kBins / kWave], n_short, n_bins;
+    constexpr uint32_t kHistPer = kSlice / kHistThreads, kHistWaves = kHistThreads / kWave;
+    const Weight weight;
+    constexpr uint32_t kCopies = 4;  // neighbouring lanes count apart: equal bins of a wave's lanes collide less
+    __shared__ __attribute__((aligned(16))) unsigned long long hist[kBins][kCopies];
+    __shared__ uint32_t max_of[kHistWaves];
+    __shared__ uint32_t ends[kHistWaves], at_of[kHistWaves], n_short, n_bins;
     const uint32_t tid = threadIdx.x, s = blockIdx.x, row = blockIdx.y, lane = tid & (kWave - 1), wid = tid / kWave;
-    const float* x = a.logits + row * a.stride;
+    const float* from = a.logits + row * a.stride;
     const double rate = rate_of(a, row);
-    uint32_t key[kPer];
-    uint64_t best = 0;
+    float x[kHistPer];
+    if ((s + 1) * kSlice <= a.vocab) {
 #pragma unroll
-    for (uint32_t j = 0; j < kPer; j++) {
-        const uint32_t i = s * kSlice + j * kThreads + tid;
-        key[j] = i < a.vocab ? key_of(x[i]) : 0;
-    }
+        for (uint32_t j = 0; j < kHistPer; j++) x[j] = from[s * kSlice + j * kHistThreads + tid];
+    } else {
 #pragma unroll
-    for (uint32_t j = 0; j < kPer; j++) {
-        const uint32_t i = s * kSlice + j * kThreads + tid;
-        const uint64_t c = key[j] ? static_cast<uint64_t>(key[j]) << 32 | ~i : 0;
-        best = c > best ? c : best;
+        for (uint32_t j = 0; j < kHistPer; j++) {
+            const uint32_t i = s * kSlice + j * kHistThreads + tid;
+            x[j] = i < a.vocab ? from[i] : -INFINITY;
+        }
     }
-    best = wave_max(best);
-    if (lane == 0) best_of[wid] = best;
-    if (tid < kBins) hist[tid] = 0;
+    float mx = -INFINITY;
+#pragma unroll
+    for (uint32_t j = 0; j < kHistPer; j++) {
+        x[j] = x[j] > 3.402823466e38f ? 3.402823466e38f : x[j];  // a NaN stays one: no comparison below holds for it
+        mx = __builtin_fmaxf(mx, x[j]);
+    }
+    const uint32_t wave_key = last_lane(wave_max(key_of(mx)));
+    if (lane == 0) max_of[wid] = wave_key;
+    for (uint32_t i = tid; i < kBins * kCopies; i += kHistThreads) hist[0][i] = 0;
     if (tid == 0) n_short = n_bins = 0;
     __syncthreads();
+    uint32_t best_key = 0;
 #pragma unroll
-    for (uint32_t w = 0; w < kThreads / kWave; w++) best = best_of[w] > best ? best_of[w] : best;
+    for (uint32_t w = 0; w < kHistWaves; w++) best_key = max(best_key, max_of[w]);
+    mx = value_of(best_key);
     const size_t at = static_cast<size_t>(row) * a.slices + s;
+    const uint64_t best = static_cast<uint64_t>(best_key) << 32;
     if (best == 0 || rate == 0.0) {
-        if (tid == 0) a.info[at] = {best, 0, 0};
+        uint32_t first = 0xffffffffu;  // of the largest, for a greedy row
+#pragma unroll
+        for (uint32_t j = kHistPer; j-- > 0;)
+            if (best && x[j] == mx) first = s * kSlice + j * kHistThreads + tid;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) first = min(first, static_cast<uint32_t>(__shfl_xor(first, o)));
+        if (lane == 0) at_of[wid] = first;
+        __syncthreads();
+        if (tid == 0) {
+            for (uint32_t w = 0; w < kHistWaves; w++) first = min(first, at_of[w]);
+            a.info[at] = {best ? best | static_cast<uint32_t>(~first) : 0, 0, 0};
+        }
         return;
     }
-    const double top = __builtin_floor(static_cast<double>(value_of(static_cast<uint32_t>(best >> 32))) * rate);
-    uint32_t bin[kPer];
+    const double top = __builtin_floor(static_cast<double>(mx) * rate);
 #pragma unroll
-    for (uint32_t j = 0; j < kPer; j++) {
-        const double y = static_cast<double>(value_of(key[j])) * rate, b = __builtin_floor(y);
+    for (uint32_t j = 0; j < kHistPer; j++) {
+        const double y = static_cast<double>(x[j]) * rate, b = __builtin_floor(y);
         const double d = top - b;
-        bin[j] = kBins;
-        if (key[j] && d < static_cast<double>(kBins)) {
-            bin[j] = static_cast<uint32_t>(d);
-            atomicAdd(&hist[bin[j]], (1ull << kCountShift) + weight_of(y, b));
-        }
+        if (d < static_cast<double>(kBins)) atomicAdd(&hist[static_cast<uint32_t>(d)][tid % kCopies], (1ull << kCountShift) + weight(y - b));
     }
     __syncthreads();
-    // the bins that the short list has room for
-    uint32_t c = 0;
-    if (tid < kBins) {
-        const uint64_t h = hist[tid];
-        a.hist[at * kBins + tid] = h;
-        c = static_cast<uint32_t>(h >> kCountShift);
+    // the bins that the short list has room for: two a thread
+    uint32_t c0 = 0, c1 = 0;
+    if (tid < kBins / 2) {
+        ulonglong2 h = {0, 0};
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t y = __shfl_up(c, o);
-            if (static_cast<int>(lane) >= o) c += y;
+        for (uint32_t i = 0; i < kCopies; i++) {
+            h.x += hist[2 * tid][i];
+            h.y += hist[2 * tid + 1][i];
         }
-        if (lane == kWave - 1) ends[wid] = c;
+        reinterpret_cast<ulonglong2*>(a.hist + at * kBins)[tid] = h;
+        c0 = static_cast<uint32_t>(h.x >> kCountShift);
+        c1 = static_cast<uint32_t>(h.y >> kCountShift);
     }
+    uint32_t c = wave_scan(c0 + c1);
+    if (lane == kWave - 1) ends[wid] = c;
     __syncthreads();
-    if (tid < kBins) {
-        for (uint32_t w = 0; w < wid; w++) c += ends[w];
-        const uint64_t fits = __ballot(c <= kShort);
-        if (lane == 0 && fits) atomicAdd(&n_bins, static_cast<uint32_t>(__builtin_popcountll(fits)));
-    }
+    for (uint32_t w = 0; w < wid; w++) c += ends[w];
+    const bool two = tid < kBins / 2;
+    const uint32_t fits = __builtin_popcountll(__ballot(two && c - c1 <= kShort)) + __builtin_popcountll(__ballot(two && c <= kShort));
+    if (lane == 0 && fits) atomicAdd(&n_bins, fits);
     __syncthreads();
     const uint32_t bins = n_bins;
+    if (bins) {
+        const float least = value_of(key_at(top - static_cast<double>(bins - 1), rate));
 #pragma unroll
-    for (uint32_t j = 0; j < kPer; j++)
-        if (bin[j] < bins)
-            a.shorts[at * kShort + atomicAdd(&n_short, 1u)] =
-                static_cast<uint64_t>(key[j]) << 32 | ~(s * kSlice + j * kThreads + tid);
+        for (uint32_t j = 0; j < kHistPer; j++)
+            if (x[j] >= least) {
+                const uint32_t to = atomicAdd(&n_short, 1u);
+                if (to < kShort)
+                    a.shorts[at * kShort + to] =
+                        static_cast<uint64_t>(key_of(x[j])) << 32 | static_cast<uint32_t>(~(s * kSlice + j * kHistThreads + tid));
+            }
+    }
     __syncthreads();
-    if (tid == 0) a.info[at] = {best, bins, n_short};
+    if (tid == 0) a.info[at] = {best, n_short <= kShort ? bins : 0, n_short};
 }
 
+constexpr uint32_t kRuns = 4;   // top-k's bin, top-p's, min-p's, the draw's
+constexpr uint32_t kFinal = 64;  // tokens that a wave decides among
+
 struct Shared {
-    uint64_t list[kList];  // tokens of bins g0 .. g1 (or of a key's range), largest first: key, ~index
-    double cum[kList];     // their cumulative weights
-    double weight[kBins];  // cumulative, all bins up to and with this one
+    uint64_t list[kList];   // the tokens of the flagged bins, in no order: key, ~index
+    double weight[kBins];   // cumulative, all bins up to and with this one
     uint32_t count[kBins];
+    double scale[kBins];    // e^(-bin/16) in units of the weights
+    // sums by range of tokens
+    uint32_t sub_count[kThreads];
+    unsigned long long sub_weight[kThreads];
+    uint64_t last[kFinal];
+    uint32_t flags[kBins / 32];
+    float lo[kRuns], hi[kRuns];  // the flagged bins' runs, by value
     uint64_t best[kSlices];
     uint32_t shift[kSlices];  // a slice's top bin below the row's (kBins: no tokens with weight)
     uint32_t bins[kSlices], n_short[kSlices];
-    uint32_t need[kSlices];  // the slices to look through
-    uint32_t n_need;
-    uint32_t sub_count[kThreads];
-    unsigned long long sub_weight[kThreads];
-    double part_w[kThreads / kWave];
-    uint32_t part_c[kThreads / kWave];
-    uint32_t n, at, lo, hi;
-    double base;
+    // what the waves of a scan or search hand on: two sets, used in turn, so that a
+    // wave may start the next while others read the last
+    uint64_t part_w[2][kThreads / kWave];
+    uint32_t part_c[2][kThreads / kWave], part_i[2][kThreads / kWave];
+    uint32_t n, step_n, step_count;
+    uint64_t step_weight;
 };
 
-// Inclusive sums over the workgroup in thread order.
-__device__ __forceinline__ void block_scan(Shared& sm, uint32_t& c, double& w) {
-    const uint32_t lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave;
+// Inclusive sums over the workgroup in thread order.  `turn` alternates.
+__device__ __forceinline__ uint32_t block_scan(Shared& sm, uint32_t& turn, uint32_t c) {
+    const uint32_t wid = threadIdx.x / kWave;
+    turn ^= 1;
+    c = wave_scan(c);
+    if ((threadIdx.x & (kWave - 1)) == kWave - 1) sm.part_c[turn][wid] = c;
+    __syncthreads();
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t cc = __shfl_up(c, o);
-        const double ww = __shfl_up(w, o);
-        if (static_cast<int>(lane) >= o) {
-            c += cc;
-            w += ww;
-        }
-    }
+    for (uint32_t i = 0; i < kThreads / kWave; i++) c += i < wid ? sm.part_c[turn][i] : 0;
+    return c;
+}
+template <class T>  // double or uint64_t
+__device__ __forceinline__ T block_scan(Shared& sm, uint32_t& turn, T w) {
+    const uint32_t wid = threadIdx.x / kWave;
+    turn ^= 1;
+    w = wave_scan(w);
+    if ((threadIdx.x & (kWave - 1)) == kWave - 1) sm.part_w[turn][wid] = __builtin_bit_cast(uint64_t, w);
     __syncthreads();
-    if (lane == kWave - 1) {
-        sm.part_c[wid] = c;
-        sm.part_w[wid] = w;
-    }
-    __syncthreads();
-    uint32_t bc = 0;
-    double bw = 0.0;
-    for (uint32_t i = 0; i < wid; i++) {
-        bc += sm.part_c[i];
-        bw += sm.part_w[i];
-    }
-    c += bc;
-    w = bw + w;
+    T before = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kThreads / kWave; i++) before += i < wid ? __builtin_bit_cast(T, sm.part_w[turn][i]) : T(0);
+    return before + w;
 }
 
-// The first thread of those that say yes, or kThreads.
-__device__ __forceinline__ uint32_t first_of(Shared& sm, bool yes) {
-    __syncthreads();
-    if (threadIdx.x == 0) sm.at = kThreads;
-    __syncthreads();
+constexpr uint32_t kNone = 0xffffffffu;
+
+// The index `i` of the first thread that says yes (i does not fall with the thread), or kNone.
+__device__ __forceinline__ uint32_t first_of(Shared& sm, uint32_t& turn, bool yes, uint32_t i) {
+    turn ^= 1;
     const uint64_t m = __ballot(yes);
-    if (m && (threadIdx.x & (kWave - 1)) == 0) atomicMin(&sm.at, threadIdx.x + __builtin_ctzll(m));
+    const uint32_t own = m ? __builtin_amdgcn_readlane(i, __builtin_ctzll(m)) : kNone;
+    if ((threadIdx.x & (kWave - 1)) == 0) sm.part_i[turn][threadIdx.x / kWave] = own;
     __syncthreads();
-    return sm.at;
+    uint32_t first = kNone;
+#pragma unroll
+    for (uint32_t w = 0; w < kThreads / kWave; w++) first = min(first, sm.part_i[turn][w]);
+    return first;
 }
 
 // What a search looks for.
-enum Mode { kCount, kAtLeast, kMore, kKey };
+enum Mode { kCount, kAtLeast, kMore, kKey };  // kKey: the tokens from a key on
 struct Goal {
     Mode mode;
     double w;      // kAtLeast, kMore: the cumulative weight
@@ -234,63 +327,76 @@ struct Found {
 
 class Row {
 public:
-    __device__ Row(const Args& a, Shared& sm, uint32_t row, double rate)
-        : a_(a), sm_(sm), row_(row), rate_(rate), x_(a.logits + row * a.stride), tid_(threadIdx.x) {}
+    // What pick reads of the row at its start, all in one latency: the histograms and
+    // short lists of the first 32 slices.
+    static constexpr uint32_t kAhead = 32, kSide = kThreads / kShort;
+    struct Ahead {
+        uint64_t hist[kAhead], shorts[kAhead / kSide];
+    };
+    __device__ __forceinline__ static void read_ahead(const Args& a, uint32_t row, uint32_t s0, Ahead& h) {
+        const uint64_t* hist = a.hist + static_cast<size_t>(row) * a.slices * kBins;
+        const uint64_t* shorts = a.shorts + static_cast<size_t>(row) * a.slices * kShort;
+#pragma unroll
+        for (uint32_t j = 0; j < kAhead; j++)
+            h.hist[j] = hist[static_cast<size_t>(min(s0 + j, a.slices - 1)) * kBins + threadIdx.x];
+#pragma unroll
+        for (uint32_t j = 0; j < kAhead / kSide; j++)
+            h.shorts[j] = shorts[static_cast<size_t>(min(s0 + kSide * j + threadIdx.x / kShort, a.slices - 1)) * kShort +
+                                 threadIdx.x % kShort];
+    }
 
-    // The slices' histograms as the row's: cumulative counts and weights by bin.
-    __device__ __forceinline__ void join(uint64_t best) {
-        best_ = best;
-        top_ = edge_of(static_cast<uint32_t>(best >> 32));
+    __device__ __forceinline__ Row(const Args& a, Shared& sm, uint32_t row, double rate, uint64_t best)
+        : a_(a), sm_(sm), row_(row), rate_(rate), x_(a.logits + row * a.stride), tid_(threadIdx.x), best_(best),
+          top_(edge_of(static_cast<uint32_t>(best >> 32))) {
+        static_assert(kThreads == kBins, "a bin a thread");
+        sm_.scale[tid_] = exp(static_cast<double>(tid_) * -0.0625) / kUnit;
+        if (tid_ < kBins / 32) sm_.flags[tid_] = 0;
+        if (tid_ == 0) sm_.n = 0;
         if (tid_ < a_.slices) {
             const uint64_t b = sm_.best[tid_];
-            sm_.shift[tid_] = b ? static_cast<uint32_t>(__builtin_fmin(top_ - edge_of(static_cast<uint32_t>(b >> 32)), 1.0 * kBins)) : kBins;
-        }
-        __syncthreads();
-        // the lower half of the threads takes the even slices, the upper the odd ones
-        const uint32_t bin = tid_ % kBins;
-        uint32_t c = 0;
-        uint64_t w = 0;
-        const uint64_t* hist = a_.hist + static_cast<size_t>(row_) * a_.slices * kBins;
-#pragma unroll 4
-        for (uint32_t s = tid_ / kBins; s < a_.slices; s += kThreads / kBins) {
-            const uint32_t shift = sm_.shift[s];
-            const uint64_t h = bin >= shift ? hist[static_cast<size_t>(s) * kBins + bin - shift] : 0;
-            c += static_cast<uint32_t>(h >> kCountShift);
-            w += h & ((1ull << kCountShift) - 1);
-        }
-        if (tid_ >= kBins) {
-            sm_.sub_count[bin] = c;
-            sm_.sub_weight[bin] = w;
-        }
-        __syncthreads();
-        double ww = 0.0;
-        if (tid_ < kBins) {
-            c += sm_.sub_count[bin];
-            ww = static_cast<double>(w + sm_.sub_weight[bin]) * scale_of(bin);
-        } else {
-            c = 0;
-        }
-        block_scan(sm_, c, ww);
-        if (tid_ < kBins) {
-            sm_.count[tid_] = c;
-            sm_.weight[tid_] = ww;
+            sm_.shift[tid_] =
+                b ? static_cast<uint32_t>(__builtin_fmin(top_ - edge_of(static_cast<uint32_t>(b >> 32)), 1.0 * kBins)) : kBins;
         }
         __syncthreads();
     }
 
-    __device__ __forceinline__ double total() const { return sm_.weight[kBins - 1]; }
-    __device__ __forceinline__ uint32_t tokens() const { return sm_.count[kBins - 1]; }
-    __device__ __forceinline__ uint32_t count_to(uint32_t bin) const { return sm_.count[bin]; }
-
-    // The smallest and the largest key of a bin: the border is known to a rounding,
-    // the wave's lanes try the 64 keys around it.
-    __device__ __forceinline__ uint32_t first_key(uint32_t bin) const {
-        const double edge = top_ - static_cast<double>(bin);
-        const double e = __builtin_fmax(__builtin_fmin(edge / rate_, 3.402823466e38), -3.402823466e38);
-        const uint32_t k = key_of(static_cast<float>(e)) - 31 + (tid_ & (kWave - 1));
-        const uint64_t in = __ballot(static_cast<double>(value_of(k)) * rate_ >= edge);
-        return key_of(static_cast<float>(e)) - 31 + (in ? __builtin_ctzll(in) : kWave);
+    // The slices' histograms as the row's: cumulative counts and weights by bin.
+    __device__ __forceinline__ void join(Ahead& h) {
+        // eight slices at a time through LDS (the list's room), to their places on the row's grid
+        static_assert(8 * kBins <= kList, "room for eight histograms");
+        uint32_t count = 0;
+        uint64_t weight = 0;
+        for (uint32_t s0 = 0; s0 < a_.slices; s0 += kAhead) {
+            if (s0) read_ahead(a_, row_, s0, h);
+#pragma unroll
+            for (uint32_t j0 = 0; j0 < kAhead; j0 += 8) {
+                if (s0 + j0 >= a_.slices) break;
+                __syncthreads();
+#pragma unroll
+                for (uint32_t j = 0; j < 8; j++) sm_.list[j * kBins + tid_] = h.hist[j0 + j];
+                __syncthreads();
+#pragma unroll
+                for (uint32_t j = 0; j < 8; j++) {
+                    const uint32_t s = s0 + j0 + j, shift = sm_.shift[min(s, a_.slices - 1)];
+                    const bool has = s < a_.slices && tid_ >= shift;
+                    const uint64_t x = sm_.list[j * kBins + (has ? tid_ - shift : 0)];
+                    count += has ? static_cast<uint32_t>(x >> kCountShift) : 0;
+                    weight += has ? x & ((1ull << kCountShift) - 1) : 0;
+                }
+            }
+        }
+        const uint32_t c = block_scan(sm_, turn_, count);
+        const double w = block_scan(sm_, turn_, static_cast<double>(weight) * sm_.scale[tid_]);
+        sm_.count[tid_] = c;
+        sm_.weight[tid_] = w;
+        __syncthreads();
     }
+
+    __device__ __forceinline__ double weight_to(uint32_t end) const { return end ? sm_.weight[end - 1] : 0.0; }  // bins under `end`
+    __device__ __forceinline__ uint32_t count_to(uint32_t end) const { return end ? sm_.count[end - 1] : 0; }
+
+    // The smallest and the largest key of a bin.
+    __device__ __forceinline__ uint32_t first_key(uint32_t bin) const { return key_at(top_ - static_cast<double>(bin), rate_); }
     __device__ __forceinline__ uint32_t last_key(uint32_t bin) const {
         return bin ? first_key(bin - 1) - 1 : static_cast<uint32_t>(best_ >> 32);
     }
@@ -302,260 +408,254 @@ public:
 
     // The first bin by whose end the goal is reached (kBins: none).
     __device__ __forceinline__ uint32_t bin_for(const Goal& g) {
-        if (g.mode == kKey) return bin_of(g.n);
-        const uint32_t b = first_of(sm_, tid_ < kBins && g.reached(sm_.count[tid_ % kBins], sm_.weight[tid_ % kBins]));
-        return b < kBins ? b : kBins;
+        return min(first_of(sm_, turn_, g.reached(sm_.count[tid_], sm_.weight[tid_]), tid_), kBins);
     }
 
-    // The list: tokens of bins g0 .. g1 with keys lo .. hi, sorted, with cumulative
-    // weights from `base`.  The caller knows that there are at most kList.
-    __device__ __forceinline__ void gather(uint32_t g0, uint32_t g1, uint32_t lo, uint32_t hi, double base) {
+    // Bins b0 .. b1 are in question.
+    __device__ __forceinline__ void flag(uint32_t b0, uint32_t b1) {
+        if (tid_ >= b0 && tid_ <= b1) atomicOr(&sm_.flags[tid_ / 32], 1u << tid_ % 32);
+    }
+    __device__ __forceinline__ bool flagged(uint32_t bin) const { return sm_.flags[bin / 32] >> bin % 32 & 1; }
+
+    // The number of the flagged bins' tokens.
+    __device__ __forceinline__ uint32_t in_question() {
         __syncthreads();
-        if (tid_ == 0) sm_.n = 0;
-        mark(g0, g1, true);
-        const auto take = [&](uint32_t key, uint32_t i) {
-            if (key < lo || key > hi) return;
-            const uint32_t at = atomicAdd(&sm_.n, 1u);
-            if (at < kList) sm_.list[at] = static_cast<uint64_t>(key) << 32 | ~i;
-        };
-        // short lists, four slices at a time
-        const uint64_t* shorts = a_.shorts + static_cast<size_t>(row_) * a_.slices * kShort;
-#pragma unroll 4
-        for (uint32_t s = tid_ / kShort; s < a_.slices; s += kThreads / kShort) {
-            const uint32_t shift = sm_.shift[s];
-            if (shift > g1 || g1 - shift >= sm_.bins[s] || tid_ % kShort >= sm_.n_short[s]) continue;
-            const uint64_t t = shorts[static_cast<size_t>(s) * kShort + tid_ % kShort];
-            take(static_cast<uint32_t>(t >> 32), ~static_cast<uint32_t>(t));
+        const uint32_t c = block_scan(sm_, turn_, flagged(tid_) ? sm_.count[tid_] - count_to(tid_) : 0);
+        if (tid_ == kThreads - 1) sm_.step_n = c;
+        __syncthreads();
+        return sm_.step_n;
+    }
+
+    __device__ __forceinline__ void put(uint64_t token) {
+        const uint32_t at = atomicAdd(&sm_.n, 1u);
+        if (at < kList) sm_.list[at] = token;
+    }
+
+    // Lists the flagged bins' tokens from the slices' short lists; false where one of
+    // these ends before the last of the bins.
+    __device__ __forceinline__ bool list_shorts(Ahead& h) {
+        const uint32_t lane = tid_ & (kWave - 1), bits = lane < kBins / 32 ? sm_.flags[lane] : 0;
+        const uint32_t last = last_lane(wave_max(bits ? 32 * lane + 31 - __builtin_clz(bits) : 0u));
+        const bool open = tid_ < a_.slices && sm_.shift[tid_] <= last && last - sm_.shift[tid_] >= sm_.bins[tid_];
+        if (first_of(sm_, turn_, open, tid_) != kNone) return false;
+        const uint32_t least = first_key(last);
+        for (uint32_t s0 = 0; s0 < a_.slices; s0 += kAhead) {
+            if (a_.slices > kAhead) read_ahead(a_, row_, s0, h);
+#pragma unroll
+            for (uint32_t j = 0; j < kAhead / kSide; j++) {
+                const uint32_t s = s0 + kSide * j + tid_ / kShort, key = static_cast<uint32_t>(h.shorts[j] >> 32);
+                const bool has = s < a_.slices && tid_ % kShort < sm_.n_short[min(s, a_.slices - 1)];
+                if (!has || key < least) continue;
+                const uint32_t b = bin_of(key);
+                if (b < kBins && flagged(b)) put(h.shorts[j]);
+            }
         }
-        each_needed([&](uint32_t key, uint32_t i) { take(key, i); });
         __syncthreads();
         n_ = min(sm_.n, kList);
-        uint32_t len = 64;
-        while (len < n_) len *= 2;
-        for (uint32_t i = n_ + tid_; i < len; i += kThreads) sm_.list[i] = 0;
-        sort(len);
-        // cumulative weights, a run of tokens a thread
-        const uint32_t per = (n_ + kThreads - 1) / kThreads;
-        double w[kList / kThreads], sum = 0.0;
-#pragma unroll
-        for (uint32_t j = 0; j < kList / kThreads; j++) {
-            const uint32_t i = tid_ * per + j;
-            w[j] = j < per && i < n_ ? weight_at(static_cast<uint32_t>(sm_.list[i] >> 32)) : 0.0;
-            sum += w[j];
-        }
-        uint32_t none = 0;
-        double run = sum;
-        block_scan(sm_, none, run);
-        run = base + (run - sum);
-#pragma unroll
-        for (uint32_t j = 0; j < kList / kThreads; j++) {
-            const uint32_t i = tid_ * per + j;
-            run += w[j];
-            if (j < per && i < n_) sm_.cum[i] = run;
-        }
-        g0_ = g0;
-        g1_ = g1;
-        __syncthreads();
+        return true;
     }
 
-    __device__ __forceinline__ Found find(const Goal& g) {
-        uint32_t b = bin_for(g);
-        if (b >= kBins) {  // all that has weight (a goal missed by a rounding, or a key under all)
-            return {0, total()};
-        }
-        const uint32_t before = b ? sm_.count[b - 1] : 0;
-        const double base = b ? sm_.weight[b - 1] : 0.0;
-        if (b < g0_ || b > g1_) {
-            if (sm_.count[b] - before > kList) return refine(g, b, before, base);
-            gather(b, b, first_key(b), last_key(b), base);
-        }
-        return in_list(g, g0_ ? sm_.count[g0_ - 1] : 0, g0_ ? sm_.weight[g0_ - 1] : 0.0);
-    }
-
-    __device__ __forceinline__ double weight_at(uint32_t key) const {
-        const double y = static_cast<double>(value_of(key)) * rate_, b = __builtin_floor(y);
-        return static_cast<double>(weight_of(y, b)) * scale_of(static_cast<uint32_t>(top_ - b));
-    }
-
-private:
-    __device__ __forceinline__ static double scale_of(uint32_t bin) { return exp(static_cast<double>(bin) * -0.0625) / kUnit; }
-
-    __device__ __forceinline__ double edge_of(uint32_t key) const {
-        return __builtin_floor(static_cast<double>(value_of(key)) * rate_);
-    }
-
-    // Which slices have tokens in bins g0 .. g1 (more than one bin: may have), but not
-    // (with `beyond`) all of them in their short lists.
-    __device__ __forceinline__ void mark(uint32_t g0, uint32_t g1, bool beyond) {
-        if (tid_ == 0) sm_.n_need = 0;
-        __syncthreads();
-        if (tid_ < a_.slices) {
-            const uint32_t shift = sm_.shift[tid_];
-            bool need = shift <= g1 && !(beyond && g1 - shift < sm_.bins[tid_]);
-            if (need && g0 == g1)
-                need = (a_.hist[(static_cast<size_t>(row_) * a_.slices + tid_) * kBins + g0 - shift] >> kCountShift) != 0;
-            if (need) sm_.need[atomicAdd(&sm_.n_need, 1u)] = tid_;
-        }
-        __syncthreads();
-    }
-
-    // f(key, index) for every logit of the needed slices (key 0: not to be drawn), four
-    // slices' loads in flight at once.
-    template <class F>
-    __device__ __forceinline__ void each_needed(const F& f) const {
-        constexpr uint32_t kAtOnce = 4;
-        const uint32_t n = sm_.n_need;
-        for (uint32_t b = 0; b < n; b += kAtOnce) {
-            float x[kAtOnce][kPer];
-            uint32_t i0[kAtOnce];
-#pragma unroll
-            for (uint32_t g = 0; g < kAtOnce; g++) {
-                i0[g] = b + g < n ? sm_.need[b + g] * kSlice + tid_ : a_.vocab;
-#pragma unroll
-                for (uint32_t j = 0; j < kPer; j++)
-                    x[g][j] = i0[g] + j * kThreads < a_.vocab ? x_[i0[g] + j * kThreads] : -INFINITY;
-            }
-#pragma unroll
-            for (uint32_t g = 0; g < kAtOnce; g++)
-#pragma unroll
-                for (uint32_t j = 0; j < kPer; j++) f(key_of(x[g][j]), i0[g] + j * kThreads);
-        }
-    }
-
-    __device__ __forceinline__ void sort(uint32_t len) {  // largest first; len a power of two
-        for (uint32_t size = 2; size <= len; size *= 2)
-            for (uint32_t step = size / 2; step > 0; step /= 2) {
-                __syncthreads();
-                for (uint32_t t = tid_; t < len / 2; t += kThreads) {
-                    const uint32_t i = 2 * t - (t & (step - 1)), j = i + step;
-                    const uint64_t p = sm_.list[i], q = sm_.list[j];
-                    if ((p < q) == ((i & size) == 0)) {
-                        sm_.list[i] = q;
-                        sm_.list[j] = p;
-                    }
+    // Lists the flagged bins' tokens from the row itself.  Four logits a load, 16 loads
+    // in flight; a logit in no run costs two comparisons a run and a bit.
+    __device__ __forceinline__ void list_row() {
+        uint32_t runs = 0, prev = 0;
+        for (uint32_t w = 0; w < kBins / 32; w++) {
+            // runs begin where a bin is flagged and the one before is not
+            const uint32_t bits = sm_.flags[w], begins = bits & ~(bits << 1 | prev >> 31);
+            prev = bits;
+            for (uint32_t m = begins; m; m &= m - 1) {
+                const uint32_t b0 = 32 * w + __builtin_ctz(m);
+                uint32_t b1 = b0;
+                while (b1 + 1 < kBins && flagged(b1 + 1)) b1++;
+                const uint32_t hi = last_key(b0), lo = first_key(b1);
+                if (tid_ == 0 && runs < kRuns) {
+                    sm_.lo[runs] = value_of(lo);
+                    sm_.hi[runs] = hi >= key_of(3.402823466e38f) ? INFINITY : value_of(hi);
                 }
+                runs++;
             }
+        }
+        runs = min(runs, kRuns);
+        __syncthreads();
+        typedef float v4 __attribute__((ext_vector_type(4), aligned(4)));
+        constexpr uint32_t kLoads = 16;
+        const uint32_t n4 = a_.vocab / 4;
+        for (uint32_t c = 0; c < n4; c += kThreads * kLoads) {
+            v4 x[kLoads];
+#pragma unroll
+            for (uint32_t j = 0; j < kLoads; j++)
+                x[j] = *reinterpret_cast<const v4*>(x_ + 4 * static_cast<size_t>(min(c + j * kThreads + tid_, n4 - 1)));
+            uint32_t hit[2] = {0, 0};
+            for (uint32_t r = 0; r < runs; r++) {
+                const float lo = sm_.lo[r], hi = sm_.hi[r];
+#pragma unroll
+                for (uint32_t j = 0; j < kLoads; j++)
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; e++)
+                        hit[j / 8] |= x[j][e] >= lo && x[j][e] <= hi ? 1u << (4 * (j % 8) + e) : 0u;
+            }
+#pragma unroll
+            for (uint32_t h = 0; h < 2; h++)
+                for (uint32_t m = hit[h]; m; m &= m - 1) {
+                    const uint32_t bit = __builtin_ctz(m), v = c + (8 * h + bit / 4) * kThreads + tid_;
+                    if (v < n4) put(static_cast<uint32_t>(~(4 * v + bit % 4)));
+                }
+        }
+        const uint32_t i = 4 * n4 + tid_;  // up to three more
+        if (i < a_.vocab) {
+            bool in = false;
+            for (uint32_t r = 0; r < runs; r++) in = in || (x_[i] >= sm_.lo[r] && x_[i] <= sm_.hi[r]);
+            if (in) put(static_cast<uint32_t>(~i));
+        }
+        __syncthreads();
+        n_ = min(sm_.n, kList);
+        // the keys of those found, all at once
+        for (uint32_t k = tid_; k < n_; k += kThreads)
+            sm_.list[k] |= static_cast<uint64_t>(key_of(x_[static_cast<uint32_t>(~static_cast<uint32_t>(sm_.list[k]))])) << 32;
         __syncthreads();
     }
 
-    // The goal in the list, whose tokens come after `before` others with weight `base`.
-    __device__ __forceinline__ Found in_list(const Goal& g, uint32_t before, double base) {
-        __syncthreads();
-        if (tid_ == 0) sm_.lo = n_;
-        __syncthreads();
-        for (uint32_t i = tid_; i < n_; i += kThreads) {
-            const bool yes = g.mode == kKey ? static_cast<uint32_t>(sm_.list[i] >> 32) < g.n
-                                            : g.reached(before + i + 1, sm_.cum[i]);
-            if (yes) atomicMin(&sm_.lo, i);
+    // f(token) for the listed tokens, or for all of the row that may be drawn.
+    template <class F>
+    __device__ __forceinline__ void each(bool listed, const F& f) const {
+        if (listed) {
+            for (uint32_t i = tid_; i < n_; i += kThreads) f(sm_.list[i]);
+            return;
         }
-        __syncthreads();
-        uint32_t i = sm_.lo;
-        if (g.mode == kKey) {  // i: the first that is too small
-            if (i == 0) return {static_cast<uint64_t>(g.n) << 32, base};
-            return {static_cast<uint64_t>(g.n) << 32, sm_.cum[i - 1]};
+        for (uint32_t i0 = tid_; i0 < a_.slices * kSlice; i0 += kSlice) {
+            float x[kPer];
+#pragma unroll
+            for (uint32_t j = 0; j < kPer; j++) x[j] = x_[min(i0 + j * kThreads, a_.vocab - 1)];
+#pragma unroll
+            for (uint32_t j = 0; j < kPer; j++) {
+                const uint32_t i = i0 + j * kThreads, key = i < a_.vocab ? key_of(x[j]) : 0;
+                if (key) f(static_cast<uint64_t>(key) << 32 | static_cast<uint32_t>(~i));
+            }
         }
-        if (i >= n_) i = n_ - 1;
-        return {sm_.list[i], sm_.cum[i]};
     }
 
-    // A goal in a bin of more than kList tokens: histograms of ever narrower ranges
-    // of keys, until the list holds one, or one key is left: then its tokens count
-    // in order of their index.
-    __device__ __forceinline__ Found refine(const Goal& g, uint32_t b, uint32_t before, double base) {
-        const double scale = scale_of(b);
-        mark(b, b, false);
-        uint32_t lo = first_key(b), hi = last_key(b);
-        if (g.mode == kKey && g.n > hi) return {static_cast<uint64_t>(g.n) << 32, base};
-        for (;;) {
-            uint32_t sh = 0;
-            while (((hi - lo) >> sh) >= kThreads) sh++;
+    // Where a goal is reached.  Its bin's tokens, among those listed or in the row, are
+    // counted and weighed in 512 equal ranges of (key, ~index); so again those of the
+    // range in which it is reached, until they are few; a wave decides among these.  In
+    // a bin the weights are whole numbers, so every sum here is exact.
+    __device__ __forceinline__ Found find(const Goal& g, bool listed) {
+        const uint32_t b = g.mode == kKey ? bin_of(g.n) : bin_for(g);
+        if (b >= kBins) return {0, weight_to(kBins)};  // a key under all that has weight
+        const double base = weight_to(b), scale = sm_.scale[b];
+        const uint32_t before = count_to(b);
+        if (g.mode == kKey && !flagged(b)) {
+            // min-p's border in a bin that is in no question: another filter cuts before it
+            return {static_cast<uint64_t>(g.n) << 32, base};
+        }
+        uint64_t lo = static_cast<uint64_t>(first_key(b)) << 32, hi = static_cast<uint64_t>(last_key(b)) << 32 | 0xffffffffu;
+        uint32_t count = 0;   // of the bin's tokens above hi
+        uint64_t weight = 0;  // theirs
+        uint32_t n = sm_.count[b] - before;
+        if (g.mode == kKey) {
+            // the weight of the bin's tokens from the key on
+            lo = static_cast<uint64_t>(g.n) << 32;
+            uint64_t w = 0;
+            each(listed, [&](uint64_t t) {
+                if (t >= lo && t <= hi) w += weight_of(t);
+            });
+            w = block_scan(sm_, turn_, w);
+            __syncthreads();
+            if (tid_ == kThreads - 1) sm_.step_weight = w;
+            __syncthreads();
+            return {lo, base + static_cast<double>(sm_.step_weight) * scale};
+        }
+        while (n > kFinal) {
+            const uint32_t sh = max(64 - __builtin_clzll(hi - lo | 511), 9) - 9;  // (hi - lo) >> sh < 512
             __syncthreads();
             sm_.sub_count[tid_] = 0;
             sm_.sub_weight[tid_] = 0;
             __syncthreads();
-            each_needed([&](uint32_t key, uint32_t) {
-                if (key < lo || key > hi) return;
-                const double y = static_cast<double>(value_of(key)) * rate_;
-                atomicAdd(&sm_.sub_count[(hi - key) >> sh], 1u);
-                atomicAdd(&sm_.sub_weight[(hi - key) >> sh], static_cast<unsigned long long>(weight_of(y, __builtin_floor(y))));
+            each(listed, [&](uint64_t t) {
+                if (t < lo || t > hi) return;
+                const uint32_t at = static_cast<uint32_t>((hi - t) >> sh);
+                atomicAdd(&sm_.sub_count[at], 1u);
+                atomicAdd(&sm_.sub_weight[at], static_cast<unsigned long long>(weight_of(t)));
             });
             __syncthreads();
             const uint32_t own = sm_.sub_count[tid_];
-            const double own_w = static_cast<double>(sm_.sub_weight[tid_]);
-            uint32_t c = own;
-            double w = own_w;  // whole numbers under 2^54, sums exact to 2^53
-            block_scan(sm_, c, w);
-            uint32_t at;
-            if (g.mode == kKey) at = g.n > lo ? (hi - g.n) >> sh : (hi - lo) >> sh;
-            else at = first_of(sm_, own && g.reached(before + c, base + w * scale));
-            if (at == kThreads) at = (hi - lo) >> sh;
-            __syncthreads();
+            const uint64_t own_w = sm_.sub_weight[tid_];
+            const uint32_t c = count + block_scan(sm_, turn_, own);
+            const uint64_t w = weight + block_scan(sm_, turn_, own_w);
+            uint32_t at = first_of(sm_, turn_, own && g.reached(before + c, base + static_cast<double>(w) * scale), tid_);
+            if (at == kNone)  // missed by a rounding: the last token
+                at = kThreads - 1 - first_of(sm_, turn_, sm_.sub_count[kThreads - 1 - tid_] != 0, tid_);
             if (tid_ == at) {
-                sm_.n = own;
-                sm_.lo = before + c - own;
-                sm_.base = base + (w - own_w) * scale;
+                sm_.step_n = own;
+                sm_.step_count = c - own;
+                sm_.step_weight = w - own_w;
             }
             __syncthreads();
-            const uint32_t n = sm_.n;
-            before = sm_.lo;
-            base = sm_.base;
-            hi -= at << sh;
-            lo = max(lo, hi - ((1u << sh) - 1));
-            if (n <= kList) {
-                gather(b, b, lo, hi, base);
-                g0_ = 1;  // the list is no whole bin's
-                g1_ = 0;
-                return in_list(g, before, base);
-            }
-            if (sh == 0) return in_ties(g, b, lo, n, before, base);
+            n = sm_.step_n;
+            count = sm_.step_count;
+            weight = sm_.step_weight;
+            hi -= static_cast<uint64_t>(at) << sh;
+            const uint64_t width = (1ull << sh) - 1;
+            if (hi - lo > width) lo = hi - width;
         }
-    }
-
-    // A goal among n tokens of one key.
-    __device__ __forceinline__ Found in_ties(const Goal& g, uint32_t b, uint32_t key, uint32_t n, uint32_t before, double base) {
-        const double w = weight_at(key);
-        uint32_t t = n;  // how many of them the goal takes
-        if (g.mode == kKey) return {static_cast<uint64_t>(g.n) << 32, base + (key >= g.n ? n * w : 0.0)};
-        if (g.mode == kCount) {
-            t = g.n - before;
-        } else {
-            t = static_cast<uint32_t>(__builtin_fmin(__builtin_fmax((g.w - base) / w - 2.0, 0.0), 1.0 * n - 1)) + 1;
-            while (t < n && !g.reached(0, base + t * w)) t++;
-        }
-        t = min(max(t, 1u), n);
-        // the t-th in order of index
-        uint32_t left = t, at = 0;
-        for (uint32_t s = 0; s < a_.slices; s++) {
-            if (sm_.shift[s] > b) continue;
-            for (uint32_t j = 0; j < kPer; j++) {
-                const uint32_t i = s * kSlice + j * kThreads + tid_;
-                const bool yes = i < a_.vocab && key_of(x_[i]) == key;
-                uint32_t c = yes;
-                double none = 0.0;
-                block_scan(sm_, c, none);
-                const uint32_t hit = first_of(sm_, yes && c == left);
-                if (hit < kThreads) {
-                    at = s * kSlice + j * kThreads + hit;
-                    return {static_cast<uint64_t>(key) << 32 | ~at, base + t * w};
-                }
-                __syncthreads();
-                if (tid_ == kThreads - 1) sm_.lo = c;
-                __syncthreads();
-                left -= sm_.lo;
+        __syncthreads();
+        if (tid_ == 0) sm_.step_n = 0;
+        __syncthreads();
+        each(listed, [&](uint64_t t) {
+            if (t < lo || t > hi) return;
+            const uint32_t at = atomicAdd(&sm_.step_n, 1u);
+            if (at < kFinal) sm_.last[at] = t;
+        });
+        __syncthreads();
+        n = min(sm_.step_n, kFinal);
+        const uint32_t lane = tid_ & (kWave - 1);
+        const uint64_t own = lane < n ? sm_.last[lane] : 0, own_w = lane < n ? weight_of(own) : 0;
+        uint32_t c = count;
+        uint64_t w = weight;
+        for (uint32_t j = 0; j < n; j++) {  // lane j's token before this one, or itself
+            const uint64_t t = lane_of(own, j), tw = lane_of(own_w, j);
+            if (t >= own) {
+                c++;
+                w += tw;
             }
         }
-        return {static_cast<uint64_t>(key) << 32 | ~at, base + t * w};
+        const bool yes = lane < n && g.reached(before + c, base + static_cast<double>(w) * scale);
+        // the largest that reaches it; where none does (a rounding), the smallest of all
+        const uint64_t most = last_lane(wave_max(yes ? own : 0)), least = ~last_lane(wave_max(lane < n ? ~own : 0));
+        const uint64_t token = most ? most : least;
+        const uint64_t at = __ballot(own == token && lane < n);
+        const uint64_t sum = lane_of(w, at ? __builtin_ctzll(at) : 0);
+        __syncthreads();
+        return {token, base + static_cast<double>(sum) * scale};
     }
 
-    const Args& a_;
+    // A token's weight as the sums hold it.
+    __device__ __forceinline__ double weight_at(uint64_t token) const {
+        return static_cast<double>(weight_of(token)) * sm_.scale[min(bin_of(static_cast<uint32_t>(token >> 32)), kBins - 1)];
+    }
+
+private:
+    __device__ __forceinline__ double edge_of(uint32_t key) const {
+        return __builtin_floor(static_cast<double>(value_of(key)) * rate_);
+    }
+    __device__ __forceinline__ uint64_t weight_of(uint64_t token) const {  // in its bin's units
+        const double y = static_cast<double>(value_of(static_cast<uint32_t>(token >> 32))) * rate_;
+        return weight_(y - __builtin_floor(y));
+    }
+    __device__ __forceinline__ static uint64_t lane_of(uint64_t v, uint32_t lane) {
+        return static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), lane))) << 32 |
+               static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane));
+    }
+
+    const Args a_;
     Shared& sm_;
     uint32_t row_;
     double rate_;
     const float* x_;
     uint32_t tid_;
-    double top_ = 0.0;
-    uint64_t best_ = 0;
-    uint32_t n_ = 0, g0_ = 1, g1_ = 0;  // the list's tokens and bins
+    uint64_t best_;
+    double top_;
+    const Weight weight_;
+    uint32_t turn_ = 0, n_ = 0;  // n_: tokens listed
 };
 
 // The smallest key that min-p keeps: e^((x - max) / T) >= p (p in (0, 1]).  The
@@ -582,10 +682,37 @@ __device__ __forceinline__ uint32_t min_p_key(float top, double rate, double p) 
     return hi;
 }
 
-__device__ __forceinline__ void pick(const Args& a) {
-    __shared__ Shared sm;
-    const uint32_t tid = threadIdx.x, row = blockIdx.x;
-    const double rate = rate_of(a, row);
+// The filters of a row, and their parameters as loaded.
+struct Filters {
+    bool by_k, by_p, by_min;
+    uint32_t k, min_key;
+    double p, u;
+};
+struct Params {
+    int32_t k;
+    float p, min_p, u;
+};
+
+__device__ __forceinline__ Params params_of(const Args& a, uint32_t row) {
+    return {a.top_k ? a.top_k[row] : 0, a.top_p ? a.top_p[row] : 1.0f, a.min_p ? a.min_p[row] : 0.0f, a.u[row]};
+}
+
+__device__ __forceinline__ Filters filters_of(const Params& p, double rate, uint64_t best) {
+    Filters f;
+    f.k = static_cast<uint32_t>(p.k);
+    f.p = p.p;
+    f.by_k = p.k > 0;
+    f.by_p = p.p < 1.0f;
+    f.by_min = p.min_p > 0.0f;
+    f.min_key = f.by_min ? min_p_key(value_of(static_cast<uint32_t>(best >> 32)), rate, __builtin_fminf(p.min_p, 1.0f)) : 1;
+    // u in [0, 1): what lies outside counts as the nearest that does not
+    f.u = __builtin_fminf(__builtin_fmaxf(p.u, 0.0f), 0x1.fffffep-1f);
+    return f;
+}
+
+// A row's slices into LDS; its largest token.
+__device__ __forceinline__ uint64_t row_info(const Args& a, Shared& sm, uint32_t row) {
+    const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1);
     if (tid < a.slices) {
         const SampleSlice s = a.info[static_cast<size_t>(row) * a.slices + tid];
         sm.best[tid] = s.best;
@@ -593,10 +720,19 @@ __device__ __forceinline__ void pick(const Args& a) {
         sm.n_short[tid] = s.n;
     }
     __syncthreads();
-    const uint32_t lane = tid & (kWave - 1);
     uint64_t best = lane < a.slices ? sm.best[lane] : 0;
     if (lane + kWave < a.slices && sm.best[lane + kWave] > best) best = sm.best[lane + kWave];
-    best = wave_max(best);
+    return last_lane(wave_max(best));
+}
+
+__device__ __forceinline__ void pick(const Args& a) {
+    __shared__ Shared sm;
+    const uint32_t tid = threadIdx.x, row = blockIdx.x;
+    const Params params = params_of(a, row);
+    const double rate = rate_of(a, row);
+    Row::Ahead ahead;
+    if (rate != 0.0) Row::read_ahead(a, row, 0, ahead);
+    const uint64_t best = row_info(a, sm, row);
     if (best == 0 || rate == 0.0) {  // nothing to draw; temperature 0: the largest
         if (tid == 0) {
             a.token[row] = best ? static_cast<int32_t>(~static_cast<uint32_t>(best)) : -1;
@@ -604,49 +740,65 @@ __device__ __forceinline__ void pick(const Args& a) {
         }
         return;
     }
-    Row r(a, sm, row, rate);
-    r.join(best);
-    const int32_t k = a.top_k ? a.top_k[row] : 0;
-    const float p = a.top_p ? a.top_p[row] : 1.0f, mp = a.min_p ? a.min_p[row] : 0.0f;
-    const bool by_k = k > 0 && static_cast<uint32_t>(k) < r.tokens(), by_p = p < 1.0f, by_min = mp > 0.0f;
-    const uint32_t min_key =
-        by_min ? min_p_key(value_of(static_cast<uint32_t>(best >> 32)), rate, __builtin_fmin(mp, 1.0f)) : 1;
-    // the bins that any filter may leave: where they hold few tokens, all of these are listed at once
-    uint32_t last = kBins;
-    if (by_k) last = min(last, r.bin_for({kCount, 0.0, static_cast<uint32_t>(k)}));
-    if (by_p) last = min(last, r.bin_for({kAtLeast, r.total() * p, 0}));
-    if (by_min) last = min(last, r.bin_of(min_key));
-    last = min(last, kBins - 1);
-    if (r.count_to(last) <= kList) r.gather(0, last, r.first_key(last), r.last_key(0), 0.0);
-    // u in [0, 1): what lies outside counts as the nearest that does not
-    const double u = __builtin_fminf(__builtin_fmaxf(a.u[row], 0.0f), 0x1.fffffep-1f);
-    Found cut = {0, r.total()};  // the last token kept, and the weight of all that are
-    double p_weight = cut.weight;
+    const Filters f = filters_of(params, rate, best);
+    Row r(a, sm, row, rate, best);
+    r.join(ahead);
+    const double total = r.weight_to(kBins);
+    const bool by_k = f.by_k && f.k < r.count_to(kBins);
+    // The bins in question.  A cut falls within a bin, so the weight that is left after
+    // it lies between two bins' ends, and the next goal in the bins that these make.
+    double w0 = total, w1 = total;
+    if (by_k) {
+        const uint32_t b = r.bin_for({kCount, 0.0, f.k});
+        r.flag(b, b);
+        w0 = r.weight_to(b);
+        w1 = r.weight_to(b + 1);
+    }
+    if (f.by_p) {
+        const uint32_t b0 = r.bin_for({kAtLeast, w0 * f.p, 0}), b1 = min(r.bin_for({kAtLeast, w1 * f.p, 0}), kBins - 1);
+        r.flag(b0, b1);
+        w0 = r.weight_to(min(b0, kBins - 1));
+        w1 = __builtin_fmin(w1, r.weight_to(b1 + 1));
+    }
+    if (f.by_min) {
+        const uint32_t b = r.bin_of(f.min_key);
+        if (b < kBins && r.weight_to(b) < w1) {
+            r.flag(b, b);
+            w0 = __builtin_fmin(w0, r.weight_to(b));
+            w1 = __builtin_fmin(w1, r.weight_to(b + 1));
+        }
+    }
+    r.flag(r.bin_for({kMore, w0 * f.u, 0}), min(r.bin_for({kMore, w1 * f.u, 0}), kBins - 1));
+    const bool listed = r.in_question() <= kList;
+    if (listed && !r.list_shorts(ahead)) r.list_row();
+    // the filters in turn, then the draw
+    Found cut = {0, total};  // the last token kept, and the weight of all that are
+    double p_weight = total;
     for (int step = 0; step < 4; step++) {
-        Goal g = {kMore, cut.weight * u, 0};  // the draw
+        Goal g = {kMore, cut.weight * f.u, 0};  // the draw
         if (step == 0) {
             if (!by_k) continue;
-            g = {kCount, 0.0, static_cast<uint32_t>(k)};
+            g = {kCount, 0.0, f.k};
         } else if (step == 1) {
-            p_weight = cut.weight * p;  // top-p is of what top-k left
-            if (!by_min || min_key <= cut.token >> 32) continue;
-            g = {kKey, 0.0, min_key};
+            p_weight = cut.weight * f.p;  // top-p is of what top-k left
+            if (!f.by_min || f.min_key <= cut.token >> 32) continue;
+            g = {kKey, 0.0, f.min_key};
         } else if (step == 2) {
-            if (!by_p || p_weight >= cut.weight) continue;
+            if (!f.by_p || p_weight >= cut.weight) continue;
             g = {kAtLeast, p_weight, 0};
         }
-        const Found f = r.find(g);
+        const Found t = r.find(g, listed);
         if (step < 3) {
-            if (f.token > cut.token) cut = f;
+            if (t.token > cut.token) cut = t;
         } else if (tid == 0) {
-            a.token[row] = static_cast<int32_t>(~static_cast<uint32_t>(f.token));
-            if (a.prob)
-                a.prob[row] = static_cast<float>(r.weight_at(static_cast<uint32_t>(f.token >> 32)) / cut.weight);
+            a.token[row] = static_cast<int32_t>(~static_cast<uint32_t>(t.token));
+            if (a.prob) a.prob[row] = static_cast<float>(r.weight_at(t.token) / cut.weight);
         }
     }
 }
 
 }  // namespace
 
-extern "C" __global__ void __launch_bounds__(1024) zlm_sample_hist(Args a) { slice_hist(a); }
-extern "C" __global__ void __launch_bounds__(1024) zlm_sample_pick(Args a) { pick(a); }
+extern "C" __global__ void __launch_bounds__(256, 8) zlm_sample_hist(Args a) { slice_hist<256>(a); }
+extern "C" __global__ void __launch_bounds__(1024) zlm_sample_hist_wide(Args a) { slice_hist<1024>(a); }
+extern "C" __global__ void __launch_bounds__(512) zlm_sample_pick(Args a) { pick(a); }
