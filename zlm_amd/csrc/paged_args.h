@@ -41,7 +41,8 @@ struct PagedAttend {
     Paged p;
     const float* q;
     float* out;
-    float* part;  // the shares' partial results
+    float* part;       // the shares' partial results
+    uint32_t* counts;  // a counter for every share, 0 between calls
     uint32_t n_heads, group;
     uint32_t window;  // 0: all
     float scale;      // times log2(e)

@@ -223,8 +223,9 @@ struct zlm_device {
     // the paged cache's kernels, by cache type (f16, q4_0) and head size (kPagedDims)
     hipModule_t paged_mod = nullptr;
     struct PagedKernels {
-        hipFunction_t append = nullptr, read = nullptr, few = nullptr, merge_few = nullptr, many = nullptr, merge_many = nullptr;
+        hipFunction_t append = nullptr, read = nullptr, few = nullptr, many = nullptr, merge_many = nullptr;
     } paged[2][3];
+    uint32_t* paged_counts = nullptr;  // the few-row attention's counters, one a workgroup; 0 between calls
     hipModule_t sample_mod = nullptr;
     hipFunction_t sample_hist = nullptr;
     hipFunction_t sample_hist_wide = nullptr;
@@ -404,7 +405,7 @@ bool load_kernels(zlm_device* d) {
             const struct {
                 hipFunction_t* f;
                 const char* name;
-            } fns[] = {{&k.append, "append"}, {&k.read, "read"}, {&k.few, "attend_few"}, {&k.merge_few, "merge_few"},
+            } fns[] = {{&k.append, "append"}, {&k.read, "read"}, {&k.few, "attend_few"},
                        {&k.many, "attend_many"}, {&k.merge_many, "merge_many"}};
             for (const auto& fn : fns) {
                 snprintf(nm, sizeof nm, "zlm_paged_%s_%s_%d", fn.name, t ? "q4_0" : "f16", kPagedDims[i]);
@@ -1842,6 +1843,7 @@ extern "C" void zlm_gpu_deinit(zlm_device* d) {
         if (d->d_y) hipFree(d->d_y);
         if (d->h_y) hipHostFree(d->h_y);
         if (d->attn_part) hipFree(d->attn_part);
+        if (d->paged_counts) hipFree(d->paged_counts);
         if (d->d_mid) hipFree(d->d_mid);
         if (d->d_bx) hipFree(d->d_bx);
         if (d->s_raw) hipFree(d->s_raw);
@@ -3015,6 +3017,23 @@ bool paged_block(zlm_device* d, const zlm_paged_cache* c, const zlm_paged_batch*
     return true;
 }
 
+// The few-row attention's counters: allocated and cleared by the first call, which
+// has to be an eager one.
+bool ensure_paged_counts(zlm_device* d, uint32_t n) {
+    if (d->paged_counts) return true;
+    if (d->capturing) return fail(d, "the attention's counters must be made by an eager call before capture");
+    const std::vector<uint32_t> zero(n, 0u);
+    uint32_t* p = nullptr;
+    if (!ok(d, hipMalloc(reinterpret_cast<void**>(&p), n * sizeof(uint32_t)), "hipMalloc")) return false;
+    if (!ok(d, hipMemcpyAsync(p, zero.data(), n * sizeof(uint32_t), hipMemcpyHostToDevice, d->stream), "upload") ||
+        !ok(d, hipStreamSynchronize(d->stream), "sync")) {
+        hipFree(p);
+        return false;
+    }
+    d->paged_counts = p;
+    return true;
+}
+
 }  // namespace
 
 extern "C" uint64_t zlm_gpu_paged_page_bytes(uint32_t type, uint32_t n_kv_heads, uint32_t head_dim, uint32_t page_size) {
@@ -3089,8 +3108,8 @@ extern "C" bool zlm_gpu_paged_attention_enqueue(zlm_device* d, const zlm_paged_c
         return fail(d, "q and out need 16-byte alignment");
     const uint32_t hd = cache->head_dim, group = n_heads / cache->n_kv_heads;
     const uint64_t tiles = static_cast<uint64_t>(batch->n_tokens) * group / 16 + batch->n_seqs;
-    const uint64_t depth = (static_cast<uint64_t>(batch->table_stride) * cache->page_size) / 128 + 2;
-    if (tiles * cache->n_kv_heads * std::min<uint64_t>(depth, (1u << 24) + 2) >= (1ull << 31))
+    const uint64_t depth = (static_cast<uint64_t>(batch->table_stride) * cache->page_size) / 128 + 4;  // units, and an item's own cost
+    if (tiles * cache->n_kv_heads * std::min<uint64_t>(depth, (1u << 24) + 4) >= (1ull << 31) - 1)
         return fail(d, "attention of %u tokens over up to %u pages a sequence is too large for one call",
                     batch->n_tokens, batch->table_stride);
     // Sequences of more than kFewRows rows go to the many-row kernel.  Which there
@@ -3112,24 +3131,23 @@ extern "C" bool zlm_gpu_paged_attention_enqueue(zlm_device* d, const zlm_paged_c
     const size_t few_part = few ? static_cast<size_t>(grid) * 2 * 16 * (hd + 2) : 0;
     const size_t many_part = splits > 1 ? items * splits * tile_rows * (hd + 2) : 0;
     if (!ensure_attn_scratch(d, std::max({few_part, many_part, kServingScratch / sizeof(float)}))) return false;
+    if (!ensure_paged_counts(d, grid)) return false;
     a.q = q;
     a.out = out;
     a.part = d->attn_part;
+    a.counts = d->paged_counts;
     a.n_heads = n_heads;
     a.group = group;
     a.window = window;
     a.scale = scale * 1.44269504088896340736f;
     a.few_rows = many ? kFewRows : 0xffffffffu;
     a.splits = splits;
-    uint32_t g = grid;
-    void* args[] = {&a, &g};
+    void* args[] = {&a};
     if (many && !(launch(d, k->many, static_cast<uint32_t>(items * splits), 256, args, "paged attention of many rows") &&
                   (splits == 1 || launch3(d, k->merge_many, static_cast<uint32_t>(items), tile_rows / 16, 1, 256, args,
                                           "paged attention of many rows, merge"))))
         return false;
-    if (!few) return true;
-    return launch(d, k->few, grid, 256, args, "paged attention") &&
-           launch(d, k->merge_few, grid - 1, 256, args, "paged attention merge");
+    return !few || launch(d, k->few, grid, 256, args, "paged attention");
 }
 
 // ---- sampling ----

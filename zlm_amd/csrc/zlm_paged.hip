@@ -356,6 +356,10 @@ __device__ __forceinline__ void read_rows(const ReadArgs& a) {
 // has the accuracy of f32 products at half of f16's matrix rate.  q is scaled by a
 // power of two of its row's own, so neither part leaves f16's range.
 constexpr uint32_t kUnit = 128;  // positions of a unit of work: 32 for each of a workgroup's 4 waves
+// What an item costs besides its units, in units: its q and first K and V come one
+// after another, and its sums are joined. Measured at 64 sequences of 820
+// to 8192 positions and 8 heads: 90.3 us with none, 86.6 with two or four, 88.6 with eight.
+constexpr uint32_t kItem = 2;
 
 // Over the four lanes of a query row (lane % 16): a swap gives a lane both its own
 // and the other's value, in some order.
@@ -379,9 +383,12 @@ __device__ __forceinline__ float sum_over_q(float x) {
 // Eight 4-bit values of a word as f16, in the order nibble 0, 4, 1, 5, 2, 6, 3, 7.
 // A nibble in mantissa bits 9..6 of 16.0 is 16 + n; (16 + n) d - 24 d is exact.
 __device__ __forceinline__ v8h decode8(uint32_t w, v2h d0, v2h d1, v2h d2, v2h d3) {
-    constexpr uint32_t kMask = 0x03c003c0u, kOr = 0x4c004c00u;
-    const v2h x0 = __builtin_bit_cast(v2h, ((w << 6) & kMask) | kOr), x1 = __builtin_bit_cast(v2h, ((w << 2) & kMask) | kOr);
-    const v2h x2 = __builtin_bit_cast(v2h, ((w >> 2) & kMask) | kOr), x3 = __builtin_bit_cast(v2h, ((w >> 6) & kMask) | kOr);
+    // one scalar and one vector register: v_and_or_b32 takes no two literals
+    uint32_t mask = 0x03c003c0u, sixteen = 0x4c004c00u;
+    asm("" : "+s"(mask));
+    asm("" : "+v"(sixteen));
+    const auto at = [&](uint32_t x) { return __builtin_bit_cast(v2h, (x & mask) | sixteen); };
+    const v2h x0 = at(w << 6), x1 = at(w << 2), x2 = at(w >> 2), x3 = at(w >> 6);
     const v2h c = {static_cast<_Float16>(-24.0f), static_cast<_Float16>(-24.0f)};
     const v2h y0 = __builtin_elementwise_fma(x0, d0, c * d0), y1 = __builtin_elementwise_fma(x1, d1, c * d1);
     const v2h y2 = __builtin_elementwise_fma(x2, d2, c * d2), y3 = __builtin_elementwise_fma(x3, d3, c * d3);
@@ -392,7 +399,7 @@ __device__ __forceinline__ v8h decode8(uint32_t w, v2h d0, v2h d1, v2h d2, v2h d
 template <int HD, bool Q4>
 struct KRaw {
     uint32_t w[2][HD / 32][Q4 ? 1 : 4];
-    uint16_t d[2][HD / 128 ? HD / 128 : 1];
+    uint32_t d[2][HD / 128 ? HD / 128 : 1];  // a register each: two in one would be waited for where they meet
 };
 template <int HD, bool Q4>
 struct VRaw {
@@ -402,50 +409,83 @@ struct VRaw {
 
 // The pages of a 32-position block: one, or two of 16 positions.  -1: none.
 struct Pages {
-    int32_t id[2];
+    int32_t a, b;
+    __device__ __forceinline__ int32_t of(bool second) const {
+        const int32_t x = a, y = b;
+        return second ? y : x;
+    }
 };
 
-__device__ __forceinline__ Pages pages_at(const Paged& p, uint32_t s, uint32_t kb) {
-    Pages g;
-    g.id[0] = __builtin_amdgcn_readfirstlane(page_of(p, s, static_cast<int32_t>(kb)));
-    g.id[1] = p.page_shift > 4 ? g.id[0] : __builtin_amdgcn_readfirstlane(page_of(p, s, static_cast<int32_t>(kb) + 16));
-    return g;
+// One for all of the wave, by scalar loads: a vector load here would be waited for with
+// all the K and V loads that went out before it.  What the table holds, not looked at
+// yet: that waits for it.
+__device__ __forceinline__ int32_t entry_at(const Paged& p, uint32_t s, uint32_t pos) {
+    const uint32_t i = __builtin_amdgcn_readfirstlane(min(pos >> p.page_shift, p.table_stride - 1));
+    typedef const __attribute__((address_space(4))) int32_t* Table;
+    return ((Table)(uintptr_t)p.table)[static_cast<size_t>(__builtin_amdgcn_readfirstlane(s)) * p.table_stride + i];
+}
+
+__device__ __forceinline__ Pages entries_at(const Paged& p, uint32_t s, uint32_t kb) {
+    return {entry_at(p, s, kb), entry_at(p, s, kb + 16)};
+}
+
+__device__ __forceinline__ Pages pages_of(const Paged& p, const Pages& e, uint32_t kb) {
+    return {static_cast<uint32_t>(e.a) < p.n_pages && kb >> p.page_shift < p.table_stride ? e.a : -1,
+            static_cast<uint32_t>(e.b) < p.n_pages && (kb + 16) >> p.page_shift < p.table_stride ? e.b : -1};
 }
 
 // K position of matrix row m (0..15) of tile t in a 32-position block.
 __device__ __forceinline__ uint32_t k_row(uint32_t m, int t) { return 8 * (m >> 2) + (m & 3) + 4 * t; }
 
+// A lane's addresses in a 32-position block: its K row of tile 0 and its 8 positions
+// of V, and their scales.  Tile 1's K row is the fourth on from tile 0's, in the same
+// page, so all of a block's loads are these and constants.
+struct Spots {
+    const uint8_t *k, *ks, *v, *vs;
+};
+
 template <int HD, bool Q4>
-__device__ __forceinline__ void load_k(const Paged& p, const Pages& g, uint32_t h, uint32_t kb, uint32_t lane,
-                                       KRaw<HD, Q4>& r) {
+__device__ __forceinline__ Spots spots_of(const Paged& p, const Pages& g, uint32_t h, uint32_t kb, uint32_t lane) {
     const uint32_t m = lane & 15, q = lane >> 4, page = 1u << p.page_shift;
-    const size_t b0 = head_base<HD, Q4>(p, max(g.id[0], 0), h), b1 = head_base<HD, Q4>(p, max(g.id[1], 0), h);
-    const uint8_t* base = p.k + (m >= 8 ? b1 : b0);
+    const size_t a = head_base<HD, Q4>(p, max(g.a, 0), h), b = head_base<HD, Q4>(p, max(g.b, 0), h);
+    const size_t kh = m >= 8 ? b : a, vh = q >= 2 ? b : a;
+    const uint32_t row = (kb + k_row(m, 0)) & (page - 1), grp = ((kb + 8 * q) & (page - 1)) >> 3;
+    Spots s;
+    if constexpr (!Q4) {
+        s.k = p.k + (kh + row * (HD * 2) + 16 * q);
+        s.v = p.v + (vh + (grp * HD + m) * 16);
+        s.ks = s.vs = nullptr;
+    } else {
+        s.k = p.k + (kh + row * (HD / 2) + (HD == 64 ? 8 : 16) * q);
+        s.ks = p.k + (kh + page * (HD / 2) + row * (HD / 16) + (HD == 64 ? 2 * (q >> 1) : 2 * q));
+        s.v = p.v + (vh + (grp * HD + 4 * m) * 4);
+        s.vs = p.v + (vh + page * (HD / 2) + (grp * (HD / 32) + (m >> 3)) * 16);
+    }
+    return s;
+}
+
+template <int HD, bool Q4>
+__device__ __forceinline__ void load_k(const Spots& s, KRaw<HD, Q4>& r) {
 #pragma unroll
     for (int t = 0; t < 2; t++) {
-        const uint32_t off = (kb + k_row(m, t)) & (page - 1);
         if constexpr (!Q4) {
 #pragma unroll
             for (int i = 0; i < HD / 32; i++)
-                *reinterpret_cast<v4u*>(r.w[t][i]) = *reinterpret_cast<const v4u*>(base + off * (HD * 2) + 64 * i + 16 * q);
+                *reinterpret_cast<v4u*>(r.w[t][i]) = *reinterpret_cast<const v4u*>(s.k + t * (8 * HD) + 64 * i);
+        } else if constexpr (HD == 64) {  // half of block q / 2
+            const v2u x = *reinterpret_cast<const v2u*>(s.k + t * (2 * HD));
+            r.w[t][0][0] = x.x;
+            r.w[t][1][0] = x.y;
+            r.d[t][0] = *reinterpret_cast<const uint16_t*>(s.ks + t * (HD / 4));
         } else {
-            const uint8_t* row = base + off * (HD / 2);
-            const uint16_t* sc = reinterpret_cast<const uint16_t*>(base + page * (HD / 2)) + off * (HD / 32);
-            if constexpr (HD == 64) {  // half of block q / 2
-                const v2u x = *reinterpret_cast<const v2u*>(row + 8 * q);
-                r.w[t][0][0] = x.x;
-                r.w[t][1][0] = x.y;
-                r.d[t][0] = sc[q >> 1];
-            } else {
 #pragma unroll
-                for (int b = 0; b < HD / 128; b++) {  // block q + 4 b
-                    const v4u x = *reinterpret_cast<const v4u*>(row + 16 * q + 64 * b);
-                    r.w[t][4 * b][0] = x.x;
-                    r.w[t][4 * b + 1][0] = x.y;
-                    r.w[t][4 * b + 2][0] = x.z;
-                    r.w[t][4 * b + 3][0] = x.w;
-                    r.d[t][b] = sc[q + 4 * b];
-                }
+            for (int b = 0; b < HD / 128; b++) {  // block q + 4 b
+                const v4u x = *reinterpret_cast<const v4u*>(s.k + t * (2 * HD) + 64 * b);
+                r.w[t][4 * b][0] = x.x;
+                r.w[t][4 * b + 1][0] = x.y;
+                r.w[t][4 * b + 2][0] = x.z;
+                r.w[t][4 * b + 3][0] = x.w;
+                r.d[t][b] = *reinterpret_cast<const uint16_t*>(s.ks + t * (HD / 4) + 8 * b);
             }
         }
     }
@@ -456,7 +496,7 @@ __device__ __forceinline__ v8h k_operand(const KRaw<HD, Q4>& r, int t, int i) {
     if constexpr (!Q4) {
         return __builtin_bit_cast(v8h, *reinterpret_cast<const v4u*>(r.w[t][i]));
     } else {
-        const _Float16 d = __builtin_bit_cast(_Float16, r.d[t][HD == 64 ? 0 : i / 4]);
+        const _Float16 d = __builtin_bit_cast(_Float16, static_cast<uint16_t>(r.d[t][HD == 64 ? 0 : i / 4]));
         const v2h dd = {d, d};
         return decode8(r.w[t][i][0], dd, dd, dd, dd);
     }
@@ -475,26 +515,19 @@ __device__ __forceinline__ constexpr uint32_t k_dim(uint32_t q, int i, int j) {
 }
 
 template <int HD, bool Q4>
-__device__ __forceinline__ void load_v(const Paged& p, const Pages& g, uint32_t h, uint32_t kb, uint32_t lane,
-                                       VRaw<HD, Q4>& r) {
-    const uint32_t m = lane & 15, q = lane >> 4, page = 1u << p.page_shift;
-    const size_t b0 = head_base<HD, Q4>(p, max(g.id[0], 0), h), b1 = head_base<HD, Q4>(p, max(g.id[1], 0), h);
-    const uint8_t* base = p.v + (q >= 2 ? b1 : b0);
-    const uint32_t grp = ((kb + 8 * q) & (page - 1)) >> 3;
+__device__ __forceinline__ void load_v(const Spots& s, VRaw<HD, Q4>& r) {
     if constexpr (!Q4) {
 #pragma unroll
-        for (int c = 0; c < HD / 16; c++)
-            *reinterpret_cast<v4u*>(r.w[c]) = *reinterpret_cast<const v4u*>(base + (grp * HD + 16 * c + m) * 16);
+        for (int c = 0; c < HD / 16; c++) *reinterpret_cast<v4u*>(r.w[c]) = *reinterpret_cast<const v4u*>(s.v + 256 * c);
     } else {
-        const v4u* sc = reinterpret_cast<const v4u*>(base + page * (HD / 2)) + grp * (HD / 32) + (m >> 3);
 #pragma unroll
         for (int b = 0; b < HD / 64; b++) {  // dims 64 b + 4 m + {0, 1, 2, 3}
-            const v4u x = *reinterpret_cast<const v4u*>(base + (grp * HD + 64 * b + 4 * m) * 4);
+            const v4u x = *reinterpret_cast<const v4u*>(s.v + 256 * b);
             r.w[4 * b][0] = x.x;
             r.w[4 * b + 1][0] = x.y;
             r.w[4 * b + 2][0] = x.z;
             r.w[4 * b + 3][0] = x.w;
-            r.d[b] = sc[2 * b];
+            r.d[b] = *reinterpret_cast<const v4u*>(s.vs + 32 * b);
         }
     }
 }
@@ -547,25 +580,44 @@ struct QTile {
 
 template <int HD, bool Q4>
 __device__ __forceinline__ void load_q(QTile<HD>& qt, const float* row, uint32_t q, float scale) {
+    // the lane's dims, in runs of four
     float x[HD / 32][8];
     float mx = 0.0f;
 #pragma unroll
-    for (int i = 0; i < HD / 32; i++)
+    for (int i = 0; i < HD / 32; i++) {
+        v4f run[2];
+        if constexpr (Q4) {
+            // two runs of a word: elements 4 w .. 4 w + 3 and 16 on, in the order of k_dim
+            const uint32_t d = k_dim<HD, Q4>(q, i, 0);
+            run[0] = *reinterpret_cast<const v4f*>(row + d);
+            run[1] = *reinterpret_cast<const v4f*>(row + d + 16);
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            x[i][j] = row ? row[k_dim<HD, Q4>(q, i, j)] : 0.0f;
-            mx = __builtin_fmaxf(mx, __builtin_fabsf(x[i][j]));
+            for (int j = 0; j < 8; j++) {
+                const int nib = (j >> 1) + 4 * (j & 1);
+                x[i][j] = run[nib & 1][nib / 2];
+            }
+        } else {
+            run[0] = *reinterpret_cast<const v4f*>(row + 32 * i + 8 * q);
+            run[1] = *reinterpret_cast<const v4f*>(row + 32 * i + 8 * q + 4);
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[i][j] = run[j / 4][j % 4];
         }
+#pragma unroll
+        for (int j = 0; j < 8; j++) mx = __builtin_fmaxf(mx, __builtin_fabsf(x[i][j]));
+    }
     mx = max_over_q(mx);
     // the row's largest to [2^13, 2^14); a row of zeros, infinities or NaN stays as it is
     int e = 0;
     if (mx > 0.0f && mx < INFINITY) e = 14 - __builtin_amdgcn_frexp_expf(mx);
-    qt.factor = ldexpf(scale, -e);
+    // the factor is positive: a negative scale's sign goes to q
+    // (and it is not 0, which a masked -inf must not meet)
+    qt.factor = __builtin_fmaxf(ldexpf(__builtin_fabsf(scale), -e), 0x1p-126f);
+    const float sign = scale < 0.0f ? -1.0f : 1.0f;
 #pragma unroll
     for (int i = 0; i < HD / 32; i++)
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const float y = ldexpf(x[i][j], e);
+            const float y = ldexpf(x[i][j] * sign, e);
             const _Float16 a = static_cast<_Float16>(y);
             qt.hi[i][j] = a;
             qt.lo[i][j] = static_cast<_Float16>(y - static_cast<float>(a));
@@ -595,25 +647,25 @@ __device__ __forceinline__ void soft_clear(Soft<HD>& st) {
 
 template <int HD, bool Q4>
 __device__ __forceinline__ void scores(const KRaw<HD, Q4>& k, const QTile<HD>& qt, v4f s[2]) {
+    s[0] = s[1] = v4f{0, 0, 0, 0};
 #pragma unroll
-    for (int t = 0; t < 2; t++) {
-        s[t] = v4f{0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < HD / 32; i++) {
-            const v8h a = k_operand<HD, Q4>(k, t, i);
-            s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qt.hi[i], s[t], 0, 0, 0);
-            s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qt.lo[i], s[t], 0, 0, 0);
-        }
-        s[t] *= qt.factor;
+    for (int i = 0; i < HD / 32; i++) {
+        const v8h a = k_operand<HD, Q4>(k, 0, i), b = k_operand<HD, Q4>(k, 1, i);
+        s[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qt.hi[i], s[0], 0, 0, 0);
+        s[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, qt.hi[i], s[1], 0, 0, 0);
+        s[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qt.lo[i], s[0], 0, 0, 0);
+        s[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, qt.lo[i], s[1], 0, 0, 0);
     }
 }
 
-// s: scores in units of log2; -inf where masked.  Makes the two parts of P.
+// s: products, -inf where masked; times the row's factor they are exponents of two.
+// Makes the two parts of P.
 template <int HD>
-__device__ __forceinline__ void soft_step(Soft<HD>& st, const v4f s[2], v8h& hi, v8h& lo) {
+__device__ __forceinline__ void soft_step(Soft<HD>& st, const v4f s[2], float factor, v8h& hi, v8h& lo) {
     float mx = s[0][0];
 #pragma unroll
     for (int i = 1; i < 8; i++) mx = __builtin_fmaxf(mx, s[i / 4][i % 4]);
+    mx *= factor;  // of 0 or more, so the largest stays it
     if (__any(mx > st.m + kSlack)) {
         mx = __builtin_fmaxf(max_over_q(mx), st.m);
         const float f = st.m == mx ? 1.0f : __builtin_amdgcn_exp2f(st.m - mx);  // -inf stays with -inf
@@ -622,27 +674,40 @@ __device__ __forceinline__ void soft_step(Soft<HD>& st, const v4f s[2], v8h& hi,
 #pragma unroll
         for (int c = 0; c < HD / 16; c++) st.o[c] *= f;
     }
-    const float base = (st.m == -INFINITY ? 0.0f : st.m) - kLift;
-    float sum = 0.0f;
+    const float base = kLift - (st.m == -INFINITY ? 0.0f : st.m);
+    float minus = -1.0f, sum = 0.0f;
+    asm("" : "+v"(minus));  // a constant would become a conversion and a difference
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const float e = __builtin_amdgcn_exp2f(s[i / 4][i % 4] - base);
-        sum += e;
-        const _Float16 a = static_cast<_Float16>(e);
-        hi[i] = a;
-        lo[i] = static_cast<_Float16>(e - static_cast<float>(a));
+    for (int i = 0; i < 8; i += 2) {
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][i % 4], factor, base));
+        const float f = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][i % 4 + 1], factor, base));
+        sum += e + f;
+        // the first part towards zero, two values an instruction; what it leaves is exact
+        // and goes to the second part: 21 bits and more together
+        const v2h x = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(e, f));
+        const v2h y = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf(static_cast<float>(x.x), minus, e),
+                                                                          __builtin_fmaf(static_cast<float>(x.y), minus, f)));
+        hi[i] = x.x;
+        hi[i + 1] = x.y;
+        lo[i] = y.x;
+        lo[i + 1] = y.y;
     }
     st.l += sum;
 }
 
+// A tile's second product waits for its first; the next tile's operand is decoded between.
 template <int HD, bool Q4>
 __device__ __forceinline__ void values(Soft<HD>& st, const VRaw<HD, Q4>& v, const v8h& hi, const v8h& lo) {
+    v8h before = v_operand<HD, Q4>(v, 0);
+    st.o[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(before, hi, st.o[0], 0, 0, 0);
 #pragma unroll
-    for (int c = 0; c < HD / 16; c++) {
+    for (int c = 1; c < HD / 16; c++) {
         const v8h a = v_operand<HD, Q4>(v, c);
         st.o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, hi, st.o[c], 0, 0, 0);
-        st.o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, lo, st.o[c], 0, 0, 0);
+        st.o[c - 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(before, lo, st.o[c - 1], 0, 0, 0);
+        before = a;
     }
+    st.o[HD / 16 - 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(before, lo, st.o[HD / 16 - 1], 0, 0, 0);
 }
 
 // Sequence s in units of work: its rows in tiles of 16 (rows x heads of a kv
@@ -659,12 +724,11 @@ __device__ __forceinline__ uint64_t capacity(const Paged& p) {
     return static_cast<uint64_t>(p.table_stride) << p.page_shift;
 }
 
-__device__ __forceinline__ SeqWork seq_work(const AttnArgs& a, uint32_t s) {
+__device__ __forceinline__ SeqWork seq_work(const AttnArgs& a, int32_t row0, int32_t row1, int32_t kv) {
     SeqWork w;
     const int32_t n = static_cast<int32_t>(a.p.n_tokens);
-    w.row0 = min(max(a.p.q_start[s], 0), n);
-    w.len = max(min(a.p.q_start[s + 1], n) - w.row0, 0);
-    const int32_t kv = a.p.kv_len[s];
+    w.row0 = min(max(row0, 0), n);
+    w.len = max(min(row1, n) - w.row0, 0);
     w.first = static_cast<int32_t>(static_cast<uint32_t>(kv) - static_cast<uint32_t>(w.len));
     w.end = static_cast<int32_t>(min(static_cast<uint64_t>(max(kv, 0)), capacity(a.p)));
     const int32_t lo = a.window && w.first >= static_cast<int32_t>(a.window) ? w.first - static_cast<int32_t>(a.window) + 1 : 0;
@@ -674,61 +738,81 @@ __device__ __forceinline__ SeqWork seq_work(const AttnArgs& a, uint32_t s) {
     return w;
 }
 
-// Prefix sums of the sequences' units (all tiles and heads) into LDS; returns the total.
-__device__ __forceinline__ uint32_t scan_units(const AttnArgs& a, uint32_t* prefix, uint32_t* sums) {
+__device__ __forceinline__ SeqWork seq_work(const AttnArgs& a, uint32_t s) {
+    return seq_work(a, a.p.q_start[s], a.p.q_start[s + 1], a.p.kv_len[s]);
+}
+
+// The batch's lengths, and prefix sums of its sequences' units (all tiles and heads).
+struct Units {
+    uint32_t prefix[kMaxSeqs + 1];
+    int32_t row0[kMaxSeqs], row1[kMaxSeqs], kv[kMaxSeqs];
+    uint32_t sums[4];
+};
+
+// Fills them; returns the total.  A batch whose sequences' rows are in order has fewer
+// than kUnitsMost (the host's check); sums end there, and one that reaches it is left
+// out whole: its row starts are out of order.
+constexpr uint32_t kUnitsMost = 0x7fffffffu;
+
+__device__ __forceinline__ uint32_t scan_units(const AttnArgs& a, Units& un) {
     const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1), wid = tid / kWave;
     uint32_t base = 0;
     for (uint32_t b = 0; b < a.p.n_seqs; b += 256) {
         uint32_t x = 0;
         if (b + tid < a.p.n_seqs) {
-            const SeqWork w = seq_work(a, b + tid);
-            if (static_cast<uint32_t>(w.len) * a.group <= a.few_rows) x = w.tiles * a.p.n_kv * w.units;
+            const int32_t row0 = a.p.q_start[b + tid], row1 = a.p.q_start[b + tid + 1], kv = a.p.kv_len[b + tid];
+            un.row0[b + tid] = row0;
+            un.row1[b + tid] = row1;
+            un.kv[b + tid] = kv;
+            const SeqWork w = seq_work(a, row0, row1, kv);
+            if (static_cast<uint32_t>(w.len) * a.group <= a.few_rows)
+                x = static_cast<uint32_t>(min(static_cast<uint64_t>(w.tiles) * a.p.n_kv * (w.units + kItem), static_cast<uint64_t>(kUnitsMost)));
         }
         uint32_t run = x;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
             const uint32_t y = __shfl_up(run, o);
-            if (static_cast<int>(lane) >= o) run += y;
+            if (static_cast<int>(lane) >= o) run = min(run + y, kUnitsMost);
         }
-        if (lane == 63) sums[wid] = run;
+        if (lane == 63) un.sums[wid] = run;
         __syncthreads();
         uint32_t before = base, all = 0;
         for (uint32_t i = 0; i < 4; i++) {
-            if (i < wid) before += sums[i];
-            all += sums[i];
+            if (i < wid) before = min(before + un.sums[i], kUnitsMost);
+            all = min(all + un.sums[i], kUnitsMost);
         }
-        if (b + tid < a.p.n_seqs) prefix[b + tid] = before + run - x;
-        base += all;
+        if (b + tid < a.p.n_seqs) un.prefix[b + tid] = before + run - x;
+        base = min(base + all, kUnitsMost);
         __syncthreads();
     }
-    if (tid == 0) prefix[a.p.n_seqs] = base;
+    if (tid == 0) un.prefix[a.p.n_seqs] = base;
     __syncthreads();
-    return base;
+    return base == kUnitsMost ? 0 : base;
 }
 
 // Where unit u lies.
 struct Place {
-    uint32_t s, tile, h, unit;  // unit within the item (s, tile, h)
+    uint32_t s, tile, h, unit;  // within the item (s, tile, h): its cost, then its units
 };
 
-__device__ __forceinline__ Place place_of(const AttnArgs& a, const uint32_t* prefix, uint32_t u, SeqWork& w) {
-    uint32_t lo = 0, hi = a.p.n_seqs;  // prefix[lo] <= u < prefix[hi]
+__device__ __forceinline__ Place place_of(const AttnArgs& a, const Units& un, uint32_t u, SeqWork& w) {
+    uint32_t lo = 0, hi = a.p.n_seqs;  // un.prefix[lo] <= u < un.prefix[hi]
     while (hi - lo > 1) {
         const uint32_t mid = (lo + hi) / 2;
-        if (prefix[mid] <= u) lo = mid;
+        if (un.prefix[mid] <= u) lo = mid;
         else hi = mid;
     }
     Place at;
     at.s = __builtin_amdgcn_readfirstlane(lo);
-    w = seq_work(a, at.s);
-    const uint32_t r = u - prefix[at.s], item = r / w.units;
-    at.unit = __builtin_amdgcn_readfirstlane(r % w.units);
+    w = seq_work(a, un.row0[at.s], un.row1[at.s], un.kv[at.s]);
+    const uint32_t r = u - un.prefix[at.s], item = r / (w.units + kItem);
+    at.unit = __builtin_amdgcn_readfirstlane(r % (w.units + kItem));
     at.tile = __builtin_amdgcn_readfirstlane(item / a.p.n_kv);
     at.h = __builtin_amdgcn_readfirstlane(item % a.p.n_kv);
     return at;
 }
 
-// Units of each workgroup: all alike.  Every kernel of a call computes the same.
+// Units of each workgroup: all alike.
 __device__ __forceinline__ uint32_t share_of(uint32_t total, uint32_t grid) { return (total + grid - 1) / grid; }
 
 // A partial result: 16 rows of hd sums, then the rows' maxima and sums.
@@ -737,69 +821,188 @@ __device__ __forceinline__ float* part_slot(const AttnArgs& a, uint32_t slot) {
     return a.part + static_cast<size_t>(slot) * (16 * (HD + 2));
 }
 
+// A partial result is read by a workgroup on another part of the chip while its
+// kernel runs: stores and loads of agent scope go past the caches that they do not
+// share.
+__device__ __forceinline__ void put_part(float* p, float v) {
+    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float get_part(const float* p) {
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// The shares b0 .. b1 of an item added in order, and its rows written: kE values a
+// thread, kP shares at a time, all of their loads in flight at once.
+struct Join {
+    float m[16][16], l[16][16];  // of the shares at hand, then their factors in m
+    float top[16], sum[16], old[16];
+};
+
+template <int HD, int kE, int kP>
+__device__ __forceinline__ void join_parts(const AttnArgs& a, const SeqWork& w, const Place& at, uint32_t b0, uint32_t b1,
+                                           uint32_t tile_rows, Join& jn) {
+    const uint32_t tid = threadIdx.x, n = tile_rows * HD;
+    const auto part = [&](uint32_t b) { return part_slot<HD>(a, 2 * b + (b == b0 ? 1 : 0)); };
+    float o[kE];
+#pragma unroll
+    for (int k = 0; k < kE; k++) o[k] = 0.0f;
+    if (tid < 16) {
+        jn.top[tid] = -INFINITY;
+        jn.sum[tid] = 0.0f;
+    }
+    for (uint32_t b = b0; b <= b1; b += kP) {
+        float v[kE][kP];
+#pragma unroll
+        for (int j = 0; j < kP; j++) {
+            const float* p = part(min(b + j, b1));
+#pragma unroll
+            for (int k = 0; k < kE; k++) v[k][j] = get_part(p + min(tid + 256 * k, n - 1));
+        }
+        __syncthreads();
+        for (uint32_t i = tid; i < 16 * kP; i += 256) {
+            const uint32_t j = i / 16, row = i % 16;
+            const bool has = b + j <= b1 && row < tile_rows;
+            const float* p = part(min(b + j, b1)) + 16 * HD + min(row, tile_rows - 1);
+            const float m = get_part(p), l = get_part(p + 16);
+            jn.m[j][row] = has ? m : -INFINITY;
+            jn.l[j][row] = has ? l : 0.0f;
+        }
+        __syncthreads();
+        if (tid < 16) {
+            const float was = jn.top[tid];
+            float top = was;
+#pragma unroll
+            for (int j = 0; j < kP; j++) top = __builtin_fmaxf(top, jn.m[j][tid]);
+            const float old = was == top ? 1.0f : __builtin_amdgcn_exp2f(was - top);
+            float sum = jn.sum[tid] * old;
+#pragma unroll
+            for (int j = 0; j < kP; j++) {
+                // without a maximum: nothing seen, or a sum of NaN
+                const float m = jn.m[j][tid], l = jn.l[j][tid];
+                const float g = m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(m - top);
+                sum += l * g;
+                jn.m[j][tid] = g;
+            }
+            jn.top[tid] = top;
+            jn.sum[tid] = sum;
+            jn.old[tid] = old;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kE; k++) {
+            const uint32_t row = min((tid + 256 * k) / HD, 15u);
+            o[k] *= jn.old[row];
+#pragma unroll
+            for (int j = 0; j < kP; j++)
+                if (b + j <= b1) o[k] += v[k][j] * jn.m[j][row];
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kE; k++) {
+        const uint32_t e = tid + 256 * k, row = e / HD, rr = 16 * at.tile + row;
+        if (e >= n) continue;
+        const float sum = jn.sum[row];
+        const uint32_t tk = rr / a.group, hd = at.h * a.group + rr % a.group;
+        a.out[(static_cast<size_t>(w.row0 + tk) * a.n_heads + hd) * HD + e % HD] = sum != 0.0f ? o[k] / sum : o[k];
+    }
+}
+
 // Attention by few rows: the units of all sequences are laid end to end and cut
-// into equal shares, one a workgroup, whatever the lengths are; a workgroup's
-// shares of an item it does not finish alone go to memory and are joined by the
-// merge.  Within an item the four waves take every fourth 32 positions, and their
-// sums are joined through LDS.
+// into equal shares, one a workgroup, whatever the lengths are.  Within an item (a
+// tile of 16 rows and its kv head) the four waves take every fourth 32 positions, and
+// their sums are joined through LDS.  An item that shares cut is joined by the last
+// of its workgroups to be done: each puts its sums into memory, waits until they are
+// there and counts itself; the counter of an item is that of its first share, and is
+// 0 again when the item is done.  The join adds the shares in their order, so results
+// do not depend on which workgroup does it.
 template <int HD, bool Q4>
 __device__ __forceinline__ void attend_few(const AttnArgs& a) {
-    __shared__ uint32_t prefix[kMaxSeqs + 1];
-    __shared__ uint32_t sums[4];
+    __shared__ Units un;
     __shared__ float sm_m[4][16], sm_l[4][16];
     __shared__ __attribute__((aligned(16))) float sm_o[4][16][HD + 4];
+    __shared__ Join jn;
+    __shared__ uint32_t done;
     const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(tid / kWave);
     const uint32_t n = lane & 15, q = lane >> 4;
-    const uint32_t total = scan_units(a, prefix, sums);
-    const uint32_t share = share_of(total, gridDim.x);
+    const uint32_t total = scan_units(a, un);
+    const uint32_t share = share_of(total, gridDim.x);  // blockIdx.x of them: less than total + gridDim.x^2
+    const int32_t win = static_cast<int32_t>(a.window);
     uint32_t u = blockIdx.x * share;
     const uint32_t u_end = min(u + share, total);
     while (u < u_end) {
         SeqWork w;
-        const Place at = place_of(a, prefix, u, w);
-        const uint32_t units = min(w.units - at.unit, u_end - u);
+        Place at = place_of(a, un, u, w);
+        const uint32_t item = u - at.unit, end = min(item + kItem + w.units, u_end);
+        const uint32_t first = item + kItem;  // the item's first unit
+        at.unit = max(u, first) - first;
+        u = end;
+        if (end <= first) break;  // the share ends in the item's cost: the next one has its units
+        const uint32_t units = end - first - at.unit;
         const uint32_t rows = static_cast<uint32_t>(w.len) * a.group;
         const uint32_t r = 16 * at.tile + n;
-        const bool live = r < rows;
+        const bool live = r < rows;  // the others are computed and dropped
         const uint32_t tok = live ? r / a.group : 0, head = at.h * a.group + (live ? r % a.group : 0);
         const int32_t pos = w.first + static_cast<int32_t>(tok);
-        const int32_t hi = live ? pos + 1 : 0;
-        const int32_t lo = a.window && hi > static_cast<int32_t>(a.window) ? hi - static_cast<int32_t>(a.window) : 0;
-        // what any row of the tile sees, for V; rows are in order of position
-        const uint32_t last_tok = (min(16 * at.tile + 16, rows) - 1) / a.group;
-        const int32_t tile_hi = min(w.first + static_cast<int32_t>(last_tok) + 1, w.end);
-        const int32_t first_hi = w.first + static_cast<int32_t>(16 * at.tile / a.group) + 1;
-        const int32_t tile_lo =
-            a.window && first_hi > static_cast<int32_t>(a.window) ? first_hi - static_cast<int32_t>(a.window) : 0;
+        const int32_t hi = pos + 1, lo = win && hi > win ? hi - win : 0;
+        // what any row of the tile sees and what all of them see; rows are in order of position
+        const uint32_t tok_b = (min(16 * at.tile + 16, rows) - 1) / a.group;
+        const int32_t hi_a = w.first + static_cast<int32_t>(16 * at.tile / a.group) + 1;
+        const int32_t hi_b = w.first + static_cast<int32_t>(tok_b) + 1;
+        const int32_t tile_hi = min(hi_b, w.end);
+        const int32_t tile_lo = win && hi_a > win ? hi_a - win : 0, all_lo = win && hi_b > win ? hi_b - win : 0;
+        // this wave's blocks: every 128 positions from kb0, those that any row sees
+        const int32_t kb0 = w.lo + static_cast<int32_t>(at.unit * kUnit + 32 * wid);
+        const int32_t skip = max(tile_lo - 31 - kb0, 0);
+        const uint32_t i0 = (static_cast<uint32_t>(skip) + kUnit - 1) / kUnit;
+        const uint32_t i1 = tile_hi > kb0 ? min(units, (static_cast<uint32_t>(tile_hi - kb0) + kUnit - 1) / kUnit) : 0;
+        // The next block's K is on its way from the moment that this one's scores are
+        // done, its V from when this one's is used: no register waits for its turn.  (A
+        // second set of them, loaded a block ahead, measured 93 us where this takes 90, at
+        // 64 sequences of 820 to 8192 positions and 8 heads; f16, 6 of up to 32001: 119 and
+        // 107.)  Past the last block that one is loaded again: loads under a condition
+        // would be waited for where it ends.
+        KRaw<HD, Q4> kr;
+        VRaw<HD, Q4> vr;
+        Pages pg = {-1, -1}, ahead = {-1, -1};
         QTile<HD> qt;
-        load_q<HD, Q4>(qt, live ? a.q + (static_cast<size_t>(w.row0 + tok) * a.n_heads + head) * HD : nullptr, q, a.scale);
         Soft<HD> st;
+        const auto kb_of = [&](uint32_t i) { return static_cast<uint32_t>(kb0) + kUnit * min(i, i1 - 1); };
+        if (i0 < i1) ahead = entries_at(a.p, at.s, kb_of(i0));
+        load_q<HD, Q4>(qt, a.q + (static_cast<size_t>(w.row0 + tok) * a.n_heads + head) * HD, q, a.scale);
         soft_clear<HD>(st);
-        if (!live) st.m = 0.0f;  // no row: its maximum never moves
-        if (live && pos >= 0 && static_cast<uint64_t>(pos) >= capacity(a.p)) st.l = __builtin_nanf("");
-        for (uint32_t i = 0; i < units; i++) {
-            const uint32_t kb = static_cast<uint32_t>(w.lo) + (at.unit + i) * kUnit + 32 * wid;
-            if (static_cast<int32_t>(kb) >= tile_hi || static_cast<int32_t>(kb) + 32 <= tile_lo) continue;
-            const Pages g = pages_at(a.p, at.s, kb);
-            KRaw<HD, Q4> kr;
-            load_k<HD, Q4>(a.p, g, at.h, kb, lane, kr);
-            VRaw<HD, Q4> vr;
-            load_v<HD, Q4>(a.p, g, at.h, kb, lane, vr);
+        if (pos >= 0 && static_cast<uint64_t>(pos) >= capacity(a.p)) st.l = __builtin_nanf("");
+        if (i0 < i1) {
+            pg = pages_of(a.p, ahead, kb_of(i0));
+            const Spots spots = spots_of<HD, Q4>(a.p, pg, at.h, kb_of(i0), lane);
+            load_k<HD, Q4>(spots, kr);
+            load_v<HD, Q4>(spots, vr);
+            ahead = entries_at(a.p, at.s, kb_of(i0 + 1));
+        }
+        for (uint32_t i = i0; i < i1; i++) {
+            const int32_t kb = static_cast<int32_t>(kb_of(i));
             v4f s[2];
             scores<HD, Q4>(kr, qt, s);
-            const int32_t p0 = static_cast<int32_t>(kb + 8 * q);
-            const bool no_page = (q >= 2 ? g.id[1] : g.id[0]) < 0;
+            const Pages next = pages_of(a.p, ahead, kb_of(i + 1));
+            const Spots spots = spots_of<HD, Q4>(a.p, next, at.h, kb_of(i + 1), lane);
+            load_k<HD, Q4>(spots, kr);
+            ahead = entries_at(a.p, at.s, kb_of(i + 2));
+            if (kb < all_lo || kb + 32 > min(hi_a, w.end) || pg.a < 0 || pg.b < 0) {
+                const int32_t p0 = kb + static_cast<int32_t>(8 * q);
+                const bool no_page = pg.of(q >= 2) < 0;
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int32_t x = p0 + j;
-                float v = s[j / 4][j % 4];
-                if (no_page) v = __builtin_nanf("");
-                s[j / 4][j % 4] = x < lo || x >= hi ? -INFINITY : v;
+                for (int e = 0; e < 8; e++) {
+                    const int32_t x = p0 + e;
+                    float v = s[e / 4][e % 4];
+                    if (no_page) v = __builtin_nanf("");
+                    s[e / 4][e % 4] = x < lo || x >= hi ? -INFINITY : v;
+                }
+                clear_v<HD, Q4>(vr, p0, tile_lo, no_page ? tile_lo : tile_hi);
             }
-            clear_v<HD, Q4>(vr, p0, tile_lo, no_page ? tile_lo : tile_hi);
             v8h ph, pl;
-            soft_step<HD>(st, s, ph, pl);
+            soft_step<HD>(st, s, qt.factor, ph, pl);
             values<HD, Q4>(st, vr, ph, pl);
+            load_v<HD, Q4>(spots, vr);
+            pg = next;
         }
         // join the waves
         const float l = sum_over_q(st.l);
@@ -814,10 +1017,9 @@ __device__ __forceinline__ void attend_few(const AttnArgs& a) {
         __syncthreads();
         const bool whole = units == w.units;
         float* slot = part_slot<HD>(a, 2 * blockIdx.x + (at.unit == 0 ? 1 : 0));
-        for (uint32_t e = tid; e < 16 * HD / 4; e += 256) {
-            const uint32_t row = e / (HD / 4), d = 4 * (e % (HD / 4));
-            const uint32_t rr = 16 * at.tile + row;
-            if (rr >= rows) continue;
+        const uint32_t tile_rows = min(rows - 16 * at.tile, 16u);
+        for (uint32_t e = tid; e < tile_rows * HD / 4; e += 256) {
+            const uint32_t row = e / (HD / 4), d = 4 * (e % (HD / 4)), rr = 16 * at.tile + row;
             float m = sm_m[0][row];
             for (int i = 1; i < 4; i++) m = __builtin_fmaxf(m, sm_m[i][row]);
             float sum = 0.0f;
@@ -833,51 +1035,28 @@ __device__ __forceinline__ void attend_few(const AttnArgs& a) {
                 const uint32_t tk = rr / a.group, hd = at.h * a.group + rr % a.group;
                 *reinterpret_cast<v4f*>(a.out + (static_cast<size_t>(w.row0 + tk) * a.n_heads + hd) * HD + d) = o;
             } else {
-                *reinterpret_cast<v4f*>(slot + row * HD + d) = o;
+#pragma unroll
+                for (int i = 0; i < 4; i++) put_part(slot + row * HD + d + i, o[i]);
                 if (d == 0) {
-                    slot[16 * HD + row] = m;
-                    slot[16 * HD + 16 + row] = sum;
+                    put_part(slot + 16 * HD + row, m);
+                    put_part(slot + 16 * HD + 16 + row, sum);
                 }
             }
         }
-        __syncthreads();
-        u += units;
-    }
-}
-
-// The join of an item's shares: the workgroup of the first cut through the item
-// (blockIdx.x + 1 shares lie before it) adds them in the order of the shares.
-template <int HD, bool Q4>
-__device__ __forceinline__ void merge_few(const AttnArgs& a, uint32_t grid) {
-    __shared__ uint32_t prefix[kMaxSeqs + 1];
-    __shared__ uint32_t sums[4];
-    const uint32_t total = scan_units(a, prefix, sums);
-    const uint32_t share = share_of(total, grid);
-    const uint32_t u = (blockIdx.x + 1) * share;
-    if (u >= total) return;
-    SeqWork w;
-    const Place at = place_of(a, prefix, u, w);
-    if (at.unit == 0 || u - at.unit < blockIdx.x * share) return;  // no item cut here, or cut before
-    const uint32_t last = (u - at.unit + w.units - 1) / share;      // the item's last share
-    const uint32_t all = static_cast<uint32_t>(w.len) * a.group;
-    const uint32_t rows = all > 16 * at.tile ? min(all - 16 * at.tile, 16u) : 0u;
-    for (uint32_t e = threadIdx.x; e < rows * HD / 4; e += 256) {
-        const uint32_t row = e / (HD / 4), d = 4 * (e % (HD / 4));
-        float m = -INFINITY;
-        for (uint32_t b = blockIdx.x; b <= last; b++)
-            m = __builtin_fmaxf(m, part_slot<HD>(a, 2 * b + (b == blockIdx.x ? 1 : 0))[16 * HD + row]);
-        float sum = 0.0f;
-        v4f o = {0, 0, 0, 0};
-        for (uint32_t b = blockIdx.x; b <= last; b++) {
-            const float* slot = part_slot<HD>(a, 2 * b + (b == blockIdx.x ? 1 : 0));
-            const float pm = slot[16 * HD + row], pl = slot[16 * HD + 16 + row];
-            const float f = pm == -INFINITY ? (pl == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(pm - m);
-            sum += pl * f;
-            o += *reinterpret_cast<const v4f*>(slot + row * HD + d) * f;
+        if (!whole) {
+            const uint32_t b0 = first / share, b1 = (first + w.units - 1) / share;
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's part is in memory
+            __syncthreads();                                   // and every wave's
+            if (tid == 0)
+                done = __hip_atomic_fetch_add(a.counts + b0, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == b1 - b0;
+            __syncthreads();
+            if (done) {
+                if (tile_rows * HD <= 512) join_parts<HD, 2, 16>(a, w, at, b0, b1, tile_rows, jn);
+                else join_parts<HD, HD / 16, 4>(a, w, at, b0, b1, tile_rows, jn);
+                if (tid == 0) __hip_atomic_store(a.counts + b0, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
         }
-        if (sum != 0.0f) o /= sum;
-        const uint32_t rr = 16 * at.tile + row, tk = rr / a.group, hd = at.h * a.group + rr % a.group;
-        *reinterpret_cast<v4f*>(a.out + (static_cast<size_t>(w.row0 + tk) * a.n_heads + hd) * HD + d) = o;
+        __syncthreads();
     }
 }
 
@@ -930,7 +1109,7 @@ template <int HD, bool Q4>
 __device__ __forceinline__ void share_load(const Paged& p, const Job<HD>& job, uint32_t h, uint32_t lane,
                                            Share<HD, Q4>& r) {
     const uint32_t m = lane & 15, q = lane >> 4, page = 1u << p.page_shift;
-    const size_t b0 = head_base<HD, Q4>(p, max(r.g.id[0], 0), h), b1 = head_base<HD, Q4>(p, max(r.g.id[1], 0), h);
+    const size_t b0 = head_base<HD, Q4>(p, max(r.g.a, 0), h), b1 = head_base<HD, Q4>(p, max(r.g.b, 0), h);
     const uint8_t* kbase = p.k + (m >= 8 ? b1 : b0);
     const uint8_t* vbase = p.v + (q >= 2 ? b1 : b0);
     const uint32_t grp = ((r.kb + 8 * q) & (page - 1)) >> 3;
@@ -979,12 +1158,12 @@ template <int HD, bool Q4>
 __device__ __forceinline__ void share_store(const Job<HD>& job, Share<HD, Q4>& r, Operands<HD>& to, uint32_t lane,
                                             int32_t lo, int32_t hi) {
     const uint32_t m = lane & 15, q = lane >> 4;
-    const bool edge = static_cast<int32_t>(r.kb) < lo || static_cast<int32_t>(r.kb) + 32 > hi || r.g.id[0] < 0 || r.g.id[1] < 0;
+    const bool edge = static_cast<int32_t>(r.kb) < lo || static_cast<int32_t>(r.kb) + 32 > hi || r.g.a < 0 || r.g.b < 0;
     v4u keep = {~0u, ~0u, ~0u, ~0u};
     bool no_k = false;
     if (edge) {
-        no_k = (m >= 8 ? r.g.id[1] : r.g.id[0]) < 0;
-        const int32_t at = static_cast<int32_t>(r.kb + 8 * q), end = (q >= 2 ? r.g.id[1] : r.g.id[0]) < 0 ? lo : hi;
+        no_k = r.g.of(m >= 8) < 0;
+        const int32_t at = static_cast<int32_t>(r.kb + 8 * q), end = r.g.of(q >= 2) < 0 ? lo : hi;
         uint32_t x[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -1146,7 +1325,7 @@ __device__ __forceinline__ void attend_many(const AttnArgs& a) {
         const int32_t pos = w.first + static_cast<int32_t>(tok);
         hi[i] = live ? pos + 1 : 0;
         lo[i] = a.window && hi[i] > static_cast<int32_t>(a.window) ? hi[i] - static_cast<int32_t>(a.window) : 0;
-        load_q<HD, Q4>(qt[i], live ? a.q + (static_cast<size_t>(w.row0 + tok) * a.n_heads + head) * HD : nullptr, q, a.scale);
+        load_q<HD, Q4>(qt[i], a.q + (static_cast<size_t>(w.row0 + tok) * a.n_heads + head) * HD, q, a.scale);
         soft_clear<HD>(st[i]);
         if (!live) st[i].m = 0.0f;
         if (live && pos >= 0 && static_cast<uint64_t>(pos) >= capacity(a.p)) st[i].l = __builtin_nanf("");
@@ -1161,14 +1340,17 @@ __device__ __forceinline__ void attend_many(const AttnArgs& a) {
 
     const Job<HD> job = job_of<HD>(wid);
     Share<HD, Q4> sh;
+    Pages ahead = {-1, -1};  // of the stage after the one that is loaded next
     const auto start_load = [&](uint32_t at) {
         sh.kb = at + 32 * job.blk;
-        sh.g = pages_at(a.p, it.s, sh.kb);
+        sh.g = pages_of(a.p, ahead, sh.kb);
         share_load<HD, Q4>(a.p, job, it.h, lane, sh);
+        ahead = entries_at(a.p, it.s, sh.kb + M::kStage);
     };
     uint32_t at = static_cast<uint32_t>(sp.from), buf = 0;
     const uint32_t to = static_cast<uint32_t>(sp.to);
     if (at < to) {
+        ahead = entries_at(a.p, it.s, at + 32 * job.blk);
         start_load(at);
         share_store<HD, Q4>(job, sh, ops[0], lane, sp.lo, sp.hi);
     }
@@ -1190,17 +1372,14 @@ __device__ __forceinline__ void attend_many(const AttnArgs& a) {
                 for (int t = 0; t < 2; t++) {
                     const v8h x = op.k[b][t][i][lane];
 #pragma unroll
-                    for (int r = 0; r < M::kRt; r++) {
-                        s[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qt[r].hi[i], s[r][t], 0, 0, 0);
-                        s[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qt[r].lo[i], s[r][t], 0, 0, 0);
-                    }
+                    for (int r = 0; r < M::kRt; r++) s[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qt[r].hi[i], s[r][t], 0, 0, 0);
+#pragma unroll
+                    for (int r = 0; r < M::kRt; r++) s[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qt[r].lo[i], s[r][t], 0, 0, 0);
                 }
             v8h ph[M::kRt], pl[M::kRt];
             const bool masked = kb < all_lo || kb + 32 > hi_a || !full_tile;
 #pragma unroll
             for (int r = 0; r < M::kRt; r++) {
-                s[r][0] *= qt[r].factor;
-                s[r][1] *= qt[r].factor;
                 if (masked) {
 #pragma unroll
                     for (int j = 0; j < 8; j++) {
@@ -1208,16 +1387,15 @@ __device__ __forceinline__ void attend_many(const AttnArgs& a) {
                         s[r][j / 4][j % 4] = x < lo[r] || x >= hi[r] ? -INFINITY : s[r][j / 4][j % 4];
                     }
                 }
-                soft_step<HD>(st[r], s[r], ph[r], pl[r]);
+                soft_step<HD>(st[r], s[r], qt[r].factor, ph[r], pl[r]);
             }
 #pragma unroll
             for (int c = 0; c < HD / 16; c++) {
                 const v8h x = op.v[b][c][lane];
 #pragma unroll
-                for (int r = 0; r < M::kRt; r++) {
-                    st[r].o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, ph[r], st[r].o[c], 0, 0, 0);
-                    st[r].o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, pl[r], st[r].o[c], 0, 0, 0);
-                }
+                for (int r = 0; r < M::kRt; r++) st[r].o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, ph[r], st[r].o[c], 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < M::kRt; r++) st[r].o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, pl[r], st[r].o[c], 0, 0, 0);
             }
         }
         if (more) share_store<HD, Q4>(job, sh, ops[buf ^ 1], lane, sp.lo, sp.hi);
@@ -1298,11 +1476,8 @@ __device__ __forceinline__ void merge_many(const AttnArgs& a) {
     extern "C" __global__ void __launch_bounds__(256) zlm_paged_read_##NAME##_##HD(ReadArgs a) {              \
         read_rows<HD, Q4>(a);                                                                                 \
     }                                                                                                         \
-    extern "C" __global__ void __launch_bounds__(256) zlm_paged_attend_few_##NAME##_##HD(AttnArgs a) {        \
+    extern "C" __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) zlm_paged_attend_few_##NAME##_##HD(AttnArgs a) { \
         attend_few<HD, Q4>(a);                                                                                \
-    }                                                                                                         \
-    extern "C" __global__ void __launch_bounds__(256) zlm_paged_merge_few_##NAME##_##HD(AttnArgs a, uint32_t grid) { \
-        merge_few<HD, Q4>(a, grid);                                                                           \
     }                                                                                                         \
     extern "C" __global__ void __launch_bounds__(256, 2) zlm_paged_attend_many_##NAME##_##HD(AttnArgs a) {    \
         attend_many<HD, Q4>(a);                                                                               \
