@@ -27,6 +27,7 @@ struct PagedAppend {
     float* q_out;
     uint64_t stride;  // floats between rows of qkv
     uint32_t n_heads;
+    uint32_t per;     // heads a wave takes at a time: 1 or 4
     float eps;
     double base;
 };

@@ -87,94 +87,140 @@ __device__ __forceinline__ size_t head_base(const Paged& p, uint32_t page, uint3
     return (static_cast<size_t>(page) * p.n_kv + h) * head_bytes;
 }
 
-// The value of another lane: its place within the row of 16 by a DPP control, then
-// the neighbouring row and the other half by swaps.
-template <int kCtrl>
-__device__ __forceinline__ double dpp(double v) {
-    const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(u), kCtrl, 0xf, 0xf, true);
-    const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(u >> 32), kCtrl, 0xf, 0xf, true);
-    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+// The value of another lane of the row of 16, by a DPP control.
+template <int kCtrl, class T>
+__device__ __forceinline__ T dpp(T v) {
+    if constexpr (sizeof(T) == 4) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), kCtrl, 0xf, 0xf, true));
+    } else {
+        const uint64_t u = __builtin_bit_cast(uint64_t, v);
+        const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(u), kCtrl, 0xf, 0xf, true);
+        const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(u >> 32), kCtrl, 0xf, 0xf, true);
+        return __builtin_bit_cast(T, static_cast<uint64_t>(hi) << 32 | lo);
+    }
 }
 constexpr int kXor1 = 0xb1, kXor2 = 0x4e, kHalfMirror = 0x141, kMirror = 0x140;
 
-template <bool kHalves>  // rows 0 and 1 (2 and 3) exchanged, or the wave's halves
-__device__ __forceinline__ double swapped(double v) {
-    const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = static_cast<uint32_t>(u), hi = static_cast<uint32_t>(u >> 32);
-    const bool upper = (threadIdx.x & (kHalves ? 32 : 16)) != 0;
-    uint32_t x, y;
-    if constexpr (kHalves) {
-        const auto a = __builtin_amdgcn_permlane32_swap(lo, lo, false, false);
-        const auto b = __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
-        x = upper ? a[0] : a[1];
-        y = upper ? b[0] : b[1];
-    } else {
-        const auto a = __builtin_amdgcn_permlane16_swap(lo, lo, false, false);
-        const auto b = __builtin_amdgcn_permlane16_swap(hi, hi, false, false);
-        x = upper ? a[0] : a[1];
-        y = upper ? b[0] : b[1];
-    }
-    return __builtin_bit_cast(double, static_cast<uint64_t>(y) << 32 | x);
+// The value of the neighbouring row of 16 (rows 0 and 1, 2 and 3).
+__device__ __forceinline__ uint32_t next_row(uint32_t v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    const uint32_t x = a[0], y = a[1];
+    return threadIdx.x & 16 ? x : y;
 }
 
-__device__ __forceinline__ double wave_sum(double v) {
-    v += dpp<kXor1>(v);
-    v += dpp<kXor2>(v);
-    v += dpp<kHalfMirror>(v);
-    v += dpp<kMirror>(v);
-    v += swapped<false>(v);
-    return v + swapped<true>(v);
+// The value of lane + or - 32.
+__device__ __forceinline__ double other_half(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = static_cast<uint32_t>(u), hi = static_cast<uint32_t>(u >> 32);
+    const auto a = __builtin_amdgcn_permlane32_swap(lo, lo, false, false);
+    const auto b = __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
+    const uint32_t a0 = a[0], a1 = a[1], b0 = b[0], b1 = b[1];
+    const bool upper = (threadIdx.x & 32) != 0;
+    return __builtin_bit_cast(double, static_cast<uint64_t>(upper ? b0 : b1) << 32 | (upper ? a0 : a1));
+}
+
+// Two sums a step closer: x's in the lanes whose bit is clear, y's in the others.
+template <bool kHalves>  // the bit: 32, or 16
+__device__ __forceinline__ double fold(double x, double y) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x), v = __builtin_bit_cast(uint64_t, y);
+    const auto swap = [](uint64_t p, uint64_t q) {
+        const uint32_t a = static_cast<uint32_t>(p), b = static_cast<uint32_t>(q);
+        return kHalves ? __builtin_amdgcn_permlane32_swap(a, b, false, false)
+                       : __builtin_amdgcn_permlane16_swap(a, b, false, false);
+    };
+    const auto lo = swap(u, v), hi = swap(u >> 32, v >> 32);
+    const uint32_t l0 = lo[0], l1 = lo[1], h0 = hi[0], h1 = hi[1];
+    return __builtin_bit_cast(double, static_cast<uint64_t>(h0) << 32 | l0) +
+           __builtin_bit_cast(double, static_cast<uint64_t>(h1) << 32 | l1);
+}
+
+// Four sums over the wave at the price of one and a half: 0, 2, 1 and 3 in its rows.
+__device__ __forceinline__ double wave_sums(const double v[4]) {
+    double x = fold<false>(fold<true>(v[0], v[1]), fold<true>(v[2], v[3]));
+    x += dpp<kXor1>(x);
+    x += dpp<kXor2>(x);
+    x += dpp<kHalfMirror>(x);
+    return x + dpp<kMirror>(x);
+}
+__device__ __forceinline__ double of_row(double v, int row) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(u), 16 * row);
+    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(u >> 32), 16 * row);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
 }
 
 // The q4_0 block of 32 values, one a lane of each half wave: d from the first of
-// the largest, and this lane's nibble.
-__device__ __forceinline__ uint32_t quantise(double x, uint32_t lane, _Float16* d_out) {
-    const double a = __builtin_fabs(x);
-    double mx = a;
-    mx = __builtin_fmax(mx, dpp<kXor1>(mx));
-    mx = __builtin_fmax(mx, dpp<kXor2>(mx));
-    mx = __builtin_fmax(mx, dpp<kHalfMirror>(mx));
-    mx = __builtin_fmax(mx, dpp<kMirror>(mx));
-    mx = __builtin_fmax(mx, swapped<false>(mx));
-    const uint64_t at = __ballot(a == mx) >> (lane & 32);
-    const int first = at & 0xffffffffu ? __builtin_ctz(static_cast<uint32_t>(at)) : 0;
-    const double m = __shfl(x, static_cast<int>(lane & 32) + first);
-    const bool nan = ((__ballot(x != x) >> (lane & 32)) & 0xffffffffu) != 0;
+// the largest, and this lane's nibble.  T: what the values are exact in.
+template <class T>
+__device__ __forceinline__ uint32_t quantise(T x, uint32_t lane, _Float16* d_out) {
+    const float xf = static_cast<float>(x), a = __builtin_fabsf(xf);
+    float mx = a;
+    mx = __builtin_fmaxf(mx, dpp<kXor1>(mx));
+    mx = __builtin_fmaxf(mx, dpp<kXor2>(mx));
+    mx = __builtin_fmaxf(mx, dpp<kHalfMirror>(mx));
+    mx = __builtin_fmaxf(mx, dpp<kMirror>(mx));
+    mx = __builtin_fmaxf(mx, __builtin_bit_cast(float, next_row(__builtin_bit_cast(uint32_t, mx))));
+    const auto half = [&](uint64_t b) { return static_cast<uint32_t>(lane & 32 ? b >> 32 : b); };
+    const uint32_t at = half(__ballot(a == mx)), negative = half(__ballot(xf < 0.0f));
+    const bool nan = half(__ballot(xf != xf)) != 0;
+    const bool minus = (negative & at & (0u - at)) != 0;  // the first's sign
     // -m/8 to 8 significant bits (bf16), then to f16 (further only below its normal range)
-    const float f = static_cast<float>(m * -0.125);
-    const uint32_t u = __builtin_bit_cast(uint32_t, f);
+    const uint32_t u = __builtin_bit_cast(uint32_t, mx * 0.125f);
     const float r = __builtin_bit_cast(float, (u + 0x7fffu + ((u >> 16) & 1u)) & 0xffff0000u);
-    _Float16 d = static_cast<_Float16>(__builtin_fminf(__builtin_fmaxf(r, -2720.0f), 2720.0f));
-    const double dd = static_cast<double>(d);
-    const double n = dd != 0.0 ? __builtin_floor(x / dd + 8.5) : 8.0;
-    if (nan) d = __builtin_bit_cast(_Float16, static_cast<uint16_t>(0x7e00));  // a block with a NaN reads back as NaN
-    *d_out = d;
-    return static_cast<uint32_t>(__builtin_fmin(__builtin_fmax(n, 0.0), 15.0));
+    const _Float16 size = static_cast<_Float16>(__builtin_fminf(r, 2720.0f));
+    const float df = static_cast<float>(size);
+    // floor(x/d + 8.5): nearly so by a reciprocal, then what it leaves tells, exactly
+    const T xs = minus ? x : -x, dd = static_cast<T>(df);
+    float c = __builtin_floorf(__builtin_fmaf(static_cast<float>(xs), __builtin_amdgcn_rcpf(df), 8.5f));
+    c = __builtin_fminf(__builtin_fmaxf(c, -1.0f), 17.0f);
+    const bool over = __builtin_fma(static_cast<T>(8.5f - c), dd, xs) < T(0);
+    const bool under = __builtin_fma(static_cast<T>(7.5f - c), dd, xs) >= T(0);
+    c += under ? 1.0f : over ? -1.0f : 0.0f;
+    c = size != 0 ? __builtin_fminf(__builtin_fmaxf(c, 0.0f), 15.0f) : 8.0f;
+    // a block with a NaN reads back as NaN
+    *d_out = nan ? __builtin_bit_cast(_Float16, static_cast<uint16_t>(0x7e00)) : minus ? size : -size;
+    return static_cast<uint32_t>(c);
 }
 
 // A workgroup: one row; its waves (and those of the row's other workgroups) deal the
-// heads.  A lane holds dims lane + 64 j; the rotation's pair (i, i + hd/2) is in one
+// heads, four at a time, so that the sums of their norms take one pass over the lanes (or
+// one, where there are waves for all).
+// A lane holds dims lane + 64 j; the rotation's pair (i, i + hd/2) is in one
 // lane for hd 128 and 256 and in lanes i and i + 32 for hd 64.  Angles, norm,
 // rotation and the 4-bit decisions are formed in 64 bits: a rounding of the angle at
 // position 1e5 in 32 bits is 4e-3.  The angles' functions are most of the
 // arithmetic; the workgroup forms them once for all of its heads.
-// V's 8-position groups are written by the wave of the group's first row in this
-// call, which takes the group's other rows along: no two waves write one word.
+// A head of V's 8-position groups is written by one wave, all of the group's rows in
+// this call together: no two waves write one word.  The rows' workgroups take the heads
+// in turn (left to the group's first row they were all on one XCD, every eighth
+// workgroup's: prompts of 7270 rows together took 160 us, and 79 so).
 template <int HD, bool Q4>
 __device__ __forceinline__ void append(const AppendArgs& a) {
     const Paged& p = a.p;
     constexpr int N = HD / 64;  // dims a lane
+    constexpr uint32_t kH = 4;  // heads a step, at most
     __shared__ double turns[2][HD / 2];
     const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1);
     const uint32_t t = blockIdx.x;
-    const uint32_t waves = gridDim.y * 4;
-    uint32_t h = __builtin_amdgcn_readfirstlane(blockIdx.y * 4 + tid / kWave);
+    const uint32_t waves = gridDim.y * 4, wave = __builtin_amdgcn_readfirstlane(blockIdx.y * 4 + tid / kWave);
     const uint32_t heads = a.n_heads + p.n_kv;
     const float* row = a.qkv + t * a.stride + lane;
-    float next[N];  // the next head's values, on their way while this one's are worked on
+    uint32_t h = a.per * wave;
+    // the next heads' values, on their way while these are worked on; past the last head its own
+    float next[kH][N], wq[N], wk[N];
+    const auto load = [&](uint32_t h0) {
 #pragma unroll
-    for (int j = 0; j < N; j++) next[j] = h < heads ? row[static_cast<size_t>(h) * HD + 64 * j] : 0.0f;
+        for (uint32_t i = 0; i < kH; i++)
+#pragma unroll
+            for (int j = 0; j < N; j++) next[i][j] = row[static_cast<size_t>(min(h0 + i, heads - 1)) * HD + 64 * j];
+    };
+    if (h < heads) load(h);
+    const bool norm = a.q_norm != nullptr;
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+        wq[j] = norm ? a.q_norm[lane + 64 * j] : 1.0f;
+        wk[j] = norm ? a.k_norm[lane + 64 * j] : 1.0f;
+    }
     RowAt at;
     if (!row_at(p, t, lane, at)) return;  // a row behind the last sequence: left as it was
     const uint32_t s = at.s;
@@ -192,77 +238,87 @@ __device__ __forceinline__ void append(const AppendArgs& a) {
         cs[j] = turns[0][(lane + 64 * j) % (HD / 2)];
         sn[j] = turns[1][(lane + 64 * j) % (HD / 2)];
     }
-    for (; h < heads; h += waves) {
-        const bool is_q = h < a.n_heads;
-        const float* w = is_q ? a.q_norm : a.k_norm;
-        double x[N], y[N];
+    for (; h < heads; h += a.per * waves) {
+        double x[kH][N], inv = 1.0;
 #pragma unroll
-        for (int j = 0; j < N; j++) x[j] = next[j];
-        if (h + waves < heads) {
+        for (uint32_t i = 0; i < kH; i++)
 #pragma unroll
-            for (int j = 0; j < N; j++) next[j] = row[static_cast<size_t>(h + waves) * HD + 64 * j];
-        }
-        if (w) {
-            double ss = 0.0;
+            for (int j = 0; j < N; j++) x[i][j] = next[i][j];
+        load(h + a.per * waves);
+        if (norm) {
+            double ss[kH];
 #pragma unroll
-            for (int j = 0; j < N; j++) ss = __builtin_fma(x[j], x[j], ss);
-            const double inv = 1.0 / sqrt(wave_sum(ss) * (1.0 / HD) + static_cast<double>(a.eps));
+            for (uint32_t i = 0; i < kH; i++) {
+                ss[i] = 0.0;
 #pragma unroll
-            for (int j = 0; j < N; j++) x[j] = x[j] * inv * static_cast<double>(w[lane + 64 * j]);
-        }
-#pragma unroll
-        for (int j = 0; j < N; j++) {
-            double other;
-            bool upper;
-            if constexpr (HD == 64) {
-                other = swapped<true>(x[0]);
-                upper = lane >= 32;
-            } else {
-                other = x[(j + N / 2) % N];
-                upper = j >= N / 2;
+                for (int j = 0; j < N; j++) ss[i] = __builtin_fma(x[i][j], x[i][j], ss[i]);
             }
-            y[j] = x[j] * cs[j] + (upper ? other : -other) * sn[j];
+            inv = 1.0 / sqrt(wave_sums(ss) * (1.0 / HD) + static_cast<double>(a.eps));
         }
-        if (is_q) {
-            float* dst = a.q_out + (static_cast<size_t>(t) * a.n_heads + h) * HD;
 #pragma unroll
-            for (int j = 0; j < N; j++) dst[lane + 64 * j] = pos < 0 ? 0.0f : static_cast<float>(y[j]);
-            continue;
-        }
-        if (id < 0) continue;
-        uint8_t* base = p.k + head_base<HD, Q4>(p, id, h - a.n_heads);
-        const uint32_t off = static_cast<uint32_t>(pos) & (page - 1);
-        if constexpr (!Q4) {
-            _Float16* dst = reinterpret_cast<_Float16*>(base) + off * HD;
+        for (uint32_t i = 0; i < kH; i++) {
+            if (h + i >= heads || i >= a.per) break;
+            const bool is_q = h + i < a.n_heads;
+            if (norm) {
+                const double f = of_row(inv, i >> 1 | (i & 1) << 1);
 #pragma unroll
-            for (int j = 0; j < N; j++) dst[lane + 64 * j] = static_cast<_Float16>(static_cast<float>(y[j]));
-        } else {
+                for (int j = 0; j < N; j++) x[i][j] = x[i][j] * f * static_cast<double>(is_q ? wq[j] : wk[j]);
+            }
+            double y[N];
 #pragma unroll
             for (int j = 0; j < N; j++) {
-                _Float16 d;
-                const uint32_t n = quantise(y[j], lane, &d);
-                const uint32_t hi = __shfl(n, (lane & 32) + ((lane + 16) & 31));
-                const uint32_t blk = 2 * j + lane / 32, e = lane & 31;
-                if (e < 16) base[off * (HD / 2) + blk * 16 + e] = static_cast<uint8_t>(n | (hi << 4));
-                if (e == 0) reinterpret_cast<_Float16*>(base + page * (HD / 2))[off * (HD / 32) + blk] = d;
+                double other;
+                bool upper;
+                if constexpr (HD == 64) {
+                    other = other_half(x[i][0]);
+                    upper = lane >= 32;
+                } else {
+                    other = x[i][(j + N / 2) % N];
+                    upper = j >= N / 2;
+                }
+                y[j] = x[i][j] * cs[j] + (upper ? other : -other) * sn[j];
+            }
+            if (is_q) {
+                float* dst = a.q_out + (static_cast<size_t>(t) * a.n_heads + h + i) * HD;
+#pragma unroll
+                for (int j = 0; j < N; j++) dst[lane + 64 * j] = pos < 0 ? 0.0f : static_cast<float>(y[j]);
+                continue;
+            }
+            if (id < 0) continue;
+            uint8_t* base = p.k + head_base<HD, Q4>(p, id, h + i - a.n_heads);
+            const uint32_t off = static_cast<uint32_t>(pos) & (page - 1);
+            if constexpr (!Q4) {
+                _Float16* dst = reinterpret_cast<_Float16*>(base) + off * HD;
+#pragma unroll
+                for (int j = 0; j < N; j++) dst[lane + 64 * j] = static_cast<_Float16>(static_cast<float>(y[j]));
+            } else {
+#pragma unroll
+                for (int j = 0; j < N; j++) {
+                    _Float16 d;
+                    const uint32_t n = quantise(y[j], lane, &d);
+                    const uint32_t hi = next_row(n);
+                    const uint32_t blk = 2 * j + lane / 32, e = lane & 31;
+                    if (e < 16) base[off * (HD / 2) + blk * 16 + e] = static_cast<uint8_t>(n | (hi << 4));
+                    if (e == 0) reinterpret_cast<_Float16*>(base + page * (HD / 2))[off * (HD / 32) + blk] = d;
+                }
             }
         }
     }
-    if (h >= heads + p.n_kv) return;
-    // V: the first row of each 8-position group in this call
-    if (pos < 0 || ((pos & 7) != 0 && pos != at.first)) return;  // position 0 starts a group too
-    if (id < 0) return;
-    const uint32_t j0 = static_cast<uint32_t>(pos) & 7;
-    const uint32_t n_rows = min(8u - j0, static_cast<uint32_t>(at.row1) - t);
+    // V's 8-position groups: their rows of this call share their heads
+    if (pos < 0 || id < 0) return;  // position 0 starts a group too
+    const int32_t start = max(pos & ~7, at.first);
+    const uint32_t j0 = static_cast<uint32_t>(start) & 7, mine = static_cast<uint32_t>(pos - start), t0 = t - mine;
+    const uint32_t n_rows = min(8u - j0, static_cast<uint32_t>(at.row1) - t0);
     const uint32_t grp = (static_cast<uint32_t>(pos) & (page - 1)) >> 3;
-    for (; h < heads + p.n_kv; h += waves) {
-        uint8_t* base = p.v + head_base<HD, Q4>(p, id, h - heads);
-        const float* src = a.qkv + t * a.stride + static_cast<size_t>(h) * HD;
+    // the last waves first: they had the fewest heads
+    for (uint32_t g = mine + n_rows * (waves - 1 - wave); g < p.n_kv; g += n_rows * waves) {
+        uint8_t* base = p.v + head_base<HD, Q4>(p, id, g);
+        const float* src = a.qkv + t0 * a.stride + static_cast<size_t>(heads + g) * HD;
         float x[8][N];
 #pragma unroll
         for (uint32_t r = 0; r < 8; r++)
 #pragma unroll
-            for (int j = 0; j < N; j++) x[r][j] = r < n_rows ? src[r * a.stride + lane + 64 * j] : 0.0f;
+            for (int j = 0; j < N; j++) x[r][j] = src[min(r, n_rows - 1) * a.stride + lane + 64 * j];
 #pragma unroll
         for (int j = 0; j < N; j++) {
             const uint32_t dim = lane + 64 * j;
@@ -287,10 +343,10 @@ __device__ __forceinline__ void append(const AppendArgs& a) {
                     if (r < n_rows) {  // wave-uniform
                         _Float16 d;
                         const uint32_t n = quantise(x[r][j], lane, &d);
-                        const uint32_t at = j0 + r, sh = 4 * (at >> 1) + 16 * (at & 1);
+                        const uint32_t to = j0 + r, sh = 4 * (to >> 1) + 16 * (to & 1);
                         bits |= n << sh;
                         mask |= 15u << sh;
-                        if ((lane & 31) == 0) sc[at] = d;
+                        if ((lane & 31) == 0) sc[to] = d;
                     }
                 }
                 *word = n_rows == 8 ? bits : ((*word & ~mask) | bits);
