@@ -3122,14 +3122,17 @@ extern "C" bool zlm_gpu_paged_attention_enqueue(zlm_device* d, const zlm_paged_c
     const bool many = batch->n_tokens > batch->n_seqs && (rows > 512 || rows > static_cast<uint64_t>(batch->n_seqs) * kFewRows);
     const bool few = !many || batch->n_seqs > 1;
     const uint32_t grid = static_cast<uint32_t>(d->cus) * 2;
-    const uint32_t tile_rows = hd == 256 ? 64 : 128;
+    const uint32_t tile_rows = hd == 64 ? 128 : hd == 128 ? 256 : 64, many_threads = hd == 128 ? 512 : 256;
     // a tile for each tile_rows rows and one a sequence begun, as far as there are rows for it
     const uint64_t many_tiles = rows / tile_rows + std::min<uint64_t>(batch->n_seqs, rows / kFewRows);
     const uint64_t items = many_tiles * cache->n_kv_heads;
     if (many && items >= (1ull << 23)) return fail(d, "attention of %u tokens is too large for one call", batch->n_tokens);
-    // positions are split until two workgroups a CU have work
-    const uint64_t want = static_cast<uint64_t>(d->cus) * 2;
-    const uint32_t splits = many ? static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(16, want / items))) : 1;
+    // (in most batches one sequence or two are long: rows / tile_rows of these tiles are real)
+    const uint64_t likely = std::max<uint64_t>(1, rows / tile_rows) * cache->n_kv_heads;
+    // Positions are split where those leave CUs without work: the splits' sums cross
+    // memory twice (two splits of 2000 rows of 8 heads of 256 won 7 us and cost 15).
+    const uint64_t want = static_cast<uint64_t>(d->cus) * (hd == 64 ? 2 : 1);
+    const uint32_t splits = many ? static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(16, want / likely))) : 1;
     const size_t few_part = few ? static_cast<size_t>(grid) * 2 * 16 * (hd + 2) : 0;
     const size_t many_part = splits > 1 ? items * splits * tile_rows * (hd + 2) : 0;
     if (!ensure_attn_scratch(d, std::max({few_part, many_part, kServingScratch / sizeof(float)}))) return false;
@@ -3145,7 +3148,7 @@ extern "C" bool zlm_gpu_paged_attention_enqueue(zlm_device* d, const zlm_paged_c
     a.few_rows = many ? kFewRows : 0xffffffffu;
     a.splits = splits;
     void* args[] = {&a};
-    if (many && !(launch(d, k->many, static_cast<uint32_t>(items * splits), 256, args, "paged attention of many rows") &&
+    if (many && !(launch(d, k->many, static_cast<uint32_t>(items * splits), many_threads, args, "paged attention of many rows") &&
                   (splits == 1 || launch3(d, k->merge_many, static_cast<uint32_t>(items), tile_rows / 16, 1, 256, args,
                                           "paged attention of many rows, merge"))))
         return false;

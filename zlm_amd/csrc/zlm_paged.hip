@@ -714,13 +714,13 @@ __device__ __forceinline__ void scores(const KRaw<HD, Q4>& k, const QTile<HD>& q
     }
 }
 
-// s: products, -inf where masked; times the row's factor they are exponents of two.
-// Makes the two parts of P.
-template <int HD>
-__device__ __forceinline__ void soft_step(Soft<HD>& st, const v4f s[2], float factor, v8h& hi, v8h& lo) {
+// s: products of kT 16-position tiles, -inf where masked; times the row's factor they
+// are exponents of two.  Moves the maximum if it has to; returns what the exponents add.
+template <int HD, int kT>
+__device__ __forceinline__ float soft_base(Soft<HD>& st, const v4f (&s)[kT], float factor) {
     float mx = s[0][0];
 #pragma unroll
-    for (int i = 1; i < 8; i++) mx = __builtin_fmaxf(mx, s[i / 4][i % 4]);
+    for (int i = 1; i < 4 * kT; i++) mx = __builtin_fmaxf(mx, s[i / 4][i % 4]);
     mx *= factor;  // of 0 or more, so the largest stays it
     if (__any(mx > st.m + kSlack)) {
         mx = __builtin_fmaxf(max_over_q(mx), st.m);
@@ -730,25 +730,31 @@ __device__ __forceinline__ void soft_step(Soft<HD>& st, const v4f s[2], float fa
 #pragma unroll
         for (int c = 0; c < HD / 16; c++) st.o[c] *= f;
     }
-    const float base = kLift - (st.m == -INFINITY ? 0.0f : st.m);
-    float minus = -1.0f, sum = 0.0f;
-    asm("" : "+v"(minus));  // a constant would become a conversion and a difference
-#pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][i % 4], factor, base));
-        const float f = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4][i % 4 + 1], factor, base));
-        sum += e + f;
-        // the first part towards zero, two values an instruction; what it leaves is exact
-        // and goes to the second part: 21 bits and more together
-        const v2h x = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(e, f));
-        const v2h y = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf(static_cast<float>(x.x), minus, e),
-                                                                          __builtin_fmaf(static_cast<float>(x.y), minus, f)));
-        hi[i] = x.x;
-        hi[i + 1] = x.y;
-        lo[i] = y.x;
-        lo[i + 1] = y.y;
-    }
-    st.l += sum;
+    return kLift - (st.m == -INFINITY ? 0.0f : st.m);
+}
+
+// -1 that is no constant: with one what a first part leaves would become a conversion
+// and a difference.
+__device__ __forceinline__ float minus_one() {
+    float x = -1.0f;
+    asm("" : "+v"(x));
+    return x;
+}
+
+// The two parts of P of two products, to elements i and i + 1; returns their sum.
+__device__ __forceinline__ float soft_pair(float s0, float s1, float factor, float base, float minus, v8h& hi, v8h& lo, int i) {
+    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s0, factor, base));
+    const float f = __builtin_amdgcn_exp2f(__builtin_fmaf(s1, factor, base));
+    // the first part towards zero, two values an instruction; what it leaves is exact
+    // and goes to the second part: 21 bits and more together
+    const v2h x = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(e, f));
+    const v2h y = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf(static_cast<float>(x.x), minus, e),
+                                                                      __builtin_fmaf(static_cast<float>(x.y), minus, f)));
+    hi[i] = x.x;
+    hi[i + 1] = x.y;
+    lo[i] = y.x;
+    lo[i + 1] = y.y;
+    return e + f;
 }
 
 // A tile's second product waits for its first; the next tile's operand is decoded between.
@@ -1055,7 +1061,11 @@ __device__ __forceinline__ void attend_few(const AttnArgs& a) {
                 clear_v<HD, Q4>(vr, p0, tile_lo, no_page ? tile_lo : tile_hi);
             }
             v8h ph, pl;
-            soft_step<HD>(st, s, qt.factor, ph, pl);
+            const float base = soft_base<HD, 2>(st, s, qt.factor), minus = minus_one();
+            float sum = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) sum += soft_pair(s[e / 4][e % 4], s[e / 4][e % 4 + 1], qt.factor, base, minus, ph, pl, e);
+            st.l += sum;
             values<HD, Q4>(st, vr, ph, pl);
             load_v<HD, Q4>(spots, vr);
             pg = next;
@@ -1120,13 +1130,22 @@ __device__ __forceinline__ void attend_few(const AttnArgs& a) {
 //
 // A workgroup owns 16 kRt rows a wave of one kv head (the rows of consecutive
 // tokens, each with its group of q heads) and walks the positions they see, 32 kBlocks
-// at a time: the four waves load and decode a quarter each of the K and V operands
-// into LDS, in the lanes' order, while all four multiply from the other buffer.
+// at a time: the waves load and decode a share each of the K and V operands into LDS,
+// in the lanes' order, while all multiply from the other buffer.  A workgroup of eight
+// waves decodes half as often as one of four; with heads of 256 its tiles were too few
+// (1000 rows of two heads, f16, beside 15 sequences: 106 us, with four waves 102).
+//
+// What bounds it is the matrix unit: the two parts of q and of P make four products of
+// what f16 alone would take two of, and those run at 1.18 PFLOP/s where a library
+// product of two 16384 x 16384 matrices reaches 1.32 here (2048 rows of 32 q and 8 kv
+// heads of 128 over 8000 positions, q4_0: 400 us).
 template <int HD>
 struct Many {
     static constexpr int kRt = HD == 256 ? 1 : 2;      // tiles of 16 rows a wave
     static constexpr int kBlocks = HD == 256 ? 1 : 2;  // 32-position blocks a stage
-    static constexpr uint32_t kRows = 64 * kRt;
+    static constexpr uint32_t kWaves = HD == 128 ? 8 : 4;
+    static constexpr bool kBoth = HD == 256;           // a wave loads of K and of V
+    static constexpr uint32_t kRows = 16 * kRt * kWaves;
     static constexpr uint32_t kStage = 32 * kBlocks;
 };
 
@@ -1136,12 +1155,12 @@ struct Operands {  // one stage
     v8h v[Many<HD>::kBlocks][HD / 16][kWave];
 };
 
-// A wave's share of a stage as loaded: K's and V's four operands of a block (hd 64:
-// the even waves load K's, the odd ones V's).
+// A wave's share of a stage as loaded: K's or V's four operands of a block, or both
+// (hd 128: the first four waves load K's, the others V's; hd 64: the even, the odd ones).
 template <int HD, bool Q4>
 struct Share {
-    static constexpr int kN = HD == 64 ? 4 : 8;
-    v4u w[Q4 ? 2 : kN];
+    static constexpr int kOne = Q4 ? 1 : 4, kV = Many<HD>::kBoth ? kOne : 0;  // V's first
+    v4u w[kV + kOne];
     v4u vd;
     uint32_t kd;
     Pages g;
@@ -1157,7 +1176,7 @@ struct Job {  // which: block, K tile, 4-operand run of K and of V
 template <int HD>
 __device__ __forceinline__ Job<HD> job_of(uint32_t w) {
     if constexpr (HD == 256) return {0, w & 1, w >> 1, w, true, true};
-    if constexpr (HD == 128) return {w >> 1, w & 1, 0, w & 1, true, true};
+    if constexpr (HD == 128) return {w >> 1 & 1, w & 1, 0, w & 1, w < 4, w >= 4};
     return {w >> 1, 0, 0, 0, (w & 1) == 0, (w & 1) != 0};
 }
 
@@ -1197,12 +1216,12 @@ __device__ __forceinline__ void share_load(const Paged& p, const Job<HD>& job, u
     }
     if (job.v) {
         if constexpr (Q4) {
-            r.w[1] = *reinterpret_cast<const v4u*>(vbase + (grp * HD + 64 * job.vb + 4 * m) * 4);
+            r.w[r.kV] = *reinterpret_cast<const v4u*>(vbase + (grp * HD + 64 * job.vb + 4 * m) * 4);
             r.vd = reinterpret_cast<const v4u*>(vbase + page * (HD / 2))[grp * (HD / 32) + 2 * job.vb + (m >> 3)];
         } else {
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                r.w[(HD == 64 ? 0 : 4) + i] =
+                r.w[r.kV + i] =
                     *reinterpret_cast<const v4u*>(vbase + (grp * HD + 16 * (4 * job.vb + i) + m) * 16);
         }
     }
@@ -1252,7 +1271,8 @@ __device__ __forceinline__ void share_store(const Job<HD>& job, Share<HD, Q4>& r
         if constexpr (Q4) {
             const v4u d = r.vd & keep;
             const uint32_t d0 = d.x, d1 = d.y, d2 = d.z, d3 = d.w;
-            const uint32_t x[4] = {r.w[1].x, r.w[1].y, r.w[1].z, r.w[1].w};
+            const v4u y = r.w[r.kV];
+            const uint32_t x[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
             for (int i = 0; i < 4; i++)
                 to.v[job.blk][4 * job.vb + i][lane] =
@@ -1261,7 +1281,7 @@ __device__ __forceinline__ void share_store(const Job<HD>& job, Share<HD, Q4>& r
         } else {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const v4u x = r.w[(HD == 64 ? 0 : 4) + i] & keep;
+                const v4u x = r.w[r.kV + i] & keep;
                 to.v[job.blk][4 * job.vb + i][lane] = __builtin_bit_cast(v8h, x);
             }
         }
@@ -1286,7 +1306,7 @@ __device__ __forceinline__ Item item_of(const AttnArgs& a, uint32_t block, uint3
     const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1), wid = tid / kWave;
     uint32_t base = 0;
     it.any = false;
-    for (uint32_t b = 0; b < a.p.n_seqs; b += 256) {
+    for (uint32_t b = 0; b < a.p.n_seqs; b += blockDim.x) {
         uint32_t x = 0;
         if (b + tid < a.p.n_seqs) {
             const uint32_t rows = static_cast<uint32_t>(seq_work(a, b + tid).len) * a.group;
@@ -1301,7 +1321,7 @@ __device__ __forceinline__ Item item_of(const AttnArgs& a, uint32_t block, uint3
         if (lane == 63) sums[wid] = run;
         __syncthreads();
         uint32_t before = base;
-        for (uint32_t i = 0; i < 4; i++) {
+        for (uint32_t i = 0; i < blockDim.x / kWave; i++) {
             if (i < wid) before += sums[i];
             base += sums[i];
         }
@@ -1356,11 +1376,14 @@ __device__ __forceinline__ float* many_slot(const AttnArgs& a, uint32_t block) {
     return a.part + static_cast<size_t>(block) * (Many<HD>::kRows * (HD + 2));
 }
 
+// What the scheduler may move past a step of the products: all but them and their operands.
+constexpr int kMoves = 0x2 | 0x4 | 0x10;  // VALU, SALU, VMEM
+
 template <int HD, bool Q4>
 __device__ __forceinline__ void attend_many(const AttnArgs& a) {
     using M = Many<HD>;
     __shared__ __attribute__((aligned(16))) Operands<HD> ops[2];
-    __shared__ uint32_t prefix[2], sums[4];
+    __shared__ uint32_t prefix[2], sums[8];
     const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(tid / kWave);
     const uint32_t n = lane & 15, q = lane >> 4;
     SeqWork w;
@@ -1415,43 +1438,72 @@ __device__ __forceinline__ void attend_many(const AttnArgs& a) {
         const bool more = at + M::kStage < to;
         if (more) start_load(at + M::kStage);
         const Operands<HD>& op = ops[buf];
+        const int32_t kb = static_cast<int32_t>(at);
+        if (wave_live && kb < hi_b && kb + static_cast<int32_t>(M::kStage) > any_lo) {
+            // The operands of the stage in the order of their use, K's tiles, then V's: each
+            // comes from LDS kAhead steps before its products.
+            constexpr int kTiles = 2 * M::kBlocks, kK = kTiles * (HD / 32), kV = HD / 16, kAll = kK + M::kBlocks * kV;
+            constexpr int kAhead = 3;
+            v8h x[kAhead];
+            const auto operand = [&](int j) {
+                return j < kK ? op.k[j / (HD / 16)][j & 1][j / 2 % (HD / 32)][lane] : op.v[(j - kK) / kV][(j - kK) % kV][lane];
+            };
 #pragma unroll
-        for (int b = 0; b < M::kBlocks; b++) {
-            const int32_t kb = static_cast<int32_t>(at) + 32 * b;
-            if (!wave_live || kb >= hi_b || kb + 32 <= any_lo) continue;
-            v4f s[M::kRt][2];
+            for (int j = 0; j < kAhead; j++) x[j] = operand(j);
+            __builtin_amdgcn_sched_barrier(kMoves);
+            v4f s[M::kRt][kTiles];
 #pragma unroll
-            for (int r = 0; r < M::kRt; r++) s[r][0] = s[r][1] = v4f{0, 0, 0, 0};
+            for (int r = 0; r < M::kRt; r++)
 #pragma unroll
-            for (int i = 0; i < HD / 32; i++)
+                for (int i = 0; i < kTiles; i++) s[r][i] = v4f{0, 0, 0, 0};
 #pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    const v8h x = op.k[b][t][i][lane];
+            for (int j = 0; j < kK; j++) {
+                const int tile = 2 * (j / (HD / 16)) + (j & 1), i = j / 2 % (HD / 32);
+                const v8h y = x[j % kAhead];
 #pragma unroll
-                    for (int r = 0; r < M::kRt; r++) s[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qt[r].hi[i], s[r][t], 0, 0, 0);
+                for (int r = 0; r < M::kRt; r++) s[r][tile] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, qt[r].hi[i], s[r][tile], 0, 0, 0);
 #pragma unroll
-                    for (int r = 0; r < M::kRt; r++) s[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qt[r].lo[i], s[r][t], 0, 0, 0);
-                }
-            v8h ph[M::kRt], pl[M::kRt];
-            const bool masked = kb < all_lo || kb + 32 > hi_a || !full_tile;
+                for (int r = 0; r < M::kRt; r++) s[r][tile] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, qt[r].lo[i], s[r][tile], 0, 0, 0);
+                x[j % kAhead] = operand(j + kAhead);
+                __builtin_amdgcn_sched_barrier(kMoves);
+            }
+            float base[M::kRt];
+            const bool masked = kb < all_lo || kb + static_cast<int32_t>(M::kStage) > hi_a || !full_tile;
 #pragma unroll
             for (int r = 0; r < M::kRt; r++) {
                 if (masked) {
 #pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const int32_t x = kb + static_cast<int32_t>(8 * q) + j;
-                        s[r][j / 4][j % 4] = x < lo[r] || x >= hi[r] ? -INFINITY : s[r][j / 4][j % 4];
+                    for (int j = 0; j < 4 * kTiles; j++) {
+                        const int32_t p = kb + 32 * (j / 8) + static_cast<int32_t>(8 * q) + j % 8;
+                        s[r][j / 4][j % 4] = p < lo[r] || p >= hi[r] ? -INFINITY : s[r][j / 4][j % 4];
                     }
                 }
-                soft_step<HD>(st[r], s[r], qt[r].factor, ph[r], pl[r]);
+                base[r] = soft_base<HD, kTiles>(st[r], s[r], qt[r].factor);
             }
+            // Block by block: the next one's probabilities between the products of this one's.
+            v8h ph[2][M::kRt], pl[2][M::kRt];
+            const float minus = minus_one();
+            const auto pair = [&](int blk, int i) {  // of 4 kRt of a block
+                const int r = i / 4, e = 2 * (i % 4);
+                const v4f& v = s[r][2 * blk + e / 4];
+                st[r].l += soft_pair(v[e % 4], v[e % 4 + 1], qt[r].factor, base[r], minus, ph[blk & 1][r], pl[blk & 1][r], e);
+            };
 #pragma unroll
-            for (int c = 0; c < HD / 16; c++) {
-                const v8h x = op.v[b][c][lane];
+            for (int i = 0; i < 4 * M::kRt; i++) pair(0, i);
 #pragma unroll
-                for (int r = 0; r < M::kRt; r++) st[r].o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, ph[r], st[r].o[c], 0, 0, 0);
+            for (int j = kK; j < kAll; j++) {
+                const int blk = (j - kK) / kV, c = (j - kK) % kV;
+                const v8h y = x[j % kAhead];
 #pragma unroll
-                for (int r = 0; r < M::kRt; r++) st[r].o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, pl[r], st[r].o[c], 0, 0, 0);
+                for (int r = 0; r < M::kRt; r++) st[r].o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, ph[blk & 1][r], st[r].o[c], 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < M::kRt; r++) st[r].o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, pl[blk & 1][r], st[r].o[c], 0, 0, 0);
+                if (j + kAhead < kAll) x[j % kAhead] = operand(j + kAhead);
+                if (blk + 1 < M::kBlocks) {
+#pragma unroll
+                    for (int i = c * 4 * M::kRt / kV; i < (c + 1) * 4 * M::kRt / kV; i++) pair(blk + 1, i);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
         if (more) share_store<HD, Q4>(job, sh, ops[buf ^ 1], lane, sp.lo, sp.hi);
@@ -1494,32 +1546,64 @@ __device__ __forceinline__ void attend_many(const AttnArgs& a) {
 template <int HD, bool Q4>
 __device__ __forceinline__ void merge_many(const AttnArgs& a) {
     using M = Many<HD>;
-    __shared__ uint32_t prefix[2], sums[4];
+    __shared__ uint32_t prefix[2], sums[8];
     const uint32_t block = blockIdx.x / a.p.n_kv * a.p.n_kv * a.splits + blockIdx.x % a.p.n_kv;  // its first split's
     SeqWork w;
     const Item it = item_of<HD>(a, block, prefix, sums, w);
     if (!it.any) return;
     const Span sp = span_of<HD>(a, it, w);
-    if (sp.parts == 1) return;
     const uint32_t rows = static_cast<uint32_t>(w.len) * a.group;
-    for (uint32_t e = threadIdx.x; e < 16 * HD / 4; e += 256) {
-        const uint32_t row = 16 * blockIdx.y + e / (HD / 4), d = 4 * (e % (HD / 4)), rr = M::kRows * it.tile + row;
-        if (rr >= rows) continue;
-        float m = -INFINITY;
-        for (uint32_t i = 0; i < sp.parts; i++)
-            m = __builtin_fmaxf(m, many_slot<HD>(a, block + i * a.p.n_kv)[M::kRows * HD + row]);
-        float sum = 0.0f;
-        v4f o = {0, 0, 0, 0};
-        for (uint32_t i = 0; i < sp.parts; i++) {
-            const float* slot = many_slot<HD>(a, block + i * a.p.n_kv);
-            const float pm = slot[M::kRows * HD + row], pl = slot[M::kRows * HD + M::kRows + row];
-            const float f = pm == -INFINITY ? (pl == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(pm - m);
-            sum += pl * f;
-            o += *reinterpret_cast<const v4f*>(slot + row * HD + d) * f;
+    if (sp.parts == 1 || M::kRows * it.tile + 16 * blockIdx.y >= rows) return;
+    // four splits of all of a thread's values in flight at once: the call is their latency
+    constexpr int kE = HD / 64, kP = 4;
+    const uint32_t d = 4 * (threadIdx.x % (HD / 4)), row0 = 16 * blockIdx.y + threadIdx.x / (HD / 4);
+    constexpr uint32_t kStep = 256 / (HD / 4);  // rows
+    float top[kE], sum[kE];
+    v4f o[kE];
+#pragma unroll
+    for (int k = 0; k < kE; k++) {
+        top[k] = -INFINITY;
+        sum[k] = 0.0f;
+        o[k] = v4f{0, 0, 0, 0};
+    }
+    for (uint32_t i = 0; i < sp.parts; i += kP) {
+        float m[kE][kP], l[kE][kP];
+        v4f v[kE][kP];
+#pragma unroll
+        for (int j = 0; j < kP; j++) {
+            const float* slot = many_slot<HD>(a, block + min(i + j, sp.parts - 1) * a.p.n_kv);
+#pragma unroll
+            for (int k = 0; k < kE; k++) {
+                const uint32_t row = min(row0 + kStep * k, rows - 1 - M::kRows * it.tile);  // rows past the last were not written
+                m[k][j] = slot[M::kRows * HD + row];
+                l[k][j] = slot[M::kRows * HD + M::kRows + row];
+                v[k][j] = *reinterpret_cast<const v4f*>(slot + row * HD + d);
+            }
         }
-        if (sum != 0.0f) o /= sum;
+#pragma unroll
+        for (int k = 0; k < kE; k++) {
+            const float was = top[k];
+#pragma unroll
+            for (int j = 0; j < kP; j++) top[k] = __builtin_fmaxf(top[k], m[k][j]);  // the last one's twice is no harm
+            const float old = was == top[k] ? 1.0f : __builtin_amdgcn_exp2f(was - top[k]);
+            sum[k] *= old;
+            o[k] *= old;
+#pragma unroll
+            for (int j = 0; j < kP; j++) {
+                if (i + j >= sp.parts) break;
+                const float f = m[k][j] == -INFINITY ? (l[k][j] == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(m[k][j] - top[k]);
+                sum[k] += l[k][j] * f;
+                o[k] += v[k][j] * f;
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kE; k++) {
+        const uint32_t rr = M::kRows * it.tile + row0 + kStep * k;
+        if (rr >= rows) continue;
         const uint32_t tk = rr / a.group, hd = it.h * a.group + rr % a.group;
-        *reinterpret_cast<v4f*>(a.out + (static_cast<size_t>(w.row0 + tk) * a.n_heads + hd) * HD + d) = o;
+        if (sum[k] != 0.0f) o[k] /= sum[k];
+        *reinterpret_cast<v4f*>(a.out + (static_cast<size_t>(w.row0 + tk) * a.n_heads + hd) * HD + d) = o[k];
     }
 }
 
@@ -1535,7 +1619,7 @@ __device__ __forceinline__ void merge_many(const AttnArgs& a) {
     extern "C" __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) zlm_paged_attend_few_##NAME##_##HD(AttnArgs a) { \
         attend_few<HD, Q4>(a);                                                                                \
     }                                                                                                         \
-    extern "C" __global__ void __launch_bounds__(256, 2) zlm_paged_attend_many_##NAME##_##HD(AttnArgs a) {    \
+    extern "C" __global__ void __launch_bounds__(64 * Many<HD>::kWaves, 2) zlm_paged_attend_many_##NAME##_##HD(AttnArgs a) {    \
         attend_many<HD, Q4>(a);                                                                               \
     }                                                                                                         \
     extern "C" __global__ void __launch_bounds__(256) zlm_paged_merge_many_##NAME##_##HD(AttnArgs a) {        \
