@@ -133,27 +133,29 @@ def test_sampling_scratch_is_sized_eagerly(box):
     d.graph_destroy(d.capture_end())
 
 
-@pytest.mark.parametrize("seqs,tokens,group,want", [
+@pytest.mark.parametrize("type,seqs,tokens,group,want", [
     # one token a sequence, and few tokens each: the few-row kernel alone
-    (1, 1, 4, ["few"]), (64, 64, 8, ["few"]), (8, 40, 4, ["few"]), (2, 2, 33, ["few"]),
+    (zd.Q4_0, 1, 1, 4, ["few"]), (zd.Q4_0, 64, 64, 8, ["few"]), (zd.Q4_0, 8, 40, 4, ["few"]),
+    (zd.Q4_0, 2, 2, 33, ["few"]), (zd.F16, 2, 2, 33, ["few"]), (zd.Q4_0, 1, 32, 4, ["few"]), (zd.F16, 1, 8, 4, ["few"]),
     # one sequence of more rows than it takes: the many-row kernel alone, its positions split while it has few items
-    (1, 9, 4, ["many", "merge"]), (1, 2048, 4, ["many"]), (1, 300, 4, ["many", "merge"]),
+    (zd.F16, 1, 9, 4, ["many", "merge"]), (zd.Q4_0, 1, 33, 4, ["many", "merge"]), (zd.Q4_0, 1, 2048, 4, ["many"]),
+    (zd.Q4_0, 1, 300, 4, ["many", "merge"]),
     # prompts beside other sequences: both
-    (16, 1015, 2, ["many", "merge", "few"]), (200, 500, 4, ["many", "few"]), (2, 4000, 4, ["many", "few"])])
-def test_attention_routes(box, seqs, tokens, group, want):
+    (zd.Q4_0, 16, 1015, 2, ["many", "merge", "few"]), (zd.F16, 200, 3000, 4, ["many", "few"]),
+    (zd.Q4_0, 2, 4000, 4, ["many", "few"])])
+def test_attention_routes(box, type, seqs, tokens, group, want):
     d, p = box.dev, 1 << 16
     d.launch_log(True)
-    assert d.paged_attention_enqueue(_cache(box.mod, kv=8), _batch(box.mod, seqs=seqs, tokens=tokens), p, p, 8 * group,
-                                     0.1), d.last_error()
+    assert d.paged_attention_enqueue(_cache(box.mod, kv=8, type=type), _batch(box.mod, seqs=seqs, tokens=tokens), p, p,
+                                     8 * group, 0.1), d.last_error()
     names = {"paged attention of many rows": "many", "paged attention of many rows, merge": "merge",
              "paged attention": "few"}
     log = d.launch_log_read()
     assert [names[r["what"]] for r in log if r["what"] in names] == want
-    # a workgroup for every tile that the rows may make, kv head and split
+    # a workgroup for every tile of 256 rows that the batch may make, kv head and split
     for r in log:
         if r["what"] == "paged attention of many rows":
-            rows = tokens * group
-            assert r["grid_x"] % 8 == 0 and r["grid_x"] // 8 >= -(-rows // 128)
+            assert r["grid_x"] % 8 == 0 and r["grid_x"] // 8 >= -(-tokens * group // 256)
 
 
 def test_page_bytes():

@@ -3114,17 +3114,21 @@ extern "C" bool zlm_gpu_paged_attention_enqueue(zlm_device* d, const zlm_paged_c
     if (tiles * cache->n_kv_heads * std::min<uint64_t>(depth, (1u << 24) + 4) >= (1ull << 31) - 1)
         return fail(d, "attention of %u tokens over up to %u pages a sequence is too large for one call",
                     batch->n_tokens, batch->table_stride);
-    // Sequences of more than kFewRows rows go to the many-row kernel.  Which there
+    // Sequences of more than few_rows rows go to the many-row kernel.  Which there
     // are is known on the device only: both kernels run where the batch may hold such
-    // a sequence beside others, or is made of them.
-    constexpr uint32_t kFewRows = 32;
+    // a sequence beside others, or is made of them.  The few-row kernel reads K and V
+    // again for every 16 rows, the other one has work for few waves: 8 sequences of about
+    // 3700 positions, heads of 128, 64 and 192 rows each: f16 73 and 182 us by few rows,
+    // 79 and 96 by many; q4_0 39 and 87, 78 and 100 (32 sequences: 118 and 292, 198 and
+    // 225); heads of 256, q4_0: 82 and 171, 69 and 197.
+    const uint32_t few_rows = cache->type == ZLM_GGML_Q4_0 && hd <= 128 ? 128 : 32;
     const uint64_t rows = static_cast<uint64_t>(batch->n_tokens) * group;
-    const bool many = batch->n_tokens > batch->n_seqs && (rows > 512 || rows > static_cast<uint64_t>(batch->n_seqs) * kFewRows);
+    const bool many = batch->n_tokens > batch->n_seqs && (rows > 512 || rows > static_cast<uint64_t>(batch->n_seqs) * few_rows);
     const bool few = !many || batch->n_seqs > 1;
     const uint32_t grid = static_cast<uint32_t>(d->cus) * 2;
     const uint32_t tile_rows = hd == 64 ? 128 : hd == 128 ? 256 : 64, many_threads = hd == 128 ? 512 : 256;
     // a tile for each tile_rows rows and one a sequence begun, as far as there are rows for it
-    const uint64_t many_tiles = rows / tile_rows + std::min<uint64_t>(batch->n_seqs, rows / kFewRows);
+    const uint64_t many_tiles = rows / tile_rows + std::min<uint64_t>(batch->n_seqs, rows / few_rows);
     const uint64_t items = many_tiles * cache->n_kv_heads;
     if (many && items >= (1ull << 23)) return fail(d, "attention of %u tokens is too large for one call", batch->n_tokens);
     // (in most batches one sequence or two are long: rows / tile_rows of these tiles are real)
@@ -3145,7 +3149,7 @@ extern "C" bool zlm_gpu_paged_attention_enqueue(zlm_device* d, const zlm_paged_c
     a.group = group;
     a.window = window;
     a.scale = scale * 1.44269504088896340736f;
-    a.few_rows = many ? kFewRows : 0xffffffffu;
+    a.few_rows = many ? few_rows : 0xffffffffu;
     a.splits = splits;
     void* args[] = {&a};
     if (many && !(launch(d, k->many, static_cast<uint32_t>(items * splits), many_threads, args, "paged attention of many rows") &&
