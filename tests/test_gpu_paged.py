@@ -258,6 +258,106 @@ def test_scores_far_apart(box, kind):
         assert (np.abs(got[:, h] - want[:, h]).max(1) <= sel).all(), h
 
 
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("scale", [0.0, -0.125, 1e-30])
+@pytest.mark.parametrize("lens", [[(1, 200), (2, 9)], [(150, 200)]])
+def test_other_scales(box, kind, scale, lens):
+    """A scale of 0 (the mean of V), below 0 and so small that no score differs; few rows and many."""
+    hd, page, kv, group = 64, 32, 1, 2
+    _say(f"attention kind={kind} scale={scale} {lens}")
+    rng = np.random.default_rng(31)
+    b = paged.Batch(lens, page, rng)
+    pool = paged.Pool(kind, kv, hd, page, b.n_pages)
+    paged.fill(pool, b, rng)
+    q = rng.standard_normal((b.n_tokens, kv * group, hd)).astype(np.float32)
+    cache, batch = box.cache(pool), box.batch(b)
+    d_q, d_o = box.up(q), box.up(q)
+    assert box.dev.paged_attention_enqueue(cache, batch, d_q, d_o, kv * group, scale), box.dev.last_error()
+    got = box.down(d_o, q)
+    want, bound = paged.attend(pool, b, q, kv * group, np.float64(np.float32(scale)))
+    assert (np.abs(got - want).max((1, 2)) <= bound).all()
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("long", [0, 40])
+def test_the_largest_batch(box, kind, long):
+    """1024 sequences of one token each, or with some of 40 tokens (f16: many rows) far behind the first."""
+    hd, page, kv, group = 64, 16, 1, 4
+    _say(f"attention of 1024 sequences kind={kind} long={long}")
+    rng = np.random.default_rng(32)
+    lens = [(1, 1 + i % 37) for i in range(1024)]
+    if long:
+        lens[300] = lens[1023] = (long, long + 5)
+        lens[511] = (0, 3)
+    b = paged.Batch(lens, page, rng, behind=1)
+    pool = paged.Pool(kind, kv, hd, page, b.n_pages)
+    paged.fill(pool, b, rng)
+    q = rng.standard_normal((b.n_tokens, kv * group, hd)).astype(np.float32)
+    cache, batch = box.cache(pool), box.batch(b)
+    d_q, d_o = box.up(q), box.up(np.full_like(q, 7))
+    assert box.dev.paged_attention_enqueue(cache, batch, d_q, d_o, kv * group, 0.2), box.dev.last_error()
+    got = box.down(d_o, q)
+    assert (got[-1] == 7).all()
+    want, bound = paged.attend(pool, b, q, kv * group, np.float64(np.float32(0.2)))
+    assert (np.abs(got - want).max((1, 2))[:-1] <= bound[:-1]).all()
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_pages_past_32_bits(box, kind):
+    """Pages that lie more than 2^32 bytes into the pools, few rows and many."""
+    hd, page, kv, group = 256, 256, 8, 1
+    _say(f"far pages kind={kind}")
+    rng = np.random.default_rng(33)
+    heads = kv * group
+    b = paged.Batch([(1, 300), (200, 200)], page, rng, spare=0)
+    pool = paged.Pool(kind, kv, hd, page, b.n_pages)
+    paged.fill(pool, b, rng)
+    page_bytes = zd.paged_page_bytes(kind, kv, hd, page)
+    far = (1 << 32) // page_bytes + 7
+    n_pages = far + b.n_pages
+    k, v = (box.dev.dev_malloc(n_pages * page_bytes) for _ in range(2))
+    box.bufs += [k, v]
+    box.dev.dev_upload(k + far * page_bytes, pool.k)
+    box.dev.dev_upload(v + far * page_bytes, pool.v)
+    cache = zd.PagedCache(k, v, kind, kv, hd, page, n_pages)
+    b.table = np.where((b.table >= 0) & (b.table < b.n_pages), b.table + far, -1).astype(np.int32)
+    batch = box.batch(b)
+    b.table = np.where(b.table >= 0, b.table - far, -1)  # the oracle's
+    qkv = rng.standard_normal((b.n_tokens, (heads + 2 * kv) * hd)).astype(np.float32)
+    like = np.zeros((b.n_tokens, heads, hd), np.float32)
+    d_q, d_o = box.up(like), box.up(like)
+    assert box.dev.paged_append_enqueue(cache, batch, box.up(qkv), d_q, heads, EPS, BASE), box.dev.last_error()
+    assert box.dev.paged_attention_enqueue(cache, batch, d_q, d_o, heads, hd ** -0.5), box.dev.last_error()
+    box.dev.dev_download(pool.k, k + far * page_bytes)
+    box.dev.dev_download(pool.v, v + far * page_bytes)
+    q, got = box.down(d_q, like), box.down(d_o, like)
+    read = box.up(np.zeros((b.n_tokens, kv, hd), np.float32)), box.up(np.zeros((b.n_tokens, kv, hd), np.float32))
+    assert box.dev.paged_read_enqueue(cache, batch, *read), box.dev.last_error()
+    for row, s, p in b.places():
+        page_id, off = b.spot(s, p)
+        for buf, x in zip(read, pool.rows(np.array([page_id]), np.array([off]))):
+            if row % 50 == 0:
+                np.testing.assert_array_equal(box.down(buf, like[:, :kv])[row], x[0])
+    few = [0, 1, 2, 77, 200]  # of the 201 rows
+    want, bound = paged.attend(pool, _Some(b, few), q, heads, hd ** -0.5)
+    assert (np.abs(got[few] - want[few]).max((1, 2)) <= bound[few]).all()
+    ref = paged.append(paged.Pool(kind, kv, hd, page, b.n_pages), b, qkv, heads, EPS, BASE)
+    np.testing.assert_allclose(q, ref, rtol=2.0 ** -23, atol=1e-9)
+
+
+class _Some:
+    """A batch of which only some rows are looked at."""
+
+    def __init__(self, b, rows):
+        self.b, self.rows = b, rows
+
+    def __getattr__(self, name):
+        return getattr(self.b, name)
+
+    def places(self):
+        return (x for x in self.b.places() if x[0] in self.rows)
+
+
 def test_nan_in_one_sequence_stays_there(box):
     hd, page, kv, group = 128, 16, 1, 4
     rng = np.random.default_rng(9)

@@ -80,7 +80,9 @@ def _hold(box, layer, pool, b, window):
         ref = pool.rows(np.array([page]), np.array([off]))
         pool.k, pool.v = theirs["k"], theirs["v"]
         for x, y in zip(got, ref):
-            step = np.abs(y).reshape(*y.shape[:-1], -1, 32).max(-1).repeat(32, -1) / 7 if pool.kind == zd.Q4_0 else np.abs(y) * 2.0 ** -10 + 2.0 ** -24
+            step = np.abs(y) * 2.0 ** -10 + 2.0 ** -24
+            if pool.kind == zd.Q4_0:
+                step = np.abs(y).reshape(*y.shape[:-1], -1, 32).max(-1).repeat(32, -1) / 7
             assert (np.abs(x - y) <= step).all(), (row, s, p)
     out, bound = paged.attend(pool, b, q, HEADS, SCALE, window)
     off = np.where(live, np.abs(o - np.where(live, out, 0)), 0).max((1, 2))

@@ -122,6 +122,23 @@ def test_sampling_refusals(box):
     assert raw.zlm_gpu_sample_enqueue(d._h, p, 0, 1, 10, None, p, p, None)  # all filters off
 
 
+def test_attention_workspace_is_made_eagerly(box):
+    d, p = box.dev, 1 << 16
+    call = _calls(box, _cache(box.mod), _batch(box.mod))["attention"]
+    assert d.capture_begin()
+    assert not call() and "before capture" in d.last_error()
+    d.graph_destroy(d.capture_end())
+    # the sampler's call makes the shared scratch, not the attention's counters
+    assert d.sample_enqueue(p, 4, 1000, p, p)
+    assert d.capture_begin()
+    assert not call() and "eager call before capture" in d.last_error()
+    d.graph_destroy(d.capture_end())
+    assert call(), d.last_error()
+    assert d.capture_begin()
+    assert call(), d.last_error()
+    d.graph_destroy(d.capture_end())
+
+
 def test_sampling_scratch_is_sized_eagerly(box):
     d, p = box.dev, 1 << 16
     assert d.capture_begin()
