@@ -36,7 +36,6 @@ using zlm::SampleSlice;
 constexpr uint32_t kWave = 64, kThreads = 512;  // of a row's workgroup
 constexpr uint32_t kSlice = zlm::kSampleSlice, kBins = zlm::kSampleBins, kSlices = zlm::kSampleSlices;
 constexpr uint32_t kShort = zlm::kSampleShort;
-constexpr uint32_t kPer = kSlice / kThreads;
 constexpr uint32_t kList = 4096;  // tokens that are looked at one by one
 constexpr double kUnit = 17179869184.0;  // 2^34: the weight at a bin's edge
 constexpr int kCountShift = 50;          // a bin's count above its weights: 8192 x 2^34 is 2^47
@@ -515,23 +514,45 @@ public:
         __syncthreads();
     }
 
-    // f(token) for the listed tokens, or for all of the row that may be drawn.
+    // f(token) for the listed tokens, or for those of the row with keys lo .. hi.
     template <class F>
-    __device__ __forceinline__ void each(bool listed, const F& f) const {
+    __device__ __forceinline__ void each(bool listed, uint32_t lo, uint32_t hi, const F& f) {
         if (listed) {
             for (uint32_t i = tid_; i < n_; i += kThreads) f(sm_.list[i]);
             return;
         }
-        for (uint32_t i0 = tid_; i0 < a_.slices * kSlice; i0 += kSlice) {
-            float x[kPer];
+        // Four logits a load, 16 loads in flight: a row is one CU's to read.  Where some of
+        // a thread's are in question it puts 16 of them into LDS (the list's room), so that
+        // f stands here once.
+        static_assert(16 * kThreads * sizeof(float) <= sizeof(sm_.list), "room for 16 logits a thread");
+        float* const mine = reinterpret_cast<float*>(sm_.list) + tid_;
+        const float least = value_of(lo), most = hi >= key_of(3.402823466e38f) ? INFINITY : value_of(hi);
+        const auto token = [&](float x, uint32_t i) { f(static_cast<uint64_t>(key_of(x)) << 32 | static_cast<uint32_t>(~i)); };
+        typedef float v4 __attribute__((ext_vector_type(4), aligned(4)));
+        constexpr uint32_t kLoads = 16;
+        const uint32_t n4 = a_.vocab / 4;
+        for (uint32_t c = tid_; c < n4; c += kThreads * kLoads) {
+            v4 x[kLoads];
 #pragma unroll
-            for (uint32_t j = 0; j < kPer; j++) x[j] = x_[min(i0 + j * kThreads, a_.vocab - 1)];
+            for (uint32_t j = 0; j < kLoads; j++)
+                x[j] = *reinterpret_cast<const v4*>(x_ + 4 * static_cast<size_t>(min(c + j * kThreads, n4 - 1)));
 #pragma unroll
-            for (uint32_t j = 0; j < kPer; j++) {
-                const uint32_t i = i0 + j * kThreads, key = i < a_.vocab ? key_of(x[j]) : 0;
-                if (key) f(static_cast<uint64_t>(key) << 32 | static_cast<uint32_t>(~i));
+            for (uint32_t j0 = 0; j0 < kLoads; j0 += 4) {
+                uint32_t hit = 0;
+#pragma unroll
+                for (uint32_t e = 0; e < 16; e++)
+                    hit |= x[j0 + e / 4][e % 4] >= least && x[j0 + e / 4][e % 4] <= most ? 1u << e : 0u;
+                if (!hit) continue;
+#pragma unroll
+                for (uint32_t e = 0; e < 16; e++) mine[e * kThreads] = x[j0 + e / 4][e % 4];
+                for (uint32_t m = hit; m; m &= m - 1) {
+                    const uint32_t e = __builtin_ctz(m), v = c + (j0 + e / 4) * kThreads;
+                    if (v < n4) token(mine[e * kThreads], 4 * v + e % 4);
+                }
             }
         }
+        const uint32_t i = 4 * n4 + tid_;  // up to three more
+        if (i < a_.vocab && x_[i] >= least && x_[i] <= most) token(x_[i], i);
     }
 
     // Where a goal is reached.  Its bin's tokens, among those listed or in the row, are
@@ -555,7 +576,7 @@ public:
             // the weight of the bin's tokens from the key on
             lo = static_cast<uint64_t>(g.n) << 32;
             uint64_t w = 0;
-            each(listed, [&](uint64_t t) {
+            each(listed, lo >> 32, hi >> 32, [&](uint64_t t) {
                 if (t >= lo && t <= hi) w += weight_of(t);
             });
             w = block_scan(sm_, turn_, w);
@@ -570,7 +591,7 @@ public:
             sm_.sub_count[tid_] = 0;
             sm_.sub_weight[tid_] = 0;
             __syncthreads();
-            each(listed, [&](uint64_t t) {
+            each(listed, lo >> 32, hi >> 32, [&](uint64_t t) {
                 if (t < lo || t > hi) return;
                 const uint32_t at = static_cast<uint32_t>((hi - t) >> sh);
                 atomicAdd(&sm_.sub_count[at], 1u);
@@ -600,7 +621,7 @@ public:
         __syncthreads();
         if (tid_ == 0) sm_.step_n = 0;
         __syncthreads();
-        each(listed, [&](uint64_t t) {
+        each(listed, lo >> 32, hi >> 32, [&](uint64_t t) {
             if (t < lo || t > hi) return;
             const uint32_t at = atomicAdd(&sm_.step_n, 1u);
             if (at < kFinal) sm_.last[at] = t;
