@@ -36,7 +36,7 @@ using zlm::SampleSlice;
 constexpr uint32_t kWave = 64, kThreads = 512;  // of a row's workgroup
 constexpr uint32_t kSlice = zlm::kSampleSlice, kBins = zlm::kSampleBins, kSlices = zlm::kSampleSlices;
 constexpr uint32_t kShort = zlm::kSampleShort;
-constexpr uint32_t kList = 4096;  // tokens that are looked at one by one
+constexpr uint32_t kList = 12288;  // tokens that are looked at one by one: LDS holds them, a CU one workgroup
 constexpr double kUnit = 17179869184.0;  // 2^34: the weight at a bin's edge
 constexpr int kCountShift = 50;          // a bin's count above its weights: 8192 x 2^34 is 2^47
 
