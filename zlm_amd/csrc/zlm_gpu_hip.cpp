@@ -3125,7 +3125,10 @@ extern "C" bool zlm_gpu_paged_attention_enqueue(zlm_device* d, const zlm_paged_c
     const uint64_t rows = static_cast<uint64_t>(batch->n_tokens) * group;
     const bool many = batch->n_tokens > batch->n_seqs && (rows > 512 || rows > static_cast<uint64_t>(batch->n_seqs) * few_rows);
     const bool few = !many || batch->n_seqs > 1;
-    const uint32_t grid = static_cast<uint32_t>(d->cus) * 2;
+    // Equal shares of the few-row kernel for the workgroups that the CUs hold at once: one
+    // of heads of 256 (two rounds of them: 1 sequence of 32000 q4_0 positions 48 us, one
+    // round 27; 64 of 4096 f16 296 and 290), else two.
+    const uint32_t grid = static_cast<uint32_t>(d->cus) * (hd == 256 ? 1 : 2);
     const uint32_t tile_rows = hd == 64 ? 128 : hd == 128 ? 256 : 64, many_threads = hd == 128 ? 512 : 256;
     // a tile for each tile_rows rows and one a sequence begun, as far as there are rows for it
     const uint64_t many_tiles = rows / tile_rows + std::min<uint64_t>(batch->n_seqs, rows / few_rows);
@@ -3140,7 +3143,7 @@ extern "C" bool zlm_gpu_paged_attention_enqueue(zlm_device* d, const zlm_paged_c
     const size_t few_part = few ? static_cast<size_t>(grid) * 2 * 16 * (hd + 2) : 0;
     const size_t many_part = splits > 1 ? items * splits * tile_rows * (hd + 2) : 0;
     if (!ensure_attn_scratch(d, std::max({few_part, many_part, kServingScratch / sizeof(float)}))) return false;
-    if (!ensure_paged_counts(d, grid)) return false;
+    if (!ensure_paged_counts(d, static_cast<uint32_t>(d->cus) * 2)) return false;
     a.q = q;
     a.out = out;
     a.part = d->attn_part;
