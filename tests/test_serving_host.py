@@ -66,6 +66,7 @@ def test_other_arguments_are_refused(box):
     assert not d.paged_append_enqueue(c, b, p, p, 0, 1e-6, 1e6)
     assert not d.paged_append_enqueue(c, b, p, p, 8, 1e-6, 0.0)
     assert not d.paged_append_enqueue(c, b, p, p, 8, 1e-6, float("nan"))
+    assert not d.paged_append_enqueue(c, b, p, p, 8, 1e-6, float("inf"))
     assert not d.paged_append_enqueue(c, b, p, p, 8, 1e-6, 1e6, q_norm_w=p)  # weights of q alone
     assert not d.paged_append_enqueue(c, b, p, p, 8, 1e-6, 1e6, qkv_stride=12 * 128 - 1)
     assert d.paged_append_enqueue(c, b, p, p, 8, 1e-6, 1e6, qkv_stride=12 * 128)

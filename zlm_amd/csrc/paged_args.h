@@ -29,7 +29,7 @@ struct PagedAppend {
     uint32_t n_heads;
     uint32_t per;     // heads a wave takes at a time: 1 or 4
     float eps;
-    double base;
+    double log_base;  // of the rotation's base
 };
 
 struct PagedRead {

@@ -190,10 +190,10 @@ __device__ __forceinline__ uint32_t quantise(T x, uint32_t lane, _Float16* d_out
 // rotation and the 4-bit decisions are formed in 64 bits: a rounding of the angle at
 // position 1e5 in 32 bits is 4e-3.  The angles' functions are most of the
 // arithmetic; the workgroup forms them once for all of its heads.
-// A head of V's 8-position groups is written by one wave, all of the group's rows in
+// 64 dims of V's 8-position groups are written by one wave, all of the group's rows in
 // this call together: no two waves write one word.  The rows' workgroups take the heads
 // in turn (left to the group's first row they were all on one XCD, every eighth
-// workgroup's: prompts of 7270 rows together took 160 us, and 79 so).
+// workgroup's: prompts of 7270 rows together took 160 us, and 75 so).
 template <int HD, bool Q4>
 __device__ __forceinline__ void append(const AppendArgs& a) {
     const Paged& p = a.p;
@@ -228,7 +228,7 @@ __device__ __forceinline__ void append(const AppendArgs& a) {
     const uint32_t page = 1u << p.page_shift;
     const int32_t id = __builtin_amdgcn_readfirstlane(page_of(p, s, pos));
     if (tid < HD / 2) {
-        const double turn = static_cast<double>(pos) * pow(a.base, static_cast<double>(tid) * (-2.0 / HD));
+        const double turn = static_cast<double>(pos) * exp(a.log_base * (static_cast<double>(tid) * (-2.0 / HD)));
         sincos(turn, &turns[1][tid], &turns[0][tid]);
     }
     __syncthreads();
@@ -310,47 +310,43 @@ __device__ __forceinline__ void append(const AppendArgs& a) {
     const uint32_t j0 = static_cast<uint32_t>(start) & 7, mine = static_cast<uint32_t>(pos - start), t0 = t - mine;
     const uint32_t n_rows = min(8u - j0, static_cast<uint32_t>(at.row1) - t0);
     const uint32_t grp = (static_cast<uint32_t>(pos) & (page - 1)) >> 3;
-    // the last waves first: they had the fewest heads
-    for (uint32_t g = mine + n_rows * (waves - 1 - wave); g < p.n_kv; g += n_rows * waves) {
+    // 64 dims a wave; the last waves first: they had the fewest heads
+    const uint32_t heads_of = mine < p.n_kv ? (p.n_kv - mine + n_rows - 1) / n_rows : 0;
+    for (uint32_t i = waves - 1 - wave; i < heads_of * N; i += waves) {
+        const uint32_t g = mine + n_rows * (i / N), dim = lane + 64 * (i % N);
         uint8_t* base = p.v + head_base<HD, Q4>(p, id, g);
-        const float* src = a.qkv + t0 * a.stride + static_cast<size_t>(heads + g) * HD;
-        float x[8][N];
+        const float* src = a.qkv + t0 * a.stride + static_cast<size_t>(heads + g) * HD + dim;
+        float x[8];
 #pragma unroll
-        for (uint32_t r = 0; r < 8; r++)
+        for (uint32_t r = 0; r < 8; r++) x[r] = src[min(r, n_rows - 1) * a.stride];
+        if constexpr (!Q4) {
+            _Float16* dst = reinterpret_cast<_Float16*>(base) + (grp * HD + dim) * 8;
+            if (n_rows == 8) {
+                v8h o;
 #pragma unroll
-            for (int j = 0; j < N; j++) x[r][j] = src[min(r, n_rows - 1) * a.stride + lane + 64 * j];
-#pragma unroll
-        for (int j = 0; j < N; j++) {
-            const uint32_t dim = lane + 64 * j;
-            if constexpr (!Q4) {
-                _Float16* dst = reinterpret_cast<_Float16*>(base) + (grp * HD + dim) * 8;
-                if (n_rows == 8) {
-                    v8h o;
-#pragma unroll
-                    for (int r = 0; r < 8; r++) o[r] = static_cast<_Float16>(x[r][j]);
-                    *reinterpret_cast<v8h*>(dst) = o;
-                } else {
-#pragma unroll
-                    for (uint32_t r = 0; r < 8; r++)
-                        if (r < n_rows) dst[j0 + r] = static_cast<_Float16>(x[r][j]);
-                }
+                for (int r = 0; r < 8; r++) o[r] = static_cast<_Float16>(x[r]);
+                *reinterpret_cast<v8h*>(dst) = o;
             } else {
-                uint32_t* word = reinterpret_cast<uint32_t*>(base) + grp * HD + dim;
-                _Float16* sc = reinterpret_cast<_Float16*>(base + page * (HD / 2)) + (grp * (HD / 32) + dim / 32) * 8;
-                uint32_t bits = 0, mask = 0;
 #pragma unroll
-                for (uint32_t r = 0; r < 8; r++) {
-                    if (r < n_rows) {  // wave-uniform
-                        _Float16 d;
-                        const uint32_t n = quantise(x[r][j], lane, &d);
-                        const uint32_t to = j0 + r, sh = 4 * (to >> 1) + 16 * (to & 1);
-                        bits |= n << sh;
-                        mask |= 15u << sh;
-                        if ((lane & 31) == 0) sc[to] = d;
-                    }
-                }
-                *word = n_rows == 8 ? bits : ((*word & ~mask) | bits);
+                for (uint32_t r = 0; r < 8; r++)
+                    if (r < n_rows) dst[j0 + r] = static_cast<_Float16>(x[r]);
             }
+        } else {
+            uint32_t* word = reinterpret_cast<uint32_t*>(base) + grp * HD + dim;
+            _Float16* sc = reinterpret_cast<_Float16*>(base + page * (HD / 2)) + (grp * (HD / 32) + dim / 32) * 8;
+            uint32_t bits = 0, mask = 0;
+#pragma unroll
+            for (uint32_t r = 0; r < 8; r++) {
+                if (r < n_rows) {  // wave-uniform
+                    _Float16 d;
+                    const uint32_t n = quantise(x[r], lane, &d);
+                    const uint32_t to = j0 + r, sh = 4 * (to >> 1) + 16 * (to & 1);
+                    bits |= n << sh;
+                    mask |= 15u << sh;
+                    if ((lane & 31) == 0) sc[to] = d;
+                }
+            }
+            *word = n_rows == 8 ? bits : ((*word & ~mask) | bits);
         }
     }
 }
