@@ -278,6 +278,46 @@ def test_other_scales(box, kind, scale, lens):
     assert (np.abs(got - want).max((1, 2)) <= bound).all()
 
 
+class _Some:
+    """A batch of which only some rows are looked at."""
+
+    def __init__(self, b, rows):
+        self.b, self.rows = b, rows
+
+    def __getattr__(self, name):
+        return getattr(self.b, name)
+
+    def places(self):
+        return (x for x in self.b.places() if x[0] in self.rows)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("hd,group,lens,window", [
+    (256, 2, [(1100, 1300), (1, 9)], 0), (256, 2, [(1, 300), (1100, 1200)], 130), (256, 2, [(520, 600)], 0),
+    (128, 4, [(2100, 2100), (3, 70)], 0), (64, 4, [(1100, 1111), (40, 40)], 0)])
+def test_prompts_that_fill_the_chip(box, kind, hd, group, lens, window):
+    """More tiles of rows than CUs, so that no positions are split, and just fewer; some of the rows are looked at."""
+    page, kv = 32, 8
+    _say(f"attention of prompts kind={kind} hd={hd} {lens} window={window}")
+    rng = np.random.default_rng(35)
+    b = paged.Batch(lens, page, rng, behind=1)
+    pool = paged.Pool(kind, kv, hd, page, b.n_pages)
+    paged.fill(pool, b, rng)
+    heads = kv * group
+    q = (1.5 * rng.standard_normal((b.n_tokens, heads, hd))).astype(np.float32)
+    cache, batch = box.cache(pool), box.batch(b)
+    d_q, d_o = box.up(q), box.up(np.full_like(q, 7))
+    assert box.dev.paged_attention_enqueue(cache, batch, d_q, d_o, heads, hd ** -0.5, window=window), box.dev.last_error()
+    got = box.down(d_o, q)
+    assert (got[-1] == 7).all()
+    last = b.n_tokens - 2
+    rows = sorted({0, 1, 15, 16, 31, 32, 63, 64, 500, 519, last - 1, last} | set(rng.integers(0, last, 12).tolist()))
+    rows = [r for r in rows if r <= last]
+    want, bound = paged.attend(pool, _Some(b, rows), q, heads, hd ** -0.5, window)
+    assert (np.abs(got[rows] - want[rows]).max((1, 2)) <= bound[rows]).all()
+    assert np.isfinite(got).all()
+
+
 @pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("long", [0, 40])
 def test_the_largest_batch(box, kind, long):
@@ -343,19 +383,6 @@ def test_pages_past_32_bits(box, kind):
     assert (np.abs(got[few] - want[few]).max((1, 2)) <= bound[few]).all()
     ref = paged.append(paged.Pool(kind, kv, hd, page, b.n_pages), b, qkv, heads, EPS, BASE)
     np.testing.assert_allclose(q, ref, rtol=2.0 ** -23, atol=1e-9)
-
-
-class _Some:
-    """A batch of which only some rows are looked at."""
-
-    def __init__(self, b, rows):
-        self.b, self.rows = b, rows
-
-    def __getattr__(self, name):
-        return getattr(self.b, name)
-
-    def places(self):
-        return (x for x in self.b.places() if x[0] in self.rows)
 
 
 def test_nan_in_one_sequence_stays_there(box):

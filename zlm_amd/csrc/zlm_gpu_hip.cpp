@@ -225,6 +225,7 @@ struct zlm_device {
     hipModule_t paged_mod = nullptr;
     struct PagedKernels {
         hipFunction_t append = nullptr, read = nullptr, few = nullptr, many = nullptr, merge_many = nullptr;
+        hipFunction_t halved = nullptr;  // many's other form, heads of 256
     } paged[2][3];
     uint32_t* paged_counts = nullptr;  // the few-row attention's counters, one a workgroup; 0 between calls
     hipModule_t sample_mod = nullptr;
@@ -412,6 +413,9 @@ bool load_kernels(zlm_device* d) {
                 snprintf(nm, sizeof nm, "zlm_paged_%s_%s_%d", fn.name, t ? "q4_0" : "f16", kPagedDims[i]);
                 if (!ok(d, hipModuleGetFunction(fn.f, d->paged_mod, nm), nm)) return false;
             }
+            if (kPagedDims[i] != 256) continue;
+            snprintf(nm, sizeof nm, "zlm_paged_attend_halved_%s_256", t ? "q4_0" : "f16");
+            if (!ok(d, hipModuleGetFunction(&k.halved, d->paged_mod, nm), nm)) return false;
         }
     const std::string sp = dir + "/zlm_sample_gfx950.hsaco";
     if (!ok(d, hipModuleLoad(&d->sample_mod, sp.c_str()), sp.c_str())) return false;
@@ -3130,17 +3134,23 @@ extern "C" bool zlm_gpu_paged_attention_enqueue(zlm_device* d, const zlm_paged_c
     // of heads of 256 (two rounds of them: 1 sequence of 32000 q4_0 positions 48 us, one
     // round 27; 64 of 4096 f16 296 and 290), else two.
     const uint32_t grid = static_cast<uint32_t>(d->cus) * (hd == 256 ? 1 : 2);
-    const uint32_t tile_rows = hd == 64 ? 128 : hd == 128 ? 256 : 64, many_threads = hd == 128 ? 512 : 256;
+    const uint32_t tile_rows = hd == 64 ? 128 : hd == 128 ? 256 : 64;
     // a tile for each tile_rows rows and one a sequence begun, as far as there are rows for it
     const uint64_t many_tiles = rows / tile_rows + std::min<uint64_t>(batch->n_seqs, rows / few_rows);
     const uint64_t items = many_tiles * cache->n_kv_heads;
     if (many && items >= (1ull << 23)) return fail(d, "attention of %u tokens is too large for one call", batch->n_tokens);
     // (in most batches one sequence or two are long: rows / tile_rows of these tiles are real)
     const uint64_t likely = std::max<uint64_t>(1, rows / tile_rows) * cache->n_kv_heads;
+    // Heads of 256: two waves a SIMD from one workgroup where there are no two for each CU
+    // (512 tokens of two heads over 4000 positions q4_0 112 -> 91, f16 107 -> 95; at 512
+    // tiles 492 and 480, 493 and 521; at 1024 409 and 430, 411 and 466).
+    const bool halved = hd == 256 && likely <= static_cast<uint64_t>(d->cus);
+    const uint32_t many_threads = hd == 128 || halved ? 512 : 256;
     // Positions are split where those leave CUs without work: the splits' sums cross
     // memory twice (two splits of 2000 rows of 8 heads of 256 won 7 us and cost 15).
     const uint64_t want = static_cast<uint64_t>(d->cus) * (hd == 64 ? 2 : 1);
-    const uint32_t splits = many ? static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(16, want / likely))) : 1;
+    const uint64_t room = kServingScratch / (items * tile_rows * (hd + 2) * sizeof(float) + 1);
+    const uint32_t splits = many ? static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>({16, want / likely, room}))) : 1;
     const size_t few_part = few ? static_cast<size_t>(grid) * 2 * 16 * (hd + 2) : 0;
     const size_t many_part = splits > 1 ? items * splits * tile_rows * (hd + 2) : 0;
     if (!ensure_attn_scratch(d, std::max({few_part, many_part, kServingScratch / sizeof(float)}))) return false;
@@ -3156,7 +3166,8 @@ extern "C" bool zlm_gpu_paged_attention_enqueue(zlm_device* d, const zlm_paged_c
     a.few_rows = many ? few_rows : 0xffffffffu;
     a.splits = splits;
     void* args[] = {&a};
-    if (many && !(launch(d, k->many, static_cast<uint32_t>(items * splits), many_threads, args, "paged attention of many rows") &&
+    if (many && !(launch(d, halved ? k->halved : k->many, static_cast<uint32_t>(items * splits), many_threads, args,
+                         "paged attention of many rows") &&
                   (splits == 1 || launch3(d, k->merge_many, static_cast<uint32_t>(items), tile_rows / 16, 1, 256, args,
                                           "paged attention of many rows, merge"))))
         return false;

@@ -1128,27 +1128,30 @@ __device__ __forceinline__ void attend_few(const AttnArgs& a) {
 // tokens, each with its group of q heads) and walks the positions they see, 32 kBlocks
 // at a time: the waves load and decode a share each of the K and V operands into LDS,
 // in the lanes' order, while all multiply from the other buffer.  A workgroup of eight
-// waves decodes half as often as one of four; with heads of 256 its tiles were too few
-// (1000 rows of two heads, f16, beside 15 sequences: 106 us, with four waves 102).
+// waves decodes half as often as one of four.  With heads of 256 a tile has 64 rows;
+// kHalved: two waves share 16 of them, each with one block of a stage, and join their
+// sums at the end.
 //
 // What bounds it is the matrix unit: the two parts of q and of P make four products of
 // what f16 alone would take two of, and those run at 1.18 PFLOP/s where a library
 // product of two 16384 x 16384 matrices reaches 1.32 here (2048 rows of 32 q and 8 kv
 // heads of 128 over 8000 positions, q4_0: 400 us).
-template <int HD>
+template <int HD, bool kHalved = false>
 struct Many {
     static constexpr int kRt = HD == 256 ? 1 : 2;      // tiles of 16 rows a wave
-    static constexpr int kBlocks = HD == 256 ? 1 : 2;  // 32-position blocks a stage
-    static constexpr uint32_t kWaves = HD == 128 ? 8 : 4;
-    static constexpr bool kBoth = HD == 256;           // a wave loads of K and of V
-    static constexpr uint32_t kRows = 16 * kRt * kWaves;
+    static constexpr int kBlocks = HD == 256 && !kHalved ? 1 : 2;  // 32-position blocks a stage
+    static constexpr uint32_t kWaves = HD == 128 || kHalved ? 8 : 4;
+    static constexpr uint32_t kRowWaves = kHalved ? kWaves / 2 : kWaves;
+    static constexpr int kMine = kHalved ? kBlocks / 2 : kBlocks;  // blocks of a stage a wave multiplies
+    static constexpr bool kBoth = HD == 256;                       // a wave loads of K and of V
+    static constexpr uint32_t kRows = 16 * kRt * kRowWaves;
     static constexpr uint32_t kStage = 32 * kBlocks;
 };
 
-template <int HD>
+template <int HD, int kBlocks>
 struct Operands {  // one stage
-    v8h k[Many<HD>::kBlocks][2][HD / 32][kWave];
-    v8h v[Many<HD>::kBlocks][HD / 16][kWave];
+    v8h k[kBlocks][2][HD / 32][kWave];
+    v8h v[kBlocks][HD / 16][kWave];
 };
 
 // A wave's share of a stage as loaded: K's or V's four operands of a block, or both
@@ -1171,7 +1174,7 @@ struct Job {  // which: block, K tile, 4-operand run of K and of V
 
 template <int HD>
 __device__ __forceinline__ Job<HD> job_of(uint32_t w) {
-    if constexpr (HD == 256) return {0, w & 1, w >> 1, w, true, true};
+    if constexpr (HD == 256) return {w >> 2, w & 1, w >> 1 & 1, w & 3, true, true};  // (four waves: block 0)
     if constexpr (HD == 128) return {w >> 1 & 1, w & 1, 0, w & 1, w < 4, w >= 4};
     return {w >> 1, 0, 0, 0, (w & 1) == 0, (w & 1) != 0};
 }
@@ -1225,8 +1228,8 @@ __device__ __forceinline__ void share_load(const Paged& p, const Job<HD>& job, u
 
 // The share decoded into the stage's operands.  `edge`: positions outside [lo, hi)
 // or without a page may be among them: their V becomes 0, a K without a page NaN.
-template <int HD, bool Q4>
-__device__ __forceinline__ void share_store(const Job<HD>& job, Share<HD, Q4>& r, Operands<HD>& to, uint32_t lane,
+template <int HD, bool Q4, int kBlocks>
+__device__ __forceinline__ void share_store(const Job<HD>& job, Share<HD, Q4>& r, Operands<HD, kBlocks>& to, uint32_t lane,
                                             int32_t lo, int32_t hi) {
     const uint32_t m = lane & 15, q = lane >> 4;
     const bool edge = static_cast<int32_t>(r.kb) < lo || static_cast<int32_t>(r.kb) + 32 > hi || r.g.a < 0 || r.g.b < 0;
@@ -1357,8 +1360,8 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, const Item& it, const
     const int32_t first_hi = w.first + static_cast<int32_t>(first_tok) + 1;
     s.lo = a.window && first_hi > static_cast<int32_t>(a.window) ? first_hi - static_cast<int32_t>(a.window) : 0;
     const int32_t start = min(s.lo, s.hi) & ~31;
-    // splits of at least 256 positions, in whole stages
-    const uint32_t n = static_cast<uint32_t>(s.hi - start), step = Many<HD>::kStage;
+    // splits of at least 256 positions, in whole stages of any form
+    const uint32_t n = static_cast<uint32_t>(s.hi - start), step = 64;
     const uint32_t each = max((n + a.splits - 1) / a.splits, 256u);
     const uint32_t part = (each + step - 1) / step * step;
     s.parts = max((n + part - 1) / part, 1u);
@@ -1375,10 +1378,11 @@ __device__ __forceinline__ float* many_slot(const AttnArgs& a, uint32_t block) {
 // What the scheduler may move past a step of the products: all but them and their operands.
 constexpr int kMoves = 0x2 | 0x4 | 0x10;  // VALU, SALU, VMEM
 
-template <int HD, bool Q4>
+template <int HD, bool Q4, bool kHalved>
 __device__ __forceinline__ void attend_many(const AttnArgs& a) {
-    using M = Many<HD>;
-    __shared__ __attribute__((aligned(16))) Operands<HD> ops[2];
+    using M = Many<HD, kHalved>;
+    using Stage = Operands<HD, M::kBlocks>;
+    __shared__ __attribute__((aligned(16))) Stage ops[2];
     __shared__ uint32_t prefix[2], sums[8];
     const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(tid / kWave);
     const uint32_t n = lane & 15, q = lane >> 4;
@@ -1388,7 +1392,7 @@ __device__ __forceinline__ void attend_many(const AttnArgs& a) {
     const Span sp = span_of<HD>(a, it, w);
     if (it.split >= sp.parts) return;
     const uint32_t rows = static_cast<uint32_t>(w.len) * a.group;
-    const uint32_t row0 = M::kRows * it.tile + 16 * M::kRt * wid;
+    const uint32_t row0 = M::kRows * it.tile + 16 * M::kRt * (wid % M::kRowWaves), half = kHalved ? wid / M::kRowWaves : 0;
     QTile<HD> qt[M::kRt];
     Soft<HD> st[M::kRt];
     int32_t hi[M::kRt], lo[M::kRt];
@@ -1427,22 +1431,24 @@ __device__ __forceinline__ void attend_many(const AttnArgs& a) {
     if (at < to) {
         ahead = entries_at(a.p, it.s, at + 32 * job.blk);
         start_load(at);
-        share_store<HD, Q4>(job, sh, ops[0], lane, sp.lo, sp.hi);
+        share_store<HD, Q4, M::kBlocks>(job, sh, ops[0], lane, sp.lo, sp.hi);
     }
     __syncthreads();
     for (; at < to; at += M::kStage) {
         const bool more = at + M::kStage < to;
         if (more) start_load(at + M::kStage);
-        const Operands<HD>& op = ops[buf];
-        const int32_t kb = static_cast<int32_t>(at);
-        if (wave_live && kb < hi_b && kb + static_cast<int32_t>(M::kStage) > any_lo) {
+        const Stage& op = ops[buf];
+        constexpr int32_t kSpan = 32 * M::kMine;
+        const int32_t kb = static_cast<int32_t>(at) + kSpan * static_cast<int32_t>(half);
+        if (wave_live && kb < hi_b && kb + kSpan > any_lo) {
             // The operands of the stage in the order of their use, K's tiles, then V's: each
             // comes from LDS kAhead steps before its products.
-            constexpr int kTiles = 2 * M::kBlocks, kK = kTiles * (HD / 32), kV = HD / 16, kAll = kK + M::kBlocks * kV;
+            constexpr int kTiles = 2 * M::kMine, kK = kTiles * (HD / 32), kV = HD / 16, kAll = kK + M::kMine * kV;
             constexpr int kAhead = 3;
             v8h x[kAhead];
             const auto operand = [&](int j) {
-                return j < kK ? op.k[j / (HD / 16)][j & 1][j / 2 % (HD / 32)][lane] : op.v[(j - kK) / kV][(j - kK) % kV][lane];
+                return j < kK ? op.k[M::kMine * half + j / (HD / 16)][j & 1][j / 2 % (HD / 32)][lane]
+                              : op.v[M::kMine * half + (j - kK) / kV][(j - kK) % kV][lane];
             };
 #pragma unroll
             for (int j = 0; j < kAhead; j++) x[j] = operand(j);
@@ -1464,7 +1470,7 @@ __device__ __forceinline__ void attend_many(const AttnArgs& a) {
                 __builtin_amdgcn_sched_barrier(kMoves);
             }
             float base[M::kRt];
-            const bool masked = kb < all_lo || kb + static_cast<int32_t>(M::kStage) > hi_a || !full_tile;
+            const bool masked = kb < all_lo || kb + kSpan > hi_a || !full_tile;
 #pragma unroll
             for (int r = 0; r < M::kRt; r++) {
                 if (masked) {
@@ -1495,16 +1501,41 @@ __device__ __forceinline__ void attend_many(const AttnArgs& a) {
 #pragma unroll
                 for (int r = 0; r < M::kRt; r++) st[r].o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, pl[blk & 1][r], st[r].o[c], 0, 0, 0);
                 if (j + kAhead < kAll) x[j % kAhead] = operand(j + kAhead);
-                if (blk + 1 < M::kBlocks) {
+                if (blk + 1 < M::kMine) {
 #pragma unroll
                     for (int i = c * 4 * M::kRt / kV; i < (c + 1) * 4 * M::kRt / kV; i++) pair(blk + 1, i);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
-        if (more) share_store<HD, Q4>(job, sh, ops[buf ^ 1], lane, sp.lo, sp.hi);
+        if (more) share_store<HD, Q4, M::kBlocks>(job, sh, ops[buf ^ 1], lane, sp.lo, sp.hi);
         __syncthreads();
         buf ^= 1;
+    }
+    if constexpr (kHalved) {
+        // the other half's sums through LDS, lane by lane
+        static_assert(M::kRt == 1 && sizeof(ops) >= M::kRowWaves * kWave * (4 * HD / 16 + 2) * sizeof(float), "room for them");
+        v4f* const o = reinterpret_cast<v4f*>(ops) + (wid % M::kRowWaves) * (HD / 16) * kWave + lane;
+        float* const ml = reinterpret_cast<float*>(reinterpret_cast<v4f*>(ops) + M::kRowWaves * (HD / 16) * kWave) +
+                          (wid % M::kRowWaves) * 2 * kWave + lane;
+        if (half) {
+#pragma unroll
+            for (int c = 0; c < HD / 16; c++) o[c * kWave] = st[0].o[c];
+            ml[0] = st[0].m;
+            ml[kWave] = st[0].l;
+        }
+        __syncthreads();
+        if (half) return;
+        const float m1 = ml[0], l1 = ml[kWave], m = __builtin_fmaxf(st[0].m, m1);
+        // without a maximum: nothing seen, or a sum of NaN
+        const auto factor = [&](float mi, float li) {
+            return mi == -INFINITY ? (li == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(mi - m);
+        };
+        const float f0 = factor(st[0].m, st[0].l), f1 = factor(m1, l1);
+        st[0].m = m;
+        st[0].l = st[0].l * f0 + l1 * f1;
+#pragma unroll
+        for (int c = 0; c < HD / 16; c++) st[0].o[c] = st[0].o[c] * f0 + o[c * kWave] * f1;
     }
     float* slot = many_slot<HD>(a, blockIdx.x);
 #pragma unroll
@@ -1615,8 +1646,8 @@ __device__ __forceinline__ void merge_many(const AttnArgs& a) {
     extern "C" __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) zlm_paged_attend_few_##NAME##_##HD(AttnArgs a) { \
         attend_few<HD, Q4>(a);                                                                                \
     }                                                                                                         \
-    extern "C" __global__ void __launch_bounds__(64 * Many<HD>::kWaves, 2) zlm_paged_attend_many_##NAME##_##HD(AttnArgs a) {    \
-        attend_many<HD, Q4>(a);                                                                               \
+    extern "C" __global__ void __launch_bounds__(64 * Many<HD>::kWaves, 2) zlm_paged_attend_many_##NAME##_##HD(AttnArgs a) { \
+        attend_many<HD, Q4, false>(a);                                                                               \
     }                                                                                                         \
     extern "C" __global__ void __launch_bounds__(256) zlm_paged_merge_many_##NAME##_##HD(AttnArgs a) {        \
         merge_many<HD, Q4>(a);                                                                                \
@@ -1628,3 +1659,10 @@ ZLM_PAGED(128, f16, false)
 ZLM_PAGED(128, q4_0, true)
 ZLM_PAGED(256, f16, false)
 ZLM_PAGED(256, q4_0, true)
+
+#define ZLM_PAGED_HALVED(HD, NAME, Q4)                                                                         \
+    extern "C" __global__ void __launch_bounds__(512, 2) zlm_paged_attend_halved_##NAME##_##HD(AttnArgs a) { \
+        attend_many<HD, Q4, true>(a);                                                                         \
+    }
+ZLM_PAGED_HALVED(256, f16, false)
+ZLM_PAGED_HALVED(256, q4_0, true)
