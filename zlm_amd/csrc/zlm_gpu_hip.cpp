@@ -3123,9 +3123,9 @@ extern "C" bool zlm_gpu_paged_attention_enqueue(zlm_device* d, const zlm_paged_c
     // are is known on the device only: both kernels run where the batch may hold such
     // a sequence beside others, or is made of them.  The few-row kernel reads K and V
     // again for every 16 rows, the other one has work for few waves: 8 sequences of about
-    // 3700 positions, heads of 128, 64 and 192 rows each: f16 73 and 182 us by few rows,
-    // 79 and 96 by many; q4_0 39 and 87, 78 and 100 (32 sequences: 118 and 292, 198 and
-    // 225); heads of 256, q4_0: 82 and 171, 69 and 197.
+    // 3700 positions, heads of 128, 64 and 192 rows each: f16 73 and 181 us by few rows,
+    // 65 and 76 by many; q4_0 39 and 86, 78 and 75 (32 sequences: 119 and 307, 198 and
+    // 223); heads of 256, q4_0: 64 and 156, 56 and 136.
     const uint32_t few_rows = cache->type == ZLM_GGML_Q4_0 && hd <= 128 ? 128 : 32;
     const uint64_t rows = static_cast<uint64_t>(batch->n_tokens) * group;
     const bool many = batch->n_tokens > batch->n_seqs && (rows > 512 || rows > static_cast<uint64_t>(batch->n_seqs) * few_rows);

@@ -335,13 +335,24 @@ public:
     __device__ __forceinline__ static void read_ahead(const Args& a, uint32_t row, uint32_t s0, Ahead& h) {
         const uint64_t* hist = a.hist + static_cast<size_t>(row) * a.slices * kBins;
         const uint64_t* shorts = a.shorts + static_cast<size_t>(row) * a.slices * kShort;
+        constexpr uint32_t kStep = 8;  // slices, as far as there are any
 #pragma unroll
-        for (uint32_t j = 0; j < kAhead; j++)
-            h.hist[j] = hist[static_cast<size_t>(min(s0 + j, a.slices - 1)) * kBins + threadIdx.x];
+        for (uint32_t k = 0; k < kAhead; k += kStep) {
+            if (s0 + k < a.slices) {
 #pragma unroll
-        for (uint32_t j = 0; j < kAhead / kSide; j++)
-            h.shorts[j] = shorts[static_cast<size_t>(min(s0 + kSide * j + threadIdx.x / kShort, a.slices - 1)) * kShort +
-                                 threadIdx.x % kShort];
+                for (uint32_t j = k; j < k + kStep; j++)
+                    h.hist[j] = hist[static_cast<size_t>(min(s0 + j, a.slices - 1)) * kBins + threadIdx.x];
+#pragma unroll
+                for (uint32_t j = k / kSide; j < (k + kStep) / kSide; j++)
+                    h.shorts[j] = shorts[static_cast<size_t>(min(s0 + kSide * j + threadIdx.x / kShort, a.slices - 1)) * kShort +
+                                         threadIdx.x % kShort];
+            } else {
+#pragma unroll
+                for (uint32_t j = k; j < k + kStep; j++) h.hist[j] = 0;
+#pragma unroll
+                for (uint32_t j = k / kSide; j < (k + kStep) / kSide; j++) h.shorts[j] = 0;
+            }
+        }
     }
 
     __device__ __forceinline__ Row(const Args& a, Shared& sm, uint32_t row, double rate, uint64_t best)
