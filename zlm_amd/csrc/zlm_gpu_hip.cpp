@@ -3096,7 +3096,11 @@ extern "C" bool zlm_gpu_paged_read_enqueue(zlm_device* d, const zlm_paged_cache*
     a.k_out = k_out;
     a.v_out = v_out;
     void* args[] = {&a};
-    return launch3(d, k->read, batch->n_tokens, (cache->n_kv_heads + 3) / 4, 1, 256, args, "paged read");
+    // a head a wave while rows are few, as in the append; all of a row's in one workgroup
+    // where rows fill the CUs
+    const uint64_t fill = (8ull * d->cus + batch->n_tokens - 1) / batch->n_tokens;
+    const unsigned groups = static_cast<unsigned>(std::min<uint64_t>((cache->n_kv_heads + 3) / 4, fill));
+    return launch3(d, k->read, batch->n_tokens, groups, 1, 256, args, "paged read");
 }
 
 extern "C" bool zlm_gpu_paged_attention_enqueue(zlm_device* d, const zlm_paged_cache* cache,

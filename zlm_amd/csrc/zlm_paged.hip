@@ -361,31 +361,45 @@ __device__ __forceinline__ void read_rows(const ReadArgs& a) {
     if (!row_at(p, t, lane, at)) return;
     const int32_t pos = at.pos, id = page_of(p, at.s, pos);
     const uint32_t page = 1u << p.page_shift, off = static_cast<uint32_t>(pos) & (page - 1);
-    const uint32_t grp = off >> 3, j = off & 7;
-    for (uint32_t h = blockIdx.y * 4 + threadIdx.x / kWave; h < p.n_kv; h += gridDim.y * 4) {
-        const size_t o = (static_cast<size_t>(t) * p.n_kv + h) * HD;
+    const uint32_t grp = off >> 3, in = off & 7;
+    const uint32_t waves = gridDim.y * 4;
+    constexpr int kH = 2, N = HD / 64;  // heads at a time: their loads are in flight together
+    for (uint32_t h0 = blockIdx.y * 4 + threadIdx.x / kWave; h0 < p.n_kv; h0 += kH * waves) {
+        float k[kH][N], v[kH][N];
 #pragma unroll
-        for (int i = 0; i < HD / 64; i++) {
-            const uint32_t dim = lane + 64 * i;
-            float k = pos < 0 ? 0.0f : __builtin_nanf(""), v = k;
-            if (id >= 0) {
+        for (int i = 0; i < kH; i++) {
+            const uint32_t h = min(h0 + i * waves, p.n_kv - 1);
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                const uint32_t dim = lane + 64 * j;
+                k[i][j] = v[i][j] = pos < 0 ? 0.0f : __builtin_nanf("");
+                if (id < 0) continue;
                 const uint8_t* kb = p.k + head_base<HD, Q4>(p, id, h);
                 const uint8_t* vb = p.v + head_base<HD, Q4>(p, id, h);
                 if constexpr (!Q4) {
-                    k = static_cast<float>(reinterpret_cast<const _Float16*>(kb)[off * HD + dim]);
-                    v = static_cast<float>(reinterpret_cast<const _Float16*>(vb)[(grp * HD + dim) * 8 + j]);
+                    k[i][j] = static_cast<float>(reinterpret_cast<const _Float16*>(kb)[off * HD + dim]);
+                    v[i][j] = static_cast<float>(reinterpret_cast<const _Float16*>(vb)[(grp * HD + dim) * 8 + in]);
                 } else {
                     const uint32_t b = kb[off * (HD / 2) + dim / 32 * 16 + (dim & 15)];
                     const float dk = reinterpret_cast<const _Float16*>(kb + page * (HD / 2))[off * (HD / 32) + dim / 32];
-                    k = (static_cast<float>((b >> (dim & 16 ? 4 : 0)) & 15) - 8.0f) * dk;
+                    k[i][j] = (static_cast<float>((b >> (dim & 16 ? 4 : 0)) & 15) - 8.0f) * dk;
                     const uint32_t w = reinterpret_cast<const uint32_t*>(vb)[grp * HD + dim];
                     const float dv =
-                        reinterpret_cast<const _Float16*>(vb + page * (HD / 2))[(grp * (HD / 32) + dim / 32) * 8 + j];
-                    v = (static_cast<float>((w >> (4 * (j >> 1) + 16 * (j & 1))) & 15) - 8.0f) * dv;
+                        reinterpret_cast<const _Float16*>(vb + page * (HD / 2))[(grp * (HD / 32) + dim / 32) * 8 + in];
+                    v[i][j] = (static_cast<float>((w >> (4 * (in >> 1) + 16 * (in & 1))) & 15) - 8.0f) * dv;
                 }
             }
-            a.k_out[o + dim] = k;
-            a.v_out[o + dim] = v;
+        }
+#pragma unroll
+        for (int i = 0; i < kH; i++) {
+            const uint32_t h = h0 + i * waves;
+            if (h >= p.n_kv) break;
+            const size_t o = (static_cast<size_t>(t) * p.n_kv + h) * HD + lane;
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                a.k_out[o + 64 * j] = k[i][j];
+                a.v_out[o + 64 * j] = v[i][j];
+            }
         }
     }
 }
