@@ -454,7 +454,7 @@ typedef struct {
  * appends to; two rows of one call never write one position. */
 typedef struct {
     uint32_t n_seqs;         /* at most 1024 */
-    uint32_t n_tokens;       /* rows of the token buffers, at most 2^24 */
+    uint32_t n_tokens;       /* rows of the token buffers, below 2^24 */
     const int32_t *q_start;  /* n_seqs + 1 */
     const int32_t *kv_len;   /* n_seqs: positions of each sequence, these rows included */
     const int32_t *table;    /* n_seqs x table_stride page numbers */
@@ -468,7 +468,7 @@ uint64_t zlm_gpu_paged_page_bytes(uint32_t type, uint32_t n_kv_heads, uint32_t h
  * k: n_kv_heads*hd | v: n_kv_heads*hd] floats, qkv_stride floats apart (0:
  * packed); q_out: n_tokens x n_heads*hd floats, 0 in padding rows.  The angle
  * (position * freq_base^(-2i/hd)), the norm and the choice of 4-bit values are
- * formed in 64 bits.  q4_0: d = -m/8 of the block's value m of the largest size
+ * formed in 64 bits; freq_base is finite.  q4_0: d = -m/8 of the block's value m of the largest size
  * (the first of several), rounded to 8 significant bits, n = floor(x/d + 8.5)
  * within 0..15; a block with a NaN reads back as NaN, values past 21760 saturate.
  * f16: rounded to nearest, infinite past its range. */
@@ -487,8 +487,8 @@ bool zlm_gpu_paged_read_enqueue(zlm_device *dev, const zlm_paged_cache *cache, c
  * products and sums over the cached values.  A padding row's output is 0.  NaN or
  * infinite K reaches the rows that see its position only; such a V may make NaN
  * of other rows of its sequence in the same call, never of another sequence's.
- * Partial results live in the library scratch of zlm_gpu_attention_enqueue (call
- * once before capture). */
+ * Partial results live in the library scratch of zlm_gpu_attention_enqueue, of which
+ * 64 MiB serve every call, and counters beside it: call once before capture. */
 bool zlm_gpu_paged_attention_enqueue(zlm_device *dev, const zlm_paged_cache *cache, const zlm_paged_batch *batch,
                                      const float *q, uint32_t n_heads, uint32_t window, float scale, float *out);
 

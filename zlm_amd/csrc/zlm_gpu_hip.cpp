@@ -3356,6 +3356,7 @@ extern "C" uint64_t zlm_gpu_scratch_device_bytes(const zlm_device* d) {
     uint64_t b = (d->x_cap + d->y_cap + d->bx_cap + d->mid_cap + d->attn_part_cap) * sizeof(float) +
                  d->q_scratch_cap + d->s_raw_cap + d->s_lay_cap;
     for (const Slot& sl : d->slots) b += sl.x_cap * sizeof(float);
+    if (d->paged_counts) b += static_cast<uint64_t>(d->cus) * 2 * sizeof(uint32_t);
     return b;
 }
 
