@@ -319,6 +319,50 @@ def test_prompts_that_fill_the_chip(box, kind, hd, group, lens, window):
 
 
 @pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("live", [1, 8, 9, 32])
+def test_one_sequence_of_fewer_rows(box, kind, hd, live):
+    """One sequence that has a part of the token rows only: a prompt's last chunk in the buffers, or in the graph, of
+    a full one (4 q heads: 4, 32, 36 and 128 rows of the attention's tiles)."""
+    page, kv, group, most, kept = 32, 1, 4, 330, 45
+    dev, heads = box.dev, kv * group
+    _say(f"one sequence kind={kind} hd={hd} live={live}")
+    rng = np.random.default_rng(hd + live)
+    b = paged.Batch([(most, kept + most)], page, rng)
+    pool = paged.Pool(kind, kv, hd, page, b.n_pages)
+    paged.fill(pool, b, rng)
+    q = rng.standard_normal((most, heads, hd)).astype(np.float32)
+    cache, batch = box.cache(pool), box.batch(b)
+    d_q, d_o = box.up(q), box.up(np.full_like(q, 7))
+
+    def step():
+        assert dev.paged_attention_enqueue(cache, batch, d_q, d_o, heads, hd ** -0.5), dev.last_error()
+
+    def check(lens, rows):
+        b.lens = [lens]
+        got = box.down(d_o, q)
+        want, bound = paged.attend(pool, _Some(b, rows), q, heads, hd ** -0.5)
+        assert (np.abs(got[rows] - want[rows]).max((1, 2)) <= bound[rows]).all()
+        assert (got[lens[0]:] == 7).all()
+
+    step()
+    check((most, kept + most), [0, 17, most - 1])
+    assert dev.capture_begin(), dev.last_error()
+    step()
+    g = dev.capture_end()
+    assert g, dev.last_error()
+    try:
+        dev.dev_upload(box.q_start, np.array([0, live], np.int32))
+        dev.dev_upload(box.kv_len, np.array([kept + live], np.int32))
+        for run in (step, lambda: dev.graph_launch(g, 1), step):
+            dev.dev_upload(d_o, np.full_like(q, 7))
+            run()
+            check((live, kept + live), list(range(live)))
+    finally:
+        dev.graph_destroy(g)
+
+
+@pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("long", [0, 40])
 def test_the_largest_batch(box, kind, long):
     """1024 sequences of one token each, or with some of 40 tokens (f16: many rows) far behind the first."""

@@ -3125,7 +3125,8 @@ extern "C" bool zlm_gpu_paged_attention_enqueue(zlm_device* d, const zlm_paged_c
                     batch->n_tokens, batch->table_stride);
     // Sequences of more than few_rows rows go to the many-row kernel.  Which there
     // are is known on the device only: both kernels run where the batch may hold such
-    // a sequence beside others, or is made of them.  The few-row kernel reads K and V
+    // a sequence beside others, or is made of them.  A batch of one sequence goes to one
+    // kernel whole, however many of the token rows it has when the work runs.  The few-row kernel reads K and V
     // again for every 16 rows, the other one has work for few waves: 8 sequences of about
     // 3700 positions, heads of 128, 64 and 192 rows each: f16 73 and 181 us by few rows,
     // 65 and 76 by many; q4_0 39 and 86, 78 and 75 (32 sequences: 119 and 307, 198 and
@@ -3167,7 +3168,7 @@ extern "C" bool zlm_gpu_paged_attention_enqueue(zlm_device* d, const zlm_paged_c
     a.group = group;
     a.window = window;
     a.scale = scale * 1.44269504088896340736f;
-    a.few_rows = many ? few_rows : 0xffffffffu;
+    a.few_rows = !few ? 0 : many ? few_rows : 0xffffffffu;
     a.splits = splits;
     void* args[] = {&a};
     if (many && !(launch(d, halved ? k->halved : k->many, static_cast<uint32_t>(items * splits), many_threads, args,
