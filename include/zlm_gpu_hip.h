@@ -487,8 +487,9 @@ bool zlm_gpu_paged_read_enqueue(zlm_device *dev, const zlm_paged_cache *cache, c
  * products and sums over the cached values.  A padding row's output is 0.  NaN or
  * infinite K reaches the rows that see its position only; such a V may make NaN
  * of other rows of its sequence in the same call, never of another sequence's.
- * Partial results live in the library scratch of zlm_gpu_attention_enqueue, of which
- * 64 MiB serve every call, and counters beside it: call once before capture. */
+ * Partial results live in 64 MiB of library scratch that this call and zlm_gpu_sample_enqueue
+ * share, and counters beside it, made by their first calls and never replaced: call once
+ * before its capture. */
 bool zlm_gpu_paged_attention_enqueue(zlm_device *dev, const zlm_paged_cache *cache, const zlm_paged_batch *batch,
                                      const float *q, uint32_t n_heads, uint32_t window, float scale, float *out);
 
@@ -517,8 +518,8 @@ typedef struct {
  * packed).  u: a number in [0, 1) per row.  token[r]: the token, -1 in a row
  * whose logits are all -inf or NaN.  prob (or null): its share of the weight of
  * the tokens left (1 for the largest logit's, 0 for -1).  how null: all filters
- * off.  Histograms live in the library scratch of zlm_gpu_attention_enqueue (call
- * once before capture). */
+ * off.  Histograms live in the library scratch of zlm_gpu_paged_attention_enqueue (call
+ * once before its capture). */
 bool zlm_gpu_sample_enqueue(zlm_device *dev, const float *logits, uint64_t stride, uint32_t rows, uint32_t vocab,
                             const zlm_sampling *how, const float *u, int32_t *token, float *prob);
 

@@ -148,3 +148,51 @@ def test_prompts_then_steps(box, kind, window):
         if graph:
             dev.graph_destroy(graph)
         layer.free()
+
+
+def test_beside_a_captured_decode_step(dev):
+    """A graph of the contiguous attention replays as before while the paged attention and the sampler, which had not
+    run on this device object when it was captured, run eagerly between the replays."""
+    own = zd.Device()
+    assert own.available(), own.last_error()
+    box = _Box(own)
+    rng = np.random.default_rng(22)
+    heads, kv, hd, seq = 8, 2, 128, 300
+    q = rng.standard_normal((heads, hd)).astype(np.float32)
+    k, v = rng.standard_normal((2, kv, seq, hd)).astype(np.float16)
+    d_q, d_k, d_v, d_o = box.up(q), box.up(k), box.up(v), box.up(np.zeros_like(q))
+    pos = box.up(np.array([seq - 1], np.int32))
+
+    def contiguous():
+        assert own.attention_enqueue(d_q, d_k, d_v, heads, kv, hd, pos, seq, hd ** -0.5, d_o), own.last_error()
+
+    contiguous()
+    first = box.down(d_o, q)
+    assert np.isfinite(first).all() and first.any()
+    assert own.capture_begin(), own.last_error()
+    contiguous()
+    g = own.capture_end()
+    assert g, own.last_error()
+    b = paged.Batch([(1, 200), (3, 40)], PAGE, rng)
+    pool = paged.Pool(zd.F16, kv, hd, PAGE, b.n_pages)
+    paged.fill(pool, b, rng)
+    pq = rng.standard_normal((b.n_tokens, heads, hd)).astype(np.float32)
+    cache, batch, d_pq, d_po = box.cache(pool), box.batch(b), box.up(pq), box.up(pq)
+    x = rng.standard_normal((3, 5000)).astype(np.float32)
+    u = np.array([0.1, 0.5, 0.9], np.float32)
+    d_x, d_u, token = box.up(x), box.up(u), box.up(np.full(3, -9, np.int32))
+    try:
+        for _ in range(3):
+            assert own.sample_enqueue(d_x, 3, 5000, d_u, token), own.last_error()
+            assert own.paged_attention_enqueue(cache, batch, d_pq, d_po, heads, SCALE), own.last_error()
+            own.dev_upload(d_o, np.zeros_like(q))
+            own.graph_launch(g, 2)
+            np.testing.assert_array_equal(box.down(d_o, q), first)
+            want, bound = paged.attend(pool, b, pq, heads, SCALE)
+            assert (np.abs(box.down(d_po, pq) - want).max((1, 2)) <= bound).all()
+            got = box.down(token, np.zeros(3, np.int32))
+            assert [int(t) for t in got] == [draw(x[r], 1.0, 0, 1.0, 0.0, u[r])[0] for r in range(3)]
+    finally:
+        own.graph_destroy(g)
+        box.free()
+        own.deinit()

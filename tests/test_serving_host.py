@@ -6,7 +6,7 @@ import ctypes
 import pytest
 
 from zlm_amd import device as zd
-from tests.test_host_routes import MALLOCS, _Box, fake  # noqa: F401
+from tests.test_host_routes import FREES, MALLOCS, _Box, fake  # noqa: F401
 
 
 @pytest.fixture
@@ -138,6 +138,29 @@ def test_attention_workspace_is_made_eagerly(box):
     assert d.capture_begin()
     assert call(), d.last_error()
     d.graph_destroy(d.capture_end())
+
+
+@pytest.mark.parametrize("first", ["attention", "sample"])
+def test_serving_beside_a_captured_decode_step(box, first):
+    """A graph of the contiguous caches' attention holds its scratch; the serving calls need none of it."""
+    d, p = box.dev, 1 << 16
+    calls = {"attention": _calls(box, _cache(box.mod), _batch(box.mod))["attention"],
+             "sample": lambda: d.sample_enqueue(p, 4, 150000, p, p)}
+    contiguous = lambda: d.attention_enqueue(p, p, p, 8, 2, 128, p, 64, 0.1, p)  # noqa: E731
+    assert contiguous(), d.last_error()
+    assert d.capture_begin() and contiguous()
+    g = d.capture_end()
+    assert g, d.last_error()
+    held, freed = d.scratch_device_bytes(), box.stat(FREES)
+    for name in sorted(calls, key=lambda n: n != first):
+        assert calls[name](), (name, d.last_error())
+    assert d.scratch_device_bytes() >= held + (64 << 20) and box.stat(FREES) == freed
+    # nor do graphs of theirs hold the contiguous attention's
+    d.graph_destroy(g)
+    assert d.capture_begin() and all(call() for call in calls.values()), d.last_error()
+    g = d.capture_end()
+    assert d.attention_enqueue(p, p, p, 8, 2, 128, p, 4096, 0.1, p), d.last_error()
+    d.graph_destroy(g)
 
 
 def test_sampling_scratch_is_sized_eagerly(box):

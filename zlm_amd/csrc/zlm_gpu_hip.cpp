@@ -227,6 +227,7 @@ struct zlm_device {
         hipFunction_t append = nullptr, read = nullptr, few = nullptr, many = nullptr, merge_many = nullptr;
         hipFunction_t halved = nullptr;  // many's other form, heads of 256
     } paged[2][3];
+    float* serving = nullptr;          // kServingScratch bytes: the paged attention's partials, the sampler's histograms
     uint32_t* paged_counts = nullptr;  // the few-row attention's counters, one a workgroup; 0 between calls
     hipModule_t sample_mod = nullptr;
     hipFunction_t sample_hist = nullptr;
@@ -1848,6 +1849,7 @@ extern "C" void zlm_gpu_deinit(zlm_device* d) {
         if (d->d_y) hipFree(d->d_y);
         if (d->h_y) hipHostFree(d->h_y);
         if (d->attn_part) hipFree(d->attn_part);
+        if (d->serving) hipFree(d->serving);
         if (d->paged_counts) hipFree(d->paged_counts);
         if (d->d_mid) hipFree(d->d_mid);
         if (d->d_bx) hipFree(d->d_bx);
@@ -2860,12 +2862,11 @@ extern "C" bool zlm_gpu_qk_norm_rope_kv_enqueue(zlm_device* d, const float* qkv,
 
 namespace {
 
-// Size the attention partials (floats); the sampler's histograms live there
-// too.  Allocation happens on an eager call; a call under capture that would
-// need it fails.
-bool ensure_attn_scratch(zlm_device* d, size_t need, const char* what = "the attention scratch") {
+// Size the attention partials (floats).  Allocation happens on an eager call;
+// a call under capture that would need it fails.
+bool ensure_attn_scratch(zlm_device* d, size_t need) {
     if (need > d->attn_part_cap) {
-        if (!may_replace_scratch(d, kUsesAttn, what)) return false;
+        if (!may_replace_scratch(d, kUsesAttn, "the attention scratch")) return false;
         if (d->attn_part) {
             hipStreamSynchronize(d->stream);
             hipFree(d->attn_part);
@@ -2986,10 +2987,23 @@ extern "C" bool zlm_gpu_attention_enqueue(zlm_device* d, const float* q, const u
     return enqueue_attn_merge(d, part, nsplit, n_heads, out);
 }
 
-// The scratch that any paged attention or draw sizes at least: what the largest of
-// their launches need (34 MB the attention's partials with two workgroups a CU of
-// 256 CUs), so that a captured graph of one call never stands in another's way.
+// The scratch of the paged attention and the sampler, one buffer a device that the
+// first eager call of either makes.  Every launch of theirs fits it, so it is never
+// replaced: captured graphs hold its address without a count of them.  The few-row
+// attention's partials take two items of 16 rows a workgroup (8.5 MB at 512 workgroups
+// and heads of 128), the many-row attention's as many splits as fit, and the
+// sampler's rows go through it in as many launches as they need.
 constexpr uint64_t kServingScratch = 64ull << 20;
+
+namespace {
+
+bool ensure_serving_scratch(zlm_device* d, const char* what) {
+    if (d->serving) return true;
+    if (d->capturing) return fail(d, "%s must be made by an eager call before capture", what);
+    return ok(d, hipMalloc(reinterpret_cast<void**>(&d->serving), kServingScratch), "hipMalloc");
+}
+
+}  // namespace
 
 // ---- the paged KV cache: append, read back, attention ----
 
@@ -3156,13 +3170,11 @@ extern "C" bool zlm_gpu_paged_attention_enqueue(zlm_device* d, const zlm_paged_c
     const uint64_t want = static_cast<uint64_t>(d->cus) * (hd == 64 ? 2 : 1);
     const uint64_t room = kServingScratch / (items * tile_rows * (hd + 2) * sizeof(float) + 1);
     const uint32_t splits = many ? static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>({16, want / likely, room}))) : 1;
-    const size_t few_part = few ? static_cast<size_t>(grid) * 2 * 16 * (hd + 2) : 0;
-    const size_t many_part = splits > 1 ? items * splits * tile_rows * (hd + 2) : 0;
-    if (!ensure_attn_scratch(d, std::max({few_part, many_part, kServingScratch / sizeof(float)}))) return false;
+    if (!ensure_serving_scratch(d, "the attention's scratch")) return false;
     if (!ensure_paged_counts(d, static_cast<uint32_t>(d->cus) * 2)) return false;
     a.q = q;
     a.out = out;
-    a.part = d->attn_part;
+    a.part = d->serving;
     a.counts = d->paged_counts;
     a.n_heads = n_heads;
     a.group = group;
@@ -3199,9 +3211,9 @@ extern "C" bool zlm_gpu_sample_enqueue(zlm_device* d, const float* logits, uint6
         a.slices * ((zlm::kSampleBins + zlm::kSampleShort) * sizeof(uint64_t) + sizeof(zlm::SampleSlice));
     // rows of one launch: as many as the scratch has room for
     const uint32_t most = static_cast<uint32_t>(std::min<uint64_t>(kServingScratch / row_bytes, rows));
-    if (!ensure_attn_scratch(d, kServingScratch / sizeof(float), "the sampling scratch")) return false;
+    if (!ensure_serving_scratch(d, "the sampling scratch")) return false;
     const size_t all = static_cast<size_t>(most) * a.slices;
-    a.hist = reinterpret_cast<uint64_t*>(d->attn_part);
+    a.hist = reinterpret_cast<uint64_t*>(d->serving);
     a.shorts = a.hist + all * zlm::kSampleBins;
     a.info = reinterpret_cast<zlm::SampleSlice*>(a.shorts + all * zlm::kSampleShort);
     for (uint32_t r = 0; r < rows; r += most) {
@@ -3357,6 +3369,7 @@ extern "C" uint64_t zlm_gpu_scratch_device_bytes(const zlm_device* d) {
     uint64_t b = (d->x_cap + d->y_cap + d->bx_cap + d->mid_cap + d->attn_part_cap) * sizeof(float) +
                  d->q_scratch_cap + d->s_raw_cap + d->s_lay_cap;
     for (const Slot& sl : d->slots) b += sl.x_cap * sizeof(float);
+    if (d->serving) b += kServingScratch;
     if (d->paged_counts) b += static_cast<uint64_t>(d->cus) * 2 * sizeof(uint32_t);
     return b;
 }
