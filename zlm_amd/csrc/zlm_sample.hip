@@ -314,6 +314,7 @@ struct Goal {
     Mode mode;
     double w;      // kAtLeast, kMore: the cumulative weight
     uint32_t n;    // kCount: how many tokens; kKey: the smallest key
+    uint32_t b0 = 0, b1 = kBins - 1;  // the bins in question for it, whose tokens are listed
     __device__ bool reached(uint32_t count, double weight) const {
         return mode == kCount ? count >= n : mode == kAtLeast ? weight >= w : weight > w;
     }
@@ -404,6 +405,7 @@ public:
 
     __device__ __forceinline__ double weight_to(uint32_t end) const { return end ? sm_.weight[end - 1] : 0.0; }  // bins under `end`
     __device__ __forceinline__ uint32_t count_to(uint32_t end) const { return end ? sm_.count[end - 1] : 0; }
+    __device__ __forceinline__ uint32_t in_bin(uint32_t bin) const { return sm_.count[bin] - count_to(bin); }
 
     // The smallest and the largest key of a bin.
     __device__ __forceinline__ uint32_t first_key(uint32_t bin) const { return key_at(top_ - static_cast<double>(bin), rate_); }
@@ -416,9 +418,11 @@ public:
         return d < 1.0 * kBins ? static_cast<uint32_t>(__builtin_fmax(d, 0.0)) : kBins;
     }
 
-    // The first bin by whose end the goal is reached (kBins: none).
+    // The first bin with tokens by whose end the goal is reached; where none is (a rounding:
+    // no goal is past the row's weight), the last bin with tokens.
     __device__ __forceinline__ uint32_t bin_for(const Goal& g) {
-        return min(first_of(sm_, turn_, g.reached(sm_.count[tid_], sm_.weight[tid_]), tid_), kBins);
+        const uint32_t b = first_of(sm_, turn_, in_bin(tid_) && g.reached(sm_.count[tid_], sm_.weight[tid_]), tid_);
+        return b != kNone ? b : kBins - 1 - first_of(sm_, turn_, in_bin(kBins - 1 - tid_) != 0, tid_);
     }
 
     // Bins b0 .. b1 are in question.
@@ -430,7 +434,7 @@ public:
     // The number of the flagged bins' tokens.
     __device__ __forceinline__ uint32_t in_question() {
         __syncthreads();
-        const uint32_t c = block_scan(sm_, turn_, flagged(tid_) ? sm_.count[tid_] - count_to(tid_) : 0);
+        const uint32_t c = block_scan(sm_, turn_, flagged(tid_) ? in_bin(tid_) : 0);
         if (tid_ == kThreads - 1) sm_.step_n = c;
         __syncthreads();
         return sm_.step_n;
@@ -569,9 +573,11 @@ public:
     // Where a goal is reached.  Its bin's tokens, among those listed or in the row, are
     // counted and weighed in 512 equal ranges of (key, ~index); so again those of the
     // range in which it is reached, until they are few; a wave decides among these.  In
-    // a bin the weights are whole numbers, so every sum here is exact.
+    // a bin the weights are whole numbers, so every sum here is exact.  A goal is formed from
+    // sums in another order than the bins' ends and may lie a rounding past those of its
+    // bins in question: the nearest of these has the neighbouring token then.
     __device__ __forceinline__ Found find(const Goal& g, bool listed) {
-        const uint32_t b = g.mode == kKey ? bin_of(g.n) : bin_for(g);
+        const uint32_t b = g.mode == kKey ? bin_of(g.n) : min(max(bin_for(g), g.b0), g.b1);
         if (b >= kBins) return {0, weight_to(kBins)};  // a key under all that has weight
         const double base = weight_to(b), scale = sm_.scale[b];
         const uint32_t before = count_to(b);
@@ -614,8 +620,11 @@ public:
             const uint32_t c = count + block_scan(sm_, turn_, own);
             const uint64_t w = weight + block_scan(sm_, turn_, own_w);
             uint32_t at = first_of(sm_, turn_, own && g.reached(before + c, base + static_cast<double>(w) * scale), tid_);
-            if (at == kNone)  // missed by a rounding: the last token
-                at = kThreads - 1 - first_of(sm_, turn_, sm_.sub_count[kThreads - 1 - tid_] != 0, tid_);
+            if (at == kNone) {  // missed by a rounding: the last token
+                const uint32_t from_end = first_of(sm_, turn_, sm_.sub_count[kThreads - 1 - tid_] != 0, tid_);
+                if (from_end == kNone) break;  // no token: the logits are not those that were counted
+                at = kThreads - 1 - from_end;
+            }
             if (tid_ == at) {
                 sm_.step_n = own;
                 sm_.step_count = c - own;
@@ -657,6 +666,7 @@ public:
         const uint64_t at = __ballot(own == token && lane < n);
         const uint64_t sum = lane_of(w, at ? __builtin_ctzll(at) : 0);
         __syncthreads();
+        if (n == 0) return {0, base};
         return {token, base + static_cast<double>(sum) * scale};
     }
 
@@ -780,17 +790,19 @@ __device__ __forceinline__ void pick(const Args& a) {
     // The bins in question.  A cut falls within a bin, so the weight that is left after
     // it lies between two bins' ends, and the next goal in the bins that these make.
     double w0 = total, w1 = total;
+    uint32_t k_bin = 0, p_bins[2] = {0, 0};
     if (by_k) {
-        const uint32_t b = r.bin_for({kCount, 0.0, f.k});
-        r.flag(b, b);
-        w0 = r.weight_to(b);
-        w1 = r.weight_to(b + 1);
+        k_bin = r.bin_for({kCount, 0.0, f.k});
+        r.flag(k_bin, k_bin);
+        w0 = r.weight_to(k_bin);
+        w1 = r.weight_to(k_bin + 1);
     }
     if (f.by_p) {
-        const uint32_t b0 = r.bin_for({kAtLeast, w0 * f.p, 0}), b1 = min(r.bin_for({kAtLeast, w1 * f.p, 0}), kBins - 1);
-        r.flag(b0, b1);
-        w0 = r.weight_to(min(b0, kBins - 1));
-        w1 = __builtin_fmin(w1, r.weight_to(b1 + 1));
+        p_bins[0] = r.bin_for({kAtLeast, w0 * f.p, 0});
+        p_bins[1] = r.bin_for({kAtLeast, w1 * f.p, 0});
+        r.flag(p_bins[0], p_bins[1]);
+        w0 = r.weight_to(p_bins[0]);
+        w1 = __builtin_fmin(w1, r.weight_to(p_bins[1] + 1));
     }
     if (f.by_min) {
         const uint32_t b = r.bin_of(f.min_key);
@@ -800,31 +812,32 @@ __device__ __forceinline__ void pick(const Args& a) {
             w1 = __builtin_fmin(w1, r.weight_to(b + 1));
         }
     }
-    r.flag(r.bin_for({kMore, w0 * f.u, 0}), min(r.bin_for({kMore, w1 * f.u, 0}), kBins - 1));
+    const uint32_t u_bins[2] = {r.bin_for({kMore, w0 * f.u, 0}), r.bin_for({kMore, w1 * f.u, 0})};
+    r.flag(u_bins[0], u_bins[1]);
     const bool listed = r.in_question() <= kList;
     if (listed && !r.list_shorts(ahead)) r.list_row();
     // the filters in turn, then the draw
     Found cut = {0, total};  // the last token kept, and the weight of all that are
     double p_weight = total;
     for (int step = 0; step < 4; step++) {
-        Goal g = {kMore, cut.weight * f.u, 0};  // the draw
+        Goal g = {kMore, cut.weight * f.u, 0, u_bins[0], u_bins[1]};  // the draw
         if (step == 0) {
             if (!by_k) continue;
-            g = {kCount, 0.0, f.k};
+            g = {kCount, 0.0, f.k, k_bin, k_bin};
         } else if (step == 1) {
             p_weight = cut.weight * f.p;  // top-p is of what top-k left
             if (!f.by_min || f.min_key <= cut.token >> 32) continue;
             g = {kKey, 0.0, f.min_key};
         } else if (step == 2) {
             if (!f.by_p || p_weight >= cut.weight) continue;
-            g = {kAtLeast, p_weight, 0};
+            g = {kAtLeast, p_weight, 0, p_bins[0], p_bins[1]};
         }
         const Found t = r.find(g, listed);
         if (step < 3) {
             if (t.token > cut.token) cut = t;
         } else if (tid == 0) {
             a.token[row] = static_cast<int32_t>(~static_cast<uint32_t>(t.token));
-            if (a.prob) a.prob[row] = static_cast<float>(r.weight_at(t.token) / cut.weight);
+            if (a.prob) a.prob[row] = t.token ? static_cast<float>(r.weight_at(t.token) / cut.weight) : 0.0f;
         }
     }
 }
