@@ -396,6 +396,7 @@ public:
                 }
             }
         }
+        own_ = count;
         const uint32_t c = block_scan(sm_, turn_, count);
         const double w = block_scan(sm_, turn_, static_cast<double>(weight) * sm_.scale[tid_]);
         sm_.count[tid_] = c;
@@ -405,7 +406,6 @@ public:
 
     __device__ __forceinline__ double weight_to(uint32_t end) const { return end ? sm_.weight[end - 1] : 0.0; }  // bins under `end`
     __device__ __forceinline__ uint32_t count_to(uint32_t end) const { return end ? sm_.count[end - 1] : 0; }
-    __device__ __forceinline__ uint32_t in_bin(uint32_t bin) const { return sm_.count[bin] - count_to(bin); }
 
     // The smallest and the largest key of a bin.
     __device__ __forceinline__ uint32_t first_key(uint32_t bin) const { return key_at(top_ - static_cast<double>(bin), rate_); }
@@ -421,8 +421,8 @@ public:
     // The first bin with tokens by whose end the goal is reached; where none is (a rounding:
     // no goal is past the row's weight), the last bin with tokens.
     __device__ __forceinline__ uint32_t bin_for(const Goal& g) {
-        const uint32_t b = first_of(sm_, turn_, in_bin(tid_) && g.reached(sm_.count[tid_], sm_.weight[tid_]), tid_);
-        return b != kNone ? b : kBins - 1 - first_of(sm_, turn_, in_bin(kBins - 1 - tid_) != 0, tid_);
+        const uint32_t b = first_of(sm_, turn_, own_ && g.reached(sm_.count[tid_], sm_.weight[tid_]), tid_);
+        return b != kNone ? b : kBins - 1 - first_of(sm_, turn_, sm_.count[kBins - 1 - tid_] != count_to(kBins - 1 - tid_), tid_);
     }
 
     // Bins b0 .. b1 are in question.
@@ -434,7 +434,7 @@ public:
     // The number of the flagged bins' tokens.
     __device__ __forceinline__ uint32_t in_question() {
         __syncthreads();
-        const uint32_t c = block_scan(sm_, turn_, flagged(tid_) ? in_bin(tid_) : 0);
+        const uint32_t c = block_scan(sm_, turn_, flagged(tid_) ? own_ : 0);
         if (tid_ == kThreads - 1) sm_.step_n = c;
         __syncthreads();
         return sm_.step_n;
@@ -697,7 +697,7 @@ private:
     uint64_t best_;
     double top_;
     const Weight weight_;
-    uint32_t turn_ = 0, n_ = 0;  // n_: tokens listed
+    uint32_t turn_ = 0, n_ = 0, own_ = 0;  // n_: tokens listed; own_: the tokens of bin tid_
 };
 
 // The smallest key that min-p keeps: e^((x - max) / T) >= p (p in (0, 1]).  The
