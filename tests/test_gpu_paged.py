@@ -151,6 +151,26 @@ def test_append_of_values_at_the_borders(box, kind):
         np.testing.assert_array_equal(g, w)
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("pos", [0, 5, 90])
+def test_largest_of_a_rotated_block(box, hd, pos):
+    """Values of one size and both signs, which the rotation moves apart by less than 32 bits hold: the first of the
+    largest in 64 bits gives the scale its sign."""
+    kv, page = 2, 16
+    _say(f"append ties hd={hd} pos={pos}")
+    rng = np.random.default_rng(hd + pos)
+    b = paged.Batch([(1, pos + 1)] * 4, page, rng)
+    pool = paged.Pool(zd.Q4_0, kv, hd, page, b.n_pages, fill=rng)
+    qkv = np.zeros((4, 1 + 2 * kv, hd), np.float32)
+    qkv[:, 1:1 + kv, :hd // 2] = 8.0 * rng.choice([-1, 1], (4, kv, hd // 2))
+    cache, batch = box.cache(pool), box.batch(b)
+    d_qkv, d_q = box.up(qkv), box.up(np.zeros((4, hd), np.float32))
+    assert box.dev.paged_append_enqueue(cache, batch, d_qkv, d_q, 1, EPS, BASE), box.dev.last_error()
+    got = box.down(box.k, pool.k)
+    paged.append(pool, b, qkv.reshape(4, -1), 1, EPS, BASE)
+    np.testing.assert_array_equal(got, pool.k)
+
+
 ATTENDS = [
     # (lens, window): one position, borders of the 32-position blocks, the 128-position units and of pages
     ([(1, 1)], 0),

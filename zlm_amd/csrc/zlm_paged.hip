@@ -161,7 +161,24 @@ __device__ __forceinline__ uint32_t quantise(T x, uint32_t lane, _Float16* d_out
     mx = __builtin_fmaxf(mx, dpp<kMirror>(mx));
     mx = __builtin_fmaxf(mx, __builtin_bit_cast(float, next_row(__builtin_bit_cast(uint32_t, mx))));
     const auto half = [&](uint64_t b) { return static_cast<uint32_t>(lane & 32 ? b >> 32 : b); };
-    const uint32_t at = half(__ballot(a == mx)), negative = half(__ballot(xf < 0.0f));
+    uint64_t largest = __ballot(a == mx);
+    if constexpr (sizeof(T) > sizeof(float)) {
+        // several that are one number in 32 bits (a tie, rare past blocks of zeros): the largest in 64
+        const uint64_t low = largest & 0xffffffffull, high = largest >> 32;
+        if ((low & (low - 1)) | (high & (high - 1))) {
+            const T b = a == mx ? __builtin_fabs(x) : T(0);
+            T top = b;
+            top = __builtin_fmax(top, dpp<kXor1>(top));
+            top = __builtin_fmax(top, dpp<kXor2>(top));
+            top = __builtin_fmax(top, dpp<kHalfMirror>(top));
+            top = __builtin_fmax(top, dpp<kMirror>(top));
+            const uint64_t u = __builtin_bit_cast(uint64_t, top);
+            top = __builtin_fmax(top, __builtin_bit_cast(T, static_cast<uint64_t>(next_row(static_cast<uint32_t>(u >> 32))) << 32 |
+                                                                next_row(static_cast<uint32_t>(u))));
+            largest &= __ballot(b == top);
+        }
+    }
+    const uint32_t at = half(largest), negative = half(__ballot(xf < 0.0f));
     const bool nan = half(__ballot(xf != xf)) != 0;
     const bool minus = (negative & at & (0u - at)) != 0;  // the first's sign
     // -m/8 to 8 significant bits (bf16), then to f16 (further only below its normal range)
