@@ -307,7 +307,7 @@ __device__ __forceinline__ void append(const AppendArgs& a) {
             if constexpr (!Q4) {
                 _Float16* dst = reinterpret_cast<_Float16*>(base) + off * HD;
 #pragma unroll
-                for (int j = 0; j < N; j++) dst[lane + 64 * j] = static_cast<_Float16>(static_cast<float>(y[j]));
+                for (int j = 0; j < N; j++) dst[lane + 64 * j] = static_cast<_Float16>(y[j]);  // one rounding
             } else {
 #pragma unroll
                 for (int j = 0; j < N; j++) {
