@@ -450,7 +450,8 @@ typedef struct {
  * may have no rows.  Rows at negative positions (kv_len below the row count)
  * are padding, rows from q_start[n_seqs] on are not touched.  A page number
  * outside [0, n_pages) is no page: nothing is appended there, and what reads a
- * position there becomes NaN.  Sequences may share pages that none of them
+ * position there becomes NaN; so does the attention of rows past position
+ * 2^31 - 257.  Sequences may share pages that none of them
  * appends to; two rows of one call never write one position. */
 typedef struct {
     uint32_t n_seqs;         /* at most 1024 */

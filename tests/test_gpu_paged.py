@@ -449,6 +449,38 @@ def test_pages_past_32_bits(box, kind):
     np.testing.assert_allclose(q, ref, rtol=2.0 ** -23, atol=1e-9)
 
 
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 40])
+def test_last_positions(box, kind, hd, rows):
+    """Windows that end at the last position a sequence can have, few rows and many (one page stands for all), and rows
+    past it."""
+    page, group, window, last = 256, 4, 40, (1 << 31) - 256
+    _say(f"last positions kind={kind} hd={hd} rows={rows}")
+    rng = np.random.default_rng(hd + rows)
+    b = paged.Batch([(rows, page)], page, rng, spare=0)
+    pool = paged.Pool(kind, 1, hd, page, b.n_pages)
+    paged.fill(pool, b, rng)
+    q = rng.standard_normal((rows, group, hd)).astype(np.float32)
+    stride = (1 << 31) // page
+    kv_len, d_q, d_o = box.up(np.array([last], np.int32)), box.up(q), box.up(np.full_like(q, 7))
+    batch = zd.PagedBatch(1, rows, box.up(np.array([0, rows], np.int32)), kv_len, box.up(np.zeros((1, stride), np.int32)),
+                          stride)
+    cache = box.cache(pool)
+
+    def run():
+        assert box.dev.paged_attention_enqueue(cache, batch, d_q, d_o, group, hd ** -0.5, window=window), \
+            box.dev.last_error()
+        return box.down(d_o, q)
+
+    want, bound = paged.attend(pool, b, q, group, hd ** -0.5, window)
+    assert (np.abs(run() - want).max((1, 2)) <= bound).all()
+    for past in (1, 255):
+        box.dev.dev_upload(kv_len, np.array([last + past], np.int32))
+        got = run()
+        assert np.isnan(got[max(0, rows - past):]).all() and np.isfinite(got[:max(0, rows - past)]).all()
+
+
 def test_nan_in_one_sequence_stays_there(box):
     hd, page, kv, group = 128, 16, 1, 4
     rng = np.random.default_rng(9)

@@ -807,10 +807,11 @@ struct SeqWork {
     uint32_t tiles, units;          // per tile and head
 };
 
-// Positions that a sequence's pages can hold.  A row past them sees positions
-// that are nowhere: it becomes NaN.
+// Positions that a sequence can have: what its pages hold, and no more than leaves the
+// ends of the blocks and units around the last one below 2^31.  A row past them sees
+// positions that are nowhere: it becomes NaN.
 __device__ __forceinline__ uint64_t capacity(const Paged& p) {
-    return static_cast<uint64_t>(p.table_stride) << p.page_shift;
+    return min(static_cast<uint64_t>(p.table_stride) << p.page_shift, static_cast<uint64_t>((1u << 31) - 2 * kUnit));
 }
 
 __device__ __forceinline__ SeqWork seq_work(const AttnArgs& a, int32_t row0, int32_t row1, int32_t kv) {
