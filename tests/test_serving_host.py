@@ -76,6 +76,23 @@ def test_other_arguments_are_refused(box):
     assert not raw.zlm_gpu_paged_read_enqueue(d._h, ctypes.byref(c.c), None, p, p)
 
 
+@pytest.mark.parametrize("op", ["append", "read", "attention"])
+def test_tokens_of_a_batch_are_below_2_24(box, op):
+    cache = _cache(box.mod)
+    assert _calls(box, cache, _batch(box.mod, tokens=(1 << 24) - 1))[op](), box.dev.last_error()
+    assert not _calls(box, cache, _batch(box.mod, tokens=1 << 24))[op]()
+    assert "tokens" in box.dev.last_error()
+
+
+def test_more_attention_than_a_call_counts_is_refused(box):
+    """2^11 tokens of 128 q heads over tables of 2^24 positions; half of these is taken."""
+    d, p, cache = box.dev, 1 << 16, _cache(box.mod, kv=1)
+    ask = lambda stride: d.paged_attention_enqueue(  # noqa: E731
+        cache, _batch(box.mod, seqs=10, tokens=1 << 11, stride=stride), p, p, 128, 0.1)
+    assert not ask(1 << 18) and "too large for one call" in d.last_error()
+    assert ask(1 << 17), d.last_error()
+
+
 def test_an_empty_batch_launches_nothing(box):
     box.dev.launch_log(True)
     for empty in (dict(seqs=0), dict(tokens=0)):

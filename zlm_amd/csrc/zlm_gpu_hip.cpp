@@ -3024,7 +3024,8 @@ bool paged_block(zlm_device* d, const zlm_paged_cache* c, const zlm_paged_batch*
     while (shift < 9 && (1u << shift) != c->page_size) shift++;
     if (shift == 9) return fail(d, "pages hold 16, 32, 64, 128 or 256 positions (got %u)", c->page_size);
     if (b->n_seqs > zlm::kPagedMaxSeqs) return fail(d, "a batch holds at most %u sequences (got %u)", zlm::kPagedMaxSeqs, b->n_seqs);
-    if (b->n_tokens > (1u << 24)) return fail(d, "a batch holds at most %u tokens (got %u)", 1u << 24, b->n_tokens);
+    if (b->n_tokens >= (1u << 24))  // a workgroup of 256 threads a row: fewer than 2^32 work-items
+        return fail(d, "a batch is too large: %u tokens where at most %u go in one", b->n_tokens, (1u << 24) - 1);
     if (b->n_seqs == 0 || b->n_tokens == 0) return true;
     if (!c->k || !c->v || !b->q_start || !b->kv_len || !b->table) return fail(d, "null buffer");
     if (reinterpret_cast<uintptr_t>(c->k) % 16 || reinterpret_cast<uintptr_t>(c->v) % 16)
