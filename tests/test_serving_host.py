@@ -233,3 +233,13 @@ def test_an_inert_device_refuses():
     assert not dev.paged_read_enqueue(c, b, 16, 16)
     assert not dev.paged_attention_enqueue(c, b, 16, 16, 1, 1.0)
     dev.deinit()
+
+
+def test_rows_of_a_draw_up_to_32_bits(box):
+    """The rows go in launches of some thousands: their count ends below 2^32 rows too."""
+    d, p = box.dev, 1 << 16
+    d.launch_log(True)
+    assert d.sample_enqueue(p, (1 << 32) - 1, 1, p, p), d.last_error()
+    rows = [r["grid_x"] for r in d.launch_log_read() if r["what"] == "sample"]
+    assert len(set(rows[:-1])) == 1 and rows[0] > 1000
+    d.launch_log(False)

@@ -3217,8 +3217,8 @@ extern "C" bool zlm_gpu_sample_enqueue(zlm_device* d, const float* logits, uint6
     a.hist = reinterpret_cast<uint64_t*>(d->serving);
     a.shorts = a.hist + all * zlm::kSampleBins;
     a.info = reinterpret_cast<zlm::SampleSlice*>(a.shorts + all * zlm::kSampleShort);
-    for (uint32_t r = 0; r < rows; r += most) {
-        a.rows = std::min(most, rows - r);
+    for (uint64_t r = 0; r < rows; r += most) {  // 64 bits: the last step may pass 32
+        a.rows = static_cast<uint32_t>(std::min<uint64_t>(most, rows - r));
         a.logits = logits + r * stride;
         a.temperature = how && how->temperature ? how->temperature + r : nullptr;
         a.top_k = how && how->top_k ? how->top_k + r : nullptr;
