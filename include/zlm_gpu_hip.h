@@ -482,9 +482,10 @@ bool zlm_gpu_paged_read_enqueue(zlm_device *dev, const zlm_paged_cache *cache, c
                                 float *k_out, float *v_out);
 /* Attention of every row over the positions [max(0, p - window + 1), p] of its
  * sequence (p: the row's position; window 0: all from 0), scores scaled by
- * `scale`, q heads dealt to kv heads in order (n_heads / n_kv_heads each); q and
- * out: n_tokens x n_heads*hd floats, 16-byte aligned.  One token a sequence, a
- * prompt's chunk, or both in one batch.  The results have the accuracy of 32-bit
+ * `scale` (finite, below 2.3e38 in size), q heads dealt to kv heads in order
+ * (n_heads / n_kv_heads each); q and out: n_tokens x n_heads*hd floats, 16-byte
+ * aligned, apart from each other.  One token a sequence, a prompt's chunk, or both
+ * in one batch.  The results have the accuracy of 32-bit
  * products and sums over the cached values.  A padding row's output is 0.  NaN or
  * infinite K reaches the rows that see its position only; such a V may make NaN
  * of other rows of its sequence in the same call, never of another sequence's.

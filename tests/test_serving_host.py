@@ -93,6 +93,15 @@ def test_more_attention_than_a_call_counts_is_refused(box):
     assert ask(1 << 17), d.last_error()
 
 
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), float("-inf"), 3e38])
+def test_scales_without_a_product_are_refused(box, scale):
+    """Scores times a NaN or an infinity (3e38 times log2 e is one) are in no order."""
+    d, p = box.dev, 1 << 16
+    assert not d.paged_attention_enqueue(_cache(box.mod), _batch(box.mod), p, p, 8, scale)
+    assert "scale" in d.last_error()
+    assert d.paged_attention_enqueue(_cache(box.mod), _batch(box.mod), p, p, 8, 2e38), d.last_error()
+
+
 def test_an_empty_batch_launches_nothing(box):
     box.dev.launch_log(True)
     for empty in (dict(seqs=0), dict(tokens=0)):

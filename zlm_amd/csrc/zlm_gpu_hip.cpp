@@ -3128,6 +3128,8 @@ extern "C" bool zlm_gpu_paged_attention_enqueue(zlm_device* d, const zlm_paged_c
     if (n_heads == 0 || n_heads > 16384 || n_heads % cache->n_kv_heads)
         return fail(d, "%u q heads over %u kv heads", n_heads, cache->n_kv_heads);
     if (window > 0x7fffffffu) return fail(d, "bad attention window");
+    const float scale2 = scale * 1.44269504088896340736f;  // the exponents' base is two
+    if (!std::isfinite(scale2)) return fail(d, "the attention's scale is not finite, or past 2.3e38");
     if (!k) return true;
     if (!q || !out) return fail(d, "null buffer");
     if (reinterpret_cast<uintptr_t>(q) % 16 || reinterpret_cast<uintptr_t>(out) % 16)
@@ -3180,7 +3182,7 @@ extern "C" bool zlm_gpu_paged_attention_enqueue(zlm_device* d, const zlm_paged_c
     a.n_heads = n_heads;
     a.group = group;
     a.window = window;
-    a.scale = scale * 1.44269504088896340736f;
+    a.scale = scale2;
     a.few_rows = !few ? 0 : many ? few_rows : 0xffffffffu;
     a.splits = splits;
     void* args[] = {&a};
