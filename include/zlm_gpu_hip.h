@@ -437,7 +437,7 @@ bool zlm_gpu_attention_decode_enqueue_noalloc(zlm_device *dev, const float *qkv,
 typedef struct {
     void *k, *v;           /* device pools */
     uint32_t type;         /* ZLM_GGML_F16 or ZLM_GGML_Q4_0 */
-    uint32_t n_kv_heads;
+    uint32_t n_kv_heads;   /* 1 to 1024 */
     uint32_t head_dim;     /* 64, 128 or 256 */
     uint32_t page_size;    /* 16, 32, 64, 128 or 256 positions */
     uint32_t n_pages;

@@ -233,6 +233,12 @@ def test_page_bytes():
         assert zd.paged_page_bytes(*bad) == 0
 
 
+def test_page_bytes_of_heads_that_no_call_takes():
+    assert zd.paged_page_bytes(zd.F16, 1024, 256, 256) == 1024 * 256 * 512
+    for kv in (0, 1025, 2000, 0xFFFFFFFF):
+        assert zd.paged_page_bytes(zd.F16, kv, 128, 64) == 0
+
+
 def test_an_inert_device_refuses():
     dev = zd.Device()
     if dev.available():

@@ -52,6 +52,7 @@ constexpr uint32_t kNoLayout = 0xffffffffu;
 constexpr uint32_t kUsesAttn = 1u;  // the attention partials
 constexpr uint32_t kUsesGemm = 2u;  // the GEMM's quantized activations and the residents' GEMM tiles
 constexpr int kPagedDims[] = {64, 128, 256};  // head sizes of the paged kernels
+constexpr uint32_t kPagedKvHeads = 1024;      // their kv heads at most
 constexpr uint32_t kQ4kRecords = 0xfffffffeu;
 constexpr uint32_t kQ6kRecords = 0xfffffffdu;
 
@@ -3019,7 +3020,7 @@ bool paged_block(zlm_device* d, const zlm_paged_cache* c, const zlm_paged_batch*
     int dim = 0;
     while (dim < 3 && kPagedDims[dim] != static_cast<int>(c->head_dim)) dim++;
     if (dim == 3) return fail(d, "a paged cache has heads of 64, 128 or 256 (got %u)", c->head_dim);
-    if (c->n_kv_heads == 0 || c->n_kv_heads > 1024) return fail(d, "bad kv head count %u", c->n_kv_heads);
+    if (c->n_kv_heads == 0 || c->n_kv_heads > kPagedKvHeads) return fail(d, "bad kv head count %u", c->n_kv_heads);
     uint32_t shift = 4;
     while (shift < 9 && (1u << shift) != c->page_size) shift++;
     if (shift == 9) return fail(d, "pages hold 16, 32, 64, 128 or 256 positions (got %u)", c->page_size);
@@ -3059,7 +3060,7 @@ bool ensure_paged_counts(zlm_device* d, uint32_t n) {
 extern "C" uint64_t zlm_gpu_paged_page_bytes(uint32_t type, uint32_t n_kv_heads, uint32_t head_dim, uint32_t page_size) {
     const bool dim_ok = head_dim == 64 || head_dim == 128 || head_dim == 256;
     const bool page_ok = page_size >= 16 && page_size <= 256 && (page_size & (page_size - 1)) == 0;
-    if (!dim_ok || !page_ok || (type != ZLM_GGML_F16 && type != ZLM_GGML_Q4_0)) return 0;
+    if (!dim_ok || !page_ok || n_kv_heads > kPagedKvHeads || (type != ZLM_GGML_F16 && type != ZLM_GGML_Q4_0)) return 0;
     const uint64_t row = type == ZLM_GGML_F16 ? 2 * head_dim : head_dim / 2 + head_dim / 16;
     return row * page_size * n_kv_heads;
 }
