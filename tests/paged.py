@@ -195,3 +195,95 @@ def attend(pool, batch, q, n_heads, scale, window=0):
             e = a * (2.0 ** -22 + 2 * hd * 2.0 ** -24) + 2.0 ** -20 + (n / 32 + 64) * 2.0 ** -24 + n * 2.0 ** -30
             bound[row] = max(bound[row], 2 * e * np.abs(v[:, h // g]).max())
     return out, bound
+
+
+class TwoParts:
+    """A case of the attention whose result is known to a few 1e-6, and is off by many times that where q or the
+    probabilities enter a product as one f16 instead of two.
+
+    K of position j is g(j) c with g = 1, 0, -1, 1, .. and c of ones and minus ones; q is a sign a dim plus 2^-12 c.
+    So a row has three scores, 0 and plus and minus one number; every product and sum of q and K is exact in 32 bits;
+    and what lies behind q's first 11 bits adds up: 2^-12 hd of a raw score of hd/4 at most.  V is u(g), whole numbers,
+    so the parts of a probability that are lost add up too."""
+
+    def __init__(self, kind, n_kv, hd, group, page, lens, window=0, seed=0):
+        rng = np.random.default_rng(seed)
+        self.heads, self.hd, self.window, self.scale = n_kv * group, hd, window, np.float32(5.2 / hd)
+        self.batch = b = Batch(lens, page, rng, behind=1)
+        self.pool = Pool(kind, n_kv, hd, page, b.n_pages)
+        self.c = rng.choice([-1, 1], (n_kv, hd))
+        self.u = rng.integers(-8, 8, (3, n_kv, hd))  # by g + 1
+        self.u[:, :, 0] = [[-8], [7], [7]]  # two dims that show most of a weight
+        self.u[:, :, 1] = [[7], [7], [-8]]
+        one = np.ones((n_kv, hd // 32), np.float16)
+        for s, (_, end) in enumerate(lens):
+            for p in range(end):
+                k, v = self.g(p) * self.c, self.u[self.g(p) + 1]
+                spot = b.spot(s, p)
+                if kind == zd.F16:
+                    self.pool.write(*spot, k, v)
+                else:
+                    self.pool.put(*spot, (k + 8).astype(np.uint8), one, (v + 8).astype(np.uint8), one)
+        # signs of q: half the dims like c's and up to an eighth more, or fewer
+        m = hd // 2 + rng.integers(-(hd // 8), hd // 8 + 1, (b.n_tokens, self.heads))
+        like = rng.permuted(np.broadcast_to(np.arange(hd), (b.n_tokens, self.heads, hd)), axis=-1) < m[..., None]
+        c = np.repeat(self.c, group, 0)
+        self.signs = np.where(like, c, -c)
+        self.q = (self.signs + 2.0 ** -12 * c).astype(np.float32)
+        assert (self.q == self.signs + 2.0 ** -12 * c).all()
+
+    @staticmethod
+    def g(p):
+        return (p + 2) % 3 - 1  # 1, -1, 0, 1, ..
+
+    def _rows(self):
+        """(row, first and last position it sees) of the rows that see any."""
+        at = [(r, max(0, p - self.window + 1) if self.window else 0, p) for r, _, p in self.batch.places() if p >= 0]
+        return np.array(at).T
+
+    def want(self, q_parts=2, p_parts=2):
+        """The result in 64 bits (rows of no sequence NaN); with one part: what one f16 of q, or of the probabilities
+        (scaled as the kernels scale them: 2^6 at the largest), makes of it."""
+        out = np.full(self.q.shape, np.nan)
+        row, lo, hi = self._rows()
+        c = np.repeat(self.c, self.heads // len(self.c), 0)
+        q = self.q.astype(np.float64) if q_parts == 2 else self.q.astype(np.float16).astype(np.float64)
+        s = (q[row] * c).sum(-1) * np.float64(self.scale)  # of g = 1
+        g = np.arange(-1, 2)
+        seen = (self.g(np.arange(hi.max() + 1))[None] == g[:, None]).cumsum(1)
+        n = seen[:, hi] - np.where(lo > 0, seen[:, lo - 1], 0)  # [3, rows]
+        e = g[:, None, None] * s[None]
+        top = np.where(n[:, :, None] > 0, e, -np.inf).max(0)
+        w = np.exp(e - top) * 64
+        first = w if p_parts == 2 else w.astype(np.float16).astype(np.float64)
+        total = (n[:, :, None] * w).sum(0)
+        u = np.repeat(self.u, self.heads // len(self.c), 1).astype(np.float64)
+        out[row] = np.einsum("grh,ghd->rhd", n[:, :, None] * first, u) / total[..., None]
+        return out
+
+    def limit(self):
+        """How far the kernels may be off.  In units of 2^-24, for exponents of two of A = 2.5 at most (1.3 of the raw
+        score of hd/4 and its 2^-10, times log2 e, is 1.9): the factor of the scores is rounded twice (4 A), an
+        exponent once (2 A + 6) and its base once (A + 6), three joins of sums round a difference of maxima (2 A each):
+        times ln 2; exp2 and the joins' factors and products 2 + 3 x 3; the two parts of a probability leave 2^-20 (16).
+        That is a weight's share; the result moves by twice it, and by the roundings of the sums, eight for every 32
+        positions of a wave that takes them all and 64 for the rest, each once of the largest value, 8."""
+        a = 2.5
+        weight = np.log(2) * (4 * a + 2 * a + 6 + a + 6 + 3 * 2 * a) + 2 + 9 + 16
+        _, lo, hi = self._rows()
+        return 8 * 2.0 ** -24 * (2 * weight + (hi - lo + 1).max() / 4 + 64)
+
+
+# One case a route of the attention: (heads, rows and positions, window)
+TWO_PARTS = {
+    "few": dict(n_kv=1, hd=128, group=4, page=64, lens=[(1, 300), (2, 90)]),
+    "few, short": dict(n_kv=2, hd=64, group=8, page=16, lens=[(1, 30)] * 5),
+    "few, heads of 256": dict(n_kv=2, hd=256, group=3, page=32, lens=[(1, 200), (1, 500)]),
+    "many and merge, heads of 64": dict(n_kv=1, hd=64, group=4, page=32, lens=[(70, 700)]),
+    "many and merge": dict(n_kv=1, hd=128, group=4, page=32, lens=[(70, 700)]),
+    "halved and merge": dict(n_kv=1, hd=256, group=4, page=32, lens=[(70, 700)]),
+    "many": dict(n_kv=8, hd=128, group=4, page=64, lens=[(2100, 2100)], window=100),
+    "many, heads of 64": dict(n_kv=8, hd=64, group=8, page=64, lens=[(1050, 1050)], window=100),
+    "many, heads of 256": dict(n_kv=8, hd=256, group=2, page=64, lens=[(1100, 1100)], window=100),
+    "halved": dict(n_kv=8, hd=256, group=2, page=64, lens=[(520, 600), (1, 40)], window=100),
+}

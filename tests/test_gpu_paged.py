@@ -232,6 +232,30 @@ def test_attention_over_many_shares(box, kind, lens):
 
 
 @pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("route", paged.TWO_PARTS)
+def test_both_parts_of_q_and_of_the_probabilities(box, kind, route):
+    """Every route at the accuracy that 32-bit products have; one f16 part in place of two is off by more (shown for
+    the oracle on the CPU)."""
+    _say(f"attention parts kind={kind} {route}")
+    x = paged.TwoParts(kind, **paged.TWO_PARTS[route])
+    cache, batch = box.cache(x.pool), box.batch(x.batch)
+    d_q, d_o = box.up(x.q), box.up(np.full_like(x.q, 7))
+    assert box.dev.launch_log(True)
+    assert box.dev.paged_attention_enqueue(cache, batch, d_q, d_o, x.heads, float(x.scale), window=x.window), \
+        box.dev.last_error()
+    log = [(r["what"], r["block"]) for r in box.dev.launch_log_read()]
+    box.dev.launch_log(False)
+    names = [w for w, _ in log]
+    assert ("paged attention of many rows" in names) == ("few" not in route)
+    assert "merge" not in route or "paged attention of many rows, merge" in names
+    if x.hd == 256 and "few" not in route:
+        assert log[0][1] == (512 if "halved" in route else 256)
+    got, want = box.down(d_o, x.q).astype(np.float64), x.want()
+    assert (got[-1] == 7).all()
+    assert np.abs(got[:-1] - want[:-1]).max() <= x.limit()
+
+
+@pytest.mark.parametrize("kind", TYPES)
 def test_missing_pages_poison_the_rows_that_see_them(box, kind):
     hd, page, kv, group = 64, 16, 2, 2
     _say(f"attention missing pages kind={kind}")

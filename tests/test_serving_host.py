@@ -3,8 +3,10 @@ GPU: the host library over the stand-in runtime (tests/fake_hip.cpp), whose
 kernels do nothing.  Addresses are not read here."""
 import ctypes
 
+import numpy as np
 import pytest
 
+from tests import paged
 from zlm_amd import device as zd
 from tests.test_host_routes import FREES, MALLOCS, _Box, fake  # noqa: F401
 
@@ -258,3 +260,17 @@ def test_rows_of_a_draw_up_to_32_bits(box):
     rows = [r["grid_x"] for r in d.launch_log_read() if r["what"] == "sample"]
     assert len(set(rows[:-1])) == 1 and rows[0] > 1000
     d.launch_log(False)
+
+
+@pytest.mark.parametrize("route", paged.TWO_PARTS)
+def test_one_part_instead_of_two_shows(route):
+    """The limit that the attention's routes are held to is under what one f16 part of q, or of the probabilities,
+    would be off by: a mistake planted in the oracle."""
+    x = paged.TwoParts(zd.F16, **paged.TWO_PARTS[route])
+    want = x.want()
+    for lost in (dict(q_parts=1), dict(p_parts=1)):
+        assert np.nanmax(np.abs(x.want(**lost) - want)) > 4 * x.limit(), lost
+    row = next(x.batch.places())
+    x.batch.places = lambda: iter([row])
+    full, _ = paged.attend(x.pool, x.batch, x.q, x.heads, np.float64(x.scale), x.window)
+    assert np.abs(full[row[0]] - want[row[0]]).max() < 1e-12
