@@ -363,6 +363,29 @@ def test_prompts_that_fill_the_chip(box, kind, hd, group, lens, window):
 
 
 @pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("hd,window", [(64, 0), (128, 0), (256, 33)])
+@pytest.mark.parametrize("long", [60, 130])
+def test_a_prompt_among_drafts(box, kind, hd, window, long):
+    """Twenty sequences of a few tokens and one of many: the few-row kernel takes all of 60 tokens (8 heads: 600 to 900
+    rows of a batch), and both take those of 130."""
+    page, kv, group = 16, 1, 8
+    _say(f"prompt among drafts kind={kind} hd={hd} long={long}")
+    rng = np.random.default_rng(hd + long)
+    lens = [(1 + i % 3, 9 + 7 * i) for i in range(20)]
+    lens.insert(11, (long, long + 21))
+    b = paged.Batch(lens, page, rng, behind=2)
+    pool = paged.Pool(kind, kv, hd, page, b.n_pages)
+    paged.fill(pool, b, rng)
+    q = rng.standard_normal((b.n_tokens, kv * group, hd)).astype(np.float32)
+    cache, batch = box.cache(pool), box.batch(b)
+    d_q, d_o = box.up(q), box.up(np.full_like(q, 7))
+    assert box.dev.paged_attention_enqueue(cache, batch, d_q, d_o, kv * group, hd ** -0.5, window=window), box.dev.last_error()
+    got = box.down(d_o, q)
+    want, bound = paged.attend(pool, b, q, kv * group, hd ** -0.5, window)
+    assert (np.abs(got - want).max((1, 2))[:-2] <= bound[:-2]).all() and (got[-2:] == 7).all()
+
+
+@pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("hd", [64, 128, 256])
 @pytest.mark.parametrize("live", [1, 8, 9, 32])
 def test_one_sequence_of_fewer_rows(box, kind, hd, live):

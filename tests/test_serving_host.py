@@ -227,6 +227,18 @@ def test_attention_routes(box, type, seqs, tokens, group, want):
             assert r["grid_x"] % 8 == 0 and r["grid_x"] // 8 >= -(-tokens * group // 256)
 
 
+@pytest.mark.parametrize("type,seqs,tokens,group,want", [
+    # drafts of a serving batch, and a short prompt in one: the few-row kernel alone
+    (zd.Q4_0, 32, 160, 4, ["few"]), (zd.Q4_0, 64, 320, 4, ["few"]), (zd.F16, 32, 160, 4, ["few"]),
+    (zd.F16, 64, 320, 4, ["few"]), (zd.Q4_0, 16, 215, 4, ["few"]), (zd.Q4_0, 64, 320, 8, ["few"]),
+    # a longer prompt, also in a batch that has room for many sequences
+    (zd.Q4_0, 64, 1363, 4, ["many", "few"]), (zd.Q4_0, 16, 465, 4, ["many", "merge", "few"]),
+    (zd.Q4_0, 256, 2255, 4, ["many", "few"]), (zd.Q4_0, 1024, 2255, 4, ["many", "few"]),
+    (zd.F16, 1024, 2255, 4, ["many", "few"])])
+def test_attention_routes_of_drafts_and_prompts(box, type, seqs, tokens, group, want):
+    test_attention_routes(box, type, seqs, tokens, group, want)
+
+
 def test_page_bytes():
     assert zd.paged_page_bytes(zd.F16, 8, 128, 64) == 8 * 64 * 256
     assert zd.paged_page_bytes(zd.Q4_0, 8, 128, 64) == 8 * 64 * 72

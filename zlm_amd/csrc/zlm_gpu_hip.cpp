@@ -3141,17 +3141,23 @@ extern "C" bool zlm_gpu_paged_attention_enqueue(zlm_device* d, const zlm_paged_c
     if (tiles * cache->n_kv_heads * std::min<uint64_t>(depth, (1u << 24) + 4) >= (1ull << 31) - 1)
         return fail(d, "attention of %u tokens over up to %u pages a sequence is too large for one call",
                     batch->n_tokens, batch->table_stride);
-    // Sequences of more than few_rows rows go to the many-row kernel.  Which there
-    // are is known on the device only: both kernels run where the batch may hold such
-    // a sequence beside others, or is made of them.  A batch of one sequence goes to one
-    // kernel whole, however many of the token rows it has when the work runs.  The few-row kernel reads K and V
+    // Sequences of more than few_rows rows go to the many-row kernel.  Which there are is
+    // known on the device only.  A batch of one sequence goes to one kernel whole, however
+    // many of the token rows it has when the work runs.  The few-row kernel reads K and V
     // again for every 16 rows, the other one has work for few waves: 8 sequences of about
     // 3700 positions, heads of 128, 64 and 192 rows each: f16 73 and 181 us by few rows,
     // 65 and 76 by many; q4_0 39 and 86, 78 and 75 (32 sequences: 119 and 307, 198 and
     // 223); heads of 256, q4_0: 64 and 156, 56 and 136.
     const uint32_t few_rows = cache->type == ZLM_GGML_Q4_0 && hd <= 128 ? 128 : 32;
     const uint64_t rows = static_cast<uint64_t>(batch->n_tokens) * group;
-    const bool many = batch->n_tokens > batch->n_seqs && (rows > 512 || rows > static_cast<uint64_t>(batch->n_seqs) * few_rows);
+    // Both run where the batch may hold such a sequence beside others and enough rows for
+    // it to pay; under that the few-row kernel alone takes what there is.  3000 positions, 4
+    // heads a kv head of 128, q4_0, few alone and both: 32 sequences of 5 tokens 44 and 51 us,
+    // 64 of 5 76 and 81, of 10 125 and 131; 64 with one of 257, 500, 1000 or 1100 tokens 111,
+    // 156, 248 and 266, 126, 178, 247 and 250; 16 with one of 200, 300 or 450 63, 82 and 112,
+    // 74, 94 and 107; f16, 32 of 5 95 and 103, 64 of 5 181 and 185, with one of 257 220 and 327.
+    const uint64_t enough = std::max<uint64_t>(512, 64 * std::min<uint64_t>(batch->n_seqs, 64));
+    const bool many = batch->n_tokens > batch->n_seqs && rows > std::min<uint64_t>(static_cast<uint64_t>(batch->n_seqs) * few_rows, enough);
     const bool few = !many || batch->n_seqs > 1;
     // Equal shares of the few-row kernel for the workgroups that the CUs hold at once: one
     // of heads of 256 (two rounds of them: 1 sequence of 32000 q4_0 positions 48 us, one
