@@ -53,7 +53,7 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 
 // The weight of a token that lies f = y - floor(y) above its bin's lower edge,
 // e^((f - 1) / 16) in units of 2^-34: a polynomial of degree 5 through the
-// Chebyshev nodes of [0, 1], good to 5e-14, a six hundredth of the unit.  Its
+// Chebyshev nodes of [0, 1], good to 4e-14, a 1400th of the unit.  Its
 // coefficients stay in scalar registers.
 struct Weight {
     double c[6];
