@@ -446,8 +446,8 @@ typedef struct {
  * when the work runs: a captured graph replays with what they hold then.  Rows
  * q_start[s] .. q_start[s+1]-1 of the token buffers are sequence s's newest
  * tokens, the last at position kv_len[s] - 1; position p of s lies in page
- * table[s * table_stride + p / page_size].  q_start never decreases.  A sequence
- * may have no rows.  Rows at negative positions (kv_len below the row count)
+ * table[s * table_stride + p / page_size].  q_start begins at 0 or above, never
+ * decreases and ends at n_tokens or below.  A sequence may have no rows.  Rows at negative positions (kv_len below the row count)
  * are padding, rows from q_start[n_seqs] on are not touched.  A page number
  * outside [0, n_pages) is no page: nothing is appended there, and what reads a
  * position there becomes NaN; so does the attention of rows past position
@@ -469,8 +469,9 @@ uint64_t zlm_gpu_paged_page_bytes(uint32_t type, uint32_t n_kv_heads, uint32_t h
  * k: n_kv_heads*hd | v: n_kv_heads*hd] floats, qkv_stride floats apart (0:
  * packed); q_out: n_tokens x n_heads*hd floats, 0 in padding rows.  The angle
  * (position * freq_base^(-2i/hd)), the norm and the choice of 4-bit values are
- * formed in 64 bits; freq_base is finite.  q4_0: d = -m/8 of the block's value m of the largest size
- * (the first of several), rounded to 8 significant bits, n = floor(x/d + 8.5)
+ * formed in 64 bits; freq_base is positive and finite.  q_out lies apart from qkv.
+ * q4_0: d = -m/8 of the block's value m of the largest size (the first of
+ * several), as a 32-bit float, rounded to 8 significant bits, n = floor(x/d + 8.5)
  * within 0..15; a block with a NaN reads back as NaN, values past 21760 saturate.
  * f16: rounded to nearest, infinite past its range. */
 bool zlm_gpu_paged_append_enqueue(zlm_device *dev, const zlm_paged_cache *cache, const zlm_paged_batch *batch,
@@ -485,13 +486,14 @@ bool zlm_gpu_paged_read_enqueue(zlm_device *dev, const zlm_paged_cache *cache, c
  * `scale` (finite, below 2.3e38 in size), q heads dealt to kv heads in order
  * (n_heads / n_kv_heads each); q and out: n_tokens x n_heads*hd floats, 16-byte
  * aligned, apart from each other.  One token a sequence, a prompt's chunk, or both
- * in one batch.  The results have the accuracy of 32-bit
- * products and sums over the cached values.  A padding row's output is 0.  NaN or
- * infinite K reaches the rows that see its position only; such a V may make NaN
- * of other rows of its sequence in the same call, never of another sequence's.
- * Partial results live in 64 MiB of library scratch that this call and zlm_gpu_sample_enqueue
- * share, and counters beside it, made by their first calls and never replaced: call once
- * before its capture. */
+ * in one batch.  The results have the accuracy of 32-bit products and sums over the
+ * cached values, down to weights of 2^-30 of a row's largest and to values of
+ * 2^-14: smaller ones add with the rounding of those.  A padding row's output is 0.
+ * NaN or infinite K reaches the rows that see its position only; such a V may make
+ * NaN of other rows of its sequence in the same call, never of another sequence's.
+ * Partial results live in 64 MiB of library scratch that this call and
+ * zlm_gpu_sample_enqueue share, and counters beside it, made by their first calls
+ * and never replaced: call once before its capture. */
 bool zlm_gpu_paged_attention_enqueue(zlm_device *dev, const zlm_paged_cache *cache, const zlm_paged_batch *batch,
                                      const float *q, uint32_t n_heads, uint32_t window, float scale, float *out);
 
