@@ -366,8 +366,8 @@ def test_prompts_that_fill_the_chip(box, kind, hd, group, lens, window):
 @pytest.mark.parametrize("hd,window", [(64, 0), (128, 0), (256, 33)])
 @pytest.mark.parametrize("long", [60, 130])
 def test_a_prompt_among_drafts(box, kind, hd, window, long):
-    """Twenty sequences of a few tokens and one of many: the few-row kernel takes all of 60 tokens (8 heads: 600 to 900
-    rows of a batch), and both take those of 130."""
+    """Twenty sequences of a few tokens and one of many: with 60 tokens (8 heads, 792 rows) the few-row kernel takes
+    the batch alone, or both do (f16, heads of 256); with 130 (1352 rows) both."""
     page, kv, group = 16, 1, 8
     _say(f"prompt among drafts kind={kind} hd={hd} long={long}")
     rng = np.random.default_rng(hd + long)
@@ -526,6 +526,28 @@ def test_last_positions(box, kind, hd, rows):
         box.dev.dev_upload(kv_len, np.array([last + past], np.int32))
         got = run()
         assert np.isnan(got[max(0, rows - past):]).all() and np.isfinite(got[:max(0, rows - past)]).all()
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("lens", [[(1, 100), (1, 90), (3, 40)], [(150, 200), (1, 150), (40, 120)]])
+def test_sequences_that_share_pages(box, kind, lens):
+    """A prefix that two sequences share, one page at two places of a table, few rows and many."""
+    hd, page, kv, group = 128, 16, 1, 4
+    _say(f"shared pages kind={kind} {lens}")
+    rng = np.random.default_rng(36)
+    b = paged.Batch(lens, page, rng)
+    pool = paged.Pool(kind, kv, hd, page, b.n_pages)
+    paged.fill(pool, b, rng)
+    b.table[1:, :2] = b.table[0, :2]
+    b.table[1, :4] = b.table[0, :4]
+    b.table[2, 1] = b.table[2, 0]
+    q = rng.standard_normal((b.n_tokens, kv * group, hd)).astype(np.float32)
+    cache, batch = box.cache(pool), box.batch(b)
+    d_q, d_o = box.up(q), box.up(np.full_like(q, 7))
+    assert box.dev.paged_attention_enqueue(cache, batch, d_q, d_o, kv * group, hd ** -0.5), box.dev.last_error()
+    got = box.down(d_o, q)
+    want, bound = paged.attend(pool, b, q, kv * group, hd ** -0.5)
+    assert (np.abs(got - want).max((1, 2)) <= bound).all()
 
 
 def test_nan_in_one_sequence_stays_there(box):
