@@ -1164,10 +1164,10 @@ __device__ __forceinline__ void attend_few(const AttnArgs& a) {
 // kHalved: two waves share 16 of them, each with one block of a stage, and join their
 // sums at the end.
 //
-// What bounds it is the matrix unit: the two parts of q and of P make four products of
-// what f16 alone would take two of, and those run at 1.18 PFLOP/s where a library
-// product of two 16384 x 16384 matrices reaches 1.32 here (2048 rows of 32 q and 8 kv
-// heads of 128 over 8000 positions, q4_0: 400 us).
+// What bounds it is matrix and vector issue in turn, 59% and 32% of the CUs' cycles: the
+// two parts of q and of P make four products of what f16 alone would take two of, and those
+// run at 1.21 PFLOP/s where a library product of two 16384 x 16384 matrices reaches 1.32
+// here (2048 rows of 32 q and 8 kv heads of 128 over 8000 positions, q4_0: 387 us).
 template <int HD, bool kHalved = false>
 struct Many {
     static constexpr int kRt = HD == 256 ? 1 : 2;      // tiles of 16 rows a wave
