@@ -81,3 +81,25 @@ extern "C" int host_find(const float* logits, uint32_t vocab, uint32_t bin, int 
         }
     });
 }
+
+// The search for weight up to the end of bin `bin`, its bins in question formed from that weight
+// and one a rounding above it, in the wrong order.
+extern "C" int host_find_between(const float* logits, uint32_t vocab, uint32_t bin, int32_t* token) {
+    Call c(logits, 1, vocab);
+    if (const int e = c.count(0)) return e;
+    return host_gpu::run(512, {0, 0, 0}, kMost, [&] {
+        __shared__ Shared sm;
+        const double rate = rate_of(c.a, 0);
+        Row::Ahead ahead;
+        Row::read_ahead(c.a, 0, 0, ahead);
+        Row r(c.a, sm, 0, rate, row_info(c.a, sm, 0));
+        r.join(ahead);
+        const double end = r.weight_to(bin + 1);
+        uint32_t b[2];
+        r.bins_for(kAtLeast, nextafter(end, INFINITY), end, b);
+        const bool listed = r.in_question() <= kList;
+        if (listed && !r.list_shorts(ahead)) r.list_row();
+        const Found f = r.find({kAtLeast, end, 0, b[0], b[1]}, listed);
+        if (threadIdx.x == 0) *token = static_cast<int32_t>(~static_cast<uint32_t>(f.token));
+    });
+}

@@ -82,3 +82,15 @@ def test_a_goal_past_the_bins_in_question(host, per, bin_, past):
     w = np.exp(x[mine].astype(np.float64) - 161 / 16).sum() if past else np.exp(x[order[0]].astype(np.float64) - 161 / 16)
     # weights are whole numbers of 2^-34 of their bin's edge
     assert abs(weight.value - w) <= len(mine) * 2.0 ** -34 * np.exp(-bin_ / 16)
+
+
+@pytest.mark.parametrize("per", [3, 200])
+def test_bins_between_weights_in_the_wrong_order(host, per):
+    """The weights that a cut may leave differ by a rounding, the upper one below the lower: a bin is in question."""
+    rng = np.random.default_rng(per)
+    bins = rng.permutation(np.repeat([0, 5, 9], per))
+    x = ((160 - bins + rng.random(len(bins)) * 0.98 + 0.01) / 16).astype(np.float32)
+    token = ctypes.c_int32(-9)
+    assert host.host_find_between(_ptr(x), len(x), 0, ctypes.byref(token)) == 0
+    behind = np.flatnonzero(bins == 5)
+    assert token.value == behind[np.argmax(x[behind])]

@@ -429,6 +429,13 @@ public:
     __device__ __forceinline__ void flag(uint32_t b0, uint32_t b1) {
         if (tid_ >= b0 && tid_ <= b1) atomicOr(&sm_.flags[tid_ / 32], 1u << tid_ % 32);
     }
+    // Those of a goal between two weights are: b[0] .. b[1].  Light bins behind heavy ones add
+    // less than a rounding, so the second weight may be a rounding below the first.
+    __device__ __forceinline__ void bins_for(Mode mode, double w0, double w1, uint32_t b[2]) {
+        b[0] = bin_for({mode, w0, 0});
+        b[1] = max(bin_for({mode, w1, 0}), b[0]);
+        flag(b[0], b[1]);
+    }
     __device__ __forceinline__ bool flagged(uint32_t bin) const { return sm_.flags[bin / 32] >> bin % 32 & 1; }
 
     // The number of the flagged bins' tokens.
@@ -798,9 +805,7 @@ __device__ __forceinline__ void pick(const Args& a) {
         w1 = r.weight_to(k_bin + 1);
     }
     if (f.by_p) {
-        p_bins[0] = r.bin_for({kAtLeast, w0 * f.p, 0});
-        p_bins[1] = r.bin_for({kAtLeast, w1 * f.p, 0});
-        r.flag(p_bins[0], p_bins[1]);
+        r.bins_for(kAtLeast, w0 * f.p, w1 * f.p, p_bins);
         w0 = r.weight_to(p_bins[0]);
         w1 = __builtin_fmin(w1, r.weight_to(p_bins[1] + 1));
     }
@@ -812,8 +817,8 @@ __device__ __forceinline__ void pick(const Args& a) {
             w1 = __builtin_fmin(w1, r.weight_to(b + 1));
         }
     }
-    const uint32_t u_bins[2] = {r.bin_for({kMore, w0 * f.u, 0}), r.bin_for({kMore, w1 * f.u, 0})};
-    r.flag(u_bins[0], u_bins[1]);
+    uint32_t u_bins[2];
+    r.bins_for(kMore, w0 * f.u, w1 * f.u, u_bins);
     const bool listed = r.in_question() <= kList;
     if (listed && !r.list_shorts(ahead)) r.list_row();
     // the filters in turn, then the draw
