@@ -430,13 +430,19 @@ bool zlm_gpu_attention_decode_enqueue_noalloc(zlm_device *dev, const float *qkv,
  *      q4_0  one 32-bit word of 8 nibbles per group and dim, position j's at bits
  *            4*(j/2) + 16*(j%2), [page_size/8][head_dim], then the f16 scales
  *            [page_size/8][head_dim/32][8]
+ *   e4m3: K [page_size][head_dim] and V [page_size/8][head_dim][8] bytes, behind
+ *         each of the two 16 bytes: a scale for each block of 16 positions
+ *         (page_size/16 of them; the others are not looked at)
  * A q4_0 value is d * (nibble - 8).  d holds at most 8 significant bits and at
  * most 2720 in size, so a value is exact in f16; the append writes such scales,
- * and a cache filled elsewhere has to.  Pages need no clearing: what lies past a
+ * and a cache filled elsewhere has to.  An e4m3 value is the OCP 8-bit number (no
+ * infinities; 0x7f and 0xff NaN) times 2^(byte - 127) of its block's scale byte, which
+ * is 112 to 134 (another counts as the nearest of these): exact in f16 too.  Pages need no clearing: what lies past a
  * sequence's length is never used, whatever bits it holds. */
+enum { ZLM_CACHE_E4M3 = 0x100 };
 typedef struct {
     void *k, *v;           /* device pools */
-    uint32_t type;         /* ZLM_GGML_F16 or ZLM_GGML_Q4_0 */
+    uint32_t type;         /* ZLM_GGML_F16, ZLM_GGML_Q4_0 or ZLM_CACHE_E4M3 */
     uint32_t n_kv_heads;   /* 1 to 1024 */
     uint32_t head_dim;     /* 64, 128 or 256 */
     uint32_t page_size;    /* 16, 32, 64, 128 or 256 positions */
@@ -473,7 +479,13 @@ uint64_t zlm_gpu_paged_page_bytes(uint32_t type, uint32_t n_kv_heads, uint32_t h
  * q4_0: d = -m/8 of the block's value m of the largest size (the first of
  * several), as a 32-bit float, rounded to 8 significant bits, n = floor(x/d + 8.5)
  * within 0..15; a block with a NaN reads back as NaN, values past 21760 saturate.
- * f16: rounded to nearest, infinite past its range. */
+ * f16: rounded to nearest, infinite past its range.
+ * e4m3: a block's scale is the least that holds the largest of the rows written to it
+ * (448 times 2^k), and none below the one that it has for rows before them; where it
+ * rises those are rounded again, which changes only what becomes smaller than 2^-6 of the
+ * scale.  It falls when the block's first position is written: rows that are written over
+ * later (drafts that were not accepted) may leave it higher than it need be.  Rounded to
+ * nearest, K once from 64 bits; values past 57344 saturate, a NaN is one. */
 bool zlm_gpu_paged_append_enqueue(zlm_device *dev, const zlm_paged_cache *cache, const zlm_paged_batch *batch,
                                   const float *qkv, uint64_t qkv_stride, const float *q_norm_w,
                                   const float *k_norm_w, uint32_t n_heads, float eps, float freq_base, float *q_out);
@@ -496,6 +508,14 @@ bool zlm_gpu_paged_read_enqueue(zlm_device *dev, const zlm_paged_cache *cache, c
  * and never replaced: call once before its capture. */
 bool zlm_gpu_paged_attention_enqueue(zlm_device *dev, const zlm_paged_cache *cache, const zlm_paged_batch *batch,
                                      const float *q, uint32_t n_heads, uint32_t window, float scale, float *out);
+
+/* The same over a window and the first `sinks` positions, which stay visible: a row at
+ * p sees [max(0, p - window + 1), p] and [0, min(sinks, p + 1)).  Positions between are
+ * not read, so their pages may be given back (table entries that are no page).  window 0:
+ * all from 0, whatever sinks. */
+bool zlm_gpu_paged_attention_sinks_enqueue(zlm_device *dev, const zlm_paged_cache *cache, const zlm_paged_batch *batch,
+                                           const float *q, uint32_t n_heads, uint32_t window, uint32_t sinks,
+                                           float scale, float *out);
 
 /* ---- sampling (device buffers): a token from each row of logits ----
  * No reference counterpart on the device (its sampler runs on the CPU over the

@@ -5,6 +5,9 @@
 
 namespace zlm {
 
+// An e4m3 cache: the least and the largest byte of a block's scale, 2^(byte - 127).
+constexpr uint32_t kE8Least = 112, kE8Most = 134;
+
 constexpr uint32_t kPagedMaxSeqs = 1024;  // sequences of one call (their prefix sums live in LDS)
 
 // What every kernel takes of the cache and the batch.  `table` entries are page
@@ -49,6 +52,7 @@ struct PagedAttend {
     float scale;      // times log2(e)
     uint32_t few_rows;  // sequences with more rows (tokens x group) are the many-row kernel's
     uint32_t splits;    // its splits of the positions
+    uint32_t sinks;     // the first positions, seen beside the window's (the kernels with sinks)
 };
 
 }  // namespace zlm

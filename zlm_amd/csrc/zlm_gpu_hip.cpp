@@ -52,6 +52,11 @@ constexpr uint32_t kNoLayout = 0xffffffffu;
 constexpr uint32_t kUsesAttn = 1u;  // the attention partials
 constexpr uint32_t kUsesGemm = 2u;  // the GEMM's quantized activations and the residents' GEMM tiles
 constexpr int kPagedDims[] = {64, 128, 256};  // head sizes of the paged kernels
+// their cache types, by the names of the kernels
+constexpr struct {
+    uint32_t type;
+    const char* name;
+} kPagedTypes[] = {{ZLM_GGML_F16, "f16"}, {ZLM_GGML_Q4_0, "q4_0"}, {ZLM_CACHE_E4M3, "e4m3"}};
 constexpr uint32_t kPagedKvHeads = 1024;      // their kv heads at most
 constexpr uint32_t kQ4kRecords = 0xfffffffeu;
 constexpr uint32_t kQ6kRecords = 0xfffffffdu;
@@ -222,12 +227,15 @@ struct zlm_device {
     hipFunction_t attn_combine = nullptr;
     hipFunction_t attn_combine_wide = nullptr;
     hipFunction_t attn_decode = nullptr;
-    // the paged cache's kernels, by cache type (f16, q4_0) and head size (kPagedDims)
+    // the paged cache's kernels, by cache type (kPagedTypes) and head size (kPagedDims)
     hipModule_t paged_mod = nullptr;
     struct PagedKernels {
-        hipFunction_t append = nullptr, read = nullptr, few = nullptr, many = nullptr, merge_many = nullptr;
-        hipFunction_t halved = nullptr;  // many's other form, heads of 256
-    } paged[2][3];
+        hipFunction_t append = nullptr, read = nullptr;
+        struct Attend {
+            hipFunction_t few = nullptr, many = nullptr, merge_many = nullptr;
+            hipFunction_t halved = nullptr;  // many's other form, heads of 256
+        } attend[2];  // without sinks, with them
+    } paged[3][3];
     float* serving = nullptr;          // kServingScratch bytes: the paged attention's partials, the sampler's histograms
     uint32_t* paged_counts = nullptr;  // the few-row attention's counters, one a workgroup; 0 between calls
     hipModule_t sample_mod = nullptr;
@@ -403,21 +411,22 @@ bool load_kernels(zlm_device* d) {
     }
     const std::string pp = dir + "/zlm_paged_gfx950.hsaco";
     if (!ok(d, hipModuleLoad(&d->paged_mod, pp.c_str()), pp.c_str())) return false;
-    for (int t = 0; t < 2; t++)
+    for (int t = 0; t < 3; t++)
         for (int i = 0; i < 3; i++) {
             zlm_device::PagedKernels& k = d->paged[t][i];
-            const struct {
-                hipFunction_t* f;
-                const char* name;
-            } fns[] = {{&k.append, "append"}, {&k.read, "read"}, {&k.few, "attend_few"},
-                       {&k.many, "attend_many"}, {&k.merge_many, "merge_many"}};
-            for (const auto& fn : fns) {
-                snprintf(nm, sizeof nm, "zlm_paged_%s_%s_%d", fn.name, t ? "q4_0" : "f16", kPagedDims[i]);
-                if (!ok(d, hipModuleGetFunction(fn.f, d->paged_mod, nm), nm)) return false;
+            const auto get = [&](hipFunction_t& f, const char* op, const char* sinks) {
+                snprintf(nm, sizeof nm, "zlm_paged_%s_%s%s_%d", op, kPagedTypes[t].name, sinks, kPagedDims[i]);
+                return ok(d, hipModuleGetFunction(&f, d->paged_mod, nm), nm);
+            };
+            if (!get(k.append, "append", "") || !get(k.read, "read", "")) return false;
+            for (int j = 0; j < 2; j++) {
+                zlm_device::PagedKernels::Attend& f = k.attend[j];
+                const char* sinks = j ? "_sinks" : "";
+                if (!get(f.few, "attend_few", sinks) || !get(f.many, "attend_many", sinks) ||
+                    !get(f.merge_many, "merge_many", sinks) ||
+                    (kPagedDims[i] == 256 && !get(f.halved, "attend_halved", sinks)))
+                    return false;
             }
-            if (kPagedDims[i] != 256) continue;
-            snprintf(nm, sizeof nm, "zlm_paged_attend_halved_%s_256", t ? "q4_0" : "f16");
-            if (!ok(d, hipModuleGetFunction(&k.halved, d->paged_mod, nm), nm)) return false;
         }
     const std::string sp = dir + "/zlm_sample_gfx950.hsaco";
     if (!ok(d, hipModuleLoad(&d->sample_mod, sp.c_str()), sp.c_str())) return false;
@@ -3010,13 +3019,21 @@ bool ensure_serving_scratch(zlm_device* d, const char* what) {
 
 namespace {
 
+// The place of a cache type in kPagedTypes, or -1.
+int paged_type(uint32_t type) {
+    for (int t = 0; t < 3; t++)
+        if (kPagedTypes[t].type == type) return t;
+    return -1;
+}
+
 // Checks what can be checked on the host and fills the kernels' block.  *k =
 // the cache's kernels; null when the batch is empty (nothing to launch).
 bool paged_block(zlm_device* d, const zlm_paged_cache* c, const zlm_paged_batch* b, zlm::Paged* p,
                  const zlm_device::PagedKernels** k) {
     *k = nullptr;
     if (!c || !b) return fail(d, "null cache or batch");
-    if (c->type != ZLM_GGML_F16 && c->type != ZLM_GGML_Q4_0) return fail(d, "a paged cache is f16 or q4_0 (got type %u)", c->type);
+    const int type = paged_type(c->type);
+    if (type < 0) return fail(d, "a paged cache is f16, q4_0 or e4m3 (got type %u)", c->type);
     int dim = 0;
     while (dim < 3 && kPagedDims[dim] != static_cast<int>(c->head_dim)) dim++;
     if (dim == 3) return fail(d, "a paged cache has heads of 64, 128 or 256 (got %u)", c->head_dim);
@@ -3034,7 +3051,7 @@ bool paged_block(zlm_device* d, const zlm_paged_cache* c, const zlm_paged_batch*
     if (c->n_pages == 0 || c->n_pages > 0x7fffffffu || b->table_stride == 0) return fail(d, "no pages");
     *p = {static_cast<uint8_t*>(c->k), static_cast<uint8_t*>(c->v), b->q_start, b->kv_len, b->table, b->n_seqs,
           b->n_tokens, b->table_stride, c->n_pages, c->n_kv_heads, shift};
-    *k = &d->paged[c->type == ZLM_GGML_Q4_0][dim];
+    *k = &d->paged[type][dim];
     return true;
 }
 
@@ -3060,7 +3077,8 @@ bool ensure_paged_counts(zlm_device* d, uint32_t n) {
 extern "C" uint64_t zlm_gpu_paged_page_bytes(uint32_t type, uint32_t n_kv_heads, uint32_t head_dim, uint32_t page_size) {
     const bool dim_ok = head_dim == 64 || head_dim == 128 || head_dim == 256;
     const bool page_ok = page_size >= 16 && page_size <= 256 && (page_size & (page_size - 1)) == 0;
-    if (!dim_ok || !page_ok || n_kv_heads > kPagedKvHeads || (type != ZLM_GGML_F16 && type != ZLM_GGML_Q4_0)) return 0;
+    if (!dim_ok || !page_ok || n_kv_heads > kPagedKvHeads || paged_type(type) < 0) return 0;
+    if (type == ZLM_CACHE_E4M3) return (static_cast<uint64_t>(head_dim) * page_size + 16) * n_kv_heads;
     const uint64_t row = type == ZLM_GGML_F16 ? 2 * head_dim : head_dim / 2 + head_dim / 16;
     return row * page_size * n_kv_heads;
 }
@@ -3094,7 +3112,8 @@ extern "C" bool zlm_gpu_paged_append_enqueue(zlm_device* d, const zlm_paged_cach
     // the code then: 64 rows of 40 heads took 5.9 us so and 8.2 by four); else four a wave,
     // and a row's heads in one workgroup once rows alone fill the CUs, so that it forms
     // the rotation once (7270 rows: 75 us).
-    const uint64_t heads = static_cast<uint64_t>(n_heads) + cache->n_kv_heads;
+    // An e4m3 block's K and V are a wave's turn each.
+    const uint64_t heads = static_cast<uint64_t>(n_heads) + cache->n_kv_heads * (cache->type == ZLM_CACHE_E4M3 ? 2 : 1);
     const uint64_t fill = (8ull * d->cus + batch->n_tokens - 1) / batch->n_tokens;
     a.per = fill >= (heads + 3) / 4 ? 1 : 4;
     const unsigned groups = static_cast<unsigned>(std::min((heads + 4 * a.per - 1) / (4 * a.per), fill));
@@ -3119,9 +3138,10 @@ extern "C" bool zlm_gpu_paged_read_enqueue(zlm_device* d, const zlm_paged_cache*
     return launch3(d, k->read, batch->n_tokens, groups, 1, 256, args, "paged read");
 }
 
-extern "C" bool zlm_gpu_paged_attention_enqueue(zlm_device* d, const zlm_paged_cache* cache,
-                                                const zlm_paged_batch* batch, const float* q, uint32_t n_heads,
-                                                uint32_t window, float scale, float* out) {
+namespace {
+
+bool paged_attention(zlm_device* d, const zlm_paged_cache* cache, const zlm_paged_batch* batch, const float* q,
+                     uint32_t n_heads, uint32_t window, uint32_t sinks, float scale, float* out) {
     if (!d || !d->avail) return false;
     zlm::PagedAttend a = {};
     const zlm_device::PagedKernels* k = nullptr;
@@ -3129,6 +3149,7 @@ extern "C" bool zlm_gpu_paged_attention_enqueue(zlm_device* d, const zlm_paged_c
     if (n_heads == 0 || n_heads > 16384 || n_heads % cache->n_kv_heads)
         return fail(d, "%u q heads over %u kv heads", n_heads, cache->n_kv_heads);
     if (window > 0x7fffffffu) return fail(d, "bad attention window");
+    if (sinks > 0x7fffffffu) return fail(d, "bad count of sinks");
     const float scale2 = scale * 1.44269504088896340736f;  // the exponents' base is two
     if (!std::isfinite(scale2)) return fail(d, "the attention's scale is not finite, or past 2.3e38");
     if (!k) return true;
@@ -3192,13 +3213,29 @@ extern "C" bool zlm_gpu_paged_attention_enqueue(zlm_device* d, const zlm_paged_c
     a.scale = scale2;
     a.few_rows = !few ? 0 : many ? few_rows : 0xffffffffu;
     a.splits = splits;
+    a.sinks = sinks;
     void* args[] = {&a};
-    if (many && !(launch(d, halved ? k->halved : k->many, static_cast<uint32_t>(items * splits), many_threads, args,
+    const zlm_device::PagedKernels::Attend& f = k->attend[window && sinks];  // without a window all is seen
+    if (many && !(launch(d, halved ? f.halved : f.many, static_cast<uint32_t>(items * splits), many_threads, args,
                          "paged attention of many rows") &&
-                  (splits == 1 || launch3(d, k->merge_many, static_cast<uint32_t>(items), tile_rows / 16, 1, 256, args,
+                  (splits == 1 || launch3(d, f.merge_many, static_cast<uint32_t>(items), tile_rows / 16, 1, 256, args,
                                           "paged attention of many rows, merge"))))
         return false;
-    return !few || launch(d, k->few, grid, 256, args, "paged attention");
+    return !few || launch(d, f.few, grid, 256, args, "paged attention");
+}
+
+}  // namespace
+
+extern "C" bool zlm_gpu_paged_attention_enqueue(zlm_device* d, const zlm_paged_cache* cache,
+                                                const zlm_paged_batch* batch, const float* q, uint32_t n_heads,
+                                                uint32_t window, float scale, float* out) {
+    return paged_attention(d, cache, batch, q, n_heads, window, 0, scale, out);
+}
+
+extern "C" bool zlm_gpu_paged_attention_sinks_enqueue(zlm_device* d, const zlm_paged_cache* cache,
+                                                      const zlm_paged_batch* batch, const float* q, uint32_t n_heads,
+                                                      uint32_t window, uint32_t sinks, float scale, float* out) {
+    return paged_attention(d, cache, batch, q, n_heads, window, sinks, scale, out);
 }
 
 // ---- sampling ----

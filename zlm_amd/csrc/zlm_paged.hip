@@ -36,9 +36,13 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 
-template <int HD, bool Q4>
+// What a cache holds.  kE8: e4m3 numbers, a scale for each 16 positions and head.
+enum Cache : int { kF16, kQ4, kE8 };
+
+template <int HD, Cache C>
 struct Row {
-    static constexpr uint32_t kBytes = Q4 ? HD / 2 + HD / 16 : HD * 2;
+    static constexpr uint32_t kBytes = C == kF16 ? HD * 2 : C == kQ4 ? HD / 2 + HD / 16 : HD;
+    static constexpr uint32_t kBehind = C == kE8 ? 16 : 0;  // the scales of a head's page, behind its rows
 };
 
 // The sequence of row t (n_seqs when it lies behind the last one): the number of
@@ -81,9 +85,9 @@ __device__ __forceinline__ int32_t page_of(const Paged& p, uint32_t s, int32_t p
     return static_cast<uint32_t>(id) < p.n_pages ? id : -1;
 }
 
-template <int HD, bool Q4>
+template <int HD, Cache C>
 __device__ __forceinline__ size_t head_base(const Paged& p, uint32_t page, uint32_t h) {
-    const uint32_t head_bytes = Row<HD, Q4>::kBytes << p.page_shift;
+    const uint32_t head_bytes = (Row<HD, C>::kBytes << p.page_shift) + Row<HD, C>::kBehind;
     return (static_cast<size_t>(page) * p.n_kv + h) * head_bytes;
 }
 
@@ -117,6 +121,12 @@ __device__ __forceinline__ double other_half(double v) {
     const uint32_t a0 = a[0], a1 = a[1], b0 = b[0], b1 = b[1];
     const bool upper = (threadIdx.x & 32) != 0;
     return __builtin_bit_cast(double, static_cast<uint64_t>(upper ? b0 : b1) << 32 | (upper ? a0 : a1));
+}
+
+// An e4m3 block's scale 2^(byte - 127).  The append writes 112 to 134, for which every
+// value is exact in f16; another byte counts as the nearest of those.
+__device__ __forceinline__ float e8_scale(uint32_t byte) {
+    return __builtin_bit_cast(float, min(max(byte, zlm::kE8Least), zlm::kE8Most) << 23);
 }
 
 // Two sums a step closer: x's in the lanes whose bit is clear, y's in the others.
@@ -199,6 +209,224 @@ __device__ __forceinline__ uint32_t quantise(T x, uint32_t lane, _Float16* d_out
     return static_cast<uint32_t>(c);
 }
 
+// An e4m3 cache's blocks of 16 positions of a head.  Their scale is the least power of
+// two that holds the largest of the block's values, so one wave takes all of the block's
+// rows in this call (and, where they begin inside it, the scale that it has: a scale
+// never falls, and where it rises the codes before them are rounded again, which changes
+// none but those that become subnormal).  The rows' workgroups take the heads' K and V in
+// turn.  K's rotation goes from row to row by the turn of one position, 16 at most: a
+// sine and cosine a row would be most of the call.
+// 2^-k x is exact in 32 bits, so a 64-bit K is taken to them with its last bit set where
+// that is not exact: every comparison and rounding below then sees the right side.
+__device__ __forceinline__ float to_odd(double x) {
+    const float f = static_cast<float>(x);
+    uint32_t u = __builtin_bit_cast(uint32_t, f);
+    if (static_cast<double>(f) != x) {
+        u -= __builtin_fabs(static_cast<double>(f)) > __builtin_fabs(x) ? 1u : 0u;
+        u |= 1u;
+    }
+    return x == x ? __builtin_bit_cast(float, u) : f;
+}
+
+// The scale byte for a largest of m (0 and above): the least k with m <= 448 2^k.
+__device__ __forceinline__ uint32_t e8_byte(float m) {
+    const int e = __builtin_amdgcn_frexp_expf(m);  // m = f 2^e, f in [0.5, 1); 448 = 0.875 2^9
+    const int k = e - (__builtin_amdgcn_frexp_mantf(m) > 0.875f ? 8 : 9);
+    const int least = static_cast<int>(zlm::kE8Least) - 127, most = static_cast<int>(zlm::kE8Most) - 127;
+    return static_cast<uint32_t>((m >= 0x1p-60f ? min(max(k, least), most) : least) + 127);
+}
+
+// The largest of the wave.
+__device__ __forceinline__ float wave_most(float v) {
+    v = __builtin_fmaxf(v, dpp<kXor1>(v));
+    v = __builtin_fmaxf(v, dpp<kXor2>(v));
+    v = __builtin_fmaxf(v, dpp<kHalfMirror>(v));
+    v = __builtin_fmaxf(v, dpp<kMirror>(v));
+    v = __builtin_fmaxf(v, __builtin_bit_cast(float, next_row(__builtin_bit_cast(uint32_t, v))));
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t a0 = a[0], a1 = a[1];
+    return __builtin_fmaxf(__builtin_bit_cast(float, a0), __builtin_bit_cast(float, a1));
+}
+
+template <int HD>
+__device__ __forceinline__ void append_blocks(const AppendArgs& a, const RowAt& at, uint32_t t, uint32_t id, uint32_t wave,
+                                              uint32_t waves, const double (&turns)[6][HD / 2], const float (&wk)[HD / 64]) {
+    const Paged& p = a.p;
+    constexpr int N = HD / 64, kRows = 16;
+    constexpr float kMost = 57344.0f;  // 448 at the largest scale
+    const uint32_t lane = threadIdx.x & (kWave - 1), page = 1u << p.page_shift;
+    const int32_t start = max(at.pos & ~15, at.first);
+    const uint32_t j0 = static_cast<uint32_t>(start) & 15, mine = static_cast<uint32_t>(at.pos - start), t0 = t - mine;
+    const uint32_t n_rows = __builtin_amdgcn_readfirstlane(min(16u - j0, static_cast<uint32_t>(at.row1) - t0));
+    const uint32_t blk = (static_cast<uint32_t>(start) & (page - 1)) / 16;
+    for (uint32_t task = mine + n_rows * wave; task < 2 * p.n_kv; task += n_rows * waves) {
+        const bool is_k = task < p.n_kv;
+        const uint32_t head = is_k ? task : task - p.n_kv;
+        uint8_t* base = (is_k ? p.k : p.v) + head_base<HD, kE8>(p, id, head);
+        uint8_t* scale = base + page * HD + blk;
+        const float* src = a.qkv + t0 * a.stride + static_cast<size_t>(a.n_heads + task) * HD + lane;
+        float x[kRows][N];
+#pragma unroll
+        for (int r = 0; r < kRows; r++)
+#pragma unroll
+            for (int j = 0; j < N; j++) x[r][j] = src[min(static_cast<uint32_t>(r), n_rows - 1) * a.stride + 64 * j];
+        const uint32_t had = j0 ? min(max(static_cast<uint32_t>(*scale), zlm::kE8Least), zlm::kE8Most) : 0;
+        v2u old[N][2];
+        uint8_t* const to_v = base + (static_cast<size_t>(2 * blk) * HD + lane) * 8;
+        if (!is_k && n_rows < kRows) {
+#pragma unroll
+            for (int j = 0; j < N; j++)
+#pragma unroll
+                for (int g = 0; g < 2; g++) old[j][g] = *reinterpret_cast<const v2u*>(to_v + (g * HD + 64 * j) * 8);
+        }
+        if (is_k) {
+            double cs[N], sn[N], c1[N], s1[N];
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                const uint32_t i = (lane + 64 * j) % (HD / 2);
+                cs[j] = turns[2][i];
+                sn[j] = turns[3][i];
+                c1[j] = turns[4][i];
+                s1[j] = turns[5][i];
+            }
+#pragma unroll
+            for (int r0 = 0; r0 < kRows; r0 += 4) {
+                if (static_cast<uint32_t>(r0) >= n_rows) break;
+                double inv = 1.0;
+                if (a.k_norm) {
+                    double ss[4];
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        ss[r] = 0.0;
+#pragma unroll
+                        for (int j = 0; j < N; j++)
+                            ss[r] = __builtin_fma(static_cast<double>(x[r0 + r][j]), static_cast<double>(x[r0 + r][j]), ss[r]);
+                    }
+                    inv = 1.0 / sqrt(wave_sums(ss) * (1.0 / HD) + static_cast<double>(a.eps));
+                }
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    if (static_cast<uint32_t>(r0 + r) >= n_rows) break;
+                    double y[N];
+                    const double f = of_row(inv, r >> 1 | (r & 1) << 1);
+#pragma unroll
+                    for (int j = 0; j < N; j++) {
+                        y[j] = x[r0 + r][j];
+                        if (a.k_norm) y[j] = y[j] * f * static_cast<double>(wk[j]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < N; j++) {
+                        double other;
+                        bool upper;
+                        if constexpr (HD == 64) {
+                            other = other_half(y[0]);
+                            upper = lane >= 32;
+                        } else {
+                            other = y[(j + N / 2) % N];
+                            upper = j >= N / 2;
+                        }
+                        x[r0 + r][j] = to_odd(y[j] * cs[j] + (upper ? other : -other) * sn[j]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < N; j++) {  // on by a position
+                        const double c = cs[j];
+                        cs[j] = c * c1[j] - sn[j] * s1[j];
+                        sn[j] = sn[j] * c1[j] + c * s1[j];
+                    }
+                }
+            }
+        }
+        // rows past the last are the last's again: K's are its raw values
+        float m = 0.0f;
+#pragma unroll
+        for (int r = 0; r < kRows; r++) {
+            if (static_cast<uint32_t>(r) >= n_rows) break;
+#pragma unroll
+            for (int j = 0; j < N; j++) m = __builtin_fmaxf(m, __builtin_fabsf(x[r][j]));
+        }
+        m = __builtin_fminf(wave_most(m), kMost);
+        m = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, m)));
+        const uint32_t byte = max(e8_byte(m), had);
+        if (lane == 0) *scale = static_cast<uint8_t>(byte);
+        const float unit = __builtin_bit_cast(float, (254u - byte) << 23);  // 2^-k
+        const float rise = __builtin_bit_cast(float, (127u + had - byte) << 23);
+        const auto code2 = [&](float u, float v) {  // NaN stays one
+            u = u > kMost ? kMost : u < -kMost ? -kMost : u;
+            v = v > kMost ? kMost : v < -kMost ? -kMost : v;
+            return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(u * unit, v * unit, 0, false)) & 0xffffu;
+        };
+        const auto again = [&](uint32_t w) {  // four codes at the new scale
+            int o = __builtin_amdgcn_cvt_pk_fp8_f32(__builtin_amdgcn_cvt_f32_fp8(w, 0) * rise, __builtin_amdgcn_cvt_f32_fp8(w, 1) * rise, 0, false);
+            o = __builtin_amdgcn_cvt_pk_fp8_f32(__builtin_amdgcn_cvt_f32_fp8(w, 2) * rise, __builtin_amdgcn_cvt_f32_fp8(w, 3) * rise, o, true);
+            return static_cast<uint32_t>(o);
+        };
+        const bool risen = j0 != 0 && byte != had;
+        if (is_k) {
+            uint8_t* const to = base + (16 * blk) * HD;
+            if (risen) {
+                for (uint32_t i = 4 * lane; i < j0 * HD; i += 4 * kWave) {
+                    uint32_t* const w = reinterpret_cast<uint32_t*>(to + i);
+                    *w = again(*w);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < kRows; r += 2) {
+                if (static_cast<uint32_t>(r) >= n_rows) break;
+#pragma unroll
+                for (int j = 0; j < N; j++) {
+                    const uint32_t c = code2(x[r][j], x[r + 1][j]);
+                    to[(j0 + r) * HD + lane + 64 * j] = static_cast<uint8_t>(c);
+                    if (static_cast<uint32_t>(r) + 1 < n_rows) to[(j0 + r + 1) * HD + lane + 64 * j] = static_cast<uint8_t>(c >> 8);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                uint32_t w[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) w[i] = code2(x[4 * i][j], x[4 * i + 1][j]) | code2(x[4 * i + 2][j], x[4 * i + 3][j]) << 16;
+                if (n_rows < kRows) {
+                    // 16 bytes moved up by j0, between what lies before and behind
+                    const uint64_t lo = static_cast<uint64_t>(w[1]) << 32 | w[0], hi = static_cast<uint64_t>(w[3]) << 32 | w[2];
+                    const auto put = [&](uint64_t& l, uint64_t& h, uint64_t vl, uint64_t vh, uint32_t by) {
+                        const uint32_t b = 8 * (by & 7);
+                        const uint64_t up = b ? vl >> (64 - b) : 0;
+                        l = by < 8 ? vl << b : 0;
+                        h = by < 8 ? vh << b | up : vl << b;
+                    };
+                    uint64_t l, h, ml, mh, m1l, m1h;
+                    put(l, h, lo, hi, j0);
+                    put(ml, mh, ~0ull, ~0ull, j0);  // from j0 on
+                    const uint32_t e = j0 + n_rows;
+                    if (e < 16) put(m1l, m1h, ~0ull, ~0ull, e);
+                    else m1l = m1h = 0;
+                    ml &= ~m1l;
+                    mh &= ~m1h;
+                    uint64_t ol = static_cast<uint64_t>(old[j][0].y) << 32 | old[j][0].x, oh = static_cast<uint64_t>(old[j][1].y) << 32 | old[j][1].x;
+                    if (risen) {
+                        uint64_t bl, bh;  // before j0
+                        put(bl, bh, ~0ull, ~0ull, j0);
+                        const uint64_t al = static_cast<uint64_t>(again(ol >> 32)) << 32 | again(static_cast<uint32_t>(ol));
+                        const uint64_t ah = static_cast<uint64_t>(again(oh >> 32)) << 32 | again(static_cast<uint32_t>(oh));
+                        ol = (ol & bl) | (al & ~bl);
+                        oh = (oh & bh) | (ah & ~bh);
+                    }
+                    l = (ol & ~ml) | (l & ml);
+                    h = (oh & ~mh) | (h & mh);
+                    w[0] = static_cast<uint32_t>(l);
+                    w[1] = static_cast<uint32_t>(l >> 32);
+                    w[2] = static_cast<uint32_t>(h);
+                    w[3] = static_cast<uint32_t>(h >> 32);
+                }
+#pragma unroll
+                for (int g = 0; g < 2; g++)
+                    *reinterpret_cast<v2u*>(to_v + (g * HD + 64 * j) * 8) = v2u{w[2 * g], w[2 * g + 1]};
+            }
+        }
+    }
+}
+
 // A workgroup: one row; its waves (and those of the row's other workgroups) deal the
 // heads, four at a time, so that the sums of their norms take one pass over the lanes (or
 // one, where there are waves for all).
@@ -211,16 +439,16 @@ __device__ __forceinline__ uint32_t quantise(T x, uint32_t lane, _Float16* d_out
 // this call together: no two waves write one word.  The rows' workgroups take the heads
 // in turn (left to the group's first row they were all on one XCD, every eighth
 // workgroup's: prompts of 7270 rows together took 160 us, and 75 so).
-template <int HD, bool Q4>
+template <int HD, Cache C>
 __device__ __forceinline__ void append(const AppendArgs& a) {
     const Paged& p = a.p;
     constexpr int N = HD / 64;  // dims a lane
     constexpr uint32_t kH = 4;  // heads a step, at most
-    __shared__ double turns[2][HD / 2];
+    __shared__ double turns[C == kE8 ? 6 : 2][HD / 2];
     const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1);
     const uint32_t t = blockIdx.x;
     const uint32_t waves = gridDim.y * 4, wave = __builtin_amdgcn_readfirstlane(blockIdx.y * 4 + tid / kWave);
-    const uint32_t heads = a.n_heads + p.n_kv;
+    const uint32_t heads = C == kE8 ? a.n_heads : a.n_heads + p.n_kv;  // kE8: K goes by blocks, below
     const float* row = a.qkv + t * a.stride + lane;
     uint32_t h = a.per * wave;
     // the next heads' values, on their way while these are worked on; past the last head its own
@@ -244,7 +472,14 @@ __device__ __forceinline__ void append(const AppendArgs& a) {
     const int32_t pos = at.pos;
     const uint32_t page = 1u << p.page_shift;
     const int32_t id = __builtin_amdgcn_readfirstlane(page_of(p, s, pos));
-    if (tid < HD / 2) {
+    if constexpr (C == kE8) {  // of the block's first row too, and of one position
+        for (uint32_t i = tid; i < 3 * HD / 2; i += 256) {
+            const uint32_t j = i % (HD / 2), which = i / (HD / 2);
+            const double of = which == 0 ? pos : which == 1 ? max(pos & ~15, at.first) : 1;
+            const double turn = of * exp(a.log_base * (static_cast<double>(j) * (-2.0 / HD)));
+            sincos(turn, &turns[2 * which + 1][j], &turns[2 * which][j]);
+        }
+    } else if (tid < HD / 2) {
         const double turn = static_cast<double>(pos) * exp(a.log_base * (static_cast<double>(tid) * (-2.0 / HD)));
         sincos(turn, &turns[1][tid], &turns[0][tid]);
     }
@@ -301,10 +536,10 @@ __device__ __forceinline__ void append(const AppendArgs& a) {
                 for (int j = 0; j < N; j++) dst[lane + 64 * j] = pos < 0 ? 0.0f : static_cast<float>(y[j]);
                 continue;
             }
-            if (id < 0) continue;
-            uint8_t* base = p.k + head_base<HD, Q4>(p, id, h + i - a.n_heads);
+            if (C == kE8 || id < 0) continue;
+            uint8_t* base = p.k + head_base<HD, C>(p, id, h + i - a.n_heads);
             const uint32_t off = static_cast<uint32_t>(pos) & (page - 1);
-            if constexpr (!Q4) {
+            if constexpr (C == kF16) {
                 _Float16* dst = reinterpret_cast<_Float16*>(base) + off * HD;
 #pragma unroll
                 for (int j = 0; j < N; j++) dst[lane + 64 * j] = static_cast<_Float16>(y[j]);  // one rounding
@@ -321,8 +556,12 @@ __device__ __forceinline__ void append(const AppendArgs& a) {
             }
         }
     }
-    // V's 8-position groups: their rows of this call share their heads
     if (pos < 0 || id < 0) return;  // position 0 starts a group too
+    if constexpr (C == kE8) {
+        append_blocks<HD>(a, at, t, static_cast<uint32_t>(id), waves - 1 - wave, waves, turns, wk);
+        return;
+    }
+    // V's 8-position groups: their rows of this call share their heads
     const int32_t start = max(pos & ~7, at.first);
     const uint32_t j0 = static_cast<uint32_t>(start) & 7, mine = static_cast<uint32_t>(pos - start), t0 = t - mine;
     const uint32_t n_rows = min(8u - j0, static_cast<uint32_t>(at.row1) - t0);
@@ -331,12 +570,12 @@ __device__ __forceinline__ void append(const AppendArgs& a) {
     const uint32_t heads_of = mine < p.n_kv ? (p.n_kv - mine + n_rows - 1) / n_rows : 0;
     for (uint32_t i = waves - 1 - wave; i < heads_of * N; i += waves) {
         const uint32_t g = mine + n_rows * (i / N), dim = lane + 64 * (i % N);
-        uint8_t* base = p.v + head_base<HD, Q4>(p, id, g);
+        uint8_t* base = p.v + head_base<HD, C>(p, id, g);
         const float* src = a.qkv + t0 * a.stride + static_cast<size_t>(heads + g) * HD + dim;
         float x[8];
 #pragma unroll
         for (uint32_t r = 0; r < 8; r++) x[r] = src[min(r, n_rows - 1) * a.stride];
-        if constexpr (!Q4) {
+        if constexpr (C == kF16) {
             _Float16* dst = reinterpret_cast<_Float16*>(base) + (grp * HD + dim) * 8;
             if (n_rows == 8) {
                 v8h o;
@@ -370,7 +609,7 @@ __device__ __forceinline__ void append(const AppendArgs& a) {
 
 // The batch's rows of the cache as f32, [n_tokens][n_kv][hd]; NaN where a
 // position has no page, rows of negative positions 0.
-template <int HD, bool Q4>
+template <int HD, Cache C>
 __device__ __forceinline__ void read_rows(const ReadArgs& a) {
     const Paged& p = a.p;
     const uint32_t lane = threadIdx.x & (kWave - 1), t = blockIdx.x;
@@ -391,11 +630,15 @@ __device__ __forceinline__ void read_rows(const ReadArgs& a) {
                 const uint32_t dim = lane + 64 * j;
                 k[i][j] = v[i][j] = pos < 0 ? 0.0f : __builtin_nanf("");
                 if (id < 0) continue;
-                const uint8_t* kb = p.k + head_base<HD, Q4>(p, id, h);
-                const uint8_t* vb = p.v + head_base<HD, Q4>(p, id, h);
-                if constexpr (!Q4) {
+                const uint8_t* kb = p.k + head_base<HD, C>(p, id, h);
+                const uint8_t* vb = p.v + head_base<HD, C>(p, id, h);
+                if constexpr (C == kF16) {
                     k[i][j] = static_cast<float>(reinterpret_cast<const _Float16*>(kb)[off * HD + dim]);
                     v[i][j] = static_cast<float>(reinterpret_cast<const _Float16*>(vb)[(grp * HD + dim) * 8 + in]);
+                } else if constexpr (C == kE8) {
+                    const float dk = e8_scale(kb[page * HD + off / 16]), dv = e8_scale(vb[page * HD + off / 16]);
+                    k[i][j] = __builtin_amdgcn_cvt_f32_fp8(kb[off * HD + dim], 0) * dk;
+                    v[i][j] = __builtin_amdgcn_cvt_f32_fp8(vb[(grp * HD + dim) * 8 + in], 0) * dv;
                 } else {
                     const uint32_t b = kb[off * (HD / 2) + dim / 32 * 16 + (dim & 15)];
                     const float dk = reinterpret_cast<const _Float16*>(kb + page * (HD / 2))[off * (HD / 32) + dim / 32];
@@ -478,16 +721,26 @@ __device__ __forceinline__ v8h decode8(uint32_t w, v2h d0, v2h d1, v2h d2, v2h d
     return v8h{y0.x, y0.y, y1.x, y1.y, y2.x, y2.y, y3.x, y3.y};
 }
 
+// Eight e4m3 values of two words as f16, exactly: a conversion of two with their scale.
+__device__ __forceinline__ v8h decode_e8(uint32_t lo, uint32_t hi, float scale) {
+    const v2h a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, scale, false);
+    const v2h b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, scale, true);
+    const v2h c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, scale, false);
+    const v2h d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, scale, true);
+    return v8h{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+
 // The operands of 32 positions as loaded.
-template <int HD, bool Q4>
+template <int HD, Cache C>
 struct KRaw {
-    uint32_t w[2][HD / 32][Q4 ? 1 : 4];
+    uint32_t w[2][HD / 32][C == kF16 ? 4 : C == kQ4 ? 1 : 2];
     uint32_t d[2][HD / 128 ? HD / 128 : 1];  // a register each: two in one would be waited for where they meet
 };
-template <int HD, bool Q4>
+template <int HD, Cache C>
 struct VRaw {
-    uint32_t w[HD / 16][Q4 ? 1 : 4];
-    v4u d[Q4 ? HD / 64 : 1];
+    uint32_t w[HD / 16][C == kF16 ? 4 : C == kQ4 ? 1 : 2];
+    v4u d[C == kQ4 ? HD / 64 : 1];
+    uint32_t s;  // kE8: the scale byte of the lane's 8 positions
 };
 
 // The pages of a 32-position block: one, or two of 16 positions.  -1: none.
@@ -527,17 +780,22 @@ struct Spots {
     const uint8_t *k, *ks, *v, *vs;
 };
 
-template <int HD, bool Q4>
+template <int HD, Cache C>
 __device__ __forceinline__ Spots spots_of(const Paged& p, const Pages& g, uint32_t h, uint32_t kb, uint32_t lane) {
     const uint32_t m = lane & 15, q = lane >> 4, page = 1u << p.page_shift;
-    const size_t a = head_base<HD, Q4>(p, max(g.a, 0), h), b = head_base<HD, Q4>(p, max(g.b, 0), h);
+    const size_t a = head_base<HD, C>(p, max(g.a, 0), h), b = head_base<HD, C>(p, max(g.b, 0), h);
     const size_t kh = m >= 8 ? b : a, vh = q >= 2 ? b : a;
     const uint32_t row = (kb + k_row(m, 0)) & (page - 1), grp = ((kb + 8 * q) & (page - 1)) >> 3;
     Spots s;
-    if constexpr (!Q4) {
+    if constexpr (C == kF16) {
         s.k = p.k + (kh + row * (HD * 2) + 16 * q);
         s.v = p.v + (vh + (grp * HD + m) * 16);
         s.ks = s.vs = nullptr;
+    } else if constexpr (C == kE8) {  // a lane's K rows lie in one block of 16 positions, as its V's do
+        s.k = p.k + (kh + row * HD + 16 * q);
+        s.ks = p.k + (kh + page * HD + row / 16);
+        s.v = p.v + (vh + (grp * HD + 2 * m) * 8);
+        s.vs = p.v + (vh + page * HD + grp / 2);
     } else {
         s.k = p.k + (kh + row * (HD / 2) + (HD == 64 ? 8 : 16) * q);
         s.ks = p.k + (kh + page * (HD / 2) + row * (HD / 16) + (HD == 64 ? 2 * (q >> 1) : 2 * q));
@@ -547,14 +805,24 @@ __device__ __forceinline__ Spots spots_of(const Paged& p, const Pages& g, uint32
     return s;
 }
 
-template <int HD, bool Q4>
-__device__ __forceinline__ void load_k(const Spots& s, KRaw<HD, Q4>& r) {
+template <int HD, Cache C>
+__device__ __forceinline__ void load_k(const Spots& s, KRaw<HD, C>& r) {
 #pragma unroll
     for (int t = 0; t < 2; t++) {
-        if constexpr (!Q4) {
+        if constexpr (C == kF16) {
 #pragma unroll
             for (int i = 0; i < HD / 32; i++)
                 *reinterpret_cast<v4u*>(r.w[t][i]) = *reinterpret_cast<const v4u*>(s.k + t * (8 * HD) + 64 * i);
+        } else if constexpr (C == kE8) {
+#pragma unroll
+            for (int i = 0; i < HD / 64; i++) {
+                const v4u x = *reinterpret_cast<const v4u*>(s.k + t * (4 * HD) + 64 * i);
+                r.w[t][2 * i][0] = x.x;
+                r.w[t][2 * i][1] = x.y;
+                r.w[t][2 * i + 1][0] = x.z;
+                r.w[t][2 * i + 1][1] = x.w;
+            }
+            if (t == 0) r.d[0][0] = *s.ks;
         } else if constexpr (HD == 64) {  // half of block q / 2
             const v2u x = *reinterpret_cast<const v2u*>(s.k + t * (2 * HD));
             r.w[t][0][0] = x.x;
@@ -574,10 +842,12 @@ __device__ __forceinline__ void load_k(const Spots& s, KRaw<HD, Q4>& r) {
     }
 }
 
-template <int HD, bool Q4>
-__device__ __forceinline__ v8h k_operand(const KRaw<HD, Q4>& r, int t, int i) {
-    if constexpr (!Q4) {
+template <int HD, Cache C>
+__device__ __forceinline__ v8h k_operand(const KRaw<HD, C>& r, int t, int i) {
+    if constexpr (C == kF16) {
         return __builtin_bit_cast(v8h, *reinterpret_cast<const v4u*>(r.w[t][i]));
+    } else if constexpr (C == kE8) {
+        return decode_e8(r.w[t][i][0], r.w[t][i][1], e8_scale(r.d[0][0]));
     } else {
         const _Float16 d = __builtin_bit_cast(_Float16, static_cast<uint16_t>(r.d[t][HD == 64 ? 0 : i / 4]));
         const v2h dd = {d, d};
@@ -587,9 +857,10 @@ __device__ __forceinline__ v8h k_operand(const KRaw<HD, Q4>& r, int t, int i) {
 
 // The dim of slot j (0..7) of k-step i for lane quarter q: the order in which
 // load_k's operands hold the head's dims.
-template <int HD, bool Q4>
+template <int HD, Cache C>
 __device__ __forceinline__ constexpr uint32_t k_dim(uint32_t q, int i, int j) {
-    if (!Q4) return 32 * i + 8 * q + j;
+    if (C == kF16) return 32 * i + 8 * q + j;
+    if (C == kE8) return 64 * (i / 2) + 16 * q + 8 * (i & 1) + j;
     // word w of block b: nibbles 0, 4, 1, 5, 2, 6, 3, 7; nibble n of a GGUF block word is
     // element 4 w + n / 2 + 16 (n % 2)
     const uint32_t b = HD == 64 ? q >> 1 : q + 4 * (i / 4), w = HD == 64 ? 2 * (q & 1) + i : i % 4;
@@ -597,11 +868,21 @@ __device__ __forceinline__ constexpr uint32_t k_dim(uint32_t q, int i, int j) {
     return 32 * b + 4 * w + n / 2 + 16 * (n & 1);
 }
 
-template <int HD, bool Q4>
-__device__ __forceinline__ void load_v(const Spots& s, VRaw<HD, Q4>& r) {
-    if constexpr (!Q4) {
+template <int HD, Cache C>
+__device__ __forceinline__ void load_v(const Spots& s, VRaw<HD, C>& r) {
+    if constexpr (C == kF16) {
 #pragma unroll
         for (int c = 0; c < HD / 16; c++) *reinterpret_cast<v4u*>(r.w[c]) = *reinterpret_cast<const v4u*>(s.v + 256 * c);
+    } else if constexpr (C == kE8) {
+#pragma unroll
+        for (int b = 0; b < HD / 32; b++) {  // dims 32 b + 2 m + {0, 1}
+            const v4u x = *reinterpret_cast<const v4u*>(s.v + 256 * b);
+            r.w[2 * b][0] = x.x;
+            r.w[2 * b][1] = x.y;
+            r.w[2 * b + 1][0] = x.z;
+            r.w[2 * b + 1][1] = x.w;
+        }
+        r.s = *s.vs;
     } else {
 #pragma unroll
         for (int b = 0; b < HD / 64; b++) {  // dims 64 b + 4 m + {0, 1, 2, 3}
@@ -616,15 +897,17 @@ __device__ __forceinline__ void load_v(const Spots& s, VRaw<HD, Q4>& r) {
 }
 
 // The dim of matrix row m of V's tile c.
-template <int HD, bool Q4>
+template <int HD, Cache C>
 __device__ __forceinline__ constexpr uint32_t v_dim(int c, uint32_t m) {
-    return Q4 ? 64 * (c / 4) + 4 * m + c % 4 : 16 * c + m;
+    return C == kQ4 ? 64 * (c / 4) + 4 * m + c % 4 : C == kE8 ? 32 * (c / 2) + 2 * m + c % 2 : 16 * c + m;
 }
 
-template <int HD, bool Q4>
-__device__ __forceinline__ v8h v_operand(const VRaw<HD, Q4>& r, int c) {
-    if constexpr (!Q4) {
+template <int HD, Cache C>
+__device__ __forceinline__ v8h v_operand(const VRaw<HD, C>& r, int c) {
+    if constexpr (C == kF16) {
         return __builtin_bit_cast(v8h, *reinterpret_cast<const v4u*>(r.w[c]));
+    } else if constexpr (C == kE8) {
+        return decode_e8(r.w[c][0], r.w[c][1], e8_scale(r.s));
     } else {
         // (a bit cast of a vector's element takes the first one's bits: each goes through a scalar)
         const uint32_t d0 = r.d[c / 4].x, d1 = r.d[c / 4].y, d2 = r.d[c / 4].z, d3 = r.d[c / 4].w;
@@ -633,18 +916,26 @@ __device__ __forceinline__ v8h v_operand(const VRaw<HD, Q4>& r, int c) {
     }
 }
 
-// V's operands with the positions outside [lo, hi) zero: what lies there may be
-// anything, and 0 times a NaN is a NaN.
-template <int HD, bool Q4>
-__device__ __forceinline__ void clear_v(VRaw<HD, Q4>& r, int32_t at, int32_t lo, int32_t hi) {
+// V's operands with the positions that `seen` does not hold for zero: what lies there
+// may be anything, and 0 times a NaN is a NaN.
+template <int HD, Cache C, class Seen>
+__device__ __forceinline__ void clear_v(VRaw<HD, C>& r, int32_t at, const Seen& seen) {
+    if constexpr (C == kE8) {  // a byte of 0 makes the value 0
+        uint32_t keep[2] = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 8; i++) keep[i / 4] |= seen(at + i) ? 0xffu << (8 * (i % 4)) : 0u;
+#pragma unroll
+        for (int c = 0; c < HD / 16; c++) {
+            r.w[c][0] &= keep[0];
+            r.w[c][1] &= keep[1];
+        }
+        return;
+    }
     uint32_t keep[4];  // by pair of positions
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int32_t a = at + 2 * i;
-        keep[i] = (a >= lo && a < hi ? 0xffffu : 0u) | (a + 1 >= lo && a + 1 < hi ? 0xffff0000u : 0u);
-    }
+    for (int i = 0; i < 4; i++) keep[i] = (seen(at + 2 * i) ? 0xffffu : 0u) | (seen(at + 2 * i + 1) ? 0xffff0000u : 0u);
     const v4u k = {keep[0], keep[1], keep[2], keep[3]};
-    if constexpr (Q4) {  // a scale of 0 makes the value 0
+    if constexpr (C == kQ4) {  // a scale of 0 makes the value 0
 #pragma unroll
         for (int b = 0; b < HD / 64; b++) r.d[b] &= k;
     } else {
@@ -661,7 +952,7 @@ struct QTile {
     float factor;
 };
 
-template <int HD, bool Q4>
+template <int HD, Cache C>
 __device__ __forceinline__ void load_q(QTile<HD>& qt, const float* row, uint32_t q, float scale) {
     // the lane's dims, in runs of four
     float x[HD / 32][8];
@@ -669,9 +960,9 @@ __device__ __forceinline__ void load_q(QTile<HD>& qt, const float* row, uint32_t
 #pragma unroll
     for (int i = 0; i < HD / 32; i++) {
         v4f run[2];
-        if constexpr (Q4) {
+        if constexpr (C == kQ4) {
             // two runs of a word: elements 4 w .. 4 w + 3 and 16 on, in the order of k_dim
-            const uint32_t d = k_dim<HD, Q4>(q, i, 0);
+            const uint32_t d = k_dim<HD, C>(q, i, 0);
             run[0] = *reinterpret_cast<const v4f*>(row + d);
             run[1] = *reinterpret_cast<const v4f*>(row + d + 16);
 #pragma unroll
@@ -680,8 +971,9 @@ __device__ __forceinline__ void load_q(QTile<HD>& qt, const float* row, uint32_t
                 x[i][j] = run[nib & 1][nib / 2];
             }
         } else {
-            run[0] = *reinterpret_cast<const v4f*>(row + 32 * i + 8 * q);
-            run[1] = *reinterpret_cast<const v4f*>(row + 32 * i + 8 * q + 4);
+            const uint32_t d = k_dim<HD, C>(q, i, 0);
+            run[0] = *reinterpret_cast<const v4f*>(row + d);
+            run[1] = *reinterpret_cast<const v4f*>(row + d + 4);
 #pragma unroll
             for (int j = 0; j < 8; j++) x[i][j] = run[j / 4][j % 4];
         }
@@ -728,12 +1020,12 @@ __device__ __forceinline__ void soft_clear(Soft<HD>& st) {
     for (int c = 0; c < HD / 16; c++) st.o[c] = v4f{0, 0, 0, 0};
 }
 
-template <int HD, bool Q4>
-__device__ __forceinline__ void scores(const KRaw<HD, Q4>& k, const QTile<HD>& qt, v4f s[2]) {
+template <int HD, Cache C>
+__device__ __forceinline__ void scores(const KRaw<HD, C>& k, const QTile<HD>& qt, v4f s[2]) {
     s[0] = s[1] = v4f{0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < HD / 32; i++) {
-        const v8h a = k_operand<HD, Q4>(k, 0, i), b = k_operand<HD, Q4>(k, 1, i);
+        const v8h a = k_operand<HD, C>(k, 0, i), b = k_operand<HD, C>(k, 1, i);
         s[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qt.hi[i], s[0], 0, 0, 0);
         s[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, qt.hi[i], s[1], 0, 0, 0);
         s[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qt.lo[i], s[0], 0, 0, 0);
@@ -785,13 +1077,13 @@ __device__ __forceinline__ float soft_pair(float s0, float s1, float factor, flo
 }
 
 // A tile's second product waits for its first; the next tile's operand is decoded between.
-template <int HD, bool Q4>
-__device__ __forceinline__ void values(Soft<HD>& st, const VRaw<HD, Q4>& v, const v8h& hi, const v8h& lo) {
-    v8h before = v_operand<HD, Q4>(v, 0);
+template <int HD, Cache C>
+__device__ __forceinline__ void values(Soft<HD>& st, const VRaw<HD, C>& v, const v8h& hi, const v8h& lo) {
+    v8h before = v_operand<HD, C>(v, 0);
     st.o[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(before, hi, st.o[0], 0, 0, 0);
 #pragma unroll
     for (int c = 1; c < HD / 16; c++) {
-        const v8h a = v_operand<HD, Q4>(v, c);
+        const v8h a = v_operand<HD, C>(v, c);
         st.o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, hi, st.o[c], 0, 0, 0);
         st.o[c - 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(before, lo, st.o[c - 1], 0, 0, 0);
         before = a;
@@ -805,7 +1097,18 @@ struct SeqWork {
     int32_t row0, len, end, first;  // rows, positions with them, position of the first row
     int32_t lo;                     // first position any row sees, down to a multiple of 32
     uint32_t tiles, units;          // per tile and head
+    int32_t sink;                   // with sinks: the positions in front of `lo` that count, in whole blocks
 };
+
+// Sinks.  The positions that an item walks are its sinks' whole blocks, then those from
+// its window's first block on: along an axis without the gap between, where the blocks
+// stay whole.  `sink` positions come before it, 0 where there is no gap.
+__device__ __forceinline__ int32_t sink_blocks(const AttnArgs& a, int32_t& lo, uint32_t block) {
+    const uint64_t up = (static_cast<uint64_t>(a.sinks) + block - 1) / block * block;
+    if (static_cast<uint64_t>(lo) > up) return static_cast<int32_t>(up);
+    lo = 0;
+    return 0;
+}
 
 // Positions that a sequence can have: what its pages hold, and no more than leaves the
 // ends of the blocks and units around the last one below 2^31.  A row past them sees
@@ -814,6 +1117,7 @@ __device__ __forceinline__ uint64_t capacity(const Paged& p) {
     return min(static_cast<uint64_t>(p.table_stride) << p.page_shift, static_cast<uint64_t>((1u << 31) - 2 * kUnit));
 }
 
+template <bool kSinks>
 __device__ __forceinline__ SeqWork seq_work(const AttnArgs& a, int32_t row0, int32_t row1, int32_t kv) {
     SeqWork w;
     const int32_t n = static_cast<int32_t>(a.p.n_tokens);
@@ -824,12 +1128,14 @@ __device__ __forceinline__ SeqWork seq_work(const AttnArgs& a, int32_t row0, int
     const int32_t lo = a.window && w.first >= static_cast<int32_t>(a.window) ? w.first - static_cast<int32_t>(a.window) + 1 : 0;
     w.lo = min(lo, w.end) & ~31;
     w.tiles = (static_cast<uint32_t>(w.len) * a.group + 15) / 16;
-    w.units = max((static_cast<uint32_t>(w.end - w.lo) + kUnit - 1) / kUnit, 1u);
+    w.sink = kSinks ? sink_blocks(a, w.lo, 32) : 0;
+    w.units = max((static_cast<uint32_t>(w.end - w.lo + w.sink) + kUnit - 1) / kUnit, 1u);
     return w;
 }
 
+template <bool kSinks>
 __device__ __forceinline__ SeqWork seq_work(const AttnArgs& a, uint32_t s) {
-    return seq_work(a, a.p.q_start[s], a.p.q_start[s + 1], a.p.kv_len[s]);
+    return seq_work<kSinks>(a, a.p.q_start[s], a.p.q_start[s + 1], a.p.kv_len[s]);
 }
 
 // The batch's lengths, and prefix sums of its sequences' units (all tiles and heads).
@@ -844,6 +1150,7 @@ struct Units {
 // out whole: its row starts are out of order.
 constexpr uint32_t kUnitsMost = 0x7fffffffu;
 
+template <bool kSinks>
 __device__ __forceinline__ uint32_t scan_units(const AttnArgs& a, Units& un) {
     const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1), wid = tid / kWave;
     uint32_t base = 0;
@@ -854,7 +1161,7 @@ __device__ __forceinline__ uint32_t scan_units(const AttnArgs& a, Units& un) {
             un.row0[b + tid] = row0;
             un.row1[b + tid] = row1;
             un.kv[b + tid] = kv;
-            const SeqWork w = seq_work(a, row0, row1, kv);
+            const SeqWork w = seq_work<kSinks>(a, row0, row1, kv);
             if (static_cast<uint32_t>(w.len) * a.group <= a.few_rows)
                 x = static_cast<uint32_t>(min(static_cast<uint64_t>(w.tiles) * a.p.n_kv * (w.units + kItem), static_cast<uint64_t>(kUnitsMost)));
         }
@@ -885,6 +1192,7 @@ struct Place {
     uint32_t s, tile, h, unit;  // within the item (s, tile, h): its cost, then its units
 };
 
+template <bool kSinks>
 __device__ __forceinline__ Place place_of(const AttnArgs& a, const Units& un, uint32_t u, SeqWork& w) {
     uint32_t lo = 0, hi = a.p.n_seqs;  // un.prefix[lo] <= u < un.prefix[hi]
     while (hi - lo > 1) {
@@ -894,7 +1202,7 @@ __device__ __forceinline__ Place place_of(const AttnArgs& a, const Units& un, ui
     }
     Place at;
     at.s = __builtin_amdgcn_readfirstlane(lo);
-    w = seq_work(a, un.row0[at.s], un.row1[at.s], un.kv[at.s]);
+    w = seq_work<kSinks>(a, un.row0[at.s], un.row1[at.s], un.kv[at.s]);
     const uint32_t r = u - un.prefix[at.s], item = r / (w.units + kItem);
     at.unit = __builtin_amdgcn_readfirstlane(r % (w.units + kItem));
     at.tile = __builtin_amdgcn_readfirstlane(item / a.p.n_kv);
@@ -1005,7 +1313,7 @@ __device__ __forceinline__ void join_parts(const AttnArgs& a, const SeqWork& w, 
 // there and counts itself; the counter of an item is that of its first share, and is
 // 0 again when the item is done.  The join adds the shares in their order, so results
 // do not depend on which workgroup does it.
-template <int HD, bool Q4>
+template <int HD, Cache C, bool kSinks>
 __device__ __forceinline__ void attend_few(const AttnArgs& a) {
     __shared__ Units un;
     __shared__ float sm_m[4][16], sm_l[4][16];
@@ -1014,14 +1322,14 @@ __device__ __forceinline__ void attend_few(const AttnArgs& a) {
     __shared__ uint32_t done;
     const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(tid / kWave);
     const uint32_t n = lane & 15, q = lane >> 4;
-    const uint32_t total = scan_units(a, un);
+    const uint32_t total = scan_units<kSinks>(a, un);
     const uint32_t share = share_of(total, gridDim.x);  // blockIdx.x of them: less than total + gridDim.x^2
-    const int32_t win = static_cast<int32_t>(a.window);
+    const int32_t win = static_cast<int32_t>(a.window), sinks = static_cast<int32_t>(a.sinks);
     uint32_t u = blockIdx.x * share;
     const uint32_t u_end = min(u + share, total);
     while (u < u_end) {
         SeqWork w;
-        Place at = place_of(a, un, u, w);
+        Place at = place_of<kSinks>(a, un, u, w);
         const uint32_t item = u - at.unit, end = min(item + kItem + w.units, u_end);
         const uint32_t first = item + kItem;  // the item's first unit
         at.unit = max(u, first) - first;
@@ -1040,43 +1348,48 @@ __device__ __forceinline__ void attend_few(const AttnArgs& a) {
         const int32_t hi_b = w.first + static_cast<int32_t>(tok_b) + 1;
         const int32_t tile_hi = min(hi_b, w.end);
         const int32_t tile_lo = win && hi_a > win ? hi_a - win : 0, all_lo = win && hi_b > win ? hi_b - win : 0;
-        // this wave's blocks: every 128 positions from kb0, those that any row sees
-        const int32_t kb0 = w.lo + static_cast<int32_t>(at.unit * kUnit + 32 * wid);
-        const int32_t skip = max(tile_lo - 31 - kb0, 0);
+        // this wave's blocks: every 128 positions from kb0, those that any row sees (with
+        // sinks: from kb0 along the axis without the gap)
+        const int32_t gap = kSinks ? w.lo - w.sink : 0;
+        const int32_t kb0 = w.lo - gap + static_cast<int32_t>(at.unit * kUnit + 32 * wid) - w.sink;
+        const int32_t skip = kSinks ? 0 : max(tile_lo - 31 - kb0, 0);
         const uint32_t i0 = (static_cast<uint32_t>(skip) + kUnit - 1) / kUnit;
-        const uint32_t i1 = tile_hi > kb0 ? min(units, (static_cast<uint32_t>(tile_hi - kb0) + kUnit - 1) / kUnit) : 0;
+        const uint32_t i1 = tile_hi - gap > kb0 ? min(units, (static_cast<uint32_t>(tile_hi - gap - kb0) + kUnit - 1) / kUnit) : 0;
         // The next block's K is on its way from the moment that this one's scores are
         // done, its V from when this one's is used: no register waits for its turn.  (A
         // second set of them, loaded a block ahead, measured 93 us where this takes 90, at
         // 64 sequences of 820 to 8192 positions and 8 heads; f16, 6 of up to 32001: 119 and
         // 107.)  Past the last block that one is loaded again: loads under a condition
         // would be waited for where it ends.
-        KRaw<HD, Q4> kr;
-        VRaw<HD, Q4> vr;
+        KRaw<HD, C> kr;
+        VRaw<HD, C> vr;
         Pages pg = {-1, -1}, ahead = {-1, -1};
         QTile<HD> qt;
         Soft<HD> st;
-        const auto kb_of = [&](uint32_t i) { return static_cast<uint32_t>(kb0) + kUnit * min(i, i1 - 1); };
+        const auto kb_of = [&](uint32_t i) {
+            const uint32_t kb = static_cast<uint32_t>(kb0) + kUnit * min(i, i1 - 1);
+            return kSinks && kb >= static_cast<uint32_t>(w.sink) ? kb + static_cast<uint32_t>(gap) : kb;
+        };
         if (i0 < i1) ahead = entries_at(a.p, at.s, kb_of(i0));
-        load_q<HD, Q4>(qt, a.q + (static_cast<size_t>(w.row0 + tok) * a.n_heads + head) * HD, q, a.scale);
+        load_q<HD, C>(qt, a.q + (static_cast<size_t>(w.row0 + tok) * a.n_heads + head) * HD, q, a.scale);
         soft_clear<HD>(st);
         if (pos >= 0 && static_cast<uint64_t>(pos) >= capacity(a.p)) st.l = __builtin_nanf("");
         if (i0 < i1) {
             pg = pages_of(a.p, ahead, kb_of(i0));
-            const Spots spots = spots_of<HD, Q4>(a.p, pg, at.h, kb_of(i0), lane);
-            load_k<HD, Q4>(spots, kr);
-            load_v<HD, Q4>(spots, vr);
+            const Spots spots = spots_of<HD, C>(a.p, pg, at.h, kb_of(i0), lane);
+            load_k<HD, C>(spots, kr);
+            load_v<HD, C>(spots, vr);
             ahead = entries_at(a.p, at.s, kb_of(i0 + 1));
         }
         for (uint32_t i = i0; i < i1; i++) {
             const int32_t kb = static_cast<int32_t>(kb_of(i));
             v4f s[2];
-            scores<HD, Q4>(kr, qt, s);
+            scores<HD, C>(kr, qt, s);
             const Pages next = pages_of(a.p, ahead, kb_of(i + 1));
-            const Spots spots = spots_of<HD, Q4>(a.p, next, at.h, kb_of(i + 1), lane);
-            load_k<HD, Q4>(spots, kr);
+            const Spots spots = spots_of<HD, C>(a.p, next, at.h, kb_of(i + 1), lane);
+            load_k<HD, C>(spots, kr);
             ahead = entries_at(a.p, at.s, kb_of(i + 2));
-            if (kb < all_lo || kb + 32 > min(hi_a, w.end) || pg.a < 0 || pg.b < 0) {
+            if ((kb < all_lo && (!kSinks || kb + 32 > sinks)) || kb + 32 > min(hi_a, w.end) || pg.a < 0 || pg.b < 0) {
                 const int32_t p0 = kb + static_cast<int32_t>(8 * q);
                 const bool no_page = pg.of(q >= 2) < 0;
 #pragma unroll
@@ -1084,9 +1397,10 @@ __device__ __forceinline__ void attend_few(const AttnArgs& a) {
                     const int32_t x = p0 + e;
                     float v = s[e / 4][e % 4];
                     if (no_page) v = __builtin_nanf("");
-                    s[e / 4][e % 4] = x < lo || x >= hi ? -INFINITY : v;
+                    s[e / 4][e % 4] = (x < lo && (!kSinks || x >= sinks)) || x >= hi ? -INFINITY : v;
                 }
-                clear_v<HD, Q4>(vr, p0, tile_lo, no_page ? tile_lo : tile_hi);
+                const int32_t end = !no_page ? tile_hi : kSinks ? 0 : tile_lo;
+                clear_v<HD, C>(vr, p0, [=](int32_t x) { return (x >= tile_lo || (kSinks && x < sinks)) && x < end; });
             }
             v8h ph, pl;
             const float base = soft_base<HD, 2>(st, s, qt.factor), minus = minus_one();
@@ -1094,8 +1408,8 @@ __device__ __forceinline__ void attend_few(const AttnArgs& a) {
 #pragma unroll
             for (int e = 0; e < 8; e += 2) sum += soft_pair(s[e / 4][e % 4], s[e / 4][e % 4 + 1], qt.factor, base, minus, ph, pl, e);
             st.l += sum;
-            values<HD, Q4>(st, vr, ph, pl);
-            load_v<HD, Q4>(spots, vr);
+            values<HD, C>(st, vr, ph, pl);
+            load_v<HD, C>(spots, vr);
             pg = next;
         }
         // join the waves
@@ -1107,7 +1421,7 @@ __device__ __forceinline__ void attend_few(const AttnArgs& a) {
 #pragma unroll
         for (int c = 0; c < HD / 16; c++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) sm_o[wid][n][v_dim<HD, Q4>(c, 4 * q + i)] = st.o[c][i];
+            for (int i = 0; i < 4; i++) sm_o[wid][n][v_dim<HD, C>(c, 4 * q + i)] = st.o[c][i];
         __syncthreads();
         const bool whole = units == w.units;
         float* slot = part_slot<HD>(a, 2 * blockIdx.x + (at.unit == 0 ? 1 : 0));
@@ -1188,12 +1502,12 @@ struct Operands {  // one stage
 
 // A wave's share of a stage as loaded: K's or V's four operands of a block, or both
 // (hd 128: the first four waves load K's, the others V's; hd 64: the even, the odd ones).
-template <int HD, bool Q4>
+template <int HD, Cache C>
 struct Share {
-    static constexpr int kOne = Q4 ? 1 : 4, kV = Many<HD>::kBoth ? kOne : 0;  // V's first
+    static constexpr int kOne = C == kF16 ? 4 : C == kQ4 ? 1 : 2, kV = Many<HD>::kBoth ? kOne : 0;  // V's first
     v4u w[kV + kOne];
     v4u vd;
-    uint32_t kd;
+    uint32_t kd, vs;  // kE8: the scale bytes
     Pages g;
     uint32_t kb;
 };
@@ -1211,11 +1525,11 @@ __device__ __forceinline__ Job<HD> job_of(uint32_t w) {
     return {w >> 1, 0, 0, 0, (w & 1) == 0, (w & 1) != 0};
 }
 
-template <int HD, bool Q4>
+template <int HD, Cache C>
 __device__ __forceinline__ void share_load(const Paged& p, const Job<HD>& job, uint32_t h, uint32_t lane,
-                                           Share<HD, Q4>& r) {
+                                           Share<HD, C>& r) {
     const uint32_t m = lane & 15, q = lane >> 4, page = 1u << p.page_shift;
-    const size_t b0 = head_base<HD, Q4>(p, max(r.g.a, 0), h), b1 = head_base<HD, Q4>(p, max(r.g.b, 0), h);
+    const size_t b0 = head_base<HD, C>(p, max(r.g.a, 0), h), b1 = head_base<HD, C>(p, max(r.g.b, 0), h);
     const uint8_t* kbase = p.k + (m >= 8 ? b1 : b0);
     const uint8_t* vbase = p.v + (q >= 2 ? b1 : b0);
     const uint32_t grp = ((r.kb + 8 * q) & (page - 1)) >> 3;
@@ -1223,12 +1537,16 @@ __device__ __forceinline__ void share_load(const Paged& p, const Job<HD>& job, u
         const uint32_t off = (r.kb + k_row(m, job.t)) & (page - 1);
         if constexpr (HD == 64) {
             const uint32_t off1 = (r.kb + k_row(m, 1)) & (page - 1);
-            if constexpr (Q4) {
+            if constexpr (C == kQ4) {
                 const v2u x = *reinterpret_cast<const v2u*>(kbase + off * 32 + 8 * q);
                 const v2u y = *reinterpret_cast<const v2u*>(kbase + off1 * 32 + 8 * q);
                 r.w[0] = v4u{x.x, x.y, y.x, y.y};
                 const uint16_t* sc = reinterpret_cast<const uint16_t*>(kbase + page * 32) + (q >> 1);
                 r.kd = sc[off * 2] | static_cast<uint32_t>(sc[off1 * 2]) << 16;
+            } else if constexpr (C == kE8) {
+                r.w[0] = *reinterpret_cast<const v4u*>(kbase + off * 64 + 16 * q);
+                r.w[1] = *reinterpret_cast<const v4u*>(kbase + off1 * 64 + 16 * q);
+                r.kd = kbase[page * 64 + off / 16];  // of both rows
             } else {
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
@@ -1236,9 +1554,14 @@ __device__ __forceinline__ void share_load(const Paged& p, const Job<HD>& job, u
                     r.w[2 + i] = *reinterpret_cast<const v4u*>(kbase + off1 * 128 + 64 * i + 16 * q);
                 }
             }
-        } else if constexpr (Q4) {
+        } else if constexpr (C == kQ4) {
             r.w[0] = *reinterpret_cast<const v4u*>(kbase + off * (HD / 2) + 16 * q + 64 * job.kb);
             r.kd = reinterpret_cast<const uint16_t*>(kbase + page * (HD / 2))[off * (HD / 32) + q + 4 * job.kb];
+        } else if constexpr (C == kE8) {
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+                r.w[i] = *reinterpret_cast<const v4u*>(kbase + off * HD + 64 * (2 * job.kb + i) + 16 * q);
+            r.kd = kbase[page * HD + off / 16];
         } else {
 #pragma unroll
             for (int i = 0; i < 4; i++)
@@ -1246,9 +1569,14 @@ __device__ __forceinline__ void share_load(const Paged& p, const Job<HD>& job, u
         }
     }
     if (job.v) {
-        if constexpr (Q4) {
+        if constexpr (C == kQ4) {
             r.w[r.kV] = *reinterpret_cast<const v4u*>(vbase + (grp * HD + 64 * job.vb + 4 * m) * 4);
             r.vd = reinterpret_cast<const v4u*>(vbase + page * (HD / 2))[grp * (HD / 32) + 2 * job.vb + (m >> 3)];
+        } else if constexpr (C == kE8) {
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+                r.w[r.kV + i] = *reinterpret_cast<const v4u*>(vbase + (grp * HD + 32 * (2 * job.vb + i) + 2 * m) * 8);
+            r.vs = vbase[page * HD + grp / 2];
         } else {
 #pragma unroll
             for (int i = 0; i < 4; i++)
@@ -1258,34 +1586,49 @@ __device__ __forceinline__ void share_load(const Paged& p, const Job<HD>& job, u
     }
 }
 
+// Masks of two pairs of 16 bits as one of four bytes.
+__device__ __forceinline__ uint32_t bytes(uint32_t a, uint32_t b) {
+    return (a & 0xffu) | (a >> 8 & 0xff00u) | (b & 0xffu) << 16 | (b & 0xff000000u);
+}
+
 // The share decoded into the stage's operands.  `edge`: positions outside [lo, hi)
-// or without a page may be among them: their V becomes 0, a K without a page NaN.
-template <int HD, bool Q4, int kBlocks>
-__device__ __forceinline__ void share_store(const Job<HD>& job, Share<HD, Q4>& r, Operands<HD, kBlocks>& to, uint32_t lane,
-                                            int32_t lo, int32_t hi) {
+// (that are no sinks) or without a page may be among them: their V becomes 0, a K
+// without a page NaN.
+template <int HD, Cache C, int kBlocks, bool kSinks>
+__device__ __forceinline__ void share_store(const Job<HD>& job, Share<HD, C>& r, Operands<HD, kBlocks>& to, uint32_t lane,
+                                            int32_t lo, int32_t hi, int32_t sinks) {
     const uint32_t m = lane & 15, q = lane >> 4;
     const bool edge = static_cast<int32_t>(r.kb) < lo || static_cast<int32_t>(r.kb) + 32 > hi || r.g.a < 0 || r.g.b < 0;
     v4u keep = {~0u, ~0u, ~0u, ~0u};
     bool no_k = false;
     if (edge) {
         no_k = r.g.of(m >= 8) < 0;
-        const int32_t at = static_cast<int32_t>(r.kb + 8 * q), end = r.g.of(q >= 2) < 0 ? lo : hi;
+        const int32_t at = static_cast<int32_t>(r.kb + 8 * q), end = r.g.of(q >= 2) >= 0 ? hi : kSinks ? 0 : lo;
+        const auto seen = [=](int32_t a) { return (a >= lo || (kSinks && a < sinks)) && a < end; };
         uint32_t x[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int32_t a = at + 2 * i;
-            x[i] = (a >= lo && a < end ? 0xffffu : 0u) | (a + 1 >= lo && a + 1 < end ? 0xffff0000u : 0u);
+            x[i] = (seen(a) ? 0xffffu : 0u) | (seen(a + 1) ? 0xffff0000u : 0u);
         }
         keep = v4u{x[0], x[1], x[2], x[3]};
     }
     if (job.k) {
         v8h o[4];
-        if constexpr (Q4) {
+        if constexpr (C == kQ4) {
             const uint32_t x[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
             const uint32_t d0 = (r.kd & 0xffffu) * 0x10001u, d1 = HD == 64 ? (r.kd >> 16) * 0x10001u : d0;
             const v2h s0 = __builtin_bit_cast(v2h, d0), s1 = __builtin_bit_cast(v2h, d1);
 #pragma unroll
             for (int i = 0; i < 4; i++) o[i] = i < 2 ? decode8(x[i], s0, s0, s0, s0) : decode8(x[i], s1, s1, s1, s1);
+        } else if constexpr (C == kE8) {
+            const float d = e8_scale(r.kd);
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const uint32_t x[4] = {r.w[i].x, r.w[i].y, r.w[i].z, r.w[i].w};
+                o[2 * i] = decode_e8(x[0], x[1], d);
+                o[2 * i + 1] = decode_e8(x[2], x[3], d);
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < 4; i++) o[i] = __builtin_bit_cast(v8h, r.w[i]);
@@ -1299,7 +1642,7 @@ __device__ __forceinline__ void share_store(const Job<HD>& job, Share<HD, Q4>& r
         }
     }
     if (job.v) {
-        if constexpr (Q4) {
+        if constexpr (C == kQ4) {
             const v4u d = r.vd & keep;
             const uint32_t d0 = d.x, d1 = d.y, d2 = d.z, d3 = d.w;
             const v4u y = r.w[r.kV];
@@ -1309,6 +1652,15 @@ __device__ __forceinline__ void share_store(const Job<HD>& job, Share<HD, Q4>& r
                 to.v[job.blk][4 * job.vb + i][lane] =
                     decode8(x[i], __builtin_bit_cast(v2h, d0), __builtin_bit_cast(v2h, d1), __builtin_bit_cast(v2h, d2),
                             __builtin_bit_cast(v2h, d3));
+        } else if constexpr (C == kE8) {
+            const float d = e8_scale(r.vs);
+            const uint32_t k0 = bytes(keep.x, keep.y), k1 = bytes(keep.z, keep.w);
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const uint32_t x[4] = {r.w[r.kV + i].x & k0, r.w[r.kV + i].y & k1, r.w[r.kV + i].z & k0, r.w[r.kV + i].w & k1};
+                to.v[job.blk][4 * job.vb + 2 * i][lane] = decode_e8(x[0], x[1], d);
+                to.v[job.blk][4 * job.vb + 2 * i + 1][lane] = decode_e8(x[2], x[3], d);
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -1327,7 +1679,7 @@ struct Item {
 
 // Tiles of the sequences with more than few_rows rows, in order; the grid has one
 // workgroup for each (a bound of their number), kv head and split.
-template <int HD>
+template <int HD, bool kSinks>
 __device__ __forceinline__ Item item_of(const AttnArgs& a, uint32_t block, uint32_t* prefix, uint32_t* sums, SeqWork& w) {
     constexpr uint32_t kRows = Many<HD>::kRows;
     Item it;
@@ -1340,7 +1692,7 @@ __device__ __forceinline__ Item item_of(const AttnArgs& a, uint32_t block, uint3
     for (uint32_t b = 0; b < a.p.n_seqs; b += blockDim.x) {
         uint32_t x = 0;
         if (b + tid < a.p.n_seqs) {
-            const uint32_t rows = static_cast<uint32_t>(seq_work(a, b + tid).len) * a.group;
+            const uint32_t rows = static_cast<uint32_t>(seq_work<kSinks>(a, b + tid).len) * a.group;
             x = rows > a.few_rows ? (rows + kRows - 1) / kRows : 0;
         }
         uint32_t run = x;
@@ -1371,18 +1723,19 @@ __device__ __forceinline__ Item item_of(const AttnArgs& a, uint32_t block, uint3
     if (!it.any) return it;
     it.s = __builtin_amdgcn_readfirstlane(prefix[0]);
     it.tile = __builtin_amdgcn_readfirstlane(prefix[1]);
-    w = seq_work(a, it.s);
+    w = seq_work<kSinks>(a, it.s);
     return it;
 }
 
 // The positions that an item's rows see, and its split's part of them.
 struct Span {
-    int32_t lo, hi;      // of the item
-    int32_t from, to;    // of the split
+    int32_t lo, hi;      // of the item, its sinks apart
+    int32_t from, to;    // of the split; with sinks along the axis without the gap
+    int32_t sink, gap;   // with sinks: from `sink` on that axis a position is `gap` more
     uint32_t parts;      // splits that have any
 };
 
-template <int HD>
+template <int HD, bool kSinks>
 __device__ __forceinline__ Span span_of(const AttnArgs& a, const Item& it, const SeqWork& w) {
     constexpr uint32_t kRows = Many<HD>::kRows;
     const uint32_t rows = static_cast<uint32_t>(w.len) * a.group;
@@ -1391,14 +1744,22 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, const Item& it, const
     s.hi = max(min(w.first + static_cast<int32_t>(last_tok) + 1, w.end), 0);
     const int32_t first_hi = w.first + static_cast<int32_t>(first_tok) + 1;
     s.lo = a.window && first_hi > static_cast<int32_t>(a.window) ? first_hi - static_cast<int32_t>(a.window) : 0;
-    const int32_t start = min(s.lo, s.hi) & ~31;
+    int32_t start = min(s.lo, s.hi) & ~31;
+    s.sink = s.gap = 0;
+    if constexpr (kSinks) {
+        start &= ~63;  // a stage holds sinks or none
+        s.sink = sink_blocks(a, start, 64);
+        s.gap = start - s.sink;
+        start = 0;
+    }
     // splits of at least 256 positions, in whole stages of any form
-    const uint32_t n = static_cast<uint32_t>(s.hi - start), step = 64;
+    const uint32_t n = static_cast<uint32_t>(s.hi - s.gap - start), step = 64;
     const uint32_t each = max((n + a.splits - 1) / a.splits, 256u);
     const uint32_t part = (each + step - 1) / step * step;
     s.parts = max((n + part - 1) / part, 1u);
-    s.from = static_cast<int32_t>(min(static_cast<uint64_t>(start) + static_cast<uint64_t>(part) * it.split, static_cast<uint64_t>(s.hi)));
-    s.to = static_cast<int32_t>(min(static_cast<uint64_t>(s.from) + part, static_cast<uint64_t>(s.hi)));
+    const uint64_t end = static_cast<uint64_t>(s.hi - s.gap);
+    s.from = static_cast<int32_t>(min(static_cast<uint64_t>(start) + static_cast<uint64_t>(part) * it.split, end));
+    s.to = static_cast<int32_t>(min(static_cast<uint64_t>(s.from) + part, end));
     return s;
 }
 
@@ -1410,7 +1771,7 @@ __device__ __forceinline__ float* many_slot(const AttnArgs& a, uint32_t block) {
 // What the scheduler may move past a step of the products: all but them and their operands.
 constexpr int kMoves = 0x2 | 0x4 | 0x10;  // VALU, SALU, VMEM
 
-template <int HD, bool Q4, bool kHalved>
+template <int HD, Cache C, bool kHalved, bool kSinks>
 __device__ __forceinline__ void attend_many(const AttnArgs& a) {
     using M = Many<HD, kHalved>;
     using Stage = Operands<HD, M::kBlocks>;
@@ -1419,9 +1780,9 @@ __device__ __forceinline__ void attend_many(const AttnArgs& a) {
     const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(tid / kWave);
     const uint32_t n = lane & 15, q = lane >> 4;
     SeqWork w;
-    const Item it = item_of<HD>(a, blockIdx.x, prefix, sums, w);
+    const Item it = item_of<HD, kSinks>(a, blockIdx.x, prefix, sums, w);
     if (!it.any) return;
-    const Span sp = span_of<HD>(a, it, w);
+    const Span sp = span_of<HD, kSinks>(a, it, w);
     if (it.split >= sp.parts) return;
     const uint32_t rows = static_cast<uint32_t>(w.len) * a.group;
     const uint32_t row0 = M::kRows * it.tile + 16 * M::kRt * (wid % M::kRowWaves), half = kHalved ? wid / M::kRowWaves : 0;
@@ -1436,7 +1797,7 @@ __device__ __forceinline__ void attend_many(const AttnArgs& a) {
         const int32_t pos = w.first + static_cast<int32_t>(tok);
         hi[i] = live ? pos + 1 : 0;
         lo[i] = a.window && hi[i] > static_cast<int32_t>(a.window) ? hi[i] - static_cast<int32_t>(a.window) : 0;
-        load_q<HD, Q4>(qt[i], a.q + (static_cast<size_t>(w.row0 + tok) * a.n_heads + head) * HD, q, a.scale);
+        load_q<HD, C>(qt[i], a.q + (static_cast<size_t>(w.row0 + tok) * a.n_heads + head) * HD, q, a.scale);
         soft_clear<HD>(st[i]);
         if (!live) st[i].m = 0.0f;
         if (live && pos >= 0 && static_cast<uint64_t>(pos) >= capacity(a.p)) st[i].l = __builtin_nanf("");
@@ -1444,26 +1805,29 @@ __device__ __forceinline__ void attend_many(const AttnArgs& a) {
     // the wave's rows are in order of position: what any of them and what all of them see
     const bool wave_live = row0 < rows;
     const uint32_t tok_a = min(row0, rows - 1) / a.group, tok_b = (min(row0 + 16 * M::kRt, rows) - 1) / a.group;
-    const int32_t win = static_cast<int32_t>(a.window);
+    const int32_t win = static_cast<int32_t>(a.window), sinks = static_cast<int32_t>(a.sinks);
     const int32_t hi_a = w.first + static_cast<int32_t>(tok_a) + 1, hi_b = w.first + static_cast<int32_t>(tok_b) + 1;
     const int32_t any_lo = win && hi_a > win ? hi_a - win : 0, all_lo = win && hi_b > win ? hi_b - win : 0;
     const bool full_tile = row0 + 16 * M::kRt <= rows;
 
     const Job<HD> job = job_of<HD>(wid);
-    Share<HD, Q4> sh;
+    Share<HD, C> sh;
     Pages ahead = {-1, -1};  // of the stage after the one that is loaded next
+    const auto real = [&](uint32_t at) {
+        return kSinks && at >= static_cast<uint32_t>(sp.sink) ? at + static_cast<uint32_t>(sp.gap) : at;
+    };
     const auto start_load = [&](uint32_t at) {
-        sh.kb = at + 32 * job.blk;
+        sh.kb = real(at) + 32 * job.blk;
         sh.g = pages_of(a.p, ahead, sh.kb);
-        share_load<HD, Q4>(a.p, job, it.h, lane, sh);
-        ahead = entries_at(a.p, it.s, sh.kb + M::kStage);
+        share_load<HD, C>(a.p, job, it.h, lane, sh);
+        ahead = entries_at(a.p, it.s, kSinks ? real(at + M::kStage) + 32 * job.blk : sh.kb + M::kStage);
     };
     uint32_t at = static_cast<uint32_t>(sp.from), buf = 0;
     const uint32_t to = static_cast<uint32_t>(sp.to);
     if (at < to) {
-        ahead = entries_at(a.p, it.s, at + 32 * job.blk);
+        ahead = entries_at(a.p, it.s, real(at) + 32 * job.blk);
         start_load(at);
-        share_store<HD, Q4, M::kBlocks>(job, sh, ops[0], lane, sp.lo, sp.hi);
+        share_store<HD, C, M::kBlocks, kSinks>(job, sh, ops[0], lane, sp.lo, sp.hi, sinks);
     }
     __syncthreads();
     for (; at < to; at += M::kStage) {
@@ -1471,8 +1835,8 @@ __device__ __forceinline__ void attend_many(const AttnArgs& a) {
         if (more) start_load(at + M::kStage);
         const Stage& op = ops[buf];
         constexpr int32_t kSpan = 32 * M::kMine;
-        const int32_t kb = static_cast<int32_t>(at) + kSpan * static_cast<int32_t>(half);
-        if (wave_live && kb < hi_b && kb + kSpan > any_lo) {
+        const int32_t kb = static_cast<int32_t>(real(at)) + kSpan * static_cast<int32_t>(half);
+        if (wave_live && kb < hi_b && (kb + kSpan > any_lo || (kSinks && kb < sinks))) {
             // The operands of the stage in the order of their use, K's tiles, then V's: each
             // comes from LDS kAhead steps before its products.
             constexpr int kTiles = 2 * M::kMine, kK = kTiles * (HD / 32), kV = HD / 16, kAll = kK + M::kMine * kV;
@@ -1502,14 +1866,15 @@ __device__ __forceinline__ void attend_many(const AttnArgs& a) {
                 __builtin_amdgcn_sched_barrier(kMoves);
             }
             float base[M::kRt];
-            const bool masked = kb < all_lo || kb + kSpan > hi_a || !full_tile;
+            const bool masked = (kb < all_lo && (!kSinks || kb + kSpan > sinks)) || kb + kSpan > hi_a || !full_tile;
 #pragma unroll
             for (int r = 0; r < M::kRt; r++) {
                 if (masked) {
 #pragma unroll
                     for (int j = 0; j < 4 * kTiles; j++) {
                         const int32_t p = kb + 32 * (j / 8) + static_cast<int32_t>(8 * q) + j % 8;
-                        s[r][j / 4][j % 4] = p < lo[r] || p >= hi[r] ? -INFINITY : s[r][j / 4][j % 4];
+                        s[r][j / 4][j % 4] =
+                            (p < lo[r] && (!kSinks || p >= sinks)) || p >= hi[r] ? -INFINITY : s[r][j / 4][j % 4];
                     }
                 }
                 base[r] = soft_base<HD, kTiles>(st[r], s[r], qt[r].factor);
@@ -1540,7 +1905,7 @@ __device__ __forceinline__ void attend_many(const AttnArgs& a) {
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
-        if (more) share_store<HD, Q4, M::kBlocks>(job, sh, ops[buf ^ 1], lane, sp.lo, sp.hi);
+        if (more) share_store<HD, C, M::kBlocks, kSinks>(job, sh, ops[buf ^ 1], lane, sp.lo, sp.hi, sinks);
         __syncthreads();
         buf ^= 1;
     }
@@ -1581,13 +1946,22 @@ __device__ __forceinline__ void attend_many(const AttnArgs& a) {
         const float f = whole && l != 0.0f ? 1.0f / l : 1.0f;
 #pragma unroll
         for (int c = 0; c < HD / 16; c++) {
-            if constexpr (Q4) {
+            if constexpr (C == kQ4) {
                 // tiles 4 k .. 4 k + 3 hold runs of dims: 64 k + 16 q + 4 i + {0 .. 3}
                 if (c % 4 == 0) {
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         const v4f o = {st[i].o[c][e], st[i].o[c + 1][e], st[i].o[c + 2][e], st[i].o[c + 3][e]};
                         *reinterpret_cast<v4f*>(dst + 16 * c + 16 * q + 4 * e) = o * f;
+                    }
+                }
+            } else if constexpr (C == kE8) {
+                // tiles 2 k and 2 k + 1: runs of 32 k + 8 q + 2 i + {0, 1}
+                if (c % 2 == 0) {
+#pragma unroll
+                    for (int e = 0; e < 4; e += 2) {
+                        const v4f o = {st[i].o[c][e], st[i].o[c + 1][e], st[i].o[c][e + 1], st[i].o[c + 1][e + 1]};
+                        *reinterpret_cast<v4f*>(dst + 16 * c + 8 * q + 2 * e) = o * f;
                     }
                 }
             } else {
@@ -1602,15 +1976,15 @@ __device__ __forceinline__ void attend_many(const AttnArgs& a) {
 }
 
 // The join of an item's splits: a workgroup an item and 16 of its rows.
-template <int HD, bool Q4>
+template <int HD, bool kSinks>
 __device__ __forceinline__ void merge_many(const AttnArgs& a) {
     using M = Many<HD>;
     __shared__ uint32_t prefix[2], sums[8];
     const uint32_t block = blockIdx.x / a.p.n_kv * a.p.n_kv * a.splits + blockIdx.x % a.p.n_kv;  // its first split's
     SeqWork w;
-    const Item it = item_of<HD>(a, block, prefix, sums, w);
+    const Item it = item_of<HD, kSinks>(a, block, prefix, sums, w);
     if (!it.any) return;
-    const Span sp = span_of<HD>(a, it, w);
+    const Span sp = span_of<HD, kSinks>(a, it, w);
     const uint32_t rows = static_cast<uint32_t>(w.len) * a.group;
     if (sp.parts == 1 || M::kRows * it.tile + 16 * blockIdx.y >= rows) return;
     // four splits of all of a thread's values in flight at once: the call is their latency
@@ -1668,33 +2042,40 @@ __device__ __forceinline__ void merge_many(const AttnArgs& a) {
 
 }  // namespace
 
-#define ZLM_PAGED(HD, NAME, Q4)                                                                               \
-    extern "C" __global__ void __launch_bounds__(256) zlm_paged_append_##NAME##_##HD(AppendArgs a) {          \
-        append<HD, Q4>(a);                                                                                    \
-    }                                                                                                         \
-    extern "C" __global__ void __launch_bounds__(256) zlm_paged_read_##NAME##_##HD(ReadArgs a) {              \
-        read_rows<HD, Q4>(a);                                                                                 \
-    }                                                                                                         \
+#define ZLM_PAGED_ATTEND(HD, NAME, C, kSinks)                                                                     \
     extern "C" __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) zlm_paged_attend_few_##NAME##_##HD(AttnArgs a) { \
-        attend_few<HD, Q4>(a);                                                                                \
-    }                                                                                                         \
+        attend_few<HD, C, kSinks>(a);                                                                             \
+    }                                                                                                             \
     extern "C" __global__ void __launch_bounds__(64 * Many<HD>::kWaves, 2) zlm_paged_attend_many_##NAME##_##HD(AttnArgs a) { \
-        attend_many<HD, Q4, false>(a);                                                                               \
-    }                                                                                                         \
-    extern "C" __global__ void __launch_bounds__(256) zlm_paged_merge_many_##NAME##_##HD(AttnArgs a) {        \
-        merge_many<HD, Q4>(a);                                                                                \
+        attend_many<HD, C, false, kSinks>(a);                                                                     \
+    }                                                                                                             \
+    extern "C" __global__ void __launch_bounds__(256) zlm_paged_merge_many_##NAME##_##HD(AttnArgs a) {            \
+        merge_many<HD, kSinks>(a);                                                                                \
     }
-
-ZLM_PAGED(64, f16, false)
-ZLM_PAGED(64, q4_0, true)
-ZLM_PAGED(128, f16, false)
-ZLM_PAGED(128, q4_0, true)
-ZLM_PAGED(256, f16, false)
-ZLM_PAGED(256, q4_0, true)
-
-#define ZLM_PAGED_HALVED(HD, NAME, Q4)                                                                         \
-    extern "C" __global__ void __launch_bounds__(512, 2) zlm_paged_attend_halved_##NAME##_##HD(AttnArgs a) { \
-        attend_many<HD, Q4, true>(a);                                                                         \
+#define ZLM_PAGED_HALVED(NAME, C, kSinks)                                                                         \
+    extern "C" __global__ void __launch_bounds__(512, 2) zlm_paged_attend_halved_##NAME##_256(AttnArgs a) {       \
+        attend_many<256, C, true, kSinks>(a);                                                                     \
     }
-ZLM_PAGED_HALVED(256, f16, false)
-ZLM_PAGED_HALVED(256, q4_0, true)
+#define ZLM_PAGED_ROWS(HD, NAME, C)                                                                               \
+    extern "C" __global__ void __launch_bounds__(256) zlm_paged_append_##NAME##_##HD(AppendArgs a) {              \
+        append<HD, C>(a);                                                                                         \
+    }                                                                                                             \
+    extern "C" __global__ void __launch_bounds__(256) zlm_paged_read_##NAME##_##HD(ReadArgs a) {                  \
+        read_rows<HD, C>(a);                                                                                      \
+    }
+#define ZLM_PAGED(NAME, C)                                                                                        \
+    ZLM_PAGED_ROWS(64, NAME, C)                                                                                   \
+    ZLM_PAGED_ROWS(128, NAME, C)                                                                                  \
+    ZLM_PAGED_ROWS(256, NAME, C)                                                                                  \
+    ZLM_PAGED_ATTEND(64, NAME, C, false)                                                                          \
+    ZLM_PAGED_ATTEND(128, NAME, C, false)                                                                         \
+    ZLM_PAGED_ATTEND(256, NAME, C, false)                                                                         \
+    ZLM_PAGED_HALVED(NAME, C, false)                                                                              \
+    ZLM_PAGED_ATTEND(64, NAME##_sinks, C, true)                                                                   \
+    ZLM_PAGED_ATTEND(128, NAME##_sinks, C, true)                                                                  \
+    ZLM_PAGED_ATTEND(256, NAME##_sinks, C, true)                                                                  \
+    ZLM_PAGED_HALVED(NAME##_sinks, C, true)
+
+ZLM_PAGED(f16, kF16)
+ZLM_PAGED(q4_0, kQ4)
+ZLM_PAGED(e4m3, kE8)

@@ -33,6 +33,8 @@ NULL_HANDLE = -1
 
 # GGML type codes (reference gguf/format.zig:41-77).
 F32, F16, Q4_0, Q4_1, Q8_0, Q4_K, Q6_K, BF16 = 0, 1, 2, 3, 8, 12, 14, 30
+# A paged cache of 8-bit numbers (ZLM_CACHE_E4M3; no GGML type).
+CACHE_E4M3 = 0x100
 # GpuVariant codes (reference gpu/kernels/grid.zig:14).
 PLAIN, U4, U8, SUB, UN2, UN4, W32, W128 = range(8)
 VARIANT_NAMES = ("plain", "u4", "u8", "sub", "un2", "un4", "w32", "w128")
@@ -208,6 +210,7 @@ def lib() -> ctypes.CDLL:
         "zlm_gpu_paged_append_enqueue": (B, [P, P, P, P, ctypes.c_uint64, P, P, U, ctypes.c_float, ctypes.c_float, P]),
         "zlm_gpu_paged_read_enqueue": (B, [P, P, P, P, P]),
         "zlm_gpu_paged_attention_enqueue": (B, [P, P, P, P, U, U, ctypes.c_float, P]),
+        "zlm_gpu_paged_attention_sinks_enqueue": (B, [P, P, P, P, U, U, U, ctypes.c_float, P]),
         "zlm_gpu_sample_enqueue": (B, [P, P, ctypes.c_uint64, U, U, P, P, P, P]),
         "zlm_gpu_resident_device_bytes": (ctypes.c_uint64, [P]),
         "zlm_gpu_layout_bytes": (ctypes.c_uint64, [U, S, S, ctypes.c_bool]),
@@ -586,8 +589,13 @@ class Device:
                                                        v_out))
 
     def paged_attention_enqueue(self, cache: PagedCache, batch: PagedBatch, q: int, out: int, n_heads: int,
-                                scale: float, window: int = 0) -> bool:
-        """Attention of a batch's rows over their sequences' pages (no wait)."""
+                                scale: float, window: int = 0, sinks: int = 0) -> bool:
+        """Attention of a batch's rows over their sequences' pages (no wait); with `sinks`, the first positions stay
+        visible beside the window's."""
+        if sinks:
+            return bool(self._L.zlm_gpu_paged_attention_sinks_enqueue(self._h, ctypes.byref(cache.c),
+                                                                      ctypes.byref(batch.c), q, n_heads, window, sinks,
+                                                                      scale, out))
         return bool(self._L.zlm_gpu_paged_attention_enqueue(self._h, ctypes.byref(cache.c), ctypes.byref(batch.c), q,
                                                             n_heads, window, scale, out))
 
