@@ -503,8 +503,8 @@ bool zlm_gpu_paged_read_enqueue(zlm_device *dev, const zlm_paged_cache *cache, c
  * 2^-14: smaller ones add with the rounding of those.  A padding row's output is 0.
  * NaN or infinite K reaches the rows that see its position only; such a V may make
  * NaN of other rows of its sequence in the same call, never of another sequence's.
- * Partial results live in 64 MiB of library scratch that this call and
- * zlm_gpu_sample_enqueue share, and counters beside it, made by their first calls
+ * Partial results live in 64 MiB of library scratch that this call,
+ * zlm_gpu_sample_enqueue and zlm_gpu_lora_enqueue share, and counters beside it, made by their first calls
  * and never replaced: call once before its capture. */
 bool zlm_gpu_paged_attention_enqueue(zlm_device *dev, const zlm_paged_cache *cache, const zlm_paged_batch *batch,
                                      const float *q, uint32_t n_heads, uint32_t window, float scale, float *out);
@@ -516,6 +516,32 @@ bool zlm_gpu_paged_attention_enqueue(zlm_device *dev, const zlm_paged_cache *cac
 bool zlm_gpu_paged_attention_sinks_enqueue(zlm_device *dev, const zlm_paged_cache *cache, const zlm_paged_batch *batch,
                                            const float *q, uint32_t n_heads, uint32_t window, uint32_t sinks,
                                            float scale, float *out);
+
+/* ---- low-rank adapters of many requests beside a shared projection ----
+ * No reference counterpart.  y[t] = res[t] + scale * B (A x[t]) with the A, B and scale of
+ * token t's adapter, for any mix of adapters in a batch.  A pool holds adapters of one
+ * shape: A n_adapters x rank x k, B n_adapters x rows x rank, each 16-byte aligned. */
+typedef struct {
+    const void *a, *b;     /* device */
+    uint32_t type;         /* ZLM_GGML_F16, ZLM_GGML_BF16 or ZLM_GGML_F32 */
+    uint32_t n_adapters;   /* 1 to 4096 */
+    uint32_t rank;         /* a multiple of 8, up to 256 */
+    uint32_t rows;         /* up to 2^24 */
+    uint32_t k;            /* a multiple of 32, up to 2^24 */
+    const int32_t *ranks;  /* device, n_adapters: each adapter's own rank (0 to `rank`: its first rows of A and columns
+                            * of B; what the pool holds behind them is not used, whatever it is), or null: `rank` */
+    const float *scales;   /* device, n_adapters, or null: 1 */
+} zlm_lora;
+/* adapter: n_tokens numbers in device memory, read when the work runs; one outside
+ * [0, n_adapters) is none: y[t] = res[t].  x rows are x_stride floats apart (0: k), 16-byte
+ * aligned; res and y rows y_stride (0: rows), so that y may be a part of the rows of a packed
+ * product.  res: may be y (rows without an adapter are left alone then), or null for 0; else
+ * it lies apart from y.  Products have the accuracy of 32-bit ones over the adapters'
+ * values, sums are 32-bit; an infinite or NaN x, or weight, makes NaN of what it reaches.  A
+ * token's results depend on the other tokens of the call by how sums are split only.  Uses the
+ * library scratch of zlm_gpu_paged_attention_enqueue (call once before its capture). */
+bool zlm_gpu_lora_enqueue(zlm_device *dev, const zlm_lora *lora, uint32_t n_tokens, const int32_t *adapter,
+                          const float *x, uint64_t x_stride, const float *res, float *y, uint64_t y_stride);
 
 /* ---- sampling (device buffers): a token from each row of logits ----
  * No reference counterpart on the device (its sampler runs on the CPU over the

@@ -100,3 +100,72 @@ def test_the_oracle_of_the_e4m3_cache():
     assert (np.abs(near - m)[held] <= m[held] * 2.0 ** -4).all()
     assert list(paged_more.seen(9, 3, 2)) == [0, 1, 7, 8, 9] and list(paged_more.seen(3, 3, 9)) == [0, 1, 2, 3]
     assert paged.Pool(zd.F16, 1, 64, 16, 1).kind == zd.F16
+
+
+LORA = dict(a=1 << 20, b=1 << 21, type=zd.BF16, n_adapters=5, rank=16, rows=100, k=64)
+
+
+def _lora(mod, **how):
+    return mod.Lora(**{**LORA, **how})
+
+
+@pytest.mark.parametrize("bad", [dict(a=0), dict(b=0), dict(a=(1 << 20) + 8), dict(b=(1 << 21) + 2), dict(type=zd.Q4_0),
+                                 dict(n_adapters=0), dict(n_adapters=4097), dict(rank=0), dict(rank=12), dict(rank=264),
+                                 dict(rows=0), dict(rows=(1 << 24) + 1), dict(k=0), dict(k=48), dict(k=1 << 25)])
+def test_bad_adapters_are_refused(box, bad):
+    d, p = box.dev, 1 << 16
+    assert not d.lora_enqueue(_lora(box.mod, **bad), 3, p, p, p + 4096, res=p + 8192), bad
+    assert d.last_error()
+    assert d.lora_enqueue(_lora(box.mod), 3, p, p, p + 4096, res=p + 8192), d.last_error()
+
+
+def test_other_arguments_of_adapters(box):
+    d, p, lora = box.dev, 1 << 16, _lora(box.mod)
+    assert not d.lora_enqueue(lora, 3, 0, p, p) and not d.lora_enqueue(lora, 3, p, 0, p) and not d.lora_enqueue(lora, 3, p, p, 0)
+    assert not d.lora_enqueue(lora, 3, p, p + 4, p)  # x by 16 bytes
+    assert not d.lora_enqueue(lora, 3, p, p, p, x_stride=66)
+    assert not d.lora_enqueue(lora, 3, p, p, p, x_stride=60) and not d.lora_enqueue(lora, 3, p, p, p, y_stride=99)
+    assert d.lora_enqueue(lora, 3, p, p, p + 4, res=p + 4, x_stride=68, y_stride=101), d.last_error()
+    d.launch_log(True)
+    assert d.lora_enqueue(lora, 0, 0, 0, 0), d.last_error()
+    assert d.launch_log_read() == []
+    assert d.lora_enqueue(lora, 64, p, p, p), d.last_error()
+    assert [r["what"] for r in d.launch_log_read()] == ["adapters down", "adapters up"]
+    d.launch_log(True)
+    assert d.lora_enqueue(lora, 65, p, p, p), d.last_error()
+    assert [r["what"] for r in d.launch_log_read()] == ["adapters, tokens grouped", "adapters down", "adapters up"]
+
+
+@pytest.mark.parametrize("rank", [8, 256])
+@pytest.mark.parametrize("n_adapters", [1, 4096])
+@pytest.mark.parametrize("tokens", [1, 64, 65, 5000, 200000, 3000000])
+def test_adapters_fit_the_scratch(box, rank, n_adapters, tokens):
+    """Every launch's partials, tiles and order within the 64 MiB, whatever the sizes."""
+    d, p = box.dev, 1 << 16
+    lora = _lora(box.mod, n_adapters=n_adapters, rank=rank, k=4096)
+    d.launch_log(True)
+    assert d.lora_enqueue(lora, tokens, p, p, p + 16, res=p), d.last_error()
+    done = 0
+    for r in d.launch_log_read():
+        if r["what"] != "adapters down":
+            continue
+        tiles, splits = r["grid_x"], r["grid_y"]
+        assert tiles * splits * 16 * rank * 4 + 12 * tiles <= 64 << 20
+        assert splits == 1 or tiles * splits <= 256
+        done += 1
+    assert done >= 1
+
+
+def test_adapters_take_the_scratch_before_capture(box):
+    d, p = box.dev, 1 << 16
+    own = box.mod.Device()
+    assert own.capture_begin()
+    assert not own.lora_enqueue(_lora(box.mod), 3, p, p, p) and "before capture" in own.last_error()
+    g = own.capture_end()
+    if g:
+        own.graph_destroy(g)
+    assert own.lora_enqueue(_lora(box.mod), 3, p, p, p), own.last_error()
+    held = own.scratch_device_bytes()
+    assert own.sample_enqueue(p, 1, 100, p, p) and own.scratch_device_bytes() == held
+    own.deinit()
+    assert d.available()

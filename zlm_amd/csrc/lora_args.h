@@ -1,0 +1,40 @@
+// lora_args.h -- the argument block of the adapter kernels (zlm_lora.hip), shared with the
+// host library that fills it.
+#pragma once
+#include <stdint.h>
+
+namespace zlm {
+
+constexpr uint32_t kLoraAdapters = 4096;  // of one pool (the grouping counts their tokens in LDS)
+constexpr uint32_t kLoraRank = 256;
+constexpr uint32_t kLoraTile = 16;        // tokens of one adapter that a wave multiplies together
+constexpr uint32_t kLoraSmall = 64;       // tokens that a wave groups by itself
+constexpr uint32_t kLoraWaves = 8;        // of the first product's workgroups
+constexpr uint32_t kLoraRows = 128;       // rows of y that a wave of the second product takes
+
+// Tokens order[first .. first + n) have one adapter (kLoraAdapters and above: none).
+struct LoraTile {
+    uint32_t adapter, first, n;
+};
+
+struct LoraArgs {
+    const void* a;  // n_adapters x rank x k
+    const void* b;  // n_adapters x rows x rank
+    const int32_t* adapter;  // of each token
+    const int32_t* ranks;    // null: all `rank`
+    const float* scales;     // null: 1
+    const float* x;
+    const float* res;        // null: 0
+    float* y;
+    uint64_t x_stride, y_stride;
+    uint32_t n_adapters, rank, rows, k, n_tokens;
+    uint32_t tiles;   // of the grid: a bound of their number
+    uint32_t splits;  // of k over workgroups
+    uint32_t in_place, vectors;  // y is res; rows of y and res go by 16 bytes
+    float* part;      // splits x tiles x 16 x rank: A x
+    uint32_t* order;  // what the grouping leaves (more than kLoraSmall tokens)
+    LoraTile* tile;
+    uint32_t* n_tiles;
+};
+
+}  // namespace zlm

@@ -6,7 +6,7 @@
 // decode glue; $ZLM_HIP_CODE_OBJECT overrides its path), one
 // zlm_gemv_<quant>_gfx950.hsaco per quant with that quant's GEMV forms,
 // zlm_paged_gfx950.hsaco (the paged KV cache's append and attention) and
-// zlm_sample_gfx950.hsaco (the sampler).  One HIP
+// zlm_sample_gfx950.hsaco (the sampler), zlm_lora_gfx950.hsaco (adapters).  One HIP
 // stream per device carries every copy and launch in order, so a burst's
 // shared activation and a resident's layout conversion are ordered before the
 // kernels that read them without extra synchronisation.
@@ -21,6 +21,7 @@
 //     first submit (reference pipeline.zig:264-276 only documents it).
 #include "zlm_gpu_hip.h"
 
+#include "lora_args.h"
 #include "paged_args.h"
 #include "sample_args.h"
 #include "zlm_static_scratch.h"
@@ -51,6 +52,11 @@ constexpr uint32_t kNoLayout = 0xffffffffu;
 // Library scratch kinds a captured graph can reference.
 constexpr uint32_t kUsesAttn = 1u;  // the attention partials
 constexpr uint32_t kUsesGemm = 2u;  // the GEMM's quantized activations and the residents' GEMM tiles
+// types of adapters, by the names of their kernels
+constexpr struct {
+    uint32_t type;
+    const char* name;
+} kLoraTypes[] = {{ZLM_GGML_F16, "f16"}, {ZLM_GGML_BF16, "bf16"}, {ZLM_GGML_F32, "f32"}};
 constexpr int kPagedDims[] = {64, 128, 256};  // head sizes of the paged kernels
 // their cache types, by the names of the kernels
 constexpr struct {
@@ -238,6 +244,12 @@ struct zlm_device {
     } paged[3][3];
     float* serving = nullptr;          // kServingScratch bytes: the paged attention's partials, the sampler's histograms
     uint32_t* paged_counts = nullptr;  // the few-row attention's counters, one a workgroup; 0 between calls
+    // the adapters' kernels, by type (kLoraTypes), log2 of a step of the rank and how tokens are grouped
+    hipModule_t lora_mod = nullptr;
+    hipFunction_t lora_group = nullptr;
+    struct LoraKernels {
+        hipFunction_t down = nullptr, up = nullptr;
+    } lora[3][4][2];
     hipModule_t sample_mod = nullptr;
     hipFunction_t sample_hist = nullptr;
     hipFunction_t sample_hist_wide = nullptr;
@@ -333,7 +345,7 @@ std::string library_dir() {
 void unload_modules(zlm_device* d) {
     if (d->mod) hipModuleUnload(d->mod);
     d->mod = nullptr;
-    for (hipModule_t* m : {&d->paged_mod, &d->sample_mod}) {
+    for (hipModule_t* m : {&d->paged_mod, &d->lora_mod, &d->sample_mod}) {
         if (*m) hipModuleUnload(*m);
         *m = nullptr;
     }
@@ -426,6 +438,21 @@ bool load_kernels(zlm_device* d) {
                     !get(f.merge_many, "merge_many", sinks) ||
                     (kPagedDims[i] == 256 && !get(f.halved, "attend_halved", sinks)))
                     return false;
+            }
+        }
+    const std::string lp = dir + "/zlm_lora_gfx950.hsaco";
+    if (!ok(d, hipModuleLoad(&d->lora_mod, lp.c_str()), lp.c_str())) return false;
+    if (!ok(d, hipModuleGetFunction(&d->lora_group, d->lora_mod, "zlm_lora_group"), "zlm_lora_group")) return false;
+    for (int t = 0; t < 3; t++)
+        for (int i = 0; i < 8; i++) {
+            zlm_device::LoraKernels& k = d->lora[t][i / 2][i % 2];
+            const struct {
+                hipFunction_t* f;
+                const char* name;
+            } fns[] = {{&k.down, "down"}, {&k.up, "up"}};
+            for (const auto& fn : fns) {
+                snprintf(nm, sizeof nm, "zlm_lora_%s_%s_%d%s", fn.name, kLoraTypes[t].name, 1 << i / 2, i % 2 ? "_small" : "");
+                if (!ok(d, hipModuleGetFunction(fn.f, d->lora_mod, nm), nm)) return false;
             }
         }
     const std::string sp = dir + "/zlm_sample_gfx950.hsaco";
@@ -3279,6 +3306,86 @@ extern "C" bool zlm_gpu_sample_enqueue(zlm_device* d, const float* logits, uint6
         if (!launch3(d, wide ? d->sample_hist_wide : d->sample_hist, a.slices, a.rows, 1, wide ? 1024 : 256, args,
                      "sample histogram") ||
             !launch(d, d->sample_pick, a.rows, 512, args, "sample"))
+            return false;
+    }
+    return true;
+}
+
+// ---- low-rank adapters ----
+
+extern "C" bool zlm_gpu_lora_enqueue(zlm_device* d, const zlm_lora* lora, uint32_t n_tokens, const int32_t* adapter,
+                                     const float* x, uint64_t x_stride, const float* res, float* y, uint64_t y_stride) {
+    if (!d || !d->avail) return false;
+    if (!lora) return fail(d, "null adapters");
+    int type = 0;
+    while (type < 3 && kLoraTypes[type].type != lora->type) type++;
+    if (type == 3) return fail(d, "adapters are f16, bf16 or f32 (got type %u)", lora->type);
+    if (lora->n_adapters == 0 || lora->n_adapters > zlm::kLoraAdapters)
+        return fail(d, "a pool has 1 to %u adapters (got %u)", zlm::kLoraAdapters, lora->n_adapters);
+    if (lora->rank == 0 || lora->rank % 8 || lora->rank > zlm::kLoraRank)
+        return fail(d, "a pool's rank is a multiple of 8 up to %u (got %u)", zlm::kLoraRank, lora->rank);
+    if (lora->k == 0 || lora->k % 32 || lora->k > (1u << 24)) return fail(d, "bad k %u: a multiple of 32 up to 2^24", lora->k);
+    if (lora->rows == 0 || lora->rows > (1u << 24)) return fail(d, "bad row count %u", lora->rows);
+    if (x_stride == 0) x_stride = lora->k;
+    if (y_stride == 0) y_stride = lora->rows;
+    if (x_stride < lora->k || y_stride < lora->rows)
+        return fail(d, "rows of %llu and %llu floats overlap", static_cast<unsigned long long>(x_stride),
+                    static_cast<unsigned long long>(y_stride));
+    if (n_tokens == 0) return true;
+    if (!lora->a || !lora->b || !adapter || !x || !y) return fail(d, "null buffer");
+    const auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+    if (!aligned(lora->a) || !aligned(lora->b) || !aligned(x) || x_stride % 4)
+        return fail(d, "adapters and rows of x need 16-byte alignment");
+    zlm::LoraArgs a = {};
+    a.a = lora->a;
+    a.b = lora->b;
+    a.ranks = lora->ranks;
+    a.scales = lora->scales;
+    a.x_stride = x_stride;
+    a.y_stride = y_stride;
+    a.n_adapters = lora->n_adapters;
+    a.rank = lora->rank;
+    a.rows = lora->rows;
+    a.k = lora->k;
+    a.in_place = res == y;
+    a.vectors = lora->rows % 4 == 0 && y_stride % 4 == 0 && aligned(y) && aligned(res);
+    // Tokens of one round: as many as the scratch has room for. A tile holds up to 16 tokens
+    // of an adapter; each adapter may begin one.
+    const uint64_t groups = static_cast<uint64_t>(lora->n_adapters) + !a.in_place;
+    const auto tiles_of = [&](uint64_t n) { return n / zlm::kLoraTile + std::min(n, groups); };
+    const auto bytes_of = [&](uint64_t n, uint64_t splits) {
+        return tiles_of(n) * (splits * zlm::kLoraTile * lora->rank * sizeof(float) + sizeof(zlm::LoraTile)) + (n + 1) * sizeof(uint32_t);
+    };
+    uint64_t most = std::min<uint64_t>(n_tokens, 1u << 20);
+    while (most > zlm::kLoraSmall && bytes_of(most, 1) > kServingScratch) most = (most + 1) / 2;
+    if (!ensure_serving_scratch(d, "the adapters' scratch")) return false;
+    // matrix tiles of 16 of the rank in the first product, runs of 32 in the second
+    const auto step = [](uint32_t n) { return n <= 1 ? 0 : n <= 2 ? 1 : n <= 4 ? 2 : 3; };
+    const uint32_t m_tiles = (lora->rank + 15) / 16, k_runs = (lora->rank + 31) / 32;
+    const int down = step(m_tiles), up = step(k_runs);
+    for (uint64_t t = 0; t < n_tokens; t += most) {
+        a.n_tokens = static_cast<uint32_t>(std::min<uint64_t>(most, n_tokens - t));
+        a.adapter = adapter + t;
+        a.x = x + t * x_stride;
+        a.res = res ? res + t * y_stride : nullptr;
+        a.y = y + t * y_stride;
+        a.tiles = static_cast<uint32_t>(tiles_of(a.n_tokens));
+        // k over workgroups where tiles alone leave CUs without one, a run of 32 a wave at least
+        uint64_t splits = std::min<uint64_t>({16, std::max<uint64_t>(1, static_cast<uint64_t>(d->cus) / a.tiles),
+                                              std::max<uint64_t>(1, lora->k / (32 * zlm::kLoraWaves))});
+        while (splits > 1 && bytes_of(a.n_tokens, splits) > kServingScratch) splits--;
+        a.splits = static_cast<uint32_t>(splits);
+        a.part = d->serving;
+        a.tile = reinterpret_cast<zlm::LoraTile*>(a.part + splits * a.tiles * zlm::kLoraTile * lora->rank);
+        a.order = reinterpret_cast<uint32_t*>(a.tile + a.tiles);
+        a.n_tiles = a.order + a.n_tokens;
+        const bool small = a.n_tokens <= zlm::kLoraSmall;
+        void* args[] = {&a};
+        if ((!small && !launch(d, d->lora_group, 1, 1024, args, "adapters, tokens grouped")) ||
+            !launch3(d, d->lora[type][down][small].down, a.tiles, a.splits, (m_tiles + 7) / 8, 64 * zlm::kLoraWaves, args,
+                     "adapters down") ||
+            !launch3(d, d->lora[type][up][small].up, a.tiles, (lora->rows + 4 * zlm::kLoraRows - 1) / (4 * zlm::kLoraRows), 1,
+                     256, args, "adapters up"))
             return false;
     }
     return true;

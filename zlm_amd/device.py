@@ -24,8 +24,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_DIR = os.path.join(_HERE, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libzlm_gpu_hip.so")
 CODE_OBJECT_PATH = os.path.join(LIB_DIR, "zlm_kernels_gfx950.hsaco")
-# Every code object the library loads: the common kernels, the paged cache's, the sampler's and one GEMV object per quant.
-CODE_OBJECT_PATHS = [CODE_OBJECT_PATH] + [os.path.join(LIB_DIR, f"zlm_{n}_gfx950.hsaco") for n in ("paged", "sample")] + [os.path.join(LIB_DIR, f"zlm_gemv_{q}_gfx950.hsaco")
+# Every code object the library loads: the common kernels, the paged cache's, the adapters', the sampler's and one GEMV object per quant.
+CODE_OBJECT_PATHS = [CODE_OBJECT_PATH] + [os.path.join(LIB_DIR, f"zlm_{n}_gfx950.hsaco") for n in ("paged", "lora", "sample")] + [os.path.join(LIB_DIR, f"zlm_gemv_{q}_gfx950.hsaco")
                                           for q in ("q4_0", "q8_0", "q4_k", "q6_k", "q4_1", "f32", "f16", "bf16")]
 
 RING_SIZE = 8
@@ -211,6 +211,7 @@ def lib() -> ctypes.CDLL:
         "zlm_gpu_paged_read_enqueue": (B, [P, P, P, P, P]),
         "zlm_gpu_paged_attention_enqueue": (B, [P, P, P, P, U, U, ctypes.c_float, P]),
         "zlm_gpu_paged_attention_sinks_enqueue": (B, [P, P, P, P, U, U, U, ctypes.c_float, P]),
+        "zlm_gpu_lora_enqueue": (B, [P, P, U, P, P, ctypes.c_uint64, P, P, ctypes.c_uint64]),
         "zlm_gpu_sample_enqueue": (B, [P, P, ctypes.c_uint64, U, U, P, P, P, P]),
         "zlm_gpu_resident_device_bytes": (ctypes.c_uint64, [P]),
         "zlm_gpu_layout_bytes": (ctypes.c_uint64, [U, S, S, ctypes.c_bool]),
@@ -305,6 +306,29 @@ class PagedBatch:
 
     def __init__(self, n_seqs: int, n_tokens: int, q_start: int, kv_len: int, table: int, table_stride: int):
         self.c = _PagedBatch(n_seqs, n_tokens, q_start, kv_len, table, table_stride)
+
+
+class _Lora(ctypes.Structure):
+    _fields_ = [
+        ("a", ctypes.c_void_p),
+        ("b", ctypes.c_void_p),
+        ("type", ctypes.c_uint32),
+        ("n_adapters", ctypes.c_uint32),
+        ("rank", ctypes.c_uint32),
+        ("rows", ctypes.c_uint32),
+        ("k", ctypes.c_uint32),
+        ("ranks", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+    ]
+
+
+class Lora:
+    """A pool of low-rank adapters of one shape (zlm_lora): device addresses of A [n_adapters, rank, k], B
+    [n_adapters, rows, rank] and, where they differ, of each adapter's rank and scale."""
+
+    def __init__(self, a: int, b: int, type: int, n_adapters: int, rank: int, rows: int, k: int, ranks: int = 0,
+                 scales: int = 0):
+        self.c = _Lora(a, b, type, n_adapters, rank, rows, k, ranks or None, scales or None)
 
 
 def paged_page_bytes(type: int, n_kv_heads: int, head_dim: int, page_size: int) -> int:
@@ -598,6 +622,12 @@ class Device:
                                                                       scale, out))
         return bool(self._L.zlm_gpu_paged_attention_enqueue(self._h, ctypes.byref(cache.c), ctypes.byref(batch.c), q,
                                                             n_heads, window, scale, out))
+
+    def lora_enqueue(self, lora: Lora, n_tokens: int, adapter: int, x: int, y: int, res: int = 0, x_stride: int = 0,
+                     y_stride: int = 0) -> bool:
+        """y[t] = res[t] + scale * B (A x[t]) with each token's own adapter (no wait); res may be y, 0 is none."""
+        return bool(self._L.zlm_gpu_lora_enqueue(self._h, ctypes.byref(lora.c), n_tokens, adapter, x, x_stride,
+                                                 res or None, y, y_stride))
 
     def sample_enqueue(self, logits: int, rows: int, vocab: int, u: int, token: int, temperature: int = 0,
                        top_k: int = 0, top_p: int = 0, min_p: int = 0, prob: int = 0, stride: int = 0) -> bool:
