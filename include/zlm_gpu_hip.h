@@ -504,7 +504,7 @@ bool zlm_gpu_paged_read_enqueue(zlm_device *dev, const zlm_paged_cache *cache, c
  * NaN or infinite K reaches the rows that see its position only; such a V may make
  * NaN of other rows of its sequence in the same call, never of another sequence's.
  * Partial results live in 64 MiB of library scratch that this call,
- * zlm_gpu_sample_enqueue and zlm_gpu_lora_enqueue share, and counters beside it, made by their first calls
+ * zlm_gpu_sample_enqueue, zlm_gpu_verify_enqueue and zlm_gpu_lora_enqueue share, and counters beside it, made by their first calls
  * and never replaced: call once before its capture. */
 bool zlm_gpu_paged_attention_enqueue(zlm_device *dev, const zlm_paged_cache *cache, const zlm_paged_batch *batch,
                                      const float *q, uint32_t n_heads, uint32_t window, float scale, float *out);
@@ -572,6 +572,33 @@ typedef struct {
  * once before its capture). */
 bool zlm_gpu_sample_enqueue(zlm_device *dev, const float *logits, uint64_t stride, uint32_t rows, uint32_t vocab,
                             const zlm_sampling *how, const float *u, int32_t *token, float *prob);
+
+/* ---- verification of drafted tokens (device buffers) ----
+ * No reference counterpart.  Rows q_start[s] .. q_start[s+1]-1 of the logits are sequence
+ * s's: the target's after its last token and after each of its drafted ones, so one row
+ * more than it has drafts; draft[r] is the token drafted after row r (not looked at in a
+ * sequence's last row).  q_start (n_seqs + 1, on the device) begins at 0 or above, never
+ * decreases and ends at rows or below; at most 1024 sequences and 65536 rows.
+ * With p and q the probabilities by which zlm_gpu_sample_enqueue draws a row's token from
+ * the target's logits by `how` and from draft_logits by `draft_how` (each of one value a
+ * row; draft_logits row r is what draft[r] was drawn from): a sequence's drafts d are
+ * accepted in turn while u[r] * q(d) < p(d).  accepted[s]: how many; token holds these, in
+ * the rows after which they were drafted, then a token drawn by u_draw[s], and -1 in the
+ * sequence's other rows.  It is drawn from max(p - q, 0) of the row whose draft was not
+ * accepted (from p where that is nowhere above 0), or from p of the last row: the first
+ * token, in order of index, whose cumulative weight exceeds u_draw[s] times the weight of
+ * all.  So a token has the probability that the target's own draw has.
+ * draft_logits null: q is 1 of the drafted token (a draft that was looked up, or greedy).  A
+ * draft outside [0, vocab) is none: what follows is drawn from p.  Where all of a row's
+ * logits are -inf or NaN nothing is accepted, and -1 drawn.  Weights are those of
+ * zlm_gpu_sample_enqueue, shares and sums formed in 64 bits; numbers u in [0, 1).  token lies
+ * apart from draft.  Uses the library scratch of zlm_gpu_paged_attention_enqueue (call once
+ * before its capture). */
+bool zlm_gpu_verify_enqueue(zlm_device *dev, const float *logits, uint64_t stride, uint32_t rows, uint32_t vocab,
+                            const zlm_sampling *how, const float *draft_logits, uint64_t draft_stride,
+                            const zlm_sampling *draft_how, uint32_t n_seqs, const int32_t *q_start,
+                            const int32_t *draft, const float *u, const float *u_draw, int32_t *accepted,
+                            int32_t *token);
 
 /* ---- HIP graphs over the device stream ----
  * Everything enqueued between capture_begin and capture_end is recorded, not

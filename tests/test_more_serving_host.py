@@ -169,3 +169,56 @@ def test_adapters_take_the_scratch_before_capture(box):
     assert own.sample_enqueue(p, 1, 100, p, p) and own.scratch_device_bytes() == held
     own.deinit()
     assert d.available()
+
+
+def _verify(box, **how):
+    p = 1 << 16
+    a = dict(logits=p, rows=9, vocab=1000, n_seqs=2, q_start=p, draft=p, u=p, u_draw=p, accepted=p, token=p + 4096)
+    a.update(how)
+    return box.dev.verify_enqueue(a.pop("logits"), a.pop("rows"), a.pop("vocab"), a.pop("n_seqs"), a.pop("q_start"),
+                                  a.pop("draft"), a.pop("u"), a.pop("u_draw"), a.pop("accepted"), a.pop("token"), **a)
+
+
+@pytest.mark.parametrize("bad", [dict(vocab=0), dict(vocab=(1 << 20) + 1), dict(stride=999), dict(draft_stride=999),
+                                 dict(n_seqs=1025), dict(rows=65537), dict(logits=0), dict(q_start=0), dict(draft=0),
+                                 dict(u=0), dict(u_draw=0), dict(accepted=0), dict(token=0), dict(token=1 << 16)])
+def test_what_verification_refuses(box, bad):
+    assert not _verify(box, **bad), bad
+    assert box.dev.last_error()
+    assert _verify(box), box.dev.last_error()
+    assert _verify(box, draft_logits=1 << 20, how=box.mod.Sampling(top_k=1 << 16)), box.dev.last_error()
+
+
+def test_launches_of_a_verification(box):
+    d = box.dev
+    d.launch_log(True)
+    assert _verify(box, n_seqs=0, q_start=0, accepted=0), d.last_error()
+    assert d.launch_log_read() == []
+    assert _verify(box, rows=0, logits=0, draft=0, u=0, u_draw=0, token=0), d.last_error()
+    assert [r["what"] for r in d.launch_log_read()] == ["verify draw"]
+    d.launch_log(True)
+    assert _verify(box), d.last_error()
+    assert [(r["what"], r["grid_x"], r["grid_y"]) for r in d.launch_log_read()] == [
+        ("verify histogram", 1, 9), ("verify cuts", 9, 1), ("verify draw", 1, 2)]
+    d.launch_log(True)
+    assert _verify(box, rows=65536, vocab=1 << 20, n_seqs=1024, draft_logits=1 << 16), d.last_error()
+    log = d.launch_log_read()
+    assert log[-1]["what"] == "verify draw" and (log[-1]["grid_x"], log[-1]["grid_y"]) == (128, 1024)
+    kept = 2 * 65536 * 32 + 1024 * 128 * 16 + 1024 * 4
+    for r in log:
+        if r["what"] == "verify histogram":
+            assert kept + r["grid_x"] * r["grid_y"] * (768 * 8 + 16) <= 64 << 20
+    assert sum(r["grid_y"] for r in log if r["what"] == "verify histogram") == 2 * 65536
+
+
+def test_verification_takes_the_scratch_before_capture(box):
+    own = box.mod.Device()
+    fresh = type("", (), {"dev": own})
+    assert own.capture_begin()
+    assert not _verify(fresh) and "before capture" in own.last_error()
+    g = own.capture_end()
+    if g:
+        own.graph_destroy(g)
+    assert _verify(fresh), own.last_error()
+    own.deinit()
+    assert box.dev.available()

@@ -33,4 +33,37 @@ struct SampleArgs {
     SampleSlice* info;  // rows x slices
 };
 
+// What a draw takes a row's tokens by: those whose (key, ~index) is at least `token`, by
+// their weights' shares of `weight`; rate 0: `best` alone (0: none at all).
+struct SampleCut {
+    uint64_t token, best;
+    double weight, rate;
+};
+
+// A slice's part of what a row that ends a sequence's drafts is drawn from: the weight of
+// the target's tokens, and what of it lies above the draft's.
+struct VerifySum {
+    double rest, all;
+};
+
+constexpr uint32_t kVerifyRows = 65536;  // of a call
+
+struct VerifyArgs {
+    SampleArgs target, draft;  // the rows at hand
+    uint32_t first;            // the first of them
+    uint32_t n_rows, n_seqs;   // of the call
+    uint32_t by_logits;        // the draft has logits; else a drafted token is certain
+    const int32_t* q_start;    // n_seqs + 1: the rows of sequence s are [q_start[s], q_start[s + 1])
+    const int32_t* token;      // drafted after each row
+    const float* u;            // of each row, for its acceptance
+    const float* u_draw;       // of each sequence
+    int32_t* accepted;
+    int32_t* out;
+    const float* target_logits;  // of all rows
+    const float* draft_logits;
+    SampleCut* cuts;    // n_rows of the target, then as many of the draft
+    VerifySum* sums;    // n_seqs x slices
+    uint32_t* counts;   // of each sequence: slices that are summed up
+};
+
 }  // namespace zlm

@@ -6,7 +6,7 @@
 // decode glue; $ZLM_HIP_CODE_OBJECT overrides its path), one
 // zlm_gemv_<quant>_gfx950.hsaco per quant with that quant's GEMV forms,
 // zlm_paged_gfx950.hsaco (the paged KV cache's append and attention) and
-// zlm_sample_gfx950.hsaco (the sampler), zlm_lora_gfx950.hsaco (adapters).  One HIP
+// zlm_sample_gfx950.hsaco (the sampler), zlm_verify_gfx950.hsaco (drafts), zlm_lora_gfx950.hsaco (adapters).  One HIP
 // stream per device carries every copy and launch in order, so a burst's
 // shared activation and a resident's layout conversion are ordered before the
 // kernels that read them without extra synchronisation.
@@ -254,6 +254,11 @@ struct zlm_device {
     hipFunction_t sample_hist = nullptr;
     hipFunction_t sample_hist_wide = nullptr;
     hipFunction_t sample_pick = nullptr;
+    hipModule_t verify_mod = nullptr;
+    hipFunction_t verify_hist = nullptr;
+    hipFunction_t verify_hist_wide = nullptr;
+    hipFunction_t verify_cuts = nullptr;
+    hipFunction_t verify_draw = nullptr;
     hipFunction_t synth_blocks = nullptr;
     hipFunction_t synth_f16 = nullptr;
 
@@ -345,7 +350,7 @@ std::string library_dir() {
 void unload_modules(zlm_device* d) {
     if (d->mod) hipModuleUnload(d->mod);
     d->mod = nullptr;
-    for (hipModule_t* m : {&d->paged_mod, &d->lora_mod, &d->sample_mod}) {
+    for (hipModule_t* m : {&d->paged_mod, &d->lora_mod, &d->sample_mod, &d->verify_mod}) {
         if (*m) hipModuleUnload(*m);
         *m = nullptr;
     }
@@ -464,6 +469,15 @@ bool load_kernels(zlm_device* d) {
                     {&d->sample_pick, "zlm_sample_pick"}};
     for (const auto& m : sampling)
         if (!ok(d, hipModuleGetFunction(m.f, d->sample_mod, m.name), m.name)) return false;
+    const std::string vp = dir + "/zlm_verify_gfx950.hsaco";
+    if (!ok(d, hipModuleLoad(&d->verify_mod, vp.c_str()), vp.c_str())) return false;
+    const struct {
+        hipFunction_t* f;
+        const char* name;
+    } verifying[] = {{&d->verify_hist, "zlm_verify_hist"}, {&d->verify_hist_wide, "zlm_verify_hist_wide"},
+                     {&d->verify_cuts, "zlm_verify_cuts"}, {&d->verify_draw, "zlm_verify_draw"}};
+    for (const auto& m : verifying)
+        if (!ok(d, hipModuleGetFunction(m.f, d->verify_mod, m.name), m.name)) return false;
     return true;
 }
 
@@ -3309,6 +3323,95 @@ extern "C" bool zlm_gpu_sample_enqueue(zlm_device* d, const float* logits, uint6
             return false;
     }
     return true;
+}
+
+// ---- verification of drafted tokens ----
+
+namespace {
+
+constexpr uint64_t kSampleSliceBytes = (zlm::kSampleBins + zlm::kSampleShort) * sizeof(uint64_t) + sizeof(zlm::SampleSlice);
+
+// The sampler's block for rows r .. r + n of some logits, its scratch at *at and on.
+zlm::SampleArgs sample_block(const float* logits, uint64_t stride, uint32_t vocab, const zlm_sampling* how, uint64_t r,
+                             uint32_t n, uint8_t** at) {
+    zlm::SampleArgs a = {};
+    a.logits = logits + r * stride;
+    a.stride = stride;
+    a.rows = n;
+    a.vocab = vocab;
+    a.slices = (vocab + zlm::kSampleSlice - 1) / zlm::kSampleSlice;
+    if (how) {
+        a.temperature = how->temperature ? how->temperature + r : nullptr;
+        a.top_k = how->top_k ? how->top_k + r : nullptr;
+        a.top_p = how->top_p ? how->top_p + r : nullptr;
+        a.min_p = how->min_p ? how->min_p + r : nullptr;
+    }
+    const size_t all = static_cast<size_t>(n) * a.slices;
+    a.hist = reinterpret_cast<uint64_t*>(*at);
+    a.shorts = a.hist + all * zlm::kSampleBins;
+    a.info = reinterpret_cast<zlm::SampleSlice*>(a.shorts + all * zlm::kSampleShort);
+    *at += all * kSampleSliceBytes;
+    return a;
+}
+
+}  // namespace
+
+extern "C" bool zlm_gpu_verify_enqueue(zlm_device* d, const float* logits, uint64_t stride, uint32_t rows, uint32_t vocab,
+                                       const zlm_sampling* how, const float* draft_logits, uint64_t draft_stride,
+                                       const zlm_sampling* draft_how, uint32_t n_seqs, const int32_t* q_start,
+                                       const int32_t* draft, const float* u, const float* u_draw, int32_t* accepted,
+                                       int32_t* token) {
+    if (!d || !d->avail) return false;
+    if (vocab == 0 || vocab > zlm::kSampleSlice * zlm::kSampleSlices)
+        return fail(d, "verification takes 1 to %u logits a row (got %u)", zlm::kSampleSlice * zlm::kSampleSlices, vocab);
+    if (stride == 0) stride = vocab;
+    if (draft_stride == 0) draft_stride = vocab;
+    if (stride < vocab || draft_stride < vocab) return fail(d, "logits rows overlap");
+    if (n_seqs > zlm::kPagedMaxSeqs) return fail(d, "a call verifies at most %u sequences (got %u)", zlm::kPagedMaxSeqs, n_seqs);
+    if (rows > zlm::kVerifyRows) return fail(d, "a call verifies at most %u rows (got %u)", zlm::kVerifyRows, rows);
+    if (n_seqs == 0) return true;
+    if (!q_start || !accepted || (rows && (!logits || !draft || !u || !u_draw || !token))) return fail(d, "null buffer");
+    if (token == draft && rows) return fail(d, "the tokens that come out need a buffer of their own");
+    if (!ensure_serving_scratch(d, "the sampling scratch")) return false;
+    zlm::VerifyArgs v = {};
+    v.n_rows = rows;
+    v.n_seqs = n_seqs;
+    v.by_logits = draft_logits != nullptr;
+    v.q_start = q_start;
+    v.token = draft;
+    v.u = u;
+    v.u_draw = u_draw;
+    v.accepted = accepted;
+    v.out = token;
+    v.target_logits = logits;
+    v.draft_logits = draft_logits;
+    const uint32_t slices = (vocab + zlm::kSampleSlice - 1) / zlm::kSampleSlice;
+    // what is kept of each row and slice in front, then the histograms of as many rows as fit
+    uint8_t* const begin = reinterpret_cast<uint8_t*>(d->serving);
+    v.cuts = reinterpret_cast<zlm::SampleCut*>(begin);
+    v.sums = reinterpret_cast<zlm::VerifySum*>(v.cuts + 2 * static_cast<size_t>(rows));
+    v.counts = reinterpret_cast<uint32_t*>(v.sums + static_cast<size_t>(n_seqs) * slices);
+    uint8_t* const hists = begin + (reinterpret_cast<uint8_t*>(v.counts + n_seqs) - begin + 15) / 16 * 16;
+    const uint64_t room = kServingScratch - static_cast<uint64_t>(hists - begin);
+    const uint32_t sides = v.by_logits ? 2 : 1;
+    const uint32_t most = static_cast<uint32_t>(std::min<uint64_t>(room / (sides * slices * kSampleSliceBytes), rows));
+    void* args[] = {&v};
+    for (uint64_t r = 0; r < rows; r += most) {
+        const uint32_t n = static_cast<uint32_t>(std::min<uint64_t>(most, rows - r));
+        uint8_t* at = hists;
+        v.first = static_cast<uint32_t>(r);
+        v.target = sample_block(logits, stride, vocab, how, r, n, &at);
+        if (v.by_logits) v.draft = sample_block(draft_logits, draft_stride, vocab, draft_how, r, n, &at);
+        // up to two slices a CU: 1024 threads each, as the sampler's
+        const bool wide = static_cast<uint64_t>(slices) * n * sides <= 2ull * d->cus;
+        if (!launch3(d, wide ? d->verify_hist_wide : d->verify_hist, slices, n * sides, 1, wide ? 1024 : 256, args,
+                     "verify histogram") ||
+            !launch(d, d->verify_cuts, n * sides, 512, args, "verify cuts"))
+            return false;
+    }
+    if (rows == 0) v.target.slices = slices;
+    v.target.vocab = vocab;
+    return launch3(d, d->verify_draw, slices, n_seqs, 1, 512, args, "verify draw");
 }
 
 // ---- low-rank adapters ----

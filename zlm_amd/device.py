@@ -24,8 +24,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_DIR = os.path.join(_HERE, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libzlm_gpu_hip.so")
 CODE_OBJECT_PATH = os.path.join(LIB_DIR, "zlm_kernels_gfx950.hsaco")
-# Every code object the library loads: the common kernels, the paged cache's, the adapters', the sampler's and one GEMV object per quant.
-CODE_OBJECT_PATHS = [CODE_OBJECT_PATH] + [os.path.join(LIB_DIR, f"zlm_{n}_gfx950.hsaco") for n in ("paged", "lora", "sample")] + [os.path.join(LIB_DIR, f"zlm_gemv_{q}_gfx950.hsaco")
+# Every code object the library loads: the common kernels, the paged cache's, the adapters', the sampler's, the drafts' and one GEMV object per quant.
+CODE_OBJECT_PATHS = [CODE_OBJECT_PATH] + [os.path.join(LIB_DIR, f"zlm_{n}_gfx950.hsaco") for n in ("paged", "lora", "sample", "verify")] + [os.path.join(LIB_DIR, f"zlm_gemv_{q}_gfx950.hsaco")
                                           for q in ("q4_0", "q8_0", "q4_k", "q6_k", "q4_1", "f32", "f16", "bf16")]
 
 RING_SIZE = 8
@@ -212,6 +212,7 @@ def lib() -> ctypes.CDLL:
         "zlm_gpu_paged_attention_enqueue": (B, [P, P, P, P, U, U, ctypes.c_float, P]),
         "zlm_gpu_paged_attention_sinks_enqueue": (B, [P, P, P, P, U, U, U, ctypes.c_float, P]),
         "zlm_gpu_lora_enqueue": (B, [P, P, U, P, P, ctypes.c_uint64, P, P, ctypes.c_uint64]),
+        "zlm_gpu_verify_enqueue": (B, [P, P, ctypes.c_uint64, U, U, P, P, ctypes.c_uint64, P, U, P, P, P, P, P, P]),
         "zlm_gpu_sample_enqueue": (B, [P, P, ctypes.c_uint64, U, U, P, P, P, P]),
         "zlm_gpu_resident_device_bytes": (ctypes.c_uint64, [P]),
         "zlm_gpu_layout_bytes": (ctypes.c_uint64, [U, S, S, ctypes.c_bool]),
@@ -306,6 +307,14 @@ class PagedBatch:
 
     def __init__(self, n_seqs: int, n_tokens: int, q_start: int, kv_len: int, table: int, table_stride: int):
         self.c = _PagedBatch(n_seqs, n_tokens, q_start, kv_len, table, table_stride)
+
+
+class Sampling:
+    """How rows of logits are drawn from (zlm_sampling): device addresses of arrays of one value a row, 0 leaves a
+    filter off (temperature: 1)."""
+
+    def __init__(self, temperature: int = 0, top_k: int = 0, top_p: int = 0, min_p: int = 0):
+        self.c = _Sampling(temperature or None, top_k or None, top_p or None, min_p or None)
 
 
 class _Lora(ctypes.Structure):
@@ -622,6 +631,16 @@ class Device:
                                                                       scale, out))
         return bool(self._L.zlm_gpu_paged_attention_enqueue(self._h, ctypes.byref(cache.c), ctypes.byref(batch.c), q,
                                                             n_heads, window, scale, out))
+
+    def verify_enqueue(self, logits: int, rows: int, vocab: int, n_seqs: int, q_start: int, draft: int, u: int,
+                       u_draw: int, accepted: int, token: int, how: Optional[Sampling] = None, draft_logits: int = 0,
+                       draft_how: Optional[Sampling] = None, stride: int = 0, draft_stride: int = 0) -> bool:
+        """Accept drafted tokens against the target's logits and draw the token after them (no wait); without
+        draft_logits the drafts are certain."""
+        ref = lambda s: ctypes.byref(s.c) if s else None  # noqa: E731
+        return bool(self._L.zlm_gpu_verify_enqueue(self._h, logits, stride, rows, vocab, ref(how), draft_logits or None,
+                                                   draft_stride, ref(draft_how), n_seqs, q_start, draft, u, u_draw,
+                                                   accepted, token))
 
     def lora_enqueue(self, lora: Lora, n_tokens: int, adapter: int, x: int, y: int, res: int = 0, x_stride: int = 0,
                      y_stride: int = 0) -> bool:
