@@ -7,10 +7,11 @@ namespace zlm {
 
 constexpr uint32_t kLoraAdapters = 4096;  // of one pool (the grouping counts their tokens in LDS)
 constexpr uint32_t kLoraRank = 256;
-constexpr uint32_t kLoraTile = 16;        // tokens of one adapter that a wave multiplies together
-constexpr uint32_t kLoraSmall = 64;       // tokens that a wave groups by itself
-constexpr uint32_t kLoraWaves = 8;        // of the first product's workgroups
-constexpr uint32_t kLoraRows = 128;       // rows of y that a wave of the second product takes
+constexpr uint32_t kLoraSmall = 64;       // tokens that a wave groups by itself, in tiles of 16
+constexpr uint32_t kLoraTile = 32;        // tokens of a tile where there are more
+// Waves of the first product's workgroups, and runs of 32 of k that each has in flight (at
+// most), with tiles of 16 tokens and of 32.
+constexpr uint32_t kLoraWaves[2] = {8, 4}, kLoraRuns[2] = {4, 2};
 
 // Tokens order[first .. first + n) have one adapter (kLoraAdapters and above: none).
 struct LoraTile {
@@ -30,8 +31,9 @@ struct LoraArgs {
     uint32_t n_adapters, rank, rows, k, n_tokens;
     uint32_t tiles;   // of the grid: a bound of their number
     uint32_t splits;  // of k over workgroups
+    uint32_t wave_rows;  // of y, that a wave of the second product takes
     uint32_t in_place, vectors;  // y is res; rows of y and res go by 16 bytes
-    float* part;      // splits x tiles x 16 x rank: A x
+    float* part;      // splits x tiles x tokens of a tile x rank: A x
     uint32_t* order;  // what the grouping leaves (more than kLoraSmall tokens)
     LoraTile* tile;
     uint32_t* n_tiles;

@@ -3452,12 +3452,12 @@ extern "C" bool zlm_gpu_lora_enqueue(zlm_device* d, const zlm_lora* lora, uint32
     a.k = lora->k;
     a.in_place = res == y;
     a.vectors = lora->rows % 4 == 0 && y_stride % 4 == 0 && aligned(y) && aligned(res);
-    // Tokens of one round: as many as the scratch has room for. A tile holds up to 16 tokens
-    // of an adapter; each adapter may begin one.
+    // Tokens of one round: as many as the scratch has room for.  Each adapter may begin a tile.
     const uint64_t groups = static_cast<uint64_t>(lora->n_adapters) + !a.in_place;
-    const auto tiles_of = [&](uint64_t n) { return n / zlm::kLoraTile + std::min(n, groups); };
+    const auto tile_of = [](uint64_t n) { return n <= zlm::kLoraSmall ? 16 : zlm::kLoraTile; };
+    const auto tiles_of = [&](uint64_t n) { return n / tile_of(n) + std::min(n, groups); };
     const auto bytes_of = [&](uint64_t n, uint64_t splits) {
-        return tiles_of(n) * (splits * zlm::kLoraTile * lora->rank * sizeof(float) + sizeof(zlm::LoraTile)) + (n + 1) * sizeof(uint32_t);
+        return tiles_of(n) * (splits * tile_of(n) * lora->rank * sizeof(float) + sizeof(zlm::LoraTile)) + (n + 1) * sizeof(uint32_t);
     };
     uint64_t most = std::min<uint64_t>(n_tokens, 1u << 20);
     while (most > zlm::kLoraSmall && bytes_of(most, 1) > kServingScratch) most = (most + 1) / 2;
@@ -3473,22 +3473,35 @@ extern "C" bool zlm_gpu_lora_enqueue(zlm_device* d, const zlm_lora* lora, uint32
         a.res = res ? res + t * y_stride : nullptr;
         a.y = y + t * y_stride;
         a.tiles = static_cast<uint32_t>(tiles_of(a.n_tokens));
-        // k over workgroups where tiles alone leave CUs without one, a run of 32 a wave at least
-        uint64_t splits = std::min<uint64_t>({16, std::max<uint64_t>(1, static_cast<uint64_t>(d->cus) / a.tiles),
-                                              std::max<uint64_t>(1, lora->k / (32 * zlm::kLoraWaves))});
+        const bool small = a.n_tokens <= zlm::kLoraSmall;
+        // k over workgroups where tiles alone leave CUs without two, as many runs a wave as it has
+        // in flight at least
+        const uint64_t waves = zlm::kLoraWaves[!small], runs = 32 * waves * zlm::kLoraRuns[!small];
+        uint64_t splits = std::min<uint64_t>({16, std::max<uint64_t>(1, 2ull * d->cus / a.tiles), (lora->k + runs - 1) / runs});
         while (splits > 1 && bytes_of(a.n_tokens, splits) > kServingScratch) splits--;
         a.splits = static_cast<uint32_t>(splits);
         a.part = d->serving;
-        a.tile = reinterpret_cast<zlm::LoraTile*>(a.part + splits * a.tiles * zlm::kLoraTile * lora->rank);
+        a.tile = reinterpret_cast<zlm::LoraTile*>(a.part + splits * a.tiles * tile_of(a.n_tokens) * lora->rank);
         a.order = reinterpret_cast<uint32_t*>(a.tile + a.tiles);
         a.n_tiles = a.order + a.n_tokens;
-        const bool small = a.n_tokens <= zlm::kLoraSmall;
+        // rows of y a wave: few where tiles are few; else spans of 128, as many as leave the least
+        // work to the last round of two workgroups a CU (a span more stands for what a wave begins with)
+        const uint64_t fours = (a.tiles + 3) / 4;
+        a.wave_rows = small ? 256 : 128;
+        while (small && a.wave_rows > 32 && static_cast<uint64_t>(a.tiles) * lora->rows < 16ull * d->cus * a.wave_rows)
+            a.wave_rows /= 2;
+        const auto rounds = [&](uint64_t rows) {
+            return ((lora->rows + rows - 1) / rows * fours + 2 * d->cus - 1) / (2 * d->cus) * (rows / 128 + 1);
+        };
+        while (!small && a.wave_rows < 512 && rounds(2 * a.wave_rows) < rounds(a.wave_rows)) a.wave_rows *= 2;
+        const unsigned row_groups = static_cast<unsigned>((lora->rows + (small ? 4 : 1) * a.wave_rows - 1) / ((small ? 4 : 1) * a.wave_rows));
         void* args[] = {&a};
         if ((!small && !launch(d, d->lora_group, 1, 1024, args, "adapters, tokens grouped")) ||
-            !launch3(d, d->lora[type][down][small].down, a.tiles, a.splits, (m_tiles + 7) / 8, 64 * zlm::kLoraWaves, args,
+            !launch3(d, d->lora[type][down][small].down, a.tiles, a.splits, (m_tiles + 7) / 8,
+                     static_cast<unsigned>(64 * waves), args,
                      "adapters down") ||
-            !launch3(d, d->lora[type][up][small].up, a.tiles, (lora->rows + 4 * zlm::kLoraRows - 1) / (4 * zlm::kLoraRows), 1,
-                     256, args, "adapters up"))
+            !launch3(d, d->lora[type][up][small].up, row_groups, static_cast<unsigned>(small ? a.tiles : fours), 1, 256, args,
+                     "adapters up"))
             return false;
     }
     return true;

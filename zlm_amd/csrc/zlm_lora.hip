@@ -3,9 +3,9 @@
 //     y[t] = res[t] + scale * B (A x[t]).
 // Built as a device-only code object (hipcc --genco) and loaded by the host library.
 //
-// Tokens are taken in tiles of up to 16 with one adapter, so that a tile reads its A and B
-// once.  Up to 64 tokens every wave finds its tile by itself; more are grouped by a launch
-// before.  Then two launches: h = A x, k split over waves and workgroups, and
+// Tokens are taken in tiles with one adapter, so that a tile reads its A and B once.  Up to
+// 64 tokens every wave finds its tile, of up to 16, by itself; more are grouped by a launch
+// before, in tiles of up to 32.  Then two launches: h = A x, k split over waves and workgroups, and
 // y = res + scale * B h.
 //
 // Both products run on v_mfma_f32_16x16x32_bf16 with the tokens in the N dimension.  A
@@ -23,7 +23,8 @@ namespace {
 
 using Args = zlm::LoraArgs;
 using zlm::LoraTile;
-constexpr uint32_t kWave = 64, kTile = zlm::kLoraTile, kWaves = zlm::kLoraWaves;
+constexpr uint32_t kWave = 64;
+constexpr uint32_t kN = 16;  // tokens of a matrix tile
 
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
@@ -101,89 +102,122 @@ __device__ __forceinline__ v4f multiply(const v8b (&w)[kN], const v8b (&x)[3], v
 
 // ---- tiles ----
 
-// A tile, and this lane's token of it (lane % 16; the tile's first where it has fewer).
+// A tile, and this lane's tokens of it (lane % 16 and 16 on; the tile's first where it has
+// fewer).
+template <int kNt>
 struct Mine {
-    uint32_t adapter, n, token;
-    bool live;
+    uint32_t adapter, rank, n, token[kNt];
+    __device__ __forceinline__ bool live(int i) const { return kN * i + (threadIdx.x & (kN - 1)) < n; }
 };
 
 __device__ __forceinline__ uint32_t adapter_of(const Args& a, uint32_t t) {
     return min(static_cast<uint32_t>(a.adapter[t]), a.n_adapters);  // n_adapters: none
 }
 
+__device__ __forceinline__ uint32_t rank_of(const Args& a, uint32_t adapter) {
+    if (adapter >= a.n_adapters) return 0;
+    return a.ranks ? min(static_cast<uint32_t>(max(a.ranks[adapter], 0)), a.rank) : a.rank;
+}
+
+// What the waves of a workgroup find their tile by, up to 64 tokens.
+struct Grouping {
+    uint8_t one_of[zlm::kLoraAdapters + 2];  // a token of each adapter
+    unsigned long long with[kWave];          // all of its tokens
+};
+
 // False: there are not so many tiles.  Tokens without an adapter make tiles of their own,
 // but where y is res.
-template <bool kSmall>
-__device__ __forceinline__ bool tile_of(const Args& a, uint32_t tile, Mine& m) {
-    const uint32_t lane = threadIdx.x & (kWave - 1), j = lane & (kTile - 1);
-    if constexpr (kSmall) {
+template <int kNt>
+__device__ __forceinline__ bool tile_of(const Args& a, uint32_t tile, Mine<kNt>& m) {
+    const uint32_t lane = threadIdx.x & (kWave - 1), j = lane & (kN - 1);
+    if constexpr (kNt == 1) {
+        // the tokens of each lane's adapter, and its place among them; those at 0, 16, 32 and
+        // 48 begin tiles
+        __shared__ Grouping sm;
         const bool has = lane < a.n_tokens;
-        const uint32_t own = has ? adapter_of(a, lane) : a.n_adapters;
-        uint64_t left = __ballot(has && !(a.in_place && own == a.n_adapters));
-        while (left) {
-            const uint32_t id = __builtin_amdgcn_readlane(own, __builtin_ctzll(left));
-            uint64_t with = __ballot(own == id) & left;
-            const uint32_t n = __builtin_popcountll(with), tiles = (n + kTile - 1) / kTile;
-            if (tile < tiles) {
-                m.adapter = id;
-                m.n = min(n - kTile * tile, kTile);
-                m.live = j < m.n;
-                // the (16 tile + j)-th of them: the lane that so many come before
-                const uint32_t before = __builtin_popcountll(with & ((1ull << lane) - 1));
-                const bool in = (with >> lane & 1) != 0;
-                const uint32_t to = in ? before - kTile * tile : kWave;
-                // each of the tile's tokens tells the lane of its place
-                m.token = __builtin_ctzll(with);
-                for (uint32_t i = 0; i < m.n; i++) {
-                    const uint32_t t = __builtin_ctzll(__ballot(to == i));
-                    if (j == i) m.token = t;
-                }
-                return true;
-            }
-            tile -= tiles;
-            left &= ~with;
+        const uint32_t own = has ? adapter_of(a, lane) : a.n_adapters + 1;
+        const uint32_t rank = rank_of(a, own);
+        if (threadIdx.x < kWave) {
+            sm.with[lane] = 0;
+            sm.one_of[own] = static_cast<uint8_t>(lane);
         }
-        return false;
+        __syncthreads();
+        const uint32_t one = sm.one_of[own];
+        if (threadIdx.x < kWave) atomicOr(&sm.with[one], 1ull << lane);
+        __syncthreads();
+        const uint64_t mine = sm.with[one], below = (1ull << lane) - 1;
+        const uint32_t place = __builtin_popcountll(mine & below);
+        const bool left = has && !(a.in_place && own == a.n_adapters);
+        uint64_t begins = __ballot(left && place % kN == 0);
+        if (tile >= static_cast<uint32_t>(__builtin_popcountll(begins))) return false;
+        for (uint32_t i = 0; i < tile; i++) begins &= begins - 1;
+        const uint32_t first = __builtin_ctzll(begins);
+        m.adapter = __builtin_amdgcn_readlane(own, first);
+        m.rank = __builtin_amdgcn_readlane(rank, first);
+        const uint32_t from = __builtin_amdgcn_readlane(place, first);
+        uint64_t with = __ballot(own == m.adapter && place >= from && place < from + kN);
+        m.n = __builtin_popcountll(with);
+        m.token[0] = first;
+        for (uint32_t i = 0; i < m.n; i++) {
+            if (j == i) m.token[0] = __builtin_ctzll(with);
+            with &= with - 1;
+        }
+        return true;
     } else {
+        static_assert(kN * kNt == zlm::kLoraTile, "as the tokens are grouped");
         if (tile >= *a.n_tiles) return false;
         const LoraTile t = a.tile[tile];
         m.adapter = t.adapter;
+        m.rank = rank_of(a, t.adapter);
         m.n = t.n;
-        m.live = j < t.n;
-        m.token = a.order[t.first + (m.live ? j : 0)];
+#pragma unroll
+        for (int i = 0; i < kNt; i++) m.token[i] = a.order[t.first + (m.live(i) ? kN * i + j : 0)];
         return true;
     }
 }
 
-__device__ __forceinline__ uint32_t rank_of(const Args& a, uint32_t adapter) {
-    return a.ranks ? min(static_cast<uint32_t>(max(a.ranks[adapter], 0)), a.rank) : a.rank;
-}
-
 // The tokens by adapter: counted, their places summed up, then put there (in any order: a
-// token's result does not depend on its place).  One workgroup.
+// token's result does not depend on its place).  One workgroup; the first 8192 tokens'
+// adapters stay in registers between the two passes.
 __device__ __forceinline__ void group(const Args& a) {
     constexpr uint32_t kThreads = 1024, kMost = zlm::kLoraAdapters + 1, kPer = (kMost + kThreads - 1) / kThreads;
+    constexpr uint32_t kTile = zlm::kLoraTile, kHold = 8;
     __shared__ uint32_t count[kPer * kThreads], tiles_to[kPer * kThreads];
     __shared__ uint32_t sums[2][kThreads / kWave];
     const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1), wid = tid / kWave;
     const uint32_t groups = a.n_adapters + (a.in_place ? 0 : 1);
-    for (uint32_t i = tid; i < kPer * kThreads; i += kThreads) count[i] = 0;
-    __syncthreads();
-    for (uint32_t t = tid; t < a.n_tokens; t += kThreads) {
-        // one atomic for the tokens of a wave that are its first's
-        const uint32_t id = adapter_of(a, t);
+    uint32_t held[kHold];
+#pragma unroll
+    for (uint32_t i = 0; i < kHold; i++) held[i] = kThreads * i < a.n_tokens ? adapter_of(a, min(kThreads * i + tid, a.n_tokens - 1)) : 0;
+    // f(token, its adapter), by all lanes that have a token
+    const auto each = [&](const auto& f) {
+#pragma unroll
+        for (uint32_t i = 0; i < kHold; i++)
+            if (kThreads * i + tid < a.n_tokens) f(kThreads * i + tid, held[i]);
+        for (uint32_t t = kThreads * kHold + tid; t < a.n_tokens; t += kThreads) f(t, adapter_of(a, t));
+    };
+    // a place after `count`'s: one atomic for the tokens of a wave that are its first's
+    const auto add = [&](uint32_t id) {
         const uint32_t head = __builtin_amdgcn_readfirstlane(id);
         const uint64_t same = __ballot(id == head);
-        if (id != head) atomicAdd(&count[id], 1u);
-        else if (lane == static_cast<uint32_t>(__builtin_ctzll(same))) atomicAdd(&count[id], static_cast<uint32_t>(__builtin_popcountll(same)));
-    }
+        const uint32_t first = __builtin_ctzll(same);
+        uint32_t at = 0;
+        if (id != head) at = atomicAdd(&count[id], 1u);
+        else if (lane == first) at = atomicAdd(&count[id], static_cast<uint32_t>(__builtin_popcountll(same)));
+        const uint32_t base = __builtin_amdgcn_readlane(at, first);
+        return id == head ? base + static_cast<uint32_t>(__builtin_popcountll(same & ((1ull << lane) - 1))) : at;
+    };
+    for (uint32_t i = tid; i <= a.n_adapters + 1; i += kThreads) count[i] = 0;
+    __syncthreads();
+    each([&](uint32_t, uint32_t id) { add(id); });
     __syncthreads();
     // exclusive sums of tokens and tiles, kPer groups a thread
+    const uint32_t per = (groups + kThreads) / kThreads;
     uint32_t n = 0, k = 0, own[kPer];
 #pragma unroll
     for (uint32_t i = 0; i < kPer; i++) {
-        const uint32_t g = tid * kPer + i;
-        own[i] = g < groups ? count[g] : 0;
+        const uint32_t g = tid * per + i;
+        own[i] = i < per && g < groups ? count[g] : 0;
         n += own[i];
         k += (own[i] + kTile - 1) / kTile;
     }
@@ -202,20 +236,21 @@ __device__ __forceinline__ void group(const Args& a) {
     }
     __syncthreads();
     uint32_t all = 0;
+#pragma unroll
     for (uint32_t i = 0; i < kThreads / kWave; i++) {
-        if (i < wid) {
-            to_n += sums[0][i];
-            to_k += sums[1][i];
-        }
+        to_n += i < wid ? sums[0][i] : 0;
+        to_k += i < wid ? sums[1][i] : 0;
         all += sums[1][i];
     }
     to_n -= n;
     to_k -= k;
 #pragma unroll
     for (uint32_t i = 0; i < kPer; i++) {
-        const uint32_t g = tid * kPer + i;
-        count[g] = to_n;  // from here on the place of the group's next token
-        tiles_to[g] = to_k;
+        const uint32_t g = tid * per + i;
+        if (i < per && g <= groups) {
+            count[g] = to_n;  // from here on the place of the group's next token
+            tiles_to[g] = to_k;
+        }
         to_n += own[i];
         to_k += (own[i] + kTile - 1) / kTile;
     }
@@ -228,67 +263,63 @@ __device__ __forceinline__ void group(const Args& a) {
             else hi = mid;
         }
         const uint32_t at = kTile * (i - tiles_to[lo]);
-        const uint32_t end = lo + 1 < kPer * kThreads ? count[lo + 1] : 0;
-        a.tile[i] = {lo, count[lo] + at, min(end - count[lo] - at, kTile)};
+        a.tile[i] = {lo, count[lo] + at, min(count[lo + 1] - count[lo] - at, kTile)};
     }
     if (tid == 0) *a.n_tiles = all;
     __syncthreads();
-    for (uint32_t t = tid; t < a.n_tokens; t += kThreads) {
-        const uint32_t id = adapter_of(a, t);
-        if (id >= groups) continue;
-        const uint32_t head = __builtin_amdgcn_readfirstlane(id);
-        const uint64_t same = __ballot(id == head);
-        const uint32_t first = __builtin_ctzll(same);
-        uint32_t at = 0;
-        if (id != head) at = atomicAdd(&count[id], 1u);
-        else if (lane == first) at = atomicAdd(&count[id], static_cast<uint32_t>(__builtin_popcountll(same)));
-        const uint32_t base = __builtin_amdgcn_readlane(at, first);
-        if (id == head) at = base + __builtin_popcountll(same & ((1ull << lane) - 1));
-        a.order[at] = t;
-    }
+    each([&](uint32_t t, uint32_t id) {
+        if (id < groups) a.order[add(id)] = t;
+    });
 }
 
 // ---- h = A x ----
 //
 // A workgroup: a tile, a split of k, up to 16 kMt rows of A.  Its waves take k in turn
-// (runs of 32, the lane's eight of them together) and add up their sums through LDS.
-template <class W, int kMt, bool kSmall>
+// (runs of 32, the lane's eight of them together) and add up their sums through LDS.  5000
+// tokens of k 4096, rank 64: 30 us by tiles of 32 tokens, three splits and four waves (one
+// split 52, eight 32; by tiles of 16, which read A twice as often, 41).
+template <class W, int kMt, int kNt>
 __device__ __forceinline__ void down(const Args& a) {
-    __shared__ v4f sums[kWaves][kMt < 4 ? kMt : 4][kWave];
+    constexpr uint32_t kWaves = zlm::kLoraWaves[kNt - 1];
+    constexpr int kStep = kMt * kNt < 4 ? kMt * kNt : 4;
+    __shared__ v4f sums[kWaves][kStep][kWave];
     const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(tid / kWave);
     const uint32_t m = lane & 15, q = lane >> 4, tile = blockIdx.x, split = blockIdx.y;
-    Mine mine;
-    if (!tile_of<kSmall>(a, tile, mine) || mine.adapter >= a.n_adapters) return;
-    const uint32_t r = rank_of(a, mine.adapter), r0 = 16 * kMt * blockIdx.z;
+    Mine<kNt> mine;
+    if (!tile_of(a, tile, mine) || mine.adapter >= a.n_adapters) return;
+    const uint32_t r = mine.rank, r0 = 16 * kMt * blockIdx.z;
     if (r0 >= r) return;
     const uint32_t chunks = a.k / 32, parts = a.splits * kWaves, part = split * kWaves + wid;
     const uint32_t c0 = static_cast<uint64_t>(chunks) * part / parts, c1 = static_cast<uint64_t>(chunks) * (part + 1) / parts;
-    const float* x = a.x + mine.token * a.x_stride + 8 * q;
+    const float* x[kNt];
+#pragma unroll
+    for (int t = 0; t < kNt; t++) x[t] = a.x + mine.token[t] * a.x_stride + 8 * q;
     const uint8_t* w[kMt];
 #pragma unroll
     for (int i = 0; i < kMt; i++) {
         const uint32_t row = min(r0 + 16 * i + m, a.rank - 1);
         w[i] = static_cast<const uint8_t*>(a.a) + ((static_cast<uint64_t>(mine.adapter) * a.rank + row) * a.k + 8 * q) * W::kBytes;
     }
-    v4f acc[kMt];
+    v4f acc[kNt][kMt];
 #pragma unroll
-    for (int i = 0; i < kMt; i++) acc[i] = v4f{0, 0, 0, 0};
-    constexpr uint32_t kU = kMt <= 2 ? 4 : 2;  // runs in flight
+    for (int t = 0; t < kNt; t++)
+#pragma unroll
+        for (int i = 0; i < kMt; i++) acc[t][i] = v4f{0, 0, 0, 0};
+    // runs in flight: as many as registers hold for two waves a SIMD
+    constexpr uint32_t kU = kMt * W::kVecs <= 4 ? zlm::kLoraRuns[kNt - 1] : kMt * W::kVecs <= 8 ? 2 : 1;
     for (uint32_t c = c0; c < c1; c += kU) {
-        float xv[kU][8];
+        v4f xv[kU][kNt][2];
         v4u wv[kU][kMt][W::kVecs];
 #pragma unroll
         for (uint32_t u = 0; u < kU; u++) {
             const uint32_t at = 32 * min(c + u, c1 - 1);
-            v4f lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
-            if (mine.live) {
-                lo = *reinterpret_cast<const v4f*>(x + at);
-                hi = *reinterpret_cast<const v4f*>(x + at + 4);
-            }
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                xv[u][i] = lo[i];
-                xv[u][4 + i] = hi[i];
+            for (int t = 0; t < kNt; t++) {
+                xv[u][t][0] = xv[u][t][1] = v4f{0, 0, 0, 0};
+                if (mine.live(t)) {
+                    xv[u][t][0] = *reinterpret_cast<const v4f*>(x[t] + at);
+                    xv[u][t][1] = *reinterpret_cast<const v4f*>(x[t] + at + 4);
+                }
             }
 #pragma unroll
             for (int i = 0; i < kMt; i++)
@@ -297,147 +328,273 @@ __device__ __forceinline__ void down(const Args& a) {
 #pragma unroll
         for (uint32_t u = 0; u < kU; u++) {
             if (c + u >= c1) break;
-            v8b xp[3];
-            to_parts(xv[u], xp);
+            v8b xp[kNt][3];
+#pragma unroll
+            for (int t = 0; t < kNt; t++) {
+                const v4f lo = xv[u][t][0], hi = xv[u][t][1];
+                const float f[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                to_parts(f, xp[t]);
+            }
 #pragma unroll
             for (int i = 0; i < kMt; i++) {
                 if (r0 + 16 * i >= r) break;
                 v8b wp[W::kParts];
                 W::parts(wv[u][i], wp);
-                acc[i] = multiply(wp, xp, acc[i]);
+#pragma unroll
+                for (int t = 0; t < kNt; t++) acc[t][i] = multiply(wp, xp[t], acc[t][i]);
             }
         }
     }
-    float* to = a.part + ((static_cast<uint64_t>(split) * a.tiles + tile) * kTile) * a.rank;
-    constexpr int kStep = kMt < 4 ? kMt : 4;
+    float* to = a.part + (static_cast<uint64_t>(split) * a.tiles + tile) * (kN * kNt) * a.rank;
 #pragma unroll
-    for (int i0 = 0; i0 < kMt; i0 += kStep) {
+    for (int i0 = 0; i0 < kMt * kNt; i0 += kStep) {
         if (i0) __syncthreads();
 #pragma unroll
-        for (int i = 0; i < kStep; i++) sums[wid][i][lane] = acc[i0 + i];
+        for (int i = 0; i < kStep; i++) sums[wid][i][lane] = acc[(i0 + i) / kMt][(i0 + i) % kMt];
         __syncthreads();
         for (uint32_t i = wid; i < kStep; i += kWaves) {
             v4f s = sums[0][i][lane];
 #pragma unroll
             for (uint32_t v = 1; v < kWaves; v++) s += sums[v][i][lane];
-            const uint32_t row = r0 + 16 * (i0 + i) + 4 * q;
-            if (m < mine.n && row < a.rank) *reinterpret_cast<v4f*>(to + m * a.rank + row) = s;
+            const uint32_t row = r0 + 16 * ((i0 + i) % kMt) + 4 * q, j = kN * ((i0 + i) / kMt) + m;
+            if (j < mine.n && row < a.rank) *reinterpret_cast<v4f*>(to + j * a.rank + row) = s;
         }
     }
 }
 
 // ---- y = res + scale B h ----
-//
-// A wave: a tile and kLoraRows rows of y, 32 at a time: two matrix tiles whose rows are
-// dealt so that a lane's results are eight values of y in a row.  kKt: runs of 32 of the rank.
-template <class W, int kKt, bool kSmall>
-__device__ __forceinline__ void up(const Args& a) {
-    const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(tid / kWave);
-    const uint32_t m = lane & 15, q = lane >> 4, tile = blockIdx.x;
-    Mine mine;
-    if (!tile_of<kSmall>(a, tile, mine)) return;
-    const uint32_t n0 = (blockIdx.y * 4 + wid) * zlm::kLoraRows;
-    if (n0 >= a.rows) return;
-    const uint32_t n1 = min(n0 + zlm::kLoraRows, a.rows);
-    const bool with = mine.adapter < a.n_adapters;
-    const uint32_t r = with ? rank_of(a, mine.adapter) : 0;
-    const float scale = with && a.scales ? a.scales[mine.adapter] : 1.0f;
-    const uint64_t at = mine.token * a.y_stride;
-    v8b hp[kKt][3];
+
+// h of the lane's tokens, the sums of the splits, as parts.  kKt: runs of 32 of the rank.
+template <int kKt, int kNt>
+__device__ __forceinline__ void load_h(const Args& a, const Mine<kNt>& mine, uint32_t tile, uint32_t r, v8b (&hp)[kNt][kKt][3]) {
+    const uint32_t m = threadIdx.x & 15, q = (threadIdx.x & (kWave - 1)) >> 4;
 #pragma unroll
-    for (int c = 0; c < kKt; c++) {
-        float h[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) h[i] = 0.0f;
-        const uint32_t k = 32 * c + 8 * q;
-        if (mine.live && k < r) {
-            for (uint32_t s = 0; s < a.splits; s++) {
-                const float* p = a.part + ((static_cast<uint64_t>(s) * a.tiles + tile) * kTile + m) * a.rank + k;
-                const v4f lo = reinterpret_cast<const v4f*>(p)[0], hi = reinterpret_cast<const v4f*>(p)[1];
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    h[i] += lo[i];
-                    h[4 + i] += hi[i];
-                }
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 8; i++) h[i] = k + i < r ? h[i] : 0.0f;
-        to_parts(h, hp[c]);
-    }
-    const uint8_t* b = static_cast<const uint8_t*>(a.b) +
-                       (with ? static_cast<uint64_t>(mine.adapter) * a.rows * a.rank * W::kBytes : 0);
-    for (uint32_t n = n0; n < n1; n += 32) {
-        v4u wv[2][kKt][W::kVecs];
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-            const uint32_t row = min(n + 8 * (m >> 2) + 4 * e + (m & 3), a.rows - 1);
-            const uint8_t* p = b + (static_cast<uint64_t>(row) * a.rank + 8 * q) * W::kBytes;
-#pragma unroll
-            for (int c = 0; c < kKt; c++) {
-                const uint32_t k = 32 * c + 8 * q;
-#pragma unroll
-                for (int i = 0; i < W::kVecs; i++) wv[e][c][i] = v4u{0, 0, 0, 0};
-                if (k < r) load<W>(p + 32 * c * W::kBytes, wv[e][c]);
-            }
-        }
-        const uint32_t col = n + 8 * q;
-        float was[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) was[i] = 0.0f;
-        if (a.res && mine.live) {
-            const float* p = a.res + at + col;
-            if (a.vectors) {
-#pragma unroll
-                for (int e = 0; e < 2; e++)
-                    if (col + 4 * e < n1) {
-                        const v4f v = reinterpret_cast<const v4f*>(p)[e];
-#pragma unroll
-                        for (int i = 0; i < 4; i++) was[4 * e + i] = v[i];
-                    }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; i++)
-                    if (col + i < n1) was[i] = p[i];
-            }
-        }
-        v4f acc[2] = {v4f{0, 0, 0, 0}, v4f{0, 0, 0, 0}};
+    for (int t = 0; t < kNt; t++)
 #pragma unroll
         for (int c = 0; c < kKt; c++) {
-            if (32u * c >= r) break;
+            v4f lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
+            const uint32_t k = 32 * c + 8 * q;
+            if (mine.live(t) && k < r) {
+                const uint64_t step = static_cast<uint64_t>(a.tiles) * (kN * kNt) * a.rank;
+                const float* p = a.part + (static_cast<uint64_t>(tile) * (kN * kNt) + kN * t + m) * a.rank + k;
+                constexpr uint32_t kU = 4;  // splits in flight
+                for (uint32_t s = 0; s < a.splits; s += kU) {
+                    v4f v[kU][2];
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                if (32u * c + 32 > r) {  // weights behind the adapter's rank: there, but not its own
-                    const uint32_t k = 32 * c + 8 * q;
-#pragma unroll
-                    for (int i = 0; i < 4 * W::kVecs; i++) {
-                        const uint32_t per = 4 / W::kBytes, first = k + i * per;
-                        uint32_t keep = first < r ? ~0u : 0u;
-                        if (per == 2 && first + 1 >= r) keep &= 0xffffu;
-                        wv[e][c][i / 4][i % 4] &= keep;
+                    for (uint32_t u = 0; u < kU; u++) {
+                        const v4f* at = reinterpret_cast<const v4f*>(p + min(s + u, a.splits - 1) * step);
+                        v[u][0] = at[0];
+                        v[u][1] = at[1];
                     }
+#pragma unroll
+                    for (uint32_t u = 0; u < kU; u++)
+                        if (s + u < a.splits) {
+                            lo += v[u][0];
+                            hi += v[u][1];
+                        }
                 }
-                v8b wp[W::kParts];
-                W::parts(wv[e][c], wp);
-                acc[e] = multiply(wp, hp[c], acc[e]);
+            }
+            float h[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+#pragma unroll
+            for (int i = 0; i < 8; i++) h[i] = k + i < r ? h[i] : 0.0f;
+            to_parts(h, hp[t][c]);
+        }
+}
+
+// Sixteen rows of an adapter's B, rows n + m: the lane's eights of the rank.
+template <class W, int kKt>
+__device__ __forceinline__ void load_b(const Args& a, const uint8_t* b, uint32_t n, uint32_t r, v4u (&w)[kKt][W::kVecs]) {
+    const uint32_t m = threadIdx.x & 15, q = (threadIdx.x & (kWave - 1)) >> 4;
+    const uint8_t* p = b + (static_cast<uint64_t>(min(n + m, a.rows - 1)) * a.rank + 8 * q) * W::kBytes;
+#pragma unroll
+    for (int c = 0; c < kKt; c++) {
+#pragma unroll
+        for (int i = 0; i < W::kVecs; i++) w[c][i] = v4u{0, 0, 0, 0};
+        if (32 * c + 8 * q < r) load<W>(p + 32 * c * W::kBytes, w[c]);
+    }
+}
+
+// Their products with h.
+template <class W, int kKt, int kNt>
+__device__ __forceinline__ void multiply_b(uint32_t r, v4u (&w)[kKt][W::kVecs], const v8b (&hp)[kNt][kKt][3], v4f (&acc)[kNt]) {
+    const uint32_t q = (threadIdx.x & (kWave - 1)) >> 4;
+#pragma unroll
+    for (int t = 0; t < kNt; t++) acc[t] = v4f{0, 0, 0, 0};
+#pragma unroll
+    for (int c = 0; c < kKt; c++) {
+        if (32u * c >= r) break;
+        if (32u * c + 32 > r) {  // weights behind the adapter's rank: there, but not its own
+#pragma unroll
+            for (int i = 0; i < 4 * W::kVecs; i++) {
+                const uint32_t per = 4 / W::kBytes, first = 32 * c + 8 * q + i * per;
+                uint32_t keep = first < r ? ~0u : 0u;
+                if (per == 2 && first + 1 >= r) keep &= 0xffffu;
+                w[c][i / 4][i % 4] &= keep;
             }
         }
-        if (!mine.live) continue;
-        float* p = a.y + at + col;
+        v8b wp[W::kParts];
+        W::parts(w[c], wp);
+#pragma unroll
+        for (int t = 0; t < kNt; t++) acc[t] = multiply(wp, hp[t][c], acc[t]);
+    }
+}
+
+// y of few tokens.  A wave: a tile and some rows of y, 32 at a time (two matrix tiles); the
+// next 32 rows' B and res are on their way while these are multiplied.
+template <class W, int kKt>
+__device__ __forceinline__ void up_few(const Args& a) {
+    const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const uint32_t q = lane >> 4, tile = blockIdx.y;
+    Mine<1> mine;
+    if (!tile_of(a, tile, mine)) return;
+    const uint32_t n0 = (blockIdx.x * 4 + wid) * a.wave_rows;
+    if (n0 >= a.rows) return;
+    const uint32_t n1 = min(n0 + a.wave_rows, a.rows);
+    const bool with = mine.adapter < a.n_adapters;
+    const uint32_t r = mine.rank;
+    const float scale = with && a.scales ? a.scales[mine.adapter] : 1.0f;
+    const uint8_t* b = static_cast<const uint8_t*>(a.b) +
+                       (with ? static_cast<uint64_t>(mine.adapter) * a.rows * a.rank * W::kBytes : 0);
+    const bool live = mine.live(0);
+    const uint64_t at = mine.token[0] * a.y_stride;
+    v4u w[2][kKt][W::kVecs];
+    v4f was[2];
+    const auto load_rows = [&](uint32_t n) {
+        const uint32_t col = n + 4 * q;  // and 16 on
+#pragma unroll
+        for (int e = 0; e < 2; e++) load_b<W, kKt>(a, b, n + 16 * e, r, w[e]);
+        was[0] = was[1] = v4f{0, 0, 0, 0};
+        if (!a.res || !live) return;
+        const float* p = a.res + at + col;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            if (a.vectors) {
+                if (col + 16 * e < n1) was[e] = *reinterpret_cast<const v4f*>(p + 16 * e);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (col + 16 * e + i < n1) was[e][i] = p[16 * e + i];
+            }
+        }
+    };
+    load_rows(n0);
+    v8b hp[1][kKt][3];
+    load_h(a, mine, tile, r, hp);
+    for (uint32_t n = n0; n < n1; n += 32) {
+        v4f acc[2][1];
+#pragma unroll
+        for (int e = 0; e < 2; e++) multiply_b<W>(r, w[e], hp, acc[e]);
         v4f o[2];
 #pragma unroll
         for (int e = 0; e < 2; e++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) o[e][i] = r ? __builtin_fmaf(scale, acc[e][i], was[4 * e + i]) : was[4 * e + i];
-        if (a.vectors) {
+            for (int i = 0; i < 4; i++) o[e][i] = r ? __builtin_fmaf(scale, acc[e][0][i], was[e][i]) : was[e][i];
+        if (n + 32 < n1) load_rows(n + 32);
+        if (!live) continue;
+        const uint32_t col = n + 4 * q;
+        float* p = a.y + at + col;
 #pragma unroll
-            for (int e = 0; e < 2; e++)
-                if (col + 4 * e < n1) reinterpret_cast<v4f*>(p)[e] = o[e];
-        } else {
+        for (int e = 0; e < 2; e++) {
+            if (a.vectors) {
+                if (col + 16 * e < n1) *reinterpret_cast<v4f*>(p + 16 * e) = o[e];
+            } else {
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (col + i < n1) p[i] = o[i / 4][i % 4];
+                for (int i = 0; i < 4; i++)
+                    if (col + 16 * e + i < n1) p[16 * e + i] = o[e][i];
+            }
         }
+    }
+}
+
+// y of many tokens: bound by res and y, which meet the products in LDS so that a wave reads and
+// writes 512 bytes of a row at a time (64 bytes, straight from the matrix instruction: 150 us
+// for 5000 tokens of 12288 rows, rank 64; so 122, of which 100 without the products; a plain
+// copy of y 80).  A wave: a tile of 32 tokens (by 16, which read B twice as often: 141) and 128
+// rows of y at a time; a workgroup's waves have neighbouring tiles and the same rows of B.
+constexpr uint32_t kSpan = 128, kPitch = kSpan + 4;  // (a row of LDS begins 16 bytes past the one before's banks)
+
+template <class W, int kKt>
+__device__ __forceinline__ void up_many(const Args& a) {
+    constexpr int kNt = 2;
+    constexpr uint32_t kTokens = kN * kNt;
+    __shared__ __attribute__((aligned(16))) float rows[4][kTokens * kPitch];
+    const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const uint32_t m = lane & 15, q = lane >> 4, tile = blockIdx.y * 4 + wid;
+    Mine<kNt> mine;
+    if (!tile_of(a, tile, mine)) return;
+    const uint32_t n0 = blockIdx.x * a.wave_rows;
+    if (n0 >= a.rows) return;
+    const uint32_t n1 = min(n0 + a.wave_rows, a.rows);
+    const bool with = mine.adapter < a.n_adapters;
+    const uint32_t r = mine.rank;
+    const float scale = with && a.scales ? a.scales[mine.adapter] : 1.0f;
+    const uint8_t* b = static_cast<const uint8_t*>(a.b) +
+                       (with ? static_cast<uint64_t>(mine.adapter) * a.rows * a.rank * W::kBytes : 0);
+    float* const mem = rows[wid];
+    // matrix tiles of B in flight, and pairs of rows of res
+    constexpr uint32_t kAhead = kKt * W::kVecs <= 2 ? 4 : 2, kPairs = 8;
+    v4u w[kAhead][kKt][W::kVecs];
+    const uint32_t half = lane >> 5, col0 = 4 * (lane & 31);  // two tokens an instruction
+    v4f was[kPairs];
+    uint64_t to[kPairs];
+    const auto load_res = [&](uint32_t j0, uint32_t n, uint32_t span) {
+#pragma unroll
+        for (uint32_t j = 0; j < kPairs; j++) {
+            const uint32_t at = j0 + 2 * j + half;
+            const uint32_t t0 = __shfl(mine.token[0], at & 15), t1 = __shfl(mine.token[1], at & 15);
+            to[j] = (at < kN ? t0 : t1) * a.y_stride + n + col0;
+            was[j] = v4f{0, 0, 0, 0};
+            if (a.res && at < mine.n) {
+                if (a.vectors) {
+                    if (col0 < span) was[j] = *reinterpret_cast<const v4f*>(a.res + to[j]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (col0 + i < span) was[j][i] = a.res[to[j] + i];
+                }
+            }
+        }
+    };
+#pragma unroll
+    for (uint32_t i = 0; i < kAhead; i++) load_b<W, kKt>(a, b, n0 + 16 * i, r, w[i]);
+    load_res(0, n0, min(kSpan, n1 - n0));
+    v8b hp[kNt][kKt][3];
+    load_h(a, mine, tile, r, hp);
+    for (uint32_t n = n0; n < n1; n += kSpan) {
+        const uint32_t span = min(kSpan, n1 - n);
+        for (uint32_t e0 = 0; e0 < kSpan / 16; e0 += kAhead) {
+#pragma unroll
+            for (uint32_t i = 0; i < kAhead; i++) {
+                const uint32_t e = e0 + i;
+                v4f acc[kNt];
+                multiply_b<W>(r, w[i], hp, acc);
+                load_b<W, kKt>(a, b, n + 16 * (e + kAhead), r, w[i]);
+#pragma unroll
+                for (int t = 0; t < kNt; t++) *reinterpret_cast<v4f*>(mem + (kN * t + m) * kPitch + 16 * e + 4 * q) = acc[t];
+            }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // a wave's own: no barrier
+        for (uint32_t j0 = 0; j0 < mine.n; j0 += 2 * kPairs) {
+            if (j0) load_res(j0, n, span);
+#pragma unroll
+            for (uint32_t j = 0; j < kPairs; j++) {
+                const uint32_t at = j0 + 2 * j + half;
+                if (at >= mine.n) continue;
+                const v4f d = *reinterpret_cast<const v4f*>(mem + at * kPitch + col0);
+                v4f o;
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[i] = r ? __builtin_fmaf(scale, d[i], was[j][i]) : was[j][i];
+                if (a.vectors) {
+                    if (col0 < span) *reinterpret_cast<v4f*>(a.y + to[j]) = o;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (col0 + i < span) a.y[to[j] + i] = o[i];
+                }
+            }
+        }
+        if (n + kSpan < n1) load_res(0, n + kSpan, min(kSpan, n1 - n - kSpan));
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read before the next rows are written
     }
 }
 
@@ -445,18 +602,27 @@ __device__ __forceinline__ void up(const Args& a) {
 
 extern "C" __global__ void __launch_bounds__(1024) zlm_lora_group(Args a) { group(a); }
 
-#define ZLM_LORA(NAME, W, S, kSmall)                                                                              \
-    extern "C" __global__ void __launch_bounds__(512) zlm_lora_down_##NAME##_1##S(Args a) { down<W, 1, kSmall>(a); } \
-    extern "C" __global__ void __launch_bounds__(512) zlm_lora_down_##NAME##_2##S(Args a) { down<W, 2, kSmall>(a); } \
-    extern "C" __global__ void __launch_bounds__(512) zlm_lora_down_##NAME##_4##S(Args a) { down<W, 4, kSmall>(a); } \
-    extern "C" __global__ void __launch_bounds__(512) zlm_lora_down_##NAME##_8##S(Args a) { down<W, 8, kSmall>(a); } \
-    extern "C" __global__ void __launch_bounds__(256) zlm_lora_up_##NAME##_1##S(Args a) { up<W, 1, kSmall>(a); }     \
-    extern "C" __global__ void __launch_bounds__(256) zlm_lora_up_##NAME##_2##S(Args a) { up<W, 2, kSmall>(a); }     \
-    extern "C" __global__ void __launch_bounds__(256) zlm_lora_up_##NAME##_4##S(Args a) { up<W, 4, kSmall>(a); }     \
-    extern "C" __global__ void __launch_bounds__(256) zlm_lora_up_##NAME##_8##S(Args a) { up<W, 8, kSmall>(a); }
-ZLM_LORA(bf16, Bf16, , false)
-ZLM_LORA(f16, F16, , false)
-ZLM_LORA(f32, F32, , false)
-ZLM_LORA(bf16, Bf16, _small, true)
-ZLM_LORA(f16, F16, _small, true)
-ZLM_LORA(f32, F32, _small, true)
+#define ZLM_LORA_DOWN(NAME, W, kMt, S, kNt)                                                                       \
+    extern "C" __global__ void __launch_bounds__(64 * zlm::kLoraWaves[kNt - 1]) zlm_lora_down_##NAME##_##kMt##S(Args a) { \
+        down<W, kMt, kNt>(a);                                                                                     \
+    }
+#define ZLM_LORA_UP(NAME, W, kKt, S, kNt)                                                                         \
+    extern "C" __global__ void __launch_bounds__(256) zlm_lora_up_##NAME##_##kKt##S(Args a) {             \
+        if constexpr (kNt == 1) up_few<W, kKt>(a);                                                                \
+        else up_many<W, kKt>(a);                                                                                  \
+    }
+#define ZLM_LORA(NAME, W, S, kNt)                                                                                 \
+    ZLM_LORA_DOWN(NAME, W, 1, S, kNt)                                                                             \
+    ZLM_LORA_DOWN(NAME, W, 2, S, kNt)                                                                             \
+    ZLM_LORA_DOWN(NAME, W, 4, S, kNt)                                                                             \
+    ZLM_LORA_DOWN(NAME, W, 8, S, kNt)                                                                             \
+    ZLM_LORA_UP(NAME, W, 1, S, kNt)                                                                               \
+    ZLM_LORA_UP(NAME, W, 2, S, kNt)                                                                               \
+    ZLM_LORA_UP(NAME, W, 4, S, kNt)                                                                               \
+    ZLM_LORA_UP(NAME, W, 8, S, kNt)
+ZLM_LORA(bf16, Bf16, , 2)
+ZLM_LORA(f16, F16, , 2)
+ZLM_LORA(f32, F32, , 2)
+ZLM_LORA(bf16, Bf16, _small, 1)
+ZLM_LORA(f16, F16, _small, 1)
+ZLM_LORA(f32, F32, _small, 1)
