@@ -203,8 +203,8 @@ def test_launches_of_a_verification(box):
     d.launch_log(True)
     assert _verify(box, rows=65536, vocab=1 << 20, n_seqs=1024, draft_logits=1 << 16), d.last_error()
     log = d.launch_log_read()
-    assert log[-1]["what"] == "verify draw" and (log[-1]["grid_x"], log[-1]["grid_y"]) == (128, 1024)
-    kept = 2 * 65536 * 32 + 1024 * 128 * 16 + 1024 * 4
+    assert log[-1]["what"] == "verify draw" and (log[-1]["grid_x"], log[-1]["grid_y"]) == (256, 1024)
+    kept = 2 * 65536 * 40 + 1024 * 256 * 16 + 1024 * 4
     for r in log:
         if r["what"] == "verify histogram":
             assert kept + r["grid_x"] * r["grid_y"] * (768 * 8 + 16) <= 64 << 20

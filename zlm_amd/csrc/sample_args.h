@@ -38,10 +38,13 @@ struct SampleArgs {
 struct SampleCut {
     uint64_t token, best;
     double weight, rate;
+    double drafted;  // the share of the token drafted after the row (0 for one that is none)
 };
 
-// A slice's part of what a row that ends a sequence's drafts is drawn from: the weight of
-// the target's tokens, and what of it lies above the draft's.
+constexpr uint32_t kVerifyPart = 4096;  // tokens of a workgroup of the draw
+
+// A part of what a row that ends a sequence's drafts is drawn from: the weight of the
+// target's tokens, and what of it lies above the draft's.
 struct VerifySum {
     double rest, all;
 };
@@ -62,8 +65,9 @@ struct VerifyArgs {
     const float* target_logits;  // of all rows
     const float* draft_logits;
     SampleCut* cuts;    // n_rows of the target, then as many of the draft
-    VerifySum* sums;    // n_seqs x slices
-    uint32_t* counts;   // of each sequence: slices that are summed up
+    uint32_t parts;     // of a row
+    VerifySum* sums;    // n_seqs x parts
+    uint32_t* counts;   // of each sequence: parts that are summed up
 };
 
 }  // namespace zlm

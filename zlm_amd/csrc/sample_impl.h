@@ -36,7 +36,13 @@ using zlm::SampleSlice;
 constexpr uint32_t kWave = 64, kThreads = 512;  // of a row's workgroup
 constexpr uint32_t kSlice = zlm::kSampleSlice, kBins = zlm::kSampleBins, kSlices = zlm::kSampleSlices;
 constexpr uint32_t kShort = zlm::kSampleShort;
-constexpr uint32_t kList = 12288;  // tokens that are looked at one by one: LDS holds them, a CU one workgroup
+// Tokens that are looked at one by one, in LDS: as many as leave a CU one workgroup, or (the
+// cuts of a row without its draw, whose tokens in question are fewer) two.
+#ifdef ZLM_SAMPLE_FEW
+constexpr uint32_t kList = 4096;
+#else
+constexpr uint32_t kList = 12288;
+#endif
 constexpr double kUnit = 17179869184.0;  // 2^34: the weight at a bin's edge
 constexpr int kCountShift = 50;          // a bin's count above its weights: 8192 x 2^34 is 2^47
 
@@ -67,12 +73,17 @@ struct Weight {
         }
     }
     __device__ __forceinline__ uint64_t operator()(double f) const {
+        return __builtin_bit_cast(uint64_t, raised(f)) & 0xfffffffffffffull;
+    }
+    __device__ __forceinline__ double units(double f) const { return raised(f) - 4503599627370496.0; }  // the integer itself
+
+private:
+    __device__ __forceinline__ double raised(double f) const {
         double r = __builtin_fma(c[5], f, c[4]);
         r = __builtin_fma(r, f, c[3]);
         r = __builtin_fma(r, f, c[2]);
         r = __builtin_fma(r, f, c[1]);
-        r = __builtin_fma(r, f, c[0]) + 4503599627370496.0;  // + 2^52: the integer in the low bits
-        return __builtin_bit_cast(uint64_t, r) & 0xfffffffffffffull;
+        return __builtin_fma(r, f, c[0]) + 4503599627370496.0;  // + 2^52: the integer in the low bits
     }
 };
 
@@ -328,8 +339,8 @@ struct Found {
 class Row {
 public:
     // What pick reads of the row at its start, all in one latency: the histograms and
-    // short lists of the first 32 slices.
-    static constexpr uint32_t kAhead = 32, kSide = kThreads / kShort;
+    // short lists of the first slices, as many as registers hold.
+    static constexpr uint32_t kAhead = kList < 12288 ? 24 : 32, kSide = kThreads / kShort;
     struct Ahead {
         uint64_t hist[kAhead], shorts[kAhead / kSide];
     };
@@ -775,9 +786,9 @@ __device__ __forceinline__ uint64_t row_info(const Args& a, Shared& sm, uint32_t
     return last_lane(wave_max(best));
 }
 
-// A row's draw, or (kDraw false) what it would draw from.
+// A row's draw, or (kDraw false) what it would draw from, for thread 0, where it is true.
 template <bool kDraw>
-__device__ __forceinline__ void pick(const Args& a, uint32_t row, zlm::SampleCut* to) {
+__device__ __forceinline__ bool pick(const Args& a, uint32_t row, zlm::SampleCut& to) {
     __shared__ Shared sm;
     const uint32_t tid = threadIdx.x;
     const Params params = params_of<kDraw>(a, row);
@@ -787,12 +798,12 @@ __device__ __forceinline__ void pick(const Args& a, uint32_t row, zlm::SampleCut
     const uint64_t best = row_info(a, sm, row);
     if (best == 0 || rate == 0.0) {  // nothing to draw; temperature 0: the largest
         if (!kDraw) {
-            if (tid == 0) *to = {0, best, 0.0, 0.0};
+            to = {0, best, 0.0, 0.0, 0.0};
         } else if (tid == 0) {
             a.token[row] = best ? static_cast<int32_t>(~static_cast<uint32_t>(best)) : -1;
             if (a.prob) a.prob[row] = best ? 1.0f : 0.0f;
         }
-        return;
+        return tid == 0;
     }
     const Filters f = filters_of(params, rate, best);
     Row r(a, sm, row, rate, best);
@@ -826,8 +837,8 @@ __device__ __forceinline__ void pick(const Args& a, uint32_t row, zlm::SampleCut
     if constexpr (kDraw) {
         r.bins_for(kMore, w0 * f.u, w1 * f.u, u_bins);
     } else if (!by_k && !f.by_p && !f.by_min) {  // all that have weight
-        if (tid == 0) *to = {0, best, total, rate};
-        return;
+        to = {0, best, total, rate, 0.0};
+        return tid == 0;
     }
     const bool listed = r.in_question() <= kList;
     if (listed && !r.list_shorts(ahead)) r.list_row();
@@ -855,9 +866,8 @@ __device__ __forceinline__ void pick(const Args& a, uint32_t row, zlm::SampleCut
             if (a.prob) a.prob[row] = t.token ? static_cast<float>(r.weight_at(t.token) / cut.weight) : 0.0f;
         }
     }
-    if constexpr (!kDraw) {
-        if (tid == 0) *to = {cut.token, best, cut.weight, rate};
-    }
+    if constexpr (!kDraw) to = {cut.token, best, cut.weight, rate, 0.0};
+    return tid == 0;
 }
 
 }  // namespace

@@ -3390,7 +3390,8 @@ extern "C" bool zlm_gpu_verify_enqueue(zlm_device* d, const float* logits, uint6
     uint8_t* const begin = reinterpret_cast<uint8_t*>(d->serving);
     v.cuts = reinterpret_cast<zlm::SampleCut*>(begin);
     v.sums = reinterpret_cast<zlm::VerifySum*>(v.cuts + 2 * static_cast<size_t>(rows));
-    v.counts = reinterpret_cast<uint32_t*>(v.sums + static_cast<size_t>(n_seqs) * slices);
+    v.parts = (vocab + zlm::kVerifyPart - 1) / zlm::kVerifyPart;
+    v.counts = reinterpret_cast<uint32_t*>(v.sums + static_cast<size_t>(n_seqs) * v.parts);
     uint8_t* const hists = begin + (reinterpret_cast<uint8_t*>(v.counts + n_seqs) - begin + 15) / 16 * 16;
     const uint64_t room = kServingScratch - static_cast<uint64_t>(hists - begin);
     const uint32_t sides = v.by_logits ? 2 : 1;
@@ -3409,9 +3410,8 @@ extern "C" bool zlm_gpu_verify_enqueue(zlm_device* d, const float* logits, uint6
             !launch(d, d->verify_cuts, n * sides, 512, args, "verify cuts"))
             return false;
     }
-    if (rows == 0) v.target.slices = slices;
     v.target.vocab = vocab;
-    return launch3(d, d->verify_draw, slices, n_seqs, 1, 512, args, "verify draw");
+    return launch3(d, d->verify_draw, v.parts, n_seqs, 1, 512, args, "verify draw");
 }
 
 // ---- low-rank adapters ----

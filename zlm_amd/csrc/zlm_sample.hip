@@ -6,4 +6,7 @@
 
 extern "C" __global__ void __launch_bounds__(256, 8) zlm_sample_hist(Args a) { slice_hist<256>(a, blockIdx.y); }
 extern "C" __global__ void __launch_bounds__(1024) zlm_sample_hist_wide(Args a) { slice_hist<1024>(a, blockIdx.y); }
-extern "C" __global__ void __launch_bounds__(512) zlm_sample_pick(Args a) { pick<true>(a, blockIdx.x, nullptr); }
+extern "C" __global__ void __launch_bounds__(512) zlm_sample_pick(Args a) {
+    zlm::SampleCut none;
+    pick<true>(a, blockIdx.x, none);
+}

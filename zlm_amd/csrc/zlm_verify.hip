@@ -9,9 +9,10 @@
 // drawn from the last row's p.  Three launches:
 //   hist  the sampler's histograms of all rows, target's and draft's
 //   cuts  the sampler's search of all rows: what is kept of each, and its weight
-//   draw  a workgroup for each 8192 tokens of a sequence: it decides which row ends the
+//   draw  a workgroup for each 4096 tokens of a sequence: it decides which row ends the
 //         drafts (a few loads), and sums up its part of what is drawn from; the last of a
 //         sequence's to be done adds up the parts and looks the token up in its part
+#define ZLM_SAMPLE_FEW
 #include "sample_impl.h"
 
 namespace {
@@ -19,7 +20,7 @@ namespace {
 using VArgs = zlm::VerifyArgs;
 using Cut = zlm::SampleCut;
 using Sum = zlm::VerifySum;
-constexpr uint32_t kDrawThreads = 512, kDrawPer = kSlice / kDrawThreads;
+constexpr uint32_t kPart = zlm::kVerifyPart, kDrawThreads = 512, kVecs = kPart / (4 * kDrawThreads);
 
 // Whether a draw may look at row r: 0 no, 1 a sequence's last (the draft has none there), 2 yes.
 __device__ __forceinline__ uint32_t use_of(const VArgs& v, uint32_t r) {
@@ -50,35 +51,64 @@ __device__ __forceinline__ void hist(const VArgs& v) {
     slice_hist<kHistThreads>(draft ? v.draft : v.target, row);
 }
 
+// A value that all lanes have, in scalar registers.
+template <class T>
+__device__ __forceinline__ T uniform(T v) {
+    if constexpr (sizeof(T) == 4) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
+    } else {
+        const uint64_t u = __builtin_bit_cast(uint64_t, v);
+        const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<int>(u)), hi = __builtin_amdgcn_readfirstlane(static_cast<int>(u >> 32));
+        return __builtin_bit_cast(T, static_cast<uint64_t>(hi) << 32 | lo);
+    }
+}
+
+// A row's tokens by their shares.
+struct Share {
+    double top, rate, inv;
+    float least;    // the smallest logit that is kept, as far as `last`, the last token of that logit
+    uint32_t last;
+    __device__ __forceinline__ explicit Share(const Cut& c) {
+        // (a cut of 0 keeps all that is no -inf, a row without any has a `best` of 0)
+        const uint64_t from = c.rate == 0.0 ? c.best : c.token;
+        const float x = c.best == 0 ? INFINITY : from == 0 ? -INFINITY : value_of(static_cast<uint32_t>(from >> 32));
+        rate = uniform(c.rate);
+        top = uniform(__builtin_floor(static_cast<double>(value_of(static_cast<uint32_t>(c.best >> 32))) * c.rate));
+        inv = uniform(c.weight > 0.0 ? 1.0 / c.weight : 0.0);
+        least = uniform(x);
+        last = uniform(~static_cast<uint32_t>(from));
+    }
+    // Bin by bin down from the largest; 0 for those past kBins, which have no weight.
+    __device__ __forceinline__ double of(float x, uint32_t i, const Weight& weight, const double* scale, bool table) const {
+        x = x > 3.402823466e38f ? 3.402823466e38f : x;  // (a NaN stays one, and is not kept)
+        if (!(x > least || (x == least && i <= last))) return 0.0;
+        if (rate == 0.0) return 1.0;
+        const double y = static_cast<double>(x) * rate, b = __builtin_floor(y), d = top - b;
+        if (!(d < 1.0 * kBins)) return 0.0;
+        const double w = weight.units(y - b);
+        const uint32_t bin = static_cast<uint32_t>(__builtin_fmax(d, 0.0));
+        return w * (table ? scale[bin] : exp(static_cast<double>(bin) * -0.0625) / kUnit) * inv;
+    }
+};
+
 __device__ __forceinline__ void cuts(const VArgs& v) {
     if (v.first == 0 && blockIdx.x == 0)  // for the launch after this
         for (uint32_t s = threadIdx.x; s < v.n_seqs; s += kThreads) v.counts[s] = 0;
     bool draft;
     uint32_t row;
     if (!row_of(v, blockIdx.x, draft, row)) return;
-    pick<false>(draft ? v.draft : v.target, row, v.cuts + (draft ? v.n_rows : 0) + v.first + row);
-}
-
-// A row's tokens by their shares.
-struct Share {
+    const Args& a = draft ? v.draft : v.target;
+    // the drafted token's logit, on its way early
+    const int32_t d = v.token[v.first + row];
+    const bool is = d >= 0 && static_cast<uint32_t>(d) < a.vocab;
+    const float x = a.logits[row * a.stride + (is ? d : 0)];
+    Cut* const to = v.cuts + (draft ? v.n_rows : 0) + v.first + row;
     Cut cut;
-    double top, inv;
-    const double* scale;  // e^(-bin/16) in units of the weights
-    __device__ __forceinline__ Share(const Cut& c, const double* scales) : cut(c), scale(scales) {
-        top = __builtin_floor(static_cast<double>(value_of(static_cast<uint32_t>(c.best >> 32))) * c.rate);
-        inv = c.weight > 0.0 ? 1.0 / c.weight : 0.0;
-    }
-    // (weight: a Weight, whose coefficients stay where they are)
-    __device__ __forceinline__ double operator()(float x, uint32_t i, const Weight& weight) const {
-        const uint64_t token = static_cast<uint64_t>(key_of(x)) << 32 | static_cast<uint32_t>(~i);
-        if (cut.rate == 0.0) return token == cut.best && token >> 32 ? 1.0 : 0.0;
-        if (token >> 32 == 0 || token < cut.token) return 0.0;
-        const double y = static_cast<double>(value_of(static_cast<uint32_t>(token >> 32))) * cut.rate, b = __builtin_floor(y);
-        const double d = top - b;
-        if (!(d < 1.0 * kBins)) return 0.0;
-        return static_cast<double>(weight(y - b)) * scale[static_cast<uint32_t>(__builtin_fmax(d, 0.0))] * inv;
-    }
-};
+    if (!pick<false>(a, row, cut)) return;
+    const Weight weight;
+    cut.drafted = is ? Share(cut).of(x, d, weight, nullptr, false) : 0.0;
+    *to = cut;
+}
 
 __device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
@@ -95,164 +125,182 @@ __device__ __forceinline__ double get(const double* p) {
 
 struct DrawShared {
     double scale[kBins];
-    double part[2][kDrawThreads / kWave];
+    double part[2][kVecs][kDrawThreads / kWave];
+    uint32_t firsts[kDrawThreads / kWave], backs[kDrawThreads / kWave];
     uint32_t stop, last, at;
     double goal;
+    Cut target, draft;  // of the row that ends the drafts
 };
 
-// A thread's tokens, kDrawPer in a row: what is drawn from, and the target's shares.
+// What a row's draw goes by.
 struct Rows {
     const float *p, *q;  // q null: none, or a certain token
     Share ps, qs;
     uint32_t certain;    // that token, or none
 };
 
-__device__ __forceinline__ void weigh(const VArgs& v, const Rows& r, const Weight& weight, uint32_t i0, double (&rest)[kDrawPer],
-                                      double (&all)[kDrawPer]) {
-    const uint32_t vocab = v.target.vocab;
-    float x[kDrawPer], y[kDrawPer];
+// f(vector, element, what lies above the draft's share, the target's share) for a thread's
+// tokens: four in a row of each 2048 of the part.
+template <class F>
+__device__ __forceinline__ void weigh(const Rows& r, uint32_t vocab, const Weight& weight, const double* scale, uint32_t part, const F& f) {
     typedef float v4 __attribute__((ext_vector_type(4), aligned(4)));
-    if (i0 + kDrawPer <= vocab) {
+    float x[kVecs][4], y[kVecs][4];
+    const uint32_t i0 = part * kPart + 4 * threadIdx.x;
+    if ((part + 1) * kPart <= vocab) {
 #pragma unroll
-        for (uint32_t j = 0; j < kDrawPer; j += 4) {
-            const v4 a = *reinterpret_cast<const v4*>(r.p + i0 + j), b = *reinterpret_cast<const v4*>((r.q ? r.q : r.p) + i0 + j);
+        for (uint32_t j = 0; j < kVecs; j++) {
+            const uint32_t i = i0 + 4 * kDrawThreads * j;
+            const v4 a = *reinterpret_cast<const v4*>(r.p + i), b = *reinterpret_cast<const v4*>((r.q ? r.q : r.p) + i);
 #pragma unroll
             for (uint32_t e = 0; e < 4; e++) {
-                x[j + e] = a[e];
-                y[j + e] = b[e];
+                x[j][e] = a[e];
+                y[j][e] = b[e];
             }
         }
     } else {
 #pragma unroll
-        for (uint32_t j = 0; j < kDrawPer; j++) {
-            x[j] = i0 + j < vocab ? r.p[i0 + j] : -INFINITY;
-            y[j] = r.q && i0 + j < vocab ? r.q[i0 + j] : -INFINITY;
-        }
+        for (uint32_t j = 0; j < kVecs; j++)
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++) {
+                const uint32_t i = i0 + 4 * kDrawThreads * j + e;
+                x[j][e] = i < vocab ? r.p[i] : -INFINITY;
+                y[j][e] = r.q && i < vocab ? r.q[i] : -INFINITY;
+            }
     }
 #pragma unroll
-    for (uint32_t j = 0; j < kDrawPer; j++) {
-        const double p = r.ps(x[j], i0 + j, weight);
-        const double q = r.q ? r.qs(y[j], i0 + j, weight) : i0 + j == r.certain ? 1.0 : 0.0;
-        all[j] = p;
-        rest[j] = p > q ? p - q : 0.0;
+    for (uint32_t j = 0; j < kVecs; j++)
+#pragma unroll
+        for (uint32_t e = 0; e < 4; e++) {
+            const uint32_t i = i0 + 4 * kDrawThreads * j + e;
+            const double p = r.ps.of(x[j][e], i, weight, scale, true);
+            const double q = r.q ? r.qs.of(y[j][e], i, weight, scale, true) : i == r.certain ? 1.0 : 0.0;
+            f(j, e, p > q ? p - q : 0.0, p);
+        }
+}
+
+__device__ __forceinline__ double wave_run(double v) {  // inclusive sums
+    const uint32_t lane = threadIdx.x & (kWave - 1);
+#pragma unroll
+    for (uint32_t o = 1; o < kWave; o <<= 1) {
+        const double y = __shfl_up(v, o);
+        if (lane >= o) v += y;
     }
+    return v;
+}
+
+__device__ __forceinline__ double number(float u) {  // in [0, 1)
+    return __builtin_fminf(__builtin_fmaxf(u, 0.0f), 0x1.fffffep-1f);
 }
 
 __device__ __forceinline__ void draw(const VArgs& v) {
     __shared__ DrawShared sm;
     const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1), wid = tid / kWave;
-    const uint32_t slice = blockIdx.x, s = blockIdx.y, slices = v.target.slices;
+    const uint32_t mine = blockIdx.x, s = blockIdx.y, parts = v.parts, vocab = v.target.vocab;
     const int32_t from = v.q_start[s], to = min(v.q_start[s + 1], static_cast<int32_t>(v.n_rows));
     if (from < 0 || from >= to) {  // no rows
-        if (slice == 0 && tid == 0) v.accepted[s] = 0;
+        if (mine == 0 && tid == 0) v.accepted[s] = 0;
         return;
     }
-    const uint32_t row0 = from, n = static_cast<uint32_t>(to - from), vocab = v.target.vocab;
+    const uint32_t row0 = from, n = static_cast<uint32_t>(to - from);
+    const double u_draw = number(v.u_draw[s]);
     const Weight weight;
     sm.scale[tid] = exp(static_cast<double>(tid) * -0.0625) / kUnit;
     static_assert(kDrawThreads == kBins, "a bin a thread");
-    if (tid == 0) sm.stop = n - 1;
-    __syncthreads();
     if (wid == 0) {
-        // the first row whose drafted token is not accepted
-        for (uint32_t b = 0; b + 1 < n; b += kWave) {
-            const uint32_t i = min(b + lane, n - 2), row = row0 + i;
+        // the first row whose drafted token is not accepted, or the last
+        for (uint32_t b = 0;; b += kWave) {
+            const uint32_t i = min(b + lane, n - 1), row = row0 + i;
+            const Cut p = v.cuts[row];
+            const bool has_q = v.by_logits && i + 1 < n;
+            const Cut q = v.cuts[has_q ? v.n_rows + row : row];
             const int32_t d = v.token[row];
             const bool is = d >= 0 && static_cast<uint32_t>(d) < vocab;
-            const uint32_t at = is ? d : 0;
-            const Share ps(v.cuts[row], sm.scale);
-            const double p = ps(v.target_logits[row * v.target.stride + at], at, weight);
-            double q = 1.0;
-            if (v.by_logits) {
-                const Share qs(v.cuts[v.n_rows + row], sm.scale);
-                q = qs(v.draft_logits[row * v.draft.stride + at], at, weight);
-            }
-            const double u = __builtin_fminf(__builtin_fmaxf(v.u[row], 0.0f), 0x1.fffffep-1f);
-            const uint64_t no = __ballot(!(is && u * q < p));
+            const uint64_t no = __ballot(i + 1 == n || !(is && number(v.u[row]) * (has_q ? q.drafted : 1.0) < p.drafted));
             if (no) {
-                if (lane == 0) sm.stop = min(b + static_cast<uint32_t>(__builtin_ctzll(no)), n - 1);
+                if (lane == static_cast<uint32_t>(__builtin_ctzll(no))) {
+                    sm.stop = i;
+                    sm.target = p;
+                    sm.draft = q;
+                }
                 break;
             }
         }
     }
     __syncthreads();
     const uint32_t stop = sm.stop, row = row0 + stop;
-    const Cut cut = v.cuts[row];
     const int32_t d = stop + 1 < n ? v.token[row] : -1;
     const bool drafted = d >= 0 && static_cast<uint32_t>(d) < vocab;
     const bool by_logits = v.by_logits && drafted;
     const Rows r = {v.target_logits + row * v.target.stride, by_logits ? v.draft_logits + row * v.draft.stride : nullptr,
-                    Share(cut, sm.scale), Share(by_logits ? v.cuts[v.n_rows + row] : cut, sm.scale),
+                    Share(sm.target), Share(by_logits ? sm.draft : sm.target),
                     drafted && !by_logits ? static_cast<uint32_t>(d) : kNone};
-    double rest[kDrawPer], all[kDrawPer];
-    const auto sums_of = [&](uint32_t part, double& own, double& own_all) {
-        weigh(v, r, weight, part * kSlice + tid * kDrawPer, rest, all);
-        own = own_all = 0.0;
-#pragma unroll
-        for (uint32_t j = 0; j < kDrawPer; j++) {
-            own += rest[j];
-            own_all += all[j];
-        }
-    };
-    double own, own_all;
-    sums_of(slice, own, own_all);
+    double own = 0.0, own_all = 0.0;
+    weigh(r, vocab, weight, sm.scale, mine, [&](uint32_t, uint32_t, double rest, double all) {
+        own += rest;
+        own_all += all;
+    });
     const double a = wave_sum(own), b = wave_sum(own_all);
     if (lane == 0) {
-        sm.part[0][wid] = a;
-        sm.part[1][wid] = b;
+        sm.part[0][0][wid] = a;
+        sm.part[1][0][wid] = b;
     }
     __syncthreads();
-    Sum* const sums = v.sums + static_cast<size_t>(s) * slices;
+    Sum* const sums = v.sums + static_cast<size_t>(s) * parts;
     if (tid == 0) {
         Sum t = {0.0, 0.0};
         for (uint32_t w = 0; w < kDrawThreads / kWave; w++) {
-            t.rest += sm.part[0][w];
-            t.all += sm.part[1][w];
+            t.rest += sm.part[0][0][w];
+            t.all += sm.part[1][0][w];
         }
-        put(&sums[slice].rest, t.rest);
-        put(&sums[slice].all, t.all);
+        put(&sums[mine].rest, t.rest);
+        put(&sums[mine].all, t.all);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // they are in memory
-        sm.last = __hip_atomic_fetch_add(v.counts + s, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == slices - 1;
+        sm.last = __hip_atomic_fetch_add(v.counts + s, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
     }
     __syncthreads();
     if (!sm.last) return;
     // the part in which the goal is reached; where a rounding leaves none, the last with any weight
     if (wid == 0) {
-        static_assert(kSlices <= 2 * kWave, "two parts a lane");
-        double w[2], x[2];
+        constexpr uint32_t kEach = kSlice * kSlices / kPart / kWave;  // parts a lane
+        double w[kEach], x[kEach];
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const uint32_t at = 2 * lane + i;
-            w[i] = at < slices ? get(&sums[at].rest) : 0.0;
-            x[i] = at < slices ? get(&sums[at].all) : 0.0;
+        for (uint32_t i = 0; i < kEach; i++) {
+            const uint32_t at = min(kEach * lane + i, parts - 1);
+            const bool has = kEach * lane + i < parts;
+            const double rest = get(&sums[at].rest), all = get(&sums[at].all);
+            w[i] = has ? rest : 0.0;
+            x[i] = has ? all : 0.0;
         }
-        const bool any = __any(w[0] + w[1] > 0.0);
+        double sum = 0.0;
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; i++) sum += w[i];
+        const bool any = __any(sum > 0.0);
         if (!any) {  // p is q: what is drawn from is p
-            w[0] = x[0];
-            w[1] = x[1];
-        }
-        double run = w[0] + w[1];
+            sum = 0.0;
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const double y = __shfl_up(run, o);
-            if (static_cast<int>(lane) >= o) run += y;
+            for (uint32_t i = 0; i < kEach; i++) sum += w[i] = x[i];
         }
-        const double total = __shfl(run, 63);
-        const double u = __builtin_fminf(__builtin_fmaxf(v.u_draw[s], 0.0f), 0x1.fffffep-1f);
-        const double goal = u * total, before = run - (w[0] + w[1]);
-        // (ends of the two parts; a lane without weight is none)
-        const double mid = before + w[0];
-        const uint64_t in0 = __ballot(w[0] > 0.0 && mid > goal), in1 = __ballot(w[1] > 0.0 && run > goal);
-        const uint64_t has0 = __ballot(w[0] > 0.0), has1 = __ballot(w[1] > 0.0);
-        const uint32_t f0 = in0 ? 2 * __builtin_ctzll(in0) : kNone, f1 = in1 ? 2 * __builtin_ctzll(in1) + 1 : kNone;
-        uint32_t at = min(f0, f1);
-        if (at == kNone) {
-            const uint32_t l0 = has0 ? 2 * (63 - __builtin_clzll(has0)) : kNone, l1 = has1 ? 2 * (63 - __builtin_clzll(has1)) + 1 : kNone;
-            at = l0 == kNone ? l1 : l1 == kNone ? l0 : max(l0, l1);
+        const double run = wave_run(sum), goal = u_draw * __shfl(run, 63);
+        double at = run - sum, before = 0.0, last_before = 0.0;
+        uint32_t first = kNone, back = kNone;
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; i++) {
+            const double end = at + w[i];
+            if (w[i] > 0.0) {
+                back = kEach * lane + i;
+                last_before = at;
+                if (first == kNone && end > goal) {
+                    first = back;
+                    before = at;
+                }
+            }
+            at = end;
         }
-        if (lane == (at == kNone ? 0 : at / 2)) {
-            sm.at = at;
-            sm.goal = goal - (at % 2 ? mid : before);
+        const uint64_t in = __ballot(first != kNone), has = __ballot(back != kNone);
+        const uint32_t who = in ? __builtin_ctzll(in) : has ? 63 - __builtin_clzll(has) : 0;
+        if (lane == who) {
+            sm.at = in ? first : back;
+            sm.goal = goal - (in ? before : last_before);
             sm.last = any ? 1 : 2;
         }
     }
@@ -260,56 +308,52 @@ __device__ __forceinline__ void draw(const VArgs& v) {
     const uint32_t part = sm.at;
     int32_t token = -1;
     if (part != kNone) {
-        sums_of(part, own, own_all);
-        if (sm.last == 2) {
-            own = own_all;
+        const bool whole = sm.last == 2;
+        double sum[kVecs] = {}, run[kVecs], x[kVecs][4];
+        weigh(r, vocab, weight, sm.scale, part, [&](uint32_t j, uint32_t e, double rest, double all) {
+            x[j][e] = whole ? all : rest;
+            sum[j] += x[j][e];
+        });
 #pragma unroll
-            for (uint32_t j = 0; j < kDrawPer; j++) rest[j] = all[j];
-        }
-        double run = own;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const double y = __shfl_up(run, o);
-            if (static_cast<int>(lane) >= o) run += y;
-        }
-        const double wave = __shfl(run, 63);
-        __syncthreads();  // the sums of before are read
-        if (lane == 0) {
-            sm.part[0][wid] = wave;
-            sm.part[1][wid] = 0.0;
+        for (uint32_t j = 0; j < kVecs; j++) {
+            run[j] = wave_run(sum[j]);
+            if (lane == kWave - 1) sm.part[0][j][wid] = run[j];
         }
         __syncthreads();
-        double before = 0.0;
-        for (uint32_t w = 0; w < wid; w++) before += sm.part[0][w];
-        const double end = before + run;
-        // this thread's first token past the goal, and its last with weight
-        double at = end - own;
-        uint32_t first = kNone, back = 0;
+        // before each of this thread's vectors
+        double at[kVecs], before = 0.0;
 #pragma unroll
-        for (uint32_t j = 0; j < kDrawPer; j++) {
-            at += rest[j];
-            const uint32_t i = part * kSlice + tid * kDrawPer + j;
-            if (rest[j] > 0.0) {
-                back = i + 1;
-                if (first == kNone && at > sm.goal) first = i;
+        for (uint32_t j = 0; j < kVecs; j++) {
+            at[j] = before + run[j] - sum[j];
+            for (uint32_t w = 0; w < kDrawThreads / kWave; w++) {
+                at[j] += w < wid ? sm.part[0][j][w] : 0.0;
+                before += sm.part[0][j][w];
             }
         }
+        // its first token past the goal, and its last with weight
+        uint32_t first = kNone, back = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < kVecs; j++)
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++) {
+                const uint32_t i = part * kPart + 4 * kDrawThreads * j + 4 * tid + e;
+                at[j] += x[j][e];
+                back = x[j][e] > 0.0 ? i + 1 : back;
+                first = x[j][e] > 0.0 && at[j] > sm.goal ? min(first, i) : first;
+            }
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) {
             first = min(first, static_cast<uint32_t>(__shfl_xor(first, o)));
             back = max(back, static_cast<uint32_t>(__shfl_xor(back, o)));
         }
-        __syncthreads();
-        uint32_t* const firsts = reinterpret_cast<uint32_t*>(sm.part[0]);
-        uint32_t* const backs = reinterpret_cast<uint32_t*>(sm.part[1]);
         if (lane == 0) {
-            firsts[wid] = first;
-            backs[wid] = back;
+            sm.firsts[wid] = first;
+            sm.backs[wid] = back;
         }
         __syncthreads();
         for (uint32_t w = 0; w < kDrawThreads / kWave; w++) {
-            first = min(first, firsts[w]);
-            back = max(back, backs[w]);
+            first = min(first, sm.firsts[w]);
+            back = max(back, sm.backs[w]);
         }
         token = first != kNone ? static_cast<int32_t>(first) : static_cast<int32_t>(back) - 1;
     }
@@ -324,5 +368,5 @@ __device__ __forceinline__ void draw(const VArgs& v) {
 
 extern "C" __global__ void __launch_bounds__(256, 8) zlm_verify_hist(VArgs v) { hist<256>(v); }
 extern "C" __global__ void __launch_bounds__(1024) zlm_verify_hist_wide(VArgs v) { hist<1024>(v); }
-extern "C" __global__ void __launch_bounds__(512) zlm_verify_cuts(VArgs v) { cuts(v); }
-extern "C" __global__ void __launch_bounds__(512) zlm_verify_draw(VArgs v) { draw(v); }
+extern "C" __global__ void __launch_bounds__(512, 4) zlm_verify_cuts(VArgs v) { cuts(v); }
+extern "C" __global__ void __launch_bounds__(512, 4) zlm_verify_draw(VArgs v) { draw(v); }
