@@ -292,7 +292,7 @@ __device__ __forceinline__ void append_blocks(const AppendArgs& a, const RowAt& 
             }
 #pragma unroll
             for (int r0 = 0; r0 < kRows; r0 += 4) {
-                if (static_cast<uint32_t>(r0) >= n_rows) break;
+                if (static_cast<uint32_t>(r0) >= n_rows) continue;
                 double inv = 1.0;
                 if (a.k_norm) {
                     double ss[4];
@@ -307,7 +307,7 @@ __device__ __forceinline__ void append_blocks(const AppendArgs& a, const RowAt& 
                 }
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    if (static_cast<uint32_t>(r0 + r) >= n_rows) break;
+                    if (static_cast<uint32_t>(r0 + r) >= n_rows) continue;
                     double y[N];
                     const double f = of_row(inv, r >> 1 | (r & 1) << 1);
 #pragma unroll
@@ -341,7 +341,7 @@ __device__ __forceinline__ void append_blocks(const AppendArgs& a, const RowAt& 
         float m = 0.0f;
 #pragma unroll
         for (int r = 0; r < kRows; r++) {
-            if (static_cast<uint32_t>(r) >= n_rows) break;
+            if (static_cast<uint32_t>(r) >= n_rows) continue;
 #pragma unroll
             for (int j = 0; j < N; j++) m = __builtin_fmaxf(m, __builtin_fabsf(x[r][j]));
         }
@@ -372,7 +372,7 @@ __device__ __forceinline__ void append_blocks(const AppendArgs& a, const RowAt& 
             }
 #pragma unroll
             for (int r = 0; r < kRows; r += 2) {
-                if (static_cast<uint32_t>(r) >= n_rows) break;
+                if (static_cast<uint32_t>(r) >= n_rows) continue;
 #pragma unroll
                 for (int j = 0; j < N; j++) {
                     const uint32_t c = code2(x[r][j], x[r + 1][j]);
