@@ -3209,8 +3209,10 @@ bool paged_attention(zlm_device* d, const zlm_paged_cache* cache, const zlm_page
     // again for every 16 rows, the other one has work for few waves: 8 sequences of about
     // 3700 positions, heads of 128, 64 and 192 rows each: f16 73 and 181 us by few rows,
     // 65 and 76 by many; q4_0 39 and 86, 78 and 75 (32 sequences: 119 and 307, 198 and
-    // 223); heads of 256, q4_0: 64 and 156, 56 and 136.
-    const uint32_t few_rows = cache->type == ZLM_GGML_Q4_0 && hd <= 128 ? 128 : 32;
+    // 223); heads of 256, q4_0: 64 and 156, 56 and 136.  e4m3, 48, 64 and 96 rows each: 8
+    // sequences 45, 57 and 79 by few rows, 66, 67 and 82 by many, 32 of them 134, 166 and 242,
+    // 162, 157 and 162.
+    const uint32_t few_rows = hd > 128 ? 32 : cache->type == ZLM_GGML_Q4_0 ? 128 : cache->type == ZLM_CACHE_E4M3 ? 64 : 32;
     const uint64_t rows = static_cast<uint64_t>(batch->n_tokens) * group;
     // Both run where the batch may hold such a sequence beside others and enough rows for
     // it to pay; under that the few-row kernel alone takes what there is.  3000 positions, 4
