@@ -456,6 +456,7 @@ bool load_kernels(zlm_device* d) {
                 const char* name;
             } fns[] = {{&k.down, "down"}, {&k.up, "up"}};
             for (const auto& fn : fns) {
+                if (fn.f == &k.up && i >= 4 && i % 2 == 0) continue;  // many tokens: in passes of 64 of the rank
                 snprintf(nm, sizeof nm, "zlm_lora_%s_%s_%d%s", fn.name, kLoraTypes[t].name, 1 << i / 2, i % 2 ? "_small" : "");
                 if (!ok(d, hipModuleGetFunction(fn.f, d->lora_mod, nm), nm)) return false;
             }
@@ -3467,7 +3468,7 @@ extern "C" bool zlm_gpu_lora_enqueue(zlm_device* d, const zlm_lora* lora, uint32
     // matrix tiles of 16 of the rank in the first product, runs of 32 in the second
     const auto step = [](uint32_t n) { return n <= 1 ? 0 : n <= 2 ? 1 : n <= 4 ? 2 : 3; };
     const uint32_t m_tiles = (lora->rank + 15) / 16, k_runs = (lora->rank + 31) / 32;
-    const int down = step(m_tiles), up = step(k_runs);
+    const int down = step(m_tiles), up_small = step(k_runs), up_many = std::min(up_small, 1);
     for (uint64_t t = 0; t < n_tokens; t += most) {
         a.n_tokens = static_cast<uint32_t>(std::min<uint64_t>(most, n_tokens - t));
         a.adapter = adapter + t;
@@ -3479,7 +3480,8 @@ extern "C" bool zlm_gpu_lora_enqueue(zlm_device* d, const zlm_lora* lora, uint32
         // k over workgroups where tiles alone leave CUs without two, as many runs a wave as it has
         // in flight at least
         const uint64_t waves = zlm::kLoraWaves[!small], runs = 32 * waves * zlm::kLoraRuns[!small];
-        uint64_t splits = std::min<uint64_t>({16, std::max<uint64_t>(1, 2ull * d->cus / a.tiles), (lora->k + runs - 1) / runs});
+        uint64_t splits = std::min<uint64_t>({small ? 16u : 4u, std::max<uint64_t>(1, 2ull * d->cus / (a.tiles * ((m_tiles + 7) / 8))),
+                                              (lora->k + runs - 1) / runs});
         while (splits > 1 && bytes_of(a.n_tokens, splits) > kServingScratch) splits--;
         a.splits = static_cast<uint32_t>(splits);
         a.part = d->serving;
@@ -3502,7 +3504,7 @@ extern "C" bool zlm_gpu_lora_enqueue(zlm_device* d, const zlm_lora* lora, uint32
             !launch3(d, d->lora[type][down][small].down, a.tiles, a.splits, (m_tiles + 7) / 8,
                      static_cast<unsigned>(64 * waves), args,
                      "adapters down") ||
-            !launch3(d, d->lora[type][up][small].up, row_groups, static_cast<unsigned>(small ? a.tiles : fours), 1, 256, args,
+            !launch3(d, d->lora[type][small ? up_small : up_many][small].up, row_groups, static_cast<unsigned>(small ? a.tiles : fours), 1, 256, args,
                      "adapters up"))
             return false;
     }

@@ -357,76 +357,90 @@ __device__ __forceinline__ void down(const Args& a) {
 #pragma unroll
             for (uint32_t v = 1; v < kWaves; v++) s += sums[v][i][lane];
             const uint32_t row = r0 + 16 * ((i0 + i) % kMt) + 4 * q, j = kN * ((i0 + i) / kMt) + m;
-            if (j < mine.n && row < a.rank) *reinterpret_cast<v4f*>(to + j * a.rank + row) = s;
+            if (j >= mine.n || row >= a.rank) continue;
+            *reinterpret_cast<v4f*>(to + j * a.rank + row) = s;
         }
     }
 }
 
 // ---- y = res + scale B h ----
 
-// h of the lane's tokens, the sums of the splits, as parts.  kKt: runs of 32 of the rank.
+// h of the lane's tokens as parts, runs c0 .. c0 + kKt of 32 of the rank: the splits' sum.
 template <int kKt, int kNt>
-__device__ __forceinline__ void load_h(const Args& a, const Mine<kNt>& mine, uint32_t tile, uint32_t r, v8b (&hp)[kNt][kKt][3]) {
-    const uint32_t m = threadIdx.x & 15, q = (threadIdx.x & (kWave - 1)) >> 4;
+__device__ __forceinline__ void load_h(const Args& a, const Mine<kNt>& mine, uint32_t tile, uint32_t c0, v8b (&hp)[kNt][kKt][3]) {
+    const uint32_t m = threadIdx.x & 15, q = (threadIdx.x & (kWave - 1)) >> 4, r = mine.rank;
+    const uint64_t step = static_cast<uint64_t>(a.tiles) * (kN * kNt) * a.rank;
+    constexpr uint32_t kU = kKt * kNt <= 2 ? 4 : kKt * kNt <= 4 ? 2 : 1;  // splits in flight
+    v4f sum[kNt][kKt][2];
+#pragma unroll
+    for (int t = 0; t < kNt; t++)
+#pragma unroll
+        for (int c = 0; c < kKt; c++) sum[t][c][0] = sum[t][c][1] = v4f{0, 0, 0, 0};
+    for (uint32_t s = 0; s < a.splits; s += kU) {
+        v4f v[kU][kNt][kKt][2];
+#pragma unroll
+        for (uint32_t u = 0; u < kU; u++)
+#pragma unroll
+            for (int t = 0; t < kNt; t++)
+#pragma unroll
+                for (int c = 0; c < kKt; c++) {
+                    const uint32_t k = 32 * (c0 + c) + 8 * q;
+                    v[u][t][c][0] = v[u][t][c][1] = v4f{0, 0, 0, 0};
+                    if (mine.live(t) && k < r) {
+                        const v4f* p = reinterpret_cast<const v4f*>(
+                            a.part + min(s + u, a.splits - 1) * step + (static_cast<uint64_t>(tile) * (kN * kNt) + kN * t + m) * a.rank + k);
+                        v[u][t][c][0] = p[0];
+                        v[u][t][c][1] = p[1];
+                    }
+                }
+#pragma unroll
+        for (uint32_t u = 0; u < kU; u++) {
+            if (s + u >= a.splits) break;
+#pragma unroll
+            for (int t = 0; t < kNt; t++)
+#pragma unroll
+                for (int c = 0; c < kKt; c++) {
+                    sum[t][c][0] += v[u][t][c][0];
+                    sum[t][c][1] += v[u][t][c][1];
+                }
+        }
+    }
 #pragma unroll
     for (int t = 0; t < kNt; t++)
 #pragma unroll
         for (int c = 0; c < kKt; c++) {
-            v4f lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
-            const uint32_t k = 32 * c + 8 * q;
-            if (mine.live(t) && k < r) {
-                const uint64_t step = static_cast<uint64_t>(a.tiles) * (kN * kNt) * a.rank;
-                const float* p = a.part + (static_cast<uint64_t>(tile) * (kN * kNt) + kN * t + m) * a.rank + k;
-                constexpr uint32_t kU = 4;  // splits in flight
-                for (uint32_t s = 0; s < a.splits; s += kU) {
-                    v4f v[kU][2];
-#pragma unroll
-                    for (uint32_t u = 0; u < kU; u++) {
-                        const v4f* at = reinterpret_cast<const v4f*>(p + min(s + u, a.splits - 1) * step);
-                        v[u][0] = at[0];
-                        v[u][1] = at[1];
-                    }
-#pragma unroll
-                    for (uint32_t u = 0; u < kU; u++)
-                        if (s + u < a.splits) {
-                            lo += v[u][0];
-                            hi += v[u][1];
-                        }
-                }
-            }
+            const v4f lo = sum[t][c][0], hi = sum[t][c][1];
             float h[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 #pragma unroll
-            for (int i = 0; i < 8; i++) h[i] = k + i < r ? h[i] : 0.0f;
+            for (int i = 0; i < 8; i++) h[i] = 32 * (c0 + c) + 8 * q + i < r ? h[i] : 0.0f;
             to_parts(h, hp[t][c]);
         }
 }
 
-// Sixteen rows of an adapter's B, rows n + m: the lane's eights of the rank.
+// Sixteen rows of an adapter's B, rows n + m: the lane's eights of runs c0 and on of the rank.
 template <class W, int kKt>
-__device__ __forceinline__ void load_b(const Args& a, const uint8_t* b, uint32_t n, uint32_t r, v4u (&w)[kKt][W::kVecs]) {
+__device__ __forceinline__ void load_b(const Args& a, const uint8_t* b, uint32_t n, uint32_t r, uint32_t c0, v4u (&w)[kKt][W::kVecs]) {
     const uint32_t m = threadIdx.x & 15, q = (threadIdx.x & (kWave - 1)) >> 4;
-    const uint8_t* p = b + (static_cast<uint64_t>(min(n + m, a.rows - 1)) * a.rank + 8 * q) * W::kBytes;
+    const uint8_t* p = b + (static_cast<uint64_t>(min(n + m, a.rows - 1)) * a.rank + 32 * c0 + 8 * q) * W::kBytes;
 #pragma unroll
     for (int c = 0; c < kKt; c++) {
 #pragma unroll
         for (int i = 0; i < W::kVecs; i++) w[c][i] = v4u{0, 0, 0, 0};
-        if (32 * c + 8 * q < r) load<W>(p + 32 * c * W::kBytes, w[c]);
+        if (32 * (c0 + c) + 8 * q < r) load<W>(p + 32 * c * W::kBytes, w[c]);
     }
 }
 
-// Their products with h.
+// Their products with h, added.
 template <class W, int kKt, int kNt>
-__device__ __forceinline__ void multiply_b(uint32_t r, v4u (&w)[kKt][W::kVecs], const v8b (&hp)[kNt][kKt][3], v4f (&acc)[kNt]) {
+__device__ __forceinline__ void multiply_b(uint32_t r, uint32_t c0, v4u (&w)[kKt][W::kVecs], const v8b (&hp)[kNt][kKt][3], v4f (&acc)[kNt]) {
     const uint32_t q = (threadIdx.x & (kWave - 1)) >> 4;
 #pragma unroll
-    for (int t = 0; t < kNt; t++) acc[t] = v4f{0, 0, 0, 0};
-#pragma unroll
     for (int c = 0; c < kKt; c++) {
-        if (32u * c >= r) break;
-        if (32u * c + 32 > r) {  // weights behind the adapter's rank: there, but not its own
+        if (32 * (c0 + c) >= r) break;
+        if (32 * (c0 + c) + 32 > r) {  // weights behind the adapter's rank: there, but not its own
 #pragma unroll
             for (int i = 0; i < 4 * W::kVecs; i++) {
-                const uint32_t per = 4 / W::kBytes, first = 32 * c + 8 * q + i * per;
+                const uint32_t per = 4 / W::kBytes, first = 32 * (c0 + c) + 8 * q + i * per;
                 uint32_t keep = first < r ? ~0u : 0u;
                 if (per == 2 && first + 1 >= r) keep &= 0xffffu;
                 w[c][i / 4][i % 4] &= keep;
@@ -462,7 +476,7 @@ __device__ __forceinline__ void up_few(const Args& a) {
     const auto load_rows = [&](uint32_t n) {
         const uint32_t col = n + 4 * q;  // and 16 on
 #pragma unroll
-        for (int e = 0; e < 2; e++) load_b<W, kKt>(a, b, n + 16 * e, r, w[e]);
+        for (int e = 0; e < 2; e++) load_b<W, kKt>(a, b, n + 16 * e, r, 0, w[e]);
         was[0] = was[1] = v4f{0, 0, 0, 0};
         if (!a.res || !live) return;
         const float* p = a.res + at + col;
@@ -479,11 +493,11 @@ __device__ __forceinline__ void up_few(const Args& a) {
     };
     load_rows(n0);
     v8b hp[1][kKt][3];
-    load_h(a, mine, tile, r, hp);
+    load_h(a, mine, tile, 0, hp);
     for (uint32_t n = n0; n < n1; n += 32) {
-        v4f acc[2][1];
+        v4f acc[2][1] = {{v4f{0, 0, 0, 0}}, {v4f{0, 0, 0, 0}}};
 #pragma unroll
-        for (int e = 0; e < 2; e++) multiply_b<W>(r, w[e], hp, acc[e]);
+        for (int e = 0; e < 2; e++) multiply_b<W>(r, 0, w[e], hp, acc[e]);
         v4f o[2];
 #pragma unroll
         for (int e = 0; e < 2; e++)
@@ -510,7 +524,9 @@ __device__ __forceinline__ void up_few(const Args& a) {
 // writes 512 bytes of a row at a time (64 bytes, straight from the matrix instruction: 150 us
 // for 5000 tokens of 12288 rows, rank 64; so 122, of which 100 without the products; a plain
 // copy of y 80).  A wave: a tile of 32 tokens (by 16, which read B twice as often: 141) and 128
-// rows of y at a time; a workgroup's waves have neighbouring tiles and the same rows of B.
+// rows of y at a time; a workgroup's waves have neighbouring tiles and the same rows of B.  A
+// rank past 32 kKt goes in several passes over the span, whose sums wait in LDS: with all of
+// its h in registers a rank of 256 took 133 us for 2048 tokens of 4096 rows.
 constexpr uint32_t kSpan = 128, kPitch = kSpan + 4;  // (a row of LDS begins 16 bytes past the one before's banks)
 
 template <class W, int kKt>
@@ -532,7 +548,8 @@ __device__ __forceinline__ void up_many(const Args& a) {
                        (with ? static_cast<uint64_t>(mine.adapter) * a.rows * a.rank * W::kBytes : 0);
     float* const mem = rows[wid];
     // matrix tiles of B in flight, and pairs of rows of res
-    constexpr uint32_t kAhead = kKt * W::kVecs <= 2 ? 4 : 2, kPairs = 8;
+    constexpr uint32_t kAhead = kKt * W::kVecs <= 2 ? 4 : 2, kPairs = 8, kTiles = kSpan / 16;
+    const uint32_t passes = max((r + 32 * kKt - 1) / (32 * kKt), 1u);
     v4u w[kAhead][kKt][W::kVecs];
     const uint32_t half = lane >> 5, col0 = 4 * (lane & 31);  // two tokens an instruction
     v4f was[kPairs];
@@ -556,21 +573,32 @@ __device__ __forceinline__ void up_many(const Args& a) {
         }
     };
 #pragma unroll
-    for (uint32_t i = 0; i < kAhead; i++) load_b<W, kKt>(a, b, n0 + 16 * i, r, w[i]);
+    for (uint32_t i = 0; i < kAhead; i++) load_b<W, kKt>(a, b, n0 + 16 * i, r, 0, w[i]);
     load_res(0, n0, min(kSpan, n1 - n0));
     v8b hp[kNt][kKt][3];
-    load_h(a, mine, tile, r, hp);
     for (uint32_t n = n0; n < n1; n += kSpan) {
         const uint32_t span = min(kSpan, n1 - n);
-        for (uint32_t e0 = 0; e0 < kSpan / 16; e0 += kAhead) {
+        for (uint32_t pass = 0; pass < passes; pass++) {
+            const uint32_t c0 = kKt * pass;
+            if (passes > 1 || n == n0) load_h(a, mine, tile, c0, hp);
+            const bool last = pass + 1 == passes;
+            for (uint32_t e0 = 0; e0 < kTiles; e0 += kAhead) {
 #pragma unroll
-            for (uint32_t i = 0; i < kAhead; i++) {
-                const uint32_t e = e0 + i;
-                v4f acc[kNt];
-                multiply_b<W>(r, w[i], hp, acc);
-                load_b<W, kKt>(a, b, n + 16 * (e + kAhead), r, w[i]);
+                for (uint32_t i = 0; i < kAhead; i++) {
+                    const uint32_t e = e0 + i;
+                    v4f acc[kNt];
 #pragma unroll
-                for (int t = 0; t < kNt; t++) *reinterpret_cast<v4f*>(mem + (kN * t + m) * kPitch + 16 * e + 4 * q) = acc[t];
+                    for (int t = 0; t < kNt; t++) {
+                        acc[t] = v4f{0, 0, 0, 0};
+                        if (pass) acc[t] = *reinterpret_cast<const v4f*>(mem + (kN * t + m) * kPitch + 16 * e + 4 * q);
+                    }
+                    multiply_b<W>(r, c0, w[i], hp, acc);
+                    // the next: of this run of the rank, or the next one's first
+                    const bool on = e + kAhead < kTiles;
+                    load_b<W, kKt>(a, b, (on || !last ? n : n + kSpan) + 16 * (on ? e + kAhead : i), r, on ? c0 : last ? 0 : c0 + kKt, w[i]);
+#pragma unroll
+                    for (int t = 0; t < kNt; t++) *reinterpret_cast<v4f*>(mem + (kN * t + m) * kPitch + 16 * e + 4 * q) = acc[t];
+                }
             }
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // a wave's own: no barrier
@@ -606,23 +634,25 @@ extern "C" __global__ void __launch_bounds__(1024) zlm_lora_group(Args a) { grou
     extern "C" __global__ void __launch_bounds__(64 * zlm::kLoraWaves[kNt - 1]) zlm_lora_down_##NAME##_##kMt##S(Args a) { \
         down<W, kMt, kNt>(a);                                                                                     \
     }
-#define ZLM_LORA_UP(NAME, W, kKt, S, kNt)                                                                         \
-    extern "C" __global__ void __launch_bounds__(256) zlm_lora_up_##NAME##_##kKt##S(Args a) {             \
-        if constexpr (kNt == 1) up_few<W, kKt>(a);                                                                \
-        else up_many<W, kKt>(a);                                                                                  \
-    }
-#define ZLM_LORA(NAME, W, S, kNt)                                                                                 \
-    ZLM_LORA_DOWN(NAME, W, 1, S, kNt)                                                                             \
-    ZLM_LORA_DOWN(NAME, W, 2, S, kNt)                                                                             \
-    ZLM_LORA_DOWN(NAME, W, 4, S, kNt)                                                                             \
-    ZLM_LORA_DOWN(NAME, W, 8, S, kNt)                                                                             \
-    ZLM_LORA_UP(NAME, W, 1, S, kNt)                                                                               \
-    ZLM_LORA_UP(NAME, W, 2, S, kNt)                                                                               \
-    ZLM_LORA_UP(NAME, W, 4, S, kNt)                                                                               \
-    ZLM_LORA_UP(NAME, W, 8, S, kNt)
-ZLM_LORA(bf16, Bf16, , 2)
-ZLM_LORA(f16, F16, , 2)
-ZLM_LORA(f32, F32, , 2)
-ZLM_LORA(bf16, Bf16, _small, 1)
-ZLM_LORA(f16, F16, _small, 1)
-ZLM_LORA(f32, F32, _small, 1)
+#define ZLM_LORA_UP_FEW(NAME, W, kKt)                                                                             \
+    extern "C" __global__ void __launch_bounds__(256) zlm_lora_up_##NAME##_##kKt##_small(Args a) { up_few<W, kKt>(a); }
+#define ZLM_LORA_UP_MANY(NAME, W, kKt)                                                                            \
+    extern "C" __global__ void __launch_bounds__(256, 2) zlm_lora_up_##NAME##_##kKt(Args a) { up_many<W, kKt>(a); }
+#define ZLM_LORA(NAME, W)                                                                                         \
+    ZLM_LORA_DOWN(NAME, W, 1, , 2)                                                                                \
+    ZLM_LORA_DOWN(NAME, W, 2, , 2)                                                                                \
+    ZLM_LORA_DOWN(NAME, W, 4, , 2)                                                                                \
+    ZLM_LORA_DOWN(NAME, W, 8, , 2)                                                                                \
+    ZLM_LORA_DOWN(NAME, W, 1, _small, 1)                                                                          \
+    ZLM_LORA_DOWN(NAME, W, 2, _small, 1)                                                                          \
+    ZLM_LORA_DOWN(NAME, W, 4, _small, 1)                                                                          \
+    ZLM_LORA_DOWN(NAME, W, 8, _small, 1)                                                                          \
+    ZLM_LORA_UP_MANY(NAME, W, 1)                                                                                  \
+    ZLM_LORA_UP_MANY(NAME, W, 2)                                                                                  \
+    ZLM_LORA_UP_FEW(NAME, W, 1)                                                                                   \
+    ZLM_LORA_UP_FEW(NAME, W, 2)                                                                                   \
+    ZLM_LORA_UP_FEW(NAME, W, 4)                                                                                   \
+    ZLM_LORA_UP_FEW(NAME, W, 8)
+ZLM_LORA(bf16, Bf16)
+ZLM_LORA(f16, F16)
+ZLM_LORA(f32, F32)
