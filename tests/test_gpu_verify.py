@@ -245,6 +245,17 @@ def test_equal_weights(box):
     assert list(accepted) == [0] and list(token) == [32, -1]
 
 
+@pytest.mark.parametrize("how", [dict(k=7000), dict(p=0.3), dict(k=9000, p=0.5, mp=0.99), dict(mp=1.0)])
+def test_cuts_among_more_tokens_than_are_listed(box, how):
+    """Thousands of equal logits, or of nearly equal ones: more tokens in question than a workgroup lists."""
+    rng = np.random.default_rng(8)
+    for vocab in (12000, 30000):
+        for by_logits in (True, False):
+            c = make(rng, [3, 2], vocab, std=1e-3, near=0.5, by_logits=by_logits, how=how, draft_how=how)
+            c.target[0], c.target[3] = 1.5, 0.0
+            c.check(*c.run(box))
+
+
 @pytest.mark.parametrize("n", [64, 65, 130, 300])
 def test_many_drafts(box, n):
     rng = np.random.default_rng(n)

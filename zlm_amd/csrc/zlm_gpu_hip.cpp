@@ -3173,6 +3173,12 @@ extern "C" bool zlm_gpu_paged_read_enqueue(zlm_device* d, const zlm_paged_cache*
     a.k_out = k_out;
     a.v_out = v_out;
     void* args[] = {&a};
+    // e4m3: a wave a row, 1024 dims of it in turn while rows are few
+    if (cache->type == ZLM_CACHE_E4M3) {
+        const uint64_t blocks = (batch->n_tokens + 3) / 4, fill = (8ull * d->cus + blocks - 1) / blocks;
+        const uint64_t steps = (static_cast<uint64_t>(cache->n_kv_heads) * cache->head_dim + 1023) / 1024;
+        return launch3(d, k->read, static_cast<unsigned>(blocks), static_cast<unsigned>(std::min(steps, fill)), 1, 256, args, "paged read");
+    }
     // a head a wave while rows are few, as in the append; all of a row's in one workgroup
     // where rows fill the CUs
     const uint64_t fill = (8ull * d->cus + batch->n_tokens - 1) / batch->n_tokens;

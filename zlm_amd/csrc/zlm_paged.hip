@@ -214,7 +214,7 @@ __device__ __forceinline__ uint32_t quantise(T x, uint32_t lane, _Float16* d_out
 // rows in this call (and, where they begin inside it, the scale that it has: a scale
 // never falls, and where it rises the codes before them are rounded again, which changes
 // none but those that become subnormal).  The rows' workgroups take the heads' K and V in
-// turn.  K's rotation goes from row to row by the turn of one position, 16 at most: a
+// turn.  K's rotation goes from row to row by the turn of one position, 30 at most: a
 // sine and cosine a row would be most of the call.
 // 2^-k x is exact in 32 bits, so a 64-bit K is taken to them with its last bit set where
 // that is not exact: every comparison and rounding below then sees the right side.
@@ -249,17 +249,29 @@ __device__ __forceinline__ float wave_most(float v) {
     return __builtin_fmaxf(__builtin_bit_cast(float, a0), __builtin_bit_cast(float, a1));
 }
 
+// The rows of this call in row t's block.
+struct Block {
+    int32_t start;        // the first one's position
+    uint32_t mine, rows;  // t's place among them, their number
+};
+__device__ __forceinline__ Block block_of(const RowAt& at, uint32_t t) {
+    Block b;
+    b.start = max(at.pos & ~15, at.first);
+    b.mine = static_cast<uint32_t>(at.pos - b.start);
+    b.rows = __builtin_amdgcn_readfirstlane(min(16u - (static_cast<uint32_t>(b.start) & 15), static_cast<uint32_t>(at.row1) - (t - b.mine)));
+    return b;
+}
+
 template <int HD>
 __device__ __forceinline__ void append_blocks(const AppendArgs& a, const RowAt& at, uint32_t t, uint32_t id, uint32_t wave,
-                                              uint32_t waves, const double (&turns)[6][HD / 2], const float (&wk)[HD / 64]) {
+                                              uint32_t waves, const double (&turns)[4][HD / 2], const float (&wk)[HD / 64]) {
     const Paged& p = a.p;
     constexpr int N = HD / 64, kRows = 16;
     constexpr float kMost = 57344.0f;  // 448 at the largest scale
     const uint32_t lane = threadIdx.x & (kWave - 1), page = 1u << p.page_shift;
-    const int32_t start = max(at.pos & ~15, at.first);
-    const uint32_t j0 = static_cast<uint32_t>(start) & 15, mine = static_cast<uint32_t>(at.pos - start), t0 = t - mine;
-    const uint32_t n_rows = __builtin_amdgcn_readfirstlane(min(16u - j0, static_cast<uint32_t>(at.row1) - t0));
-    const uint32_t blk = (static_cast<uint32_t>(start) & (page - 1)) / 16;
+    const Block in = block_of(at, t);
+    const uint32_t j0 = static_cast<uint32_t>(in.start) & 15, mine = in.mine, t0 = t - mine, n_rows = in.rows;
+    const uint32_t blk = (static_cast<uint32_t>(in.start) & (page - 1)) / 16;
     for (uint32_t task = mine + n_rows * wave; task < 2 * p.n_kv; task += n_rows * waves) {
         const bool is_k = task < p.n_kv;
         const uint32_t head = is_k ? task : task - p.n_kv;
@@ -285,10 +297,18 @@ __device__ __forceinline__ void append_blocks(const AppendArgs& a, const RowAt& 
 #pragma unroll
             for (int j = 0; j < N; j++) {
                 const uint32_t i = (lane + 64 * j) % (HD / 2);
-                cs[j] = turns[2][i];
-                sn[j] = turns[3][i];
-                c1[j] = turns[4][i];
-                s1[j] = turns[5][i];
+                cs[j] = turns[0][i];
+                sn[j] = turns[1][i];
+                c1[j] = n_rows > 1 ? turns[2][i] : 1.0;
+                s1[j] = n_rows > 1 ? turns[3][i] : 0.0;
+            }
+            for (uint32_t i = 0; i < mine; i++) {  // from this row's turn back to the first's
+#pragma unroll
+                for (int j = 0; j < N; j++) {
+                    const double c = cs[j];
+                    cs[j] = c * c1[j] + sn[j] * s1[j];
+                    sn[j] = sn[j] * c1[j] - c * s1[j];
+                }
             }
 #pragma unroll
             for (int r0 = 0; r0 < kRows; r0 += 4) {
@@ -444,13 +464,15 @@ __device__ __forceinline__ void append(const AppendArgs& a) {
     const Paged& p = a.p;
     constexpr int N = HD / 64;  // dims a lane
     constexpr uint32_t kH = 4;  // heads a step, at most
-    __shared__ double turns[C == kE8 ? 6 : 2][HD / 2];
+    __shared__ double turns[C == kE8 ? 4 : 2][HD / 2];
     const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1);
     const uint32_t t = blockIdx.x;
     const uint32_t waves = gridDim.y * 4, wave = __builtin_amdgcn_readfirstlane(blockIdx.y * 4 + tid / kWave);
     const uint32_t heads = C == kE8 ? a.n_heads : a.n_heads + p.n_kv;  // kE8: K goes by blocks, below
     const float* row = a.qkv + t * a.stride + lane;
-    uint32_t h = a.per * wave;
+    // kE8: where heads go four at a time the last wave has a block's K or V alone
+    const uint32_t of_heads = C == kE8 && a.per > 1 ? waves - 1 : waves;
+    uint32_t h = C == kE8 && wave >= of_heads ? heads : a.per * wave;
     // the next heads' values, on their way while these are worked on; past the last head its own
     float next[kH][N], wq[N], wk[N];
     const auto load = [&](uint32_t h0) {
@@ -472,11 +494,12 @@ __device__ __forceinline__ void append(const AppendArgs& a) {
     const int32_t pos = at.pos;
     const uint32_t page = 1u << p.page_shift;
     const int32_t id = __builtin_amdgcn_readfirstlane(page_of(p, s, pos));
-    if constexpr (C == kE8) {  // of the block's first row too, and of one position
-        for (uint32_t i = tid; i < 3 * HD / 2; i += 256) {
+    if constexpr (C == kE8) {
+        // of one position too, where the workgroup turns several of K's rows
+        const bool steps = pos >= 0 && block_of(at, t).mine < p.n_kv && block_of(at, t).rows > 1;
+        for (uint32_t i = tid; i < (steps ? HD : HD / 2); i += 256) {
             const uint32_t j = i % (HD / 2), which = i / (HD / 2);
-            const double of = which == 0 ? pos : which == 1 ? max(pos & ~15, at.first) : 1;
-            const double turn = of * exp(a.log_base * (static_cast<double>(j) * (-2.0 / HD)));
+            const double turn = (which ? 1.0 : static_cast<double>(pos)) * exp(a.log_base * (static_cast<double>(j) * (-2.0 / HD)));
             sincos(turn, &turns[2 * which + 1][j], &turns[2 * which][j]);
         }
     } else if (tid < HD / 2) {
@@ -490,13 +513,13 @@ __device__ __forceinline__ void append(const AppendArgs& a) {
         cs[j] = turns[0][(lane + 64 * j) % (HD / 2)];
         sn[j] = turns[1][(lane + 64 * j) % (HD / 2)];
     }
-    for (; h < heads; h += a.per * waves) {
+    for (; h < heads; h += a.per * of_heads) {
         double x[kH][N], inv = 1.0;
 #pragma unroll
         for (uint32_t i = 0; i < kH; i++)
 #pragma unroll
             for (int j = 0; j < N; j++) x[i][j] = next[i][j];
-        load(h + a.per * waves);
+        load(h + a.per * of_heads);
         if (norm) {
             double ss[kH];
 #pragma unroll
@@ -635,10 +658,6 @@ __device__ __forceinline__ void read_rows(const ReadArgs& a) {
                 if constexpr (C == kF16) {
                     k[i][j] = static_cast<float>(reinterpret_cast<const _Float16*>(kb)[off * HD + dim]);
                     v[i][j] = static_cast<float>(reinterpret_cast<const _Float16*>(vb)[(grp * HD + dim) * 8 + in]);
-                } else if constexpr (C == kE8) {
-                    const float dk = e8_scale(kb[page * HD + off / 16]), dv = e8_scale(vb[page * HD + off / 16]);
-                    k[i][j] = __builtin_amdgcn_cvt_f32_fp8(kb[off * HD + dim], 0) * dk;
-                    v[i][j] = __builtin_amdgcn_cvt_f32_fp8(vb[(grp * HD + dim) * 8 + in], 0) * dv;
                 } else {
                     const uint32_t b = kb[off * (HD / 2) + dim / 32 * 16 + (dim & 15)];
                     const float dk = reinterpret_cast<const _Float16*>(kb + page * (HD / 2))[off * (HD / 32) + dim / 32];
@@ -660,6 +679,55 @@ __device__ __forceinline__ void read_rows(const ReadArgs& a) {
                 a.k_out[o + 64 * j] = k[i][j];
                 a.v_out[o + 64 * j] = v[i][j];
             }
+        }
+    }
+}
+
+// An e4m3 cache's: a wave a row, a lane four dims in a row of it, kTurns at a time (V's come
+// as the 8 positions of their group).  All of a wave's loads are in flight at once: by a
+// workgroup a row, a byte a load, 7270 rows of 8 heads of 128 took 24 us, and 17 so.
+template <int HD>
+__device__ __forceinline__ void read_e8(const ReadArgs& a) {
+    const Paged& p = a.p;
+    constexpr uint32_t kTurns = 4, kDims = 4 * kWave * kTurns;  // dims a step
+    const uint32_t lane = threadIdx.x & (kWave - 1), t = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + threadIdx.x / kWave);
+    if (t >= p.n_tokens) return;
+    RowAt at;
+    if (!row_at(p, t, lane, at)) return;
+    const int32_t pos = at.pos, id = page_of(p, at.s, pos);
+    const uint32_t page = 1u << p.page_shift, off = static_cast<uint32_t>(pos) & (page - 1), grp = off >> 3, in = off & 7;
+    const uint32_t dims = p.n_kv * HD;
+    const float none = pos < 0 ? 0.0f : __builtin_nanf("");
+    for (uint32_t d0 = blockIdx.y * kDims + 4 * lane; d0 < dims; d0 += gridDim.y * kDims) {
+        uint32_t kw[kTurns], ks[kTurns], vs[kTurns];
+        v4u vw[kTurns][2];
+#pragma unroll
+        for (uint32_t i = 0; i < kTurns; i++) {
+            const uint32_t d = min(d0 + 4 * kWave * i, dims - 4), h = d / HD, dim = d % HD;
+            const size_t base = head_base<HD, kE8>(p, max(id, 0), h);
+            kw[i] = *reinterpret_cast<const uint32_t*>(p.k + base + off * HD + dim);
+            vw[i][0] = reinterpret_cast<const v4u*>(p.v + base + (grp * HD + dim) * 8)[0];
+            vw[i][1] = reinterpret_cast<const v4u*>(p.v + base + (grp * HD + dim) * 8)[1];
+            ks[i] = p.k[base + page * HD + off / 16];
+            vs[i] = p.v[base + page * HD + off / 16];
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kTurns; i++) {
+            const uint32_t d = d0 + 4 * kWave * i;
+            if (d >= dims) break;
+            const float dk = e8_scale(ks[i]), dv = e8_scale(vs[i]);
+            v4f k, v;
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++) {
+                const uint32_t byte = kw[i] >> (8 * e), lo = vw[i][e / 2][e % 2 * 2], hi = vw[i][e / 2][e % 2 * 2 + 1];
+                k[e] = id < 0 ? none : __builtin_amdgcn_cvt_f32_fp8(byte, 0) * dk;
+                v[e] = id < 0 ? none : __builtin_amdgcn_cvt_f32_fp8((in & 4 ? hi : lo) >> (8 * (in & 3)), 0) * dv;
+            }
+            // (rows of k_out and v_out may begin at any float)
+            const size_t o = static_cast<size_t>(t) * dims + d;
+            typedef float v4a __attribute__((ext_vector_type(4), aligned(4)));
+            *reinterpret_cast<v4a*>(a.k_out + o) = k;
+            *reinterpret_cast<v4a*>(a.v_out + o) = v;
         }
     }
 }
@@ -2061,7 +2129,8 @@ __device__ __forceinline__ void merge_many(const AttnArgs& a) {
         append<HD, C>(a);                                                                                         \
     }                                                                                                             \
     extern "C" __global__ void __launch_bounds__(256) zlm_paged_read_##NAME##_##HD(ReadArgs a) {                  \
-        read_rows<HD, C>(a);                                                                                      \
+        if constexpr (C == kE8) read_e8<HD>(a);                                                                   \
+        else read_rows<HD, C>(a);                                                                                 \
     }
 #define ZLM_PAGED(NAME, C)                                                                                        \
     ZLM_PAGED_ROWS(64, NAME, C)                                                                                   \
