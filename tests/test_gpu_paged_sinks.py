@@ -73,6 +73,36 @@ def test_window_beside_sinks(box, kind, hd, page, kv, group, case):
     assert (off <= bound).all(), (off.max(), bound[off.argmax()], int(off.argmax()))
 
 
+# windows that the few-row kernel does not take alone: positions split over workgroups and joined
+MANY = [([(150, 1700), (1, 3), (40, 1500)], 1100, 17), ([(140, 1400)], 1200, 64), ([(170, 1450), (3, 20)], 1064, 200),
+        ([(130, 2000)], 1500, 1)]
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("hd,page,kv,group", [(128, 64, 1, 4), (64, 16, 2, 4), (256, 32, 1, 3)])
+@pytest.mark.parametrize("case", range(len(MANY)))
+def test_many_rows(box, kind, hd, page, kv, group, case):
+    lens, window, sinks = MANY[case]
+    _say(f"sinks many kind={kind} hd={hd} page={page} case={case}")
+    rng = np.random.default_rng(case + hd)
+    heads = kv * group
+    b = paged.Batch(lens, page, rng, behind=1)
+    pool = paged_more.pool(kind, kv, hd, page, b.n_pages)
+    paged_more.fill(pool, b, rng)
+    _hide(b, window, sinks)
+    q = (1.5 * rng.standard_normal((b.n_tokens, heads, hd))).astype(np.float32)
+    assert box.dev.launch_log(True)
+    got = _run(box, b, pool, q, heads, hd ** -0.5, window, sinks)
+    assert "paged attention of many rows, merge" in [r["what"] for r in box.dev.launch_log_read()]
+    box.dev.launch_log(False)
+    assert (got[-1] == 7).all()
+    last = b.n_tokens - 1
+    rows = sorted({0, 1, 15, 16, 31, 32, 63, 64, 127, 128, lens[0][0] - 1, last - 1} & set(range(last)))
+    want, bound = paged_more.attend(pool, _Some(b, rows), q, heads, hd ** -0.5, window, sinks)
+    assert (np.abs(got[rows] - want[rows]).max((1, 2)) <= bound[rows]).all()
+    assert np.isfinite(got).all()
+
+
 @pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("hd,group,lens,window,sinks", [
     (256, 2, [(1100, 2300), (1, 900)], 130, 40), (256, 2, [(520, 3000)], 700, 64), (128, 4, [(2100, 2400), (3, 700)], 300, 4),

@@ -65,6 +65,26 @@ def test_what_sinks_refuse(box, kind):
     assert d.launch_log_read() == []
 
 
+@pytest.mark.parametrize("kind", [zd.F16, zd.Q4_0, E4M3])
+def test_which_kernels_take_sinks(box, kind):
+    """The few-row kernel alone while its items are no more than its workgroups and windows short."""
+    d, p, c = box.dev, 1 << 16, _cache(box.mod, type=kind, kv=8)
+
+    def whats(tokens, seqs, **how):
+        d.launch_log(True)
+        assert d.paged_attention_enqueue(c, _batch(box.mod, seqs=seqs, tokens=tokens, stride=200), p, p, 32, 0.1, **how), \
+            d.last_error()
+        return [r["what"] for r in d.launch_log_read()]
+
+    few, many = "paged attention", "paged attention of many rows"
+    assert whats(256, 1, window=1000, sinks=100) == [few]
+    assert whats(256, 4, window=64, sinks=4) == [few]
+    assert many in whats(256, 1, window=1000, sinks=101)
+    assert many in whats(257, 1, window=64, sinks=4)
+    assert many in whats(256, 1, window=64)
+    assert whats(4, 4, window=5000, sinks=4) == [few]
+
+
 def test_sinks_take_the_scratch_that_the_attention_has(box):
     d, p, b, c = box.dev, 1 << 16, _batch(box.mod), _cache(box.mod, type=E4M3)
     assert d.capture_begin()

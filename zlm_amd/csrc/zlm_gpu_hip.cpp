@@ -3228,7 +3228,13 @@ bool paged_attention(zlm_device* d, const zlm_paged_cache* cache, const zlm_page
     // 156, 248 and 266, 126, 178, 247 and 250; 16 with one of 200, 300 or 450 63, 82 and 112,
     // 74, 94 and 107; f16, 32 of 5 95 and 103, 64 of 5 181 and 185, with one of 257 220 and 327.
     const uint64_t enough = std::max<uint64_t>(512, 64 * std::min<uint64_t>(batch->n_seqs, 64));
-    const bool many = batch->n_tokens > batch->n_seqs && rows > std::min<uint64_t>(static_cast<uint64_t>(batch->n_seqs) * few_rows, enough);
+    // With sinks, windows say how little a row sees: where the few-row kernel has no more items
+    // of 16 rows than workgroups, it alone is the faster (windows of 64, 256 and 1024, 4
+    // sinks: 256 tokens of 32 q and 8 kv heads of 128, e4m3 14, 16 and 23 us, both kernels 28, 33
+    // and 37, f16 15, 19 and 32, 27, 32 and 36; 1024 tokens 41, 54 and 82, 36, 44 and 63).
+    const bool shallow = window && sinks && static_cast<uint64_t>(window) + sinks <= 1100 &&
+                         (rows + 15) / 16 * cache->n_kv_heads <= 2ull * d->cus;
+    const bool many = !shallow && batch->n_tokens > batch->n_seqs && rows > std::min<uint64_t>(static_cast<uint64_t>(batch->n_seqs) * few_rows, enough);
     const bool few = !many || batch->n_seqs > 1;
     // Equal shares of the few-row kernel for the workgroups that the CUs hold at once: one
     // of heads of 256 (two rounds of them: 1 sequence of 32000 q4_0 positions 48 us, one
