@@ -75,6 +75,10 @@ struct Weight {
     __device__ __forceinline__ uint64_t operator()(double f) const {
         return __builtin_bit_cast(uint64_t, raised(f)) & 0xfffffffffffffull;
     }
+    // With a count of one above it: 2^52's exponent goes and 2^50 comes in one addition.
+    __device__ __forceinline__ uint64_t counted(double f) const {
+        return __builtin_bit_cast(uint64_t, raised(f)) + ((1ull << kCountShift) - (0x433ull << 52));
+    }
     __device__ __forceinline__ double units(double f) const { return raised(f) - 4503599627370496.0; }  // the integer itself
 
 private:
@@ -180,9 +184,11 @@ __device__ __forceinline__ void slice_hist(const Args& a, uint32_t row) {
     }
     float mx = -INFINITY;
 #pragma unroll
-    for (uint32_t j = 0; j < kHistPer; j++) {
-        x[j] = x[j] > 3.402823466e38f ? 3.402823466e38f : x[j];  // a NaN stays one: no comparison below holds for it
-        mx = __builtin_fmaxf(mx, x[j]);
+    for (uint32_t j = 0; j < kHistPer; j++) mx = __builtin_fmaxf(mx, x[j]);
+    if (__ballot(mx > 3.402823466e38f)) {  // a NaN stays one: no comparison below holds for it
+#pragma unroll
+        for (uint32_t j = 0; j < kHistPer; j++) x[j] = x[j] > 3.402823466e38f ? 3.402823466e38f : x[j];
+        mx = __builtin_fminf(mx, 3.402823466e38f);
     }
     const uint32_t wave_key = last_lane(wave_max(key_of(mx)));
     if (lane == 0) max_of[wid] = wave_key;
@@ -215,7 +221,7 @@ __device__ __forceinline__ void slice_hist(const Args& a, uint32_t row) {
     for (uint32_t j = 0; j < kHistPer; j++) {
         const double y = static_cast<double>(x[j]) * rate, b = __builtin_floor(y);
         const double d = top - b;
-        if (d < static_cast<double>(kBins)) atomicAdd(&hist[static_cast<uint32_t>(d)][tid % kCopies], (1ull << kCountShift) + weight(y - b));
+        if (d < static_cast<double>(kBins)) atomicAdd(&hist[static_cast<uint32_t>(d)][tid % kCopies], static_cast<unsigned long long>(weight.counted(y - b)));
     }
     __syncthreads();
     // the bins that the short list has room for: two a thread
