@@ -536,7 +536,7 @@ typedef struct {
  * [0, n_adapters) is none: y[t] = res[t].  x rows are x_stride floats apart (0: k), 16-byte
  * aligned; res and y rows y_stride (0: rows), so that y may be a part of the rows of a packed
  * product.  res: may be y (rows without an adapter are left alone then), or null for 0; else
- * it lies apart from y.  Products have the accuracy of 32-bit ones over the adapters'
+ * it lies apart from y, as x does.  Products have the accuracy of 32-bit ones over the adapters'
  * values, sums are 32-bit; an infinite or NaN x, or weight, makes NaN of what it reaches.  A
  * token's results depend on the other tokens of the call by how sums are split only.  Uses the
  * library scratch of zlm_gpu_paged_attention_enqueue (call once before its capture). */

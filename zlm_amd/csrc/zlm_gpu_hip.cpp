@@ -3039,12 +3039,13 @@ extern "C" bool zlm_gpu_attention_enqueue(zlm_device* d, const float* q, const u
     return enqueue_attn_merge(d, part, nsplit, n_heads, out);
 }
 
-// The scratch of the paged attention and the sampler, one buffer a device that the
-// first eager call of either makes.  Every launch of theirs fits it, so it is never
+// The scratch of the paged attention, the sampler, the verification of drafts and the
+// adapters, one buffer a device that the first eager call of any makes.  Every launch of theirs fits it, so it is never
 // replaced: captured graphs hold its address without a count of them.  The few-row
 // attention's partials take two items of 16 rows a workgroup (8.5 MB at 512 workgroups
 // and heads of 128), the many-row attention's as many splits as fit, and the
-// sampler's rows go through it in as many launches as they need.
+// sampler's and the verification's rows and the adapters' tokens go through it in as many
+// launches as they need.
 constexpr uint64_t kServingScratch = 64ull << 20;
 
 namespace {

@@ -12,7 +12,7 @@
 // 32-bit number is the sum of three bf16 (8 bits of its 24 each, cut off, so exactly), an
 // f16 of two, and a product is the sum of its parts' products without those below 2^-24 of
 // it: three instructions for a bf16 adapter, six for f16 and f32.  So the results have the
-// accuracy of 32-bit products at 10 and 5 times the rate of the 32-bit matrix instruction.
+// accuracy of 32-bit products at 5 and 2.7 times the rate of the 32-bit matrix instruction.
 // bf16 has the exponents of 32 bits: nothing is scaled.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
