@@ -130,6 +130,25 @@ def test_mixes(box, kind, tokens, mix):
     check(run(box, c, res=False), want, bound)
 
 
+@pytest.mark.parametrize("tokens", [65, 127, 192, 255, 256, 257])
+@pytest.mark.parametrize("mix", ["one", "most", "ends", "thirds", "each"])
+def test_tiles_at_the_borders(box, tokens, mix):
+    """Tokens that a workgroup groups by itself, and one more: tiles that end with the tokens or with an adapter's, of
+    pools as large as there are, adapters in any order."""
+    _say(f"lora borders tokens={tokens} mix={mix}")
+    rng = np.random.default_rng(tokens)
+    n, rank, rows, k = 4096, 8, 20, 64
+    t = np.arange(tokens)
+    adapter = {"one": t * 0 + n - 1, "most": np.where(t % 32 == 31, t, 5), "ends": np.array([0, n - 1, n, -1])[t % 4],
+               "thirds": np.where(t < 33, 2, np.where(t < 64, 1, 0)), "each": rng.permutation(n)[:tokens]}[mix]
+    c = Case(zd.F16, tokens, n, rank, rows, k, rng, adapter, rng.integers(0, rank + 1, n), rng.uniform(-2, 2, n))
+    want, bound = c.want()
+    got = run(box, c)
+    check(got, want, bound)
+    np.testing.assert_array_equal(run(box, c), got)
+    np.testing.assert_array_equal(run(box, c, in_place=True), got)
+
+
 @pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("tokens", [3, 100])
 def test_every_bit_of_a_number_counts(box, kind, tokens):
@@ -192,7 +211,7 @@ def test_rounds_of_the_scratch(box, kind):
 
 
 @pytest.mark.parametrize("rows,y_stride,at", [(100, 300, 8), (100, 301, 8), (99, 300, 8), (100, 300, 3), (64, 64, 0)])
-@pytest.mark.parametrize("tokens", [9, 200])
+@pytest.mark.parametrize("tokens", [9, 200, 300])
 def test_parts_of_wider_rows(box, rows, y_stride, at, tokens):
     """y as some columns of a packed product's rows, x as some of wider ones; what lies beside them stays."""
     k, x_stride, rank = 64, 100, 16
@@ -235,7 +254,7 @@ def test_what_is_not_a_number_stays_with_its_token(box):
     check(got[rest], want[rest], bound[rest])
 
 
-@pytest.mark.parametrize("tokens", [6, 150])
+@pytest.mark.parametrize("tokens", [6, 150, 400])
 def test_captured(box, tokens):
     """Two graphs over one scratch, replayed for other adapters, tokens and residuals, against eager calls."""
     dev = box.dev

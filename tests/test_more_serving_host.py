@@ -152,7 +152,10 @@ def test_other_arguments_of_adapters(box):
     assert d.lora_enqueue(lora, 64, p, p, p), d.last_error()
     assert [r["what"] for r in d.launch_log_read()] == ["adapters down", "adapters up"]
     d.launch_log(True)
-    assert d.lora_enqueue(lora, 65, p, p, p), d.last_error()
+    assert d.lora_enqueue(lora, 256, p, p, p), d.last_error()
+    assert [r["what"] for r in d.launch_log_read()] == ["adapters down", "adapters up"]
+    d.launch_log(True)
+    assert d.lora_enqueue(lora, 257, p, p, p), d.last_error()
     assert [r["what"] for r in d.launch_log_read()] == ["adapters, tokens grouped", "adapters down", "adapters up"]
 
 

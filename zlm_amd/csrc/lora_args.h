@@ -7,7 +7,7 @@ namespace zlm {
 
 constexpr uint32_t kLoraAdapters = 4096;  // of one pool (the grouping counts their tokens in LDS)
 constexpr uint32_t kLoraRank = 256;
-constexpr uint32_t kLoraSmall = 64;       // tokens that a wave groups by itself, in tiles of 16
+constexpr uint32_t kLoraSmall = 256;      // tokens that a workgroup groups by itself, in tiles of 16
 constexpr uint32_t kLoraTile = 32;        // tokens of a tile where there are more
 // Waves of the first product's workgroups, and runs of 32 of k that each has in flight (at
 // most), with tiles of 16 tokens and of 32.

@@ -3501,11 +3501,12 @@ extern "C" bool zlm_gpu_lora_enqueue(zlm_device* d, const zlm_lora* lora, uint32
         a.tile = reinterpret_cast<zlm::LoraTile*>(a.part + splits * a.tiles * tile_of(a.n_tokens) * lora->rank);
         a.order = reinterpret_cast<uint32_t*>(a.tile + a.tiles);
         a.n_tiles = a.order + a.n_tokens;
-        // rows of y a wave: few where tiles are few; else spans of 128, as many as leave the least
+        // rows of y a wave: few where tiles are few (eight waves a CU; with 16, 256 tokens of 40
+        // adapters of rank 64 30 us in place of 27, with four of 200 51 of 47); else spans of 128, as many as leave the least
         // work to the last round of two workgroups a CU (a span more stands for what a wave begins with)
         const uint64_t fours = (a.tiles + 3) / 4;
         a.wave_rows = small ? 256 : 128;
-        while (small && a.wave_rows > 32 && static_cast<uint64_t>(a.tiles) * lora->rows < 16ull * d->cus * a.wave_rows)
+        while (small && a.wave_rows > 32 && static_cast<uint64_t>(a.tiles) * lora->rows < 8ull * d->cus * a.wave_rows)
             a.wave_rows /= 2;
         const auto rounds = [&](uint64_t rows) {
             return ((lora->rows + rows - 1) / rows * fours + 2 * d->cus - 1) / (2 * d->cus) * (rows / 128 + 1);

@@ -4,7 +4,7 @@
 // Built as a device-only code object (hipcc --genco) and loaded by the host library.
 //
 // Tokens are taken in tiles with one adapter, so that a tile reads its A and B once.  Up to
-// 64 tokens every wave finds its tile, of up to 16, by itself; more are grouped by a launch
+// 256 tokens every workgroup finds its tile, of up to 16, by itself; more are grouped by a launch
 // before, in tiles of up to 32.  Then two launches: h = A x, k split over waves and workgroups, and
 // y = res + scale * B h.
 //
@@ -119,61 +119,127 @@ __device__ __forceinline__ uint32_t rank_of(const Args& a, uint32_t adapter) {
     return a.ranks ? min(static_cast<uint32_t>(max(a.ranks[adapter], 0)), a.rank) : a.rank;
 }
 
-// What the waves of a workgroup find their tile by, up to 64 tokens.
+// What a workgroup finds its tile by: a token of each adapter, and all of that token's
+// adapter's; the first of all tiles; its own.
+template <uint32_t kTokens>
 struct Grouping {
-    uint8_t one_of[zlm::kLoraAdapters + 2];  // a token of each adapter
-    unsigned long long with[kWave];          // all of its tokens
+    uint8_t one_of[zlm::kLoraAdapters + 2];
+    unsigned long long with[kTokens][kTokens / kWave], begins[kTokens / kWave];
+    uint32_t adapter, rank, from, n;
+    uint8_t member[kN];
 };
 
 // False: there are not so many tiles.  Tokens without an adapter make tiles of their own,
-// but where y is res.
-template <int kNt>
-__device__ __forceinline__ bool tile_of(const Args& a, uint32_t tile, Mine<kNt>& m) {
+// but where y is res.  Places and tiles follow the tokens' order, so that all workgroups of both
+// launches find the same.
+//
+// Up to 64 tokens, a wave: those of each lane's adapter, and its place among them; those at
+// 0, 16, 32 and 48 begin tiles.
+__device__ __forceinline__ bool few_tile(const Args& a, uint32_t tile, Mine<1>& m, Grouping<kWave>& sm) {
     const uint32_t lane = threadIdx.x & (kWave - 1), j = lane & (kN - 1);
-    if constexpr (kNt == 1) {
-        // the tokens of each lane's adapter, and its place among them; those at 0, 16, 32 and
-        // 48 begin tiles
-        __shared__ Grouping sm;
-        const bool has = lane < a.n_tokens;
-        const uint32_t own = has ? adapter_of(a, lane) : a.n_adapters + 1;
-        const uint32_t rank = rank_of(a, own);
-        if (threadIdx.x < kWave) {
-            sm.with[lane] = 0;
-            sm.one_of[own] = static_cast<uint8_t>(lane);
-        }
-        __syncthreads();
-        const uint32_t one = sm.one_of[own];
-        if (threadIdx.x < kWave) atomicOr(&sm.with[one], 1ull << lane);
-        __syncthreads();
-        const uint64_t mine = sm.with[one], below = (1ull << lane) - 1;
-        const uint32_t place = __builtin_popcountll(mine & below);
-        const bool left = has && !(a.in_place && own == a.n_adapters);
-        uint64_t begins = __ballot(left && place % kN == 0);
-        if (tile >= static_cast<uint32_t>(__builtin_popcountll(begins))) return false;
-        for (uint32_t i = 0; i < tile; i++) begins &= begins - 1;
-        const uint32_t first = __builtin_ctzll(begins);
-        m.adapter = __builtin_amdgcn_readlane(own, first);
-        m.rank = __builtin_amdgcn_readlane(rank, first);
-        const uint32_t from = __builtin_amdgcn_readlane(place, first);
-        uint64_t with = __ballot(own == m.adapter && place >= from && place < from + kN);
-        m.n = __builtin_popcountll(with);
-        m.token[0] = first;
-        for (uint32_t i = 0; i < m.n; i++) {
-            if (j == i) m.token[0] = __builtin_ctzll(with);
-            with &= with - 1;
-        }
-        return true;
-    } else {
-        static_assert(kN * kNt == zlm::kLoraTile, "as the tokens are grouped");
-        if (tile >= *a.n_tiles) return false;
-        const LoraTile t = a.tile[tile];
-        m.adapter = t.adapter;
-        m.rank = rank_of(a, t.adapter);
-        m.n = t.n;
-#pragma unroll
-        for (int i = 0; i < kNt; i++) m.token[i] = a.order[t.first + (m.live(i) ? kN * i + j : 0)];
-        return true;
+    const bool has = lane < a.n_tokens;
+    const uint32_t own = has ? adapter_of(a, lane) : a.n_adapters + 1;
+    const uint32_t rank = rank_of(a, own);
+    if (threadIdx.x < kWave) {
+        sm.with[lane][0] = 0;
+        sm.one_of[own] = static_cast<uint8_t>(lane);
     }
+    __syncthreads();
+    const uint32_t one = sm.one_of[own];
+    if (threadIdx.x < kWave) atomicOr(&sm.with[one][0], 1ull << lane);
+    __syncthreads();
+    const uint64_t mine = sm.with[one][0], below = (1ull << lane) - 1;
+    const uint32_t place = __builtin_popcountll(mine & below);
+    const bool left = has && !(a.in_place && own == a.n_adapters);
+    uint64_t begins = __ballot(left && place % kN == 0);
+    if (tile >= static_cast<uint32_t>(__builtin_popcountll(begins))) return false;
+    for (uint32_t i = 0; i < tile; i++) begins &= begins - 1;
+    const uint32_t first = __builtin_ctzll(begins);
+    m.adapter = __builtin_amdgcn_readlane(own, first);
+    m.rank = __builtin_amdgcn_readlane(rank, first);
+    const uint32_t from = __builtin_amdgcn_readlane(place, first);
+    uint64_t with = __ballot(own == m.adapter && place >= from && place < from + kN);
+    m.n = __builtin_popcountll(with);
+    m.token[0] = first;
+    for (uint32_t i = 0; i < m.n; i++) {
+        if (j == i) m.token[0] = __builtin_ctzll(with);
+        with &= with - 1;
+    }
+    return true;
+}
+
+// More, the first four waves: the same with a token a thread, the tile's members written
+// down by themselves.  k and rows 4096, bf16, by this and grouped by a launch in tiles of 32:
+// 65 tokens of 40 adapters of rank 16 12 and 18 us, of rank 256 63 and 65; 256 tokens of one
+// of rank 64 16 and 31, of 40 of rank 128 27 and 39, of 200 of rank 256 208 and 207.
+__device__ __forceinline__ bool small_tile(const Args& a, uint32_t tile, Mine<1>& m, Grouping<zlm::kLoraSmall>& sm) {
+    constexpr uint32_t kTokens = zlm::kLoraSmall, kWords = kTokens / kWave;
+    static_assert(kTokens <= 256, "a token in a byte, and a thread");
+    const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1), wid = tid / kWave;
+    const bool in = tid < kTokens, has = tid < a.n_tokens;
+    const uint32_t own = has ? adapter_of(a, tid) : a.n_adapters + 1;
+    const uint32_t rank = rank_of(a, own);
+    if (in) {
+#pragma unroll
+        for (uint32_t i = 0; i < kWords; i++) sm.with[tid][i] = 0;
+        sm.one_of[own] = static_cast<uint8_t>(tid);
+    }
+    if (tid == 0) sm.n = 0;
+    __syncthreads();
+    const uint32_t one = sm.one_of[own];
+    if (in) atomicOr(&sm.with[one][wid], 1ull << lane);
+    __syncthreads();
+    const uint64_t below = (1ull << lane) - 1;
+    uint32_t place = 0, all = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kWords; i++) {
+        const uint64_t with = sm.with[one][i];
+        place += __builtin_popcountll(i < wid ? with : i == wid ? with & below : 0);
+        all += __builtin_popcountll(with);
+    }
+    const bool begins = has && place % kN == 0 && !(a.in_place && own == a.n_adapters);
+    const uint64_t mine = __ballot(begins);
+    if (in && lane == 0) sm.begins[wid] = mine;
+    __syncthreads();
+    uint32_t index = __builtin_popcountll(mine & below);
+#pragma unroll
+    for (uint32_t i = 0; i < kWords; i++) index += i < wid ? __builtin_popcountll(sm.begins[i]) : 0;
+    if (begins && index == tile) {
+        sm.adapter = own;
+        sm.rank = rank;
+        sm.from = place;
+        sm.n = min(all - place, kN);
+    }
+    __syncthreads();
+    m.n = __builtin_amdgcn_readfirstlane(sm.n);
+    if (m.n == 0) return false;  // the workgroup as one
+    m.adapter = __builtin_amdgcn_readfirstlane(sm.adapter);
+    m.rank = __builtin_amdgcn_readfirstlane(sm.rank);
+    const uint32_t at = place - sm.from;
+    if (has && own == m.adapter && place >= sm.from && at < m.n) sm.member[at] = static_cast<uint8_t>(tid);
+    __syncthreads();
+    m.token[0] = sm.member[m.live(0) ? lane & (kN - 1) : 0];
+    return true;
+}
+
+__device__ __forceinline__ bool tile_of(const Args& a, uint32_t tile, Mine<1>& m) {
+    __shared__ union {
+        Grouping<kWave> few;
+        Grouping<zlm::kLoraSmall> small;
+    } sm;
+    return a.n_tokens <= kWave ? few_tile(a, tile, m, sm.few) : small_tile(a, tile, m, sm.small);
+}
+
+__device__ __forceinline__ bool tile_of(const Args& a, uint32_t tile, Mine<2>& m) {
+    static_assert(kN * 2 == zlm::kLoraTile, "as the tokens are grouped");
+    if (tile >= *a.n_tiles) return false;
+    const LoraTile t = a.tile[tile];
+    m.adapter = t.adapter;
+    m.rank = rank_of(a, t.adapter);
+    m.n = t.n;
+#pragma unroll
+    for (int i = 0; i < 2; i++) m.token[i] = a.order[t.first + (m.live(i) ? kN * i + (threadIdx.x & (kN - 1)) : 0)];
+    return true;
 }
 
 // The tokens by adapter: counted, their places summed up, then put there (in any order: a
@@ -417,6 +483,50 @@ __device__ __forceinline__ void load_h(const Args& a, const Mine<kNt>& mine, uin
         }
 }
 
+// The same by a workgroup of four waves with one tile: each sums a quarter, through LDS.
+template <int kKt>
+__device__ __forceinline__ void share_h(const Args& a, const Mine<1>& mine, uint32_t tile, v8b (&hp)[1][kKt][3]) {
+    constexpr uint32_t kPitch = 32 * kKt + 4, kPer = 8 * kKt, kEach = kN * kPer / 256;  // by four
+    __shared__ __attribute__((aligned(16))) float h[kN * kPitch];
+    const uint32_t tid = threadIdx.x, m = tid & 15, q = (tid & (kWave - 1)) >> 4, r = mine.rank;
+    const uint64_t step = static_cast<uint64_t>(a.tiles) * kN * a.rank;
+    v4f sum[kEach];
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; i++) sum[i] = v4f{0, 0, 0, 0};
+    constexpr uint32_t kU = kEach <= 2 ? 4 : 2;  // splits in flight
+    for (uint32_t s = 0; s < a.splits; s += kU) {
+        v4f v[kU][kEach];
+#pragma unroll
+        for (uint32_t u = 0; u < kU; u++)
+#pragma unroll
+            for (uint32_t i = 0; i < kEach; i++) {
+                const uint32_t at = 256 * i + tid, j = at / kPer, k = 4 * (at % kPer);
+                v[u][i] = v4f{0, 0, 0, 0};
+                if (s + u < a.splits && j < mine.n && k < r)
+                    v[u][i] = *reinterpret_cast<const v4f*>(a.part + (s + u) * step + (static_cast<uint64_t>(tile) * kN + j) * a.rank + k);
+            }
+#pragma unroll
+        for (uint32_t u = 0; u < kU; u++)
+#pragma unroll
+            for (uint32_t i = 0; i < kEach; i++) sum[i] += v[u][i];
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; i++) {
+        const uint32_t at = 256 * i + tid, j = at / kPer, k = 4 * (at % kPer);
+#pragma unroll
+        for (uint32_t e = 0; e < 4; e++) sum[i][e] = k + e < r ? sum[i][e] : 0.0f;
+        *reinterpret_cast<v4f*>(h + j * kPitch + k) = sum[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < kKt; c++) {
+        const v4f lo = *reinterpret_cast<const v4f*>(h + m * kPitch + 32 * c + 8 * q);
+        const v4f hi = *reinterpret_cast<const v4f*>(h + m * kPitch + 32 * c + 8 * q + 4);
+        const float f[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        to_parts(f, hp[0][c]);
+    }
+}
+
 // Sixteen rows of an adapter's B, rows n + m: the lane's eights of runs c0 and on of the rank.
 template <class W, int kKt>
 __device__ __forceinline__ void load_b(const Args& a, const uint8_t* b, uint32_t n, uint32_t r, uint32_t c0, v4u (&w)[kKt][W::kVecs]) {
@@ -454,7 +564,9 @@ __device__ __forceinline__ void multiply_b(uint32_t r, uint32_t c0, v4u (&w)[kKt
 }
 
 // y of few tokens.  A wave: a tile and some rows of y, 32 at a time (two matrix tiles); the
-// next 32 rows' B and res are on their way while these are multiplied.
+// next 32 rows' B and res are on their way while these are multiplied.  A workgroup's waves have
+// one tile: past a rank of 32 they sum h's splits together (256 tokens of one adapter of rank
+// 256, k and rows 4096: 22 us, each wave by itself 28).
 template <class W, int kKt>
 __device__ __forceinline__ void up_few(const Args& a) {
     const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1), wid = __builtin_amdgcn_readfirstlane(tid / kWave);
@@ -462,7 +574,7 @@ __device__ __forceinline__ void up_few(const Args& a) {
     Mine<1> mine;
     if (!tile_of(a, tile, mine)) return;
     const uint32_t n0 = (blockIdx.x * 4 + wid) * a.wave_rows;
-    if (n0 >= a.rows) return;
+    if (kKt == 1 && n0 >= a.rows) return;
     const uint32_t n1 = min(n0 + a.wave_rows, a.rows);
     const bool with = mine.adapter < a.n_adapters;
     const uint32_t r = mine.rank;
@@ -493,7 +605,8 @@ __device__ __forceinline__ void up_few(const Args& a) {
     };
     load_rows(n0);
     v8b hp[1][kKt][3];
-    load_h(a, mine, tile, 0, hp);
+    if constexpr (kKt == 1) load_h(a, mine, tile, 0, hp);
+    else share_h(a, mine, tile, hp);
     for (uint32_t n = n0; n < n1; n += 32) {
         v4f acc[2][1] = {{v4f{0, 0, 0, 0}}, {v4f{0, 0, 0, 0}}};
 #pragma unroll
