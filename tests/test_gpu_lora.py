@@ -95,7 +95,7 @@ def check(got, want, bound):
 @pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("rank", [8, 16, 24, 32, 40, 64, 72, 128, 136, 256])
 @pytest.mark.parametrize("tokens,n_adapters,rows,k", [(1, 3, 100, 64), (5, 2, 33, 32), (64, 5, 129, 288), (65, 70, 260, 96),
-                                                      (300, 4, 515, 128)])
+                                                      (300, 4, 515, 128), (1100, 4, 515, 64)])
 def test_sizes(box, kind, rank, tokens, n_adapters, rows, k):
     _say(f"lora kind={kind} rank={rank} tokens={tokens} adapters={n_adapters} rows={rows} k={k}")
     rng = np.random.default_rng(rank + tokens)
@@ -111,7 +111,7 @@ def test_sizes(box, kind, rank, tokens, n_adapters, rows, k):
 
 
 @pytest.mark.parametrize("kind", TYPES)
-@pytest.mark.parametrize("tokens", [1, 16, 17, 63, 64, 65, 128, 1000])
+@pytest.mark.parametrize("tokens", [1, 16, 17, 63, 64, 65, 128, 1000, 1024, 1025, 1500])
 @pytest.mark.parametrize("mix", ["one", "none", "each", "blocks", "two"])
 def test_mixes(box, kind, tokens, mix):
     _say(f"lora kind={kind} tokens={tokens} mix={mix}")
@@ -150,7 +150,7 @@ def test_tiles_at_the_borders(box, tokens, mix):
 
 
 @pytest.mark.parametrize("kind", TYPES)
-@pytest.mark.parametrize("tokens", [3, 100])
+@pytest.mark.parametrize("tokens", [3, 100, 1100])
 def test_every_bit_of_a_number_counts(box, kind, tokens):
     """A and B pick single numbers: the result is exact where every part of x, of h and of the weights takes part (24
     bits of x by weights of 1; of the weights by x of 1 for f32; 13 bits by 11 for f16, 16 by 8 for bf16)."""
@@ -194,6 +194,19 @@ def test_larger(box, tokens, rank, n_adapters, rows, k):
 
 
 @pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("tokens,rank", [(511, 256), (512, 256), (513, 256), (1023, 128), (1024, 128), (1025, 128)])
+def test_between_few_and_many(box, kind, tokens, rank):
+    """Where the tiles' size changes: adapters in any order, ranks of their own, rows of y that end within a span."""
+    _say(f"lora few and many kind={kind} tokens={tokens} rank={rank}")
+    rng = np.random.default_rng(tokens)
+    n = 7
+    c = Case(kind, tokens, n, rank, 150, 160, rng, rng.integers(-1, n, tokens), rng.integers(1, rank + 1, n))
+    want, bound = c.want()
+    check(run(box, c), want, bound)
+    check(run(box, c, in_place=True), want, bound)
+
+
+@pytest.mark.parametrize("kind", TYPES)
 def test_rounds_of_the_scratch(box, kind):
     """More tokens and adapters of the largest rank than the scratch holds at once."""
     tokens, n, rank, rows, k = 6000, 4096, 256, 8, 32
@@ -211,7 +224,7 @@ def test_rounds_of_the_scratch(box, kind):
 
 
 @pytest.mark.parametrize("rows,y_stride,at", [(100, 300, 8), (100, 301, 8), (99, 300, 8), (100, 300, 3), (64, 64, 0)])
-@pytest.mark.parametrize("tokens", [9, 200, 300])
+@pytest.mark.parametrize("tokens", [9, 200, 300, 1100])
 def test_parts_of_wider_rows(box, rows, y_stride, at, tokens):
     """y as some columns of a packed product's rows, x as some of wider ones; what lies beside them stays."""
     k, x_stride, rank = 64, 100, 16
@@ -254,7 +267,7 @@ def test_what_is_not_a_number_stays_with_its_token(box):
     check(got[rest], want[rest], bound[rest])
 
 
-@pytest.mark.parametrize("tokens", [6, 150, 400])
+@pytest.mark.parametrize("tokens", [6, 150, 400, 1300])
 def test_captured(box, tokens):
     """Two graphs over one scratch, replayed for other adapters, tokens and residuals, against eager calls."""
     dev = box.dev

@@ -161,7 +161,7 @@ def test_other_arguments_of_adapters(box):
 
 @pytest.mark.parametrize("rank", [8, 256])
 @pytest.mark.parametrize("n_adapters", [1, 4096])
-@pytest.mark.parametrize("tokens", [1, 64, 65, 5000, 200000, 3000000])
+@pytest.mark.parametrize("tokens", [1, 64, 65, 256, 512, 1024, 1025, 5000, 200000, 3000000])
 def test_adapters_fit_the_scratch(box, rank, n_adapters, tokens):
     """Every launch's partials, tiles and order within the 64 MiB, whatever the sizes."""
     d, p = box.dev, 1 << 16

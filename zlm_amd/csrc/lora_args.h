@@ -7,8 +7,8 @@ namespace zlm {
 
 constexpr uint32_t kLoraAdapters = 4096;  // of one pool (the grouping counts their tokens in LDS)
 constexpr uint32_t kLoraRank = 256;
-constexpr uint32_t kLoraSmall = 256;      // tokens that a workgroup groups by itself, in tiles of 16
-constexpr uint32_t kLoraTile = 32;        // tokens of a tile where there are more
+constexpr uint32_t kLoraOwn = 256;        // tokens that a workgroup groups by itself
+constexpr uint32_t kLoraTiles[2] = {32, 16};  // tokens of a tile, of many tokens and of few
 // Waves of the first product's workgroups, and runs of 32 of k that each has in flight (at
 // most), with tiles of 16 tokens and of 32.
 constexpr uint32_t kLoraWaves[2] = {8, 4}, kLoraRuns[2] = {4, 2};
@@ -30,11 +30,12 @@ struct LoraArgs {
     uint64_t x_stride, y_stride;
     uint32_t n_adapters, rank, rows, k, n_tokens;
     uint32_t tiles;   // of the grid: a bound of their number
+    uint32_t per_tile;  // tokens, of kLoraTiles
     uint32_t splits;  // of k over workgroups
     uint32_t wave_rows;  // of y, that a wave of the second product takes
     uint32_t in_place, vectors;  // y is res; rows of y and res go by 16 bytes
     float* part;      // splits x tiles x tokens of a tile x rank: A x
-    uint32_t* order;  // what the grouping leaves (more than kLoraSmall tokens)
+    uint32_t* order;  // what the grouping leaves (more than kLoraOwn tokens)
     LoraTile* tile;
     uint32_t* n_tiles;
 };

@@ -3470,13 +3470,18 @@ extern "C" bool zlm_gpu_lora_enqueue(zlm_device* d, const zlm_lora* lora, uint32
     a.vectors = lora->rows % 4 == 0 && y_stride % 4 == 0 && aligned(y) && aligned(res);
     // Tokens of one round: as many as the scratch has room for.  Each adapter may begin a tile.
     const uint64_t groups = static_cast<uint64_t>(lora->n_adapters) + !a.in_place;
-    const auto tile_of = [](uint64_t n) { return n <= zlm::kLoraSmall ? 16 : zlm::kLoraTile; };
+    // Tiles of 16 tokens and the kernels of few up to 512 to 1024 tokens: 40 adapters, k and rows
+    // 4096, by those and by tiles of 32: rank 16, 512 tokens 21 and 21 us, 1024 26 and 32, 2048 39
+    // and 39; rank 128 34 and 42, 59 and 70, 112 and 98; one adapter of rank 256, 512 tokens 35
+    // and 55, eight 57 and 56, 1024 tokens 66 and 67, 92 and 83.
+    const uint64_t few = std::min<uint64_t>(1024, 131072 / lora->rank);
+    const auto tile_of = [&](uint64_t n) { return zlm::kLoraTiles[n <= few]; };
     const auto tiles_of = [&](uint64_t n) { return n / tile_of(n) + std::min(n, groups); };
     const auto bytes_of = [&](uint64_t n, uint64_t splits) {
         return tiles_of(n) * (splits * tile_of(n) * lora->rank * sizeof(float) + sizeof(zlm::LoraTile)) + (n + 1) * sizeof(uint32_t);
     };
     uint64_t most = std::min<uint64_t>(n_tokens, 1u << 20);
-    while (most > zlm::kLoraSmall && bytes_of(most, 1) > kServingScratch) most = (most + 1) / 2;
+    while (most > few && bytes_of(most, 1) > kServingScratch) most = (most + 1) / 2;
     if (!ensure_serving_scratch(d, "the adapters' scratch")) return false;
     // matrix tiles of 16 of the rank in the first product, runs of 32 in the second
     const auto step = [](uint32_t n) { return n <= 1 ? 0 : n <= 2 ? 1 : n <= 4 ? 2 : 3; };
@@ -3489,7 +3494,8 @@ extern "C" bool zlm_gpu_lora_enqueue(zlm_device* d, const zlm_lora* lora, uint32
         a.res = res ? res + t * y_stride : nullptr;
         a.y = y + t * y_stride;
         a.tiles = static_cast<uint32_t>(tiles_of(a.n_tokens));
-        const bool small = a.n_tokens <= zlm::kLoraSmall;
+        const bool small = a.n_tokens <= few;
+        a.per_tile = tile_of(a.n_tokens);
         // k over workgroups where tiles alone leave CUs without two, as many runs a wave as it has
         // in flight at least
         const uint64_t waves = zlm::kLoraWaves[!small], runs = 32 * waves * zlm::kLoraRuns[!small];
@@ -3514,7 +3520,7 @@ extern "C" bool zlm_gpu_lora_enqueue(zlm_device* d, const zlm_lora* lora, uint32
         while (!small && a.wave_rows < 512 && rounds(2 * a.wave_rows) < rounds(a.wave_rows)) a.wave_rows *= 2;
         const unsigned row_groups = static_cast<unsigned>((lora->rows + (small ? 4 : 1) * a.wave_rows - 1) / ((small ? 4 : 1) * a.wave_rows));
         void* args[] = {&a};
-        if ((!small && !launch(d, d->lora_group, 1, 1024, args, "adapters, tokens grouped")) ||
+        if ((a.n_tokens > zlm::kLoraOwn && !launch(d, d->lora_group, 1, 1024, args, "adapters, tokens grouped")) ||
             !launch3(d, d->lora[type][down][small].down, a.tiles, a.splits, (m_tiles + 7) / 8,
                      static_cast<unsigned>(64 * waves), args,
                      "adapters down") ||

@@ -3,10 +3,10 @@
 //     y[t] = res[t] + scale * B (A x[t]).
 // Built as a device-only code object (hipcc --genco) and loaded by the host library.
 //
-// Tokens are taken in tiles with one adapter, so that a tile reads its A and B once.  Up to
-// 256 tokens every workgroup finds its tile, of up to 16, by itself; more are grouped by a launch
-// before, in tiles of up to 32.  Then two launches: h = A x, k split over waves and workgroups, and
-// y = res + scale * B h.
+// Tokens are taken in tiles with one adapter, so that a tile reads its A and B once: of up to 16
+// of few tokens, of up to 32 of many.  Up to 256 tokens every workgroup finds its tile by itself;
+// more are grouped by a launch before.  Then two launches: h = A x, k split over waves and
+// workgroups, and y = res + scale * B h.
 //
 // Both products run on v_mfma_f32_16x16x32_bf16 with the tokens in the N dimension.  A
 // 32-bit number is the sum of three bf16 (8 bits of its 24 each, cut off, so exactly), an
@@ -172,8 +172,8 @@ __device__ __forceinline__ bool few_tile(const Args& a, uint32_t tile, Mine<1>& 
 // down by themselves.  k and rows 4096, bf16, by this and grouped by a launch in tiles of 32:
 // 65 tokens of 40 adapters of rank 16 12 and 18 us, of rank 256 63 and 65; 256 tokens of one
 // of rank 64 16 and 31, of 40 of rank 128 27 and 39, of 200 of rank 256 208 and 207.
-__device__ __forceinline__ bool small_tile(const Args& a, uint32_t tile, Mine<1>& m, Grouping<zlm::kLoraSmall>& sm) {
-    constexpr uint32_t kTokens = zlm::kLoraSmall, kWords = kTokens / kWave;
+__device__ __forceinline__ bool small_tile(const Args& a, uint32_t tile, Mine<1>& m, Grouping<zlm::kLoraOwn>& sm) {
+    constexpr uint32_t kTokens = zlm::kLoraOwn, kWords = kTokens / kWave;
     static_assert(kTokens <= 256, "a token in a byte, and a thread");
     const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1), wid = tid / kWave;
     const bool in = tid < kTokens, has = tid < a.n_tokens;
@@ -222,32 +222,38 @@ __device__ __forceinline__ bool small_tile(const Args& a, uint32_t tile, Mine<1>
     return true;
 }
 
-__device__ __forceinline__ bool tile_of(const Args& a, uint32_t tile, Mine<1>& m) {
-    __shared__ union {
-        Grouping<kWave> few;
-        Grouping<zlm::kLoraSmall> small;
-    } sm;
-    return a.n_tokens <= kWave ? few_tile(a, tile, m, sm.few) : small_tile(a, tile, m, sm.small);
-}
-
-__device__ __forceinline__ bool tile_of(const Args& a, uint32_t tile, Mine<2>& m) {
-    static_assert(kN * 2 == zlm::kLoraTile, "as the tokens are grouped");
+// As the launch before has grouped them.
+template <int kNt>
+__device__ __forceinline__ bool grouped_tile(const Args& a, uint32_t tile, Mine<kNt>& m) {
     if (tile >= *a.n_tiles) return false;
     const LoraTile t = a.tile[tile];
     m.adapter = t.adapter;
     m.rank = rank_of(a, t.adapter);
     m.n = t.n;
 #pragma unroll
-    for (int i = 0; i < 2; i++) m.token[i] = a.order[t.first + (m.live(i) ? kN * i + (threadIdx.x & (kN - 1)) : 0)];
+    for (int i = 0; i < kNt; i++) m.token[i] = a.order[t.first + (m.live(i) ? kN * i + (threadIdx.x & (kN - 1)) : 0)];
     return true;
 }
+
+__device__ __forceinline__ bool tile_of(const Args& a, uint32_t tile, Mine<1>& m) {
+    __shared__ union {
+        Grouping<kWave> few;
+        Grouping<zlm::kLoraOwn> small;
+    } sm;
+    if (a.n_tokens <= kWave) return few_tile(a, tile, m, sm.few);
+    if (a.n_tokens <= zlm::kLoraOwn) return small_tile(a, tile, m, sm.small);
+    return grouped_tile(a, tile, m);
+}
+
+__device__ __forceinline__ bool tile_of(const Args& a, uint32_t tile, Mine<2>& m) { return grouped_tile(a, tile, m); }
 
 // The tokens by adapter: counted, their places summed up, then put there (in any order: a
 // token's result does not depend on its place).  One workgroup; the first 8192 tokens'
 // adapters stay in registers between the two passes.
 __device__ __forceinline__ void group(const Args& a) {
     constexpr uint32_t kThreads = 1024, kMost = zlm::kLoraAdapters + 1, kPer = (kMost + kThreads - 1) / kThreads;
-    constexpr uint32_t kTile = zlm::kLoraTile, kHold = 8;
+    constexpr uint32_t kHold = 8;
+    const uint32_t tile = a.per_tile;
     __shared__ uint32_t count[kPer * kThreads], tiles_to[kPer * kThreads];
     __shared__ uint32_t sums[2][kThreads / kWave];
     const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1), wid = tid / kWave;
@@ -285,7 +291,7 @@ __device__ __forceinline__ void group(const Args& a) {
         const uint32_t g = tid * per + i;
         own[i] = i < per && g < groups ? count[g] : 0;
         n += own[i];
-        k += (own[i] + kTile - 1) / kTile;
+        k += (own[i] + tile - 1) / tile;
     }
     uint32_t to_n = n, to_k = k;
 #pragma unroll
@@ -318,7 +324,7 @@ __device__ __forceinline__ void group(const Args& a) {
             tiles_to[g] = to_k;
         }
         to_n += own[i];
-        to_k += (own[i] + kTile - 1) / kTile;
+        to_k += (own[i] + tile - 1) / tile;
     }
     __syncthreads();
     for (uint32_t i = tid; i < all; i += kThreads) {
@@ -328,8 +334,8 @@ __device__ __forceinline__ void group(const Args& a) {
             if (tiles_to[mid] <= i) lo = mid;
             else hi = mid;
         }
-        const uint32_t at = kTile * (i - tiles_to[lo]);
-        a.tile[i] = {lo, count[lo] + at, min(count[lo + 1] - count[lo] - at, kTile)};
+        const uint32_t at = tile * (i - tiles_to[lo]);
+        a.tile[i] = {lo, count[lo] + at, min(count[lo + 1] - count[lo] - at, tile)};
     }
     if (tid == 0) *a.n_tiles = all;
     __syncthreads();
