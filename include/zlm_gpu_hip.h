@@ -537,7 +537,8 @@ typedef struct {
  * aligned; res and y rows y_stride (0: rows), so that y may be a part of the rows of a packed
  * product.  res: may be y (rows without an adapter are left alone then), or null for 0; else
  * it lies apart from y, as x does.  Products have the accuracy of 32-bit ones over the adapters'
- * values, sums are 32-bit; an infinite or NaN x, or weight, makes NaN of what it reaches.  A
+ * values (of numbers under 2^-110 what lies under 2^-133 is cut off), sums are 32-bit; an
+ * infinite or NaN x, or weight, makes NaN of what it reaches.  A
  * token's results depend on the other tokens of the call by how sums are split only.  Uses the
  * library scratch of zlm_gpu_paged_attention_enqueue (call once before its capture). */
 bool zlm_gpu_lora_enqueue(zlm_device *dev, const zlm_lora *lora, uint32_t n_tokens, const int32_t *adapter,
