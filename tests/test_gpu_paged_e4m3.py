@@ -195,6 +195,50 @@ def test_scales_at_both_ends(box, lens, std):
     assert (np.abs(got - want).max((1, 2)) <= bound).all(), np.abs(got - want).max() / bound.max()
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("lens", [[(1, 40)], [(160, 160)]])
+@pytest.mark.parametrize("scales", [(134,), (135, 255), (112,), (0, 111)])
+def test_scales_at_their_limits_and_past_them(box, hd, lens, scales):
+    """Every block that is seen at the largest scale (K and V with 57344 and -57344 in each) or at the least one, or at
+    a byte past these, which counts as them: the rows read back exactly, and the attention on both routes."""
+    page, kv, group = 16, 2, 2
+    _say(f"attention e4m3 limits hd={hd} {lens} scales={scales}")
+    rng = np.random.default_rng(hd + scales[0])
+    b = paged.Batch(lens, page, rng)
+    pool = paged_more.Pool(kv, hd, page, b.n_pages)
+    paged_more.fill(pool, b, rng)
+    used = b.table[0, :-(-lens[0][1] // page)]
+    for side in "kv":
+        codes, of_block = pool.parts(side)
+        for i, page_id in enumerate(used):
+            for h in range(kv):
+                of_block[page_id, h, 0] = scales[(i + h) % len(scales)]
+                for at, code in enumerate((126, 254)):  # 448, -448
+                    off, dim = (0, int(rng.integers(hd))) if side == "k" else (at % page, int(rng.integers(hd)))
+                    if side == "k":
+                        codes[page_id, h, off, dim] = code
+                    else:
+                        codes[page_id, h, off // 8, off % 8, dim] = code
+    offs = np.arange(lens[0][1])
+    k, v = pool.rows(used[offs // page], offs % page)
+    most = 57344 if scales[0] > 112 else 448 * 2.0 ** -15
+    assert np.abs(k).max() == most and np.abs(v).max() == most and np.isfinite(k).all() and np.isfinite(v).all()
+    q = (rng.standard_normal((b.n_tokens, kv * group, hd)) * (16 / most)).astype(np.float32)
+    cache, batch = box.cache(pool), box.batch(b)
+    n = lens[0][0]
+    like = np.zeros((n, kv, hd), np.float32)
+    d_k, d_v = box.up(like), box.up(like)
+    assert box.dev.paged_read_enqueue(cache, batch, d_k, d_v), box.dev.last_error()
+    np.testing.assert_array_equal(box.down(d_k, like), k[-n:])
+    np.testing.assert_array_equal(box.down(d_v, like), v[-n:])
+    d_q, d_o = box.up(q), box.up(q)
+    assert box.dev.paged_attention_enqueue(cache, batch, d_q, d_o, kv * group, 0.01), box.dev.last_error()
+    got = box.down(d_o, q)
+    want, bound = paged_more.attend(pool, b, q, kv * group, np.float64(np.float32(0.01)))
+    assert (np.abs(got - want).max((1, 2)) <= bound).all(), np.abs(got - want).max() / bound.max()
+    assert bound.max() <= most * 2.0 ** -10  # (tight enough to tell a scale from the next)
+
+
 @pytest.mark.parametrize("hd,group,lens,window", [
     (256, 2, [(1100, 1300), (1, 9)], 0), (256, 2, [(520, 600)], 0), (128, 4, [(2100, 2100), (3, 70)], 0),
     (64, 4, [(1100, 1111), (40, 40)], 130)])
