@@ -85,6 +85,22 @@ def test_which_kernels_take_sinks(box, kind):
     assert whats(4, 4, window=5000, sinks=4) == [few]
 
 
+@pytest.mark.parametrize("kind", [zd.F16, zd.Q4_0, E4M3])
+@pytest.mark.parametrize("hd,kv,heads,window,least,most", [
+    (128, 1, 1, 64, 2048, 4096), (128, 1, 4, 64, 1024, 2048), (128, 1, 8, 1000, 512, 1024), (128, 8, 8, 1000, 512, 1024),
+    (256, 1, 4, 64, 512, 1024), (256, 8, 8, 256, 512, 1024), (256, 8, 16, 64, 256, 512), (64, 8, 8, 64, 1024, 1025)])
+def test_long_chunks_with_sinks(box, kind, hd, kv, heads, window, least, most):
+    """An item of the few-row kernel walks from its sequence's window on, however short the window: chunks of `least`
+    tokens are its, those of `most` and more the many-row kernel's."""
+    d, p, c = box.dev, 1 << 16, _cache(box.mod, type=kind, kv=kv, hd=hd)
+    for tokens in (64, 256, least, most, 2 * most, 8192):
+        d.launch_log(True)
+        assert d.paged_attention_enqueue(c, _batch(box.mod, seqs=1, tokens=tokens, stride=2000), p, p, heads, 0.1,
+                                         window=window, sinks=4), d.last_error()
+        many = "paged attention of many rows" in [r["what"] for r in d.launch_log_read()]
+        assert many == (tokens >= most), tokens
+
+
 def test_sinks_take_the_scratch_that_the_attention_has(box):
     d, p, b, c = box.dev, 1 << 16, _batch(box.mod), _cache(box.mod, type=E4M3)
     assert d.capture_begin()

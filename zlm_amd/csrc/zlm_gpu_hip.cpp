@@ -3232,9 +3232,17 @@ bool paged_attention(zlm_device* d, const zlm_paged_cache* cache, const zlm_page
     // With sinks, windows say how little a row sees: where the few-row kernel has no more items
     // of 16 rows than workgroups, it alone is the faster (windows of 64, 256 and 1024, 4
     // sinks: 256 tokens of 32 q and 8 kv heads of 128, e4m3 14, 16 and 23 us, both kernels 28, 33
-    // and 37, f16 15, 19 and 32, 27, 32 and 36; 1024 tokens 41, 54 and 82, 36, 44 and 63).
-    const bool shallow = window && sinks && static_cast<uint64_t>(window) + sinks <= 1100 &&
-                         (rows + 15) / 16 * cache->n_kv_heads <= 2ull * d->cus;
+    // and 37, f16 15, 19 and 32, 27, 32 and 36; 1024 tokens 41, 54 and 82, 36, 44 and 63), as long
+    // as its items have not too far to go: each walks from its sequence's window on, over as many
+    // positions as the chunk has besides.  f16, windows of 64 and 1024, few rows alone and both
+    // kernels: heads of 128, one kv head of one q head 2048 tokens 25 and 31 us, 31 and 33
+    // (3000 units of 128 positions), 4096 54 and 33, 62 and 36 (8300 and more), 8192 116 and 34;
+    // of four 1024 tokens 29 and 33, 36 and 36 (4100), 2048 39 and 34, 56 and 40 (8400 and more);
+    // heads of 256, of four 512 27 and 23, 35 and 32 (600 and 1500), 1024 31 and 24, 48 and 34 (2200
+    // and more), 2048 90 and 24; heads of 64, of four 1024 18 and 24, 23 and 25, 2048 25 and 26, 33 and 28.
+    const uint64_t few_items = (rows + 15) / 16 * cache->n_kv_heads;
+    const bool shallow = window && sinks && static_cast<uint64_t>(window) + sinks <= 1100 && few_items <= 2ull * d->cus &&
+                         few_items * (batch->n_tokens + window + sinks) <= (hd > 128 ? 2048ull : 6144ull) * 128;
     const bool many = !shallow && batch->n_tokens > batch->n_seqs && rows > std::min<uint64_t>(static_cast<uint64_t>(batch->n_seqs) * few_rows, enough);
     const bool few = !many || batch->n_seqs > 1;
     // Equal shares of the few-row kernel for the workgroups that the CUs hold at once: one
