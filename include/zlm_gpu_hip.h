@@ -512,7 +512,8 @@ bool zlm_gpu_paged_attention_enqueue(zlm_device *dev, const zlm_paged_cache *cac
 /* The same over a window and the first `sinks` positions, which stay visible: a row at
  * p sees [max(0, p - window + 1), p] and [0, min(sinks, p + 1)).  Positions between are
  * not read, so their pages may be given back (table entries that are no page).  window 0:
- * all from 0, whatever sinks. */
+ * all from 0, whatever sinks.  Positions are absolute: K was rotated for its own, so the
+ * distance of a row to the sinks grows with p. */
 bool zlm_gpu_paged_attention_sinks_enqueue(zlm_device *dev, const zlm_paged_cache *cache, const zlm_paged_batch *batch,
                                            const float *q, uint32_t n_heads, uint32_t window, uint32_t sinks,
                                            float scale, float *out);
@@ -590,8 +591,9 @@ bool zlm_gpu_sample_enqueue(zlm_device *dev, const float *logits, uint64_t strid
  * token, in order of index, whose cumulative weight exceeds u_draw[s] times the weight of
  * all.  So a token has the probability that the target's own draw has.
  * draft_logits null: q is 1 of the drafted token (a draft that was looked up, or greedy).  A
- * draft outside [0, vocab) is none: what follows is drawn from p.  Where all of a row's
- * logits are -inf or NaN nothing is accepted, and -1 drawn.  Weights are those of
+ * draft outside [0, vocab) is none: what follows is drawn from p.  Where all of a row's target
+ * logits are -inf or NaN p is 0: nothing is accepted, and -1 drawn; where all of its draft
+ * logits are, q is 0: its draft is accepted if p of it is above 0.  Weights are those of
  * zlm_gpu_sample_enqueue, shares and sums formed in 64 bits; numbers u in [0, 1).  token lies
  * apart from draft.  Uses the library scratch of zlm_gpu_paged_attention_enqueue (call once
  * before its capture). */
