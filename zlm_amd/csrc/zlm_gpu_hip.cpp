@@ -3481,7 +3481,11 @@ extern "C" bool zlm_gpu_lora_enqueue(zlm_device* d, const zlm_lora* lora, uint32
     // Tiles of 16 tokens and the kernels of few up to 512 to 1024 tokens: 40 adapters, k and rows
     // 4096, by those and by tiles of 32: rank 16, 512 tokens 21 and 21 us, 1024 26 and 32, 2048 39
     // and 39; rank 128 34 and 42, 59 and 70, 112 and 98; one adapter of rank 256, 512 tokens 35
-    // and 55, eight 57 and 56, 1024 tokens 66 and 67, 92 and 83.
+    // and 55, eight 57 and 56, 1024 tokens 66 and 67, 92 and 83.  (bf16.  f16 and f32, 512 tokens:
+    // rank 128 of 40 38 and 51, 63 and 73, of 8 37 and 53, 47 and 64, rank 256 of one 41 and 66, 63 and
+    // 83, of 8 64 and 67, 98 and 86; 1024 tokens: rank 16 of 40 27 and 35, 29 and 40, rank 128 66 and 77,
+    // 87 and 117, of 8 59 and 61, 78 and 73, rank 256 104 and 88, 153 and 113.  14336 rows, or k: alike,
+    // but f32 of rank 256 of one 146 and 129, 117 and 130.)
     const uint64_t few = std::min<uint64_t>(1024, 131072 / lora->rank);
     const auto tile_of = [&](uint64_t n) { return zlm::kLoraTiles[n <= few]; };
     const auto tiles_of = [&](uint64_t n) { return n / tile_of(n) + std::min(n, groups); };
