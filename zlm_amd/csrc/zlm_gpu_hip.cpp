@@ -3236,8 +3236,8 @@ bool paged_attention(zlm_device* d, const zlm_paged_cache* cache, const zlm_page
     // as its items have not too far to go: each walks from its sequence's window on, over as many
     // positions as the chunk has besides.  f16, windows of 64 and 1024, few rows alone and both
     // kernels: heads of 128, one kv head of one q head 2048 tokens 25 and 31 us, 31 and 33
-    // (3000 units of 128 positions), 4096 54 and 33, 62 and 36 (8300 and more), 8192 116 and 34;
-    // of four 1024 tokens 29 and 33, 36 and 36 (4100), 2048 39 and 34, 56 and 40 (8400 and more);
+    // (2100 and 3000 units of 128 positions), 4096 54 and 33, 62 and 36 (8300 and more), 8192 116 and 34;
+    // of four 1024 tokens 29 and 33, 36 and 36 (2200 and 4100), 2048 39 and 34, 56 and 40 (8400 and more);
     // heads of 256, of four 512 27 and 23, 35 and 32 (600 and 1500), 1024 31 and 24, 48 and 34 (2200
     // and more), 2048 90 and 24; heads of 64, of four 1024 18 and 24, 23 and 25, 2048 25 and 26, 33 and 28.
     const uint64_t few_items = (rows + 15) / 16 * cache->n_kv_heads;
